@@ -185,7 +185,7 @@ def _write(cache, rows, offsets, pages, slots, d):
     rows, pages, slots = rows[keep], pages[keep].long(), slots[keep].long()
     x = torch.where(torch.isnan(rows), torch.zeros_like(rows), rows).clamp(-LIMIT, LIMIT)
     low, high = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
-    scale, low = ((high - low) / 15).bfloat16(), low.bfloat16()
+    scale, low = ((high - low) / torch.full_like(low, 15.0)).bfloat16(), low.bfloat16()             # (a divisor that is a plain number would be a product)
     code = ((x.double() - low.double()) / scale.double()).round().clamp(0, 15)                       # in 64 bits: values lie next to a border
     code = torch.where(scale.double() > 0, code, torch.zeros_like(code)).to(torch.uint8)
     byte = code[..., 0::2] | code[..., 1::2] << 4
