@@ -30,7 +30,7 @@ def _add_gen_args(p):
     p.add_argument("--gpu", dest="gpu", action="store_true", default=None)
     p.add_argument("--no-gpu", dest="gpu", action="store_false")
     p.add_argument("--max-seq-len", type=int, default=4096)
-    p.add_argument("--kv-dtype", choices=["bf16", "q8"], default="bf16", help="KV cache rows on the GPU engine")
+    p.add_argument("--kv-dtype", choices=["bf16", "q8", "q4"], default="bf16", help="KV cache rows on the GPU engine")
 
 
 def build_parser() -> argparse.ArgumentParser:
@@ -45,7 +45,7 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--model", default=None); s.add_argument("--host", default="127.0.0.1"); s.add_argument("--port", type=int, default=8080)
     s.add_argument("--demo", action="store_true"); s.add_argument("--max-batch", type=int, default=4); s.add_argument("--max-seq-len", type=int, default=4096)
     s.add_argument("--gpu", dest="gpu", action="store_true", default=None); s.add_argument("--no-gpu", dest="gpu", action="store_false")
-    s.add_argument("--kv-dtype", choices=["bf16", "q8"], default="bf16"); s.add_argument("--no-warmup", action="store_true"); s.add_argument("--classical", default=None, help="classical-ML .apr model behind /v1/predict")
+    s.add_argument("--kv-dtype", choices=["bf16", "q8", "q4"], default="bf16"); s.add_argument("--no-warmup", action="store_true"); s.add_argument("--classical", default=None, help="classical-ML .apr model behind /v1/predict")
     s.add_argument("--tp-comm", choices=["fused", "nccl"], default="fused", help="tensor parallel (under torch.distributed.run): in-kernel collectives or NCCL")
     s.add_argument("--draft-layers", type=int, default=0, help="self-speculative decoding for lone greedy streams: layers in the draft (0 = off)")
     s.add_argument("--prefill-chunk", type=int, default=256, help="prompt tokens run between two decode steps")

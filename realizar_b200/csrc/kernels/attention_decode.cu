@@ -21,6 +21,7 @@
 #include <stdlib.h>
 #include "attn_decode_static.h"
 #include "attention_decode_body.cuh"
+#include "attention_q4.cuh"
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <math.h>
@@ -80,6 +81,7 @@ namespace rlz {
 
 // Validate and launch: picks the head-group tile, the K/V access mode and the merge strategy.
 static int attn_decode_dispatch(const AttnDecodeParams& p, cudaStream_t st) {
+  if (p.kv_q8 == 2) return attn_decode_q4_dispatch(p, st);
   if (p.head_dim % 8 || p.head_dim > 128 || p.head_dim < 8) return -1;
   if (p.n_kv_heads < 1 || p.n_heads % p.n_kv_heads || p.splits < 1 || p.batch < 1) return -2;
   if (p.rope_dim > p.head_dim || (p.rope_dim & 1)) return -3;

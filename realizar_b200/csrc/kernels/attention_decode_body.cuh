@@ -40,7 +40,7 @@ struct AttnDecodeParams {
   int32_t window;                      // > 0: attend to positions (pos - window, pos] only
   int32_t rope_table_len;              // positions covered by rope_table
   const float2* rope_table;            // [rope_table_len, rope_dim / 2] (cos, sin) or null
-  int32_t kv_q8;                       // 1: int8 cache rows of head_dim + 16 bytes (codes, then the fp32 scale of the row)
+  int32_t kv_q8;                       // 1: int8 cache rows of head_dim + 16 bytes (codes, then the fp32 scale of the row); 2: pages of 4-bit rows (kv_q4.cuh)
   int32_t num_pages;                   // pages in the cache (0: unknown, page ids are not checked)
 };
 

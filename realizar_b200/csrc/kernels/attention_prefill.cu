@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "tcgen05_common.cuh"
 #include "attention_decode_body.cuh"
+#include "attention_q4.cuh"
 #include <stdlib.h>
 
 namespace rlz {
@@ -27,21 +28,6 @@ __device__ int g_prefill_attn_error = 0;
 constexpr int FP_THREADS = 128;
 constexpr int FP_PAGE = 16;
 constexpr int FP_SLAB = 128 * 128;           // one [128 rows x 64 bf16] swizzled slab
-
-struct AttnPrefillParams {
-  const float* qkv;            // [T, ld_qkv] fp32, q section already rotated
-  float* out;                  // [T, ld_out] fp32, head-major
-  const __nv_bfloat16* k_cache;
-  const __nv_bfloat16* v_cache;
-  const int32_t* page_table;   // [max_pages] of this sequence
-  int64_t ld_qkv, ld_out;
-  int32_t n_heads, n_kv_heads, head_dim, q_off;
-  int32_t n_tokens, pos0;      // chunk rows are positions pos0 .. pos0 + n_tokens - 1
-  int32_t window, kv_q8;       // kv_q8: int8 cache rows of head_dim + 16 bytes (codes, then the fp32 row scale)
-  float scale;
-  int32_t out_bf16;            // 1: `out` is bf16 [T, ld_out] (the operand of the output projection GEMM), else fp32
-  const int32_t* pos0_ptr;     // when set, the position of row 0 is read from here (a launch captured in a CUDA graph serves any chunk)
-};
 
 template <int D>
 __global__ void __launch_bounds__(FP_THREADS) attn_prefill_tcgen05_kernel(const __grid_constant__ AttnPrefillParams p) {
@@ -505,6 +491,7 @@ int rlz_attn_prefill_impl(const rlz::AttnPrefillParams* pp, void* stream, int im
   if (p.n_tokens < 1 || p.n_kv_heads < 1 || p.n_heads % p.n_kv_heads || p.pos0 < 0 || p.window < 0) return -2;
   if (((uintptr_t)p.k_cache & 15) || ((uintptr_t)p.v_cache & 15) || ((uintptr_t)p.out & 15) || (p.ld_out & (p.out_bf16 ? 7 : 3)) || (p.head_dim & 7)) return -4;
   cudaStream_t st = (cudaStream_t)stream;
+  if (p.kv_q8 == 2) return impl == 1 ? -5 : attn_prefill_q4_dispatch(p, st);
   // implementation: "mma" (16-query tiles on mma.sync, bf16 caches) or "tc" (128-query tiles on tcgen05, also int8 caches);
   // RLZ_PREFILL_ATT forces one
   static const int impl_env = [] { const char* e = getenv("RLZ_PREFILL_ATT"); return !e ? -1 : (e[0] == 'm' ? 1 : 0); }();

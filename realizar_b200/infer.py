@@ -34,7 +34,7 @@ class InferenceConfig:
     trace_output: Optional[str] = None
     max_seq_len: int = 2048
     verbose: bool = False
-    kv_dtype: str = "bf16"                 # "q8": int8 KV cache on the GPU engine
+    kv_dtype: str = "bf16"                 # "q8" / "q4": int8 / 4-bit KV cache on the GPU engine
 
     def with_prompt(self, p): self.prompt = p; return self
     def with_max_tokens(self, n): self.max_tokens = n; return self

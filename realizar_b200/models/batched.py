@@ -57,7 +57,9 @@ class BatchedForward:
         self.k_cache, self.v_cache = k_cache, v_cache
         self.max_pages = max_pages
         self.splits = 1
-        self.attn_partial, self.attn_counters = ops.attn_decode_scratch(T, model.heads, self.splits, cfg.head_dim, dev)
+        self.kv_q4 = ops.kv_format(k_cache, cfg.head_dim) == ops.KV_Q4
+        self.attn_partial, self.attn_counters = ops.attn_decode_scratch(T, model.heads, self.splits, cfg.head_dim, dev, "q4" if self.kv_q4 else "bf16")
+        self.prefill_scratch = ops.attn_prefill_scratch(T, model.heads, model.kv_heads, cfg.head_dim, dev) if self.kv_q4 else None
         self.launches_per_pass = 0
         self.flash_ok = ops.attn_prefill_supported(cfg.head_dim) and self.attn.stride(0) % 4 == 0
         self.flash_min_tokens = 16
@@ -207,17 +209,22 @@ class BatchedForward:
                 up_fused = self._gemm_to_operand(L.up, xb, self.act_b[:, L.down_in_off:], T, L.up_b, act_code)
                 if not up_fused:
                     self._gemm(L.up, xb, self.gate, T, bias=L.up_b)    # activation applied when the bf16 operand is produced
-            if L.q_norm_w is not None:
-                ops.head_rmsnorm_(qkv, L.q_norm_w, m.heads, hd, cfg.eps)
-                ops.head_rmsnorm_(qkv[:, qd:], L.k_norm_w, m.kv_heads, hd, cfg.eps)
-                self.launches_per_pass += 2
-            if cfg.uses_rope:                                  # the k heads follow the q heads in a row: one launch rotates both
-                ops.rope_(qkv, self.positions[:T], m.heads + m.kv_heads, hd, cfg.rope_dim, cfg.rope_type, cfg.rope_theta, table=m.rope_table)
-                self.launches_per_pass += 1
-            ops.kv_append(qkv[:, qd:], qkv[:, qd + kvd:], self.k_cache[l], self.v_cache[l], self.positions[:T], self.page_rows[:T], m.kv_heads, hd)
+            if self.kv_q4:                                     # one launch: norm, rotation and the write of the 4-bit rows
+                ops.qk_norm_rope_append(qkv, self.positions[:T], self.page_rows[:T], self.k_cache[l], self.v_cache[l], m.heads, m.kv_heads, hd,
+                                        q_norm_w=L.q_norm_w, k_norm_w=L.k_norm_w, eps=cfg.eps, rope_dim=cfg.rope_dim if cfg.uses_rope else 0,
+                                        rope_type=cfg.rope_type, rope_table=m.rope_table if cfg.uses_rope else None, rope_theta=cfg.rope_theta)
+            else:
+                if L.q_norm_w is not None:
+                    ops.head_rmsnorm_(qkv, L.q_norm_w, m.heads, hd, cfg.eps)
+                    ops.head_rmsnorm_(qkv[:, qd:], L.k_norm_w, m.kv_heads, hd, cfg.eps)
+                    self.launches_per_pass += 2
+                if cfg.uses_rope:                                  # the k heads follow the q heads in a row: one launch rotates both
+                    ops.rope_(qkv, self.positions[:T], m.heads + m.kv_heads, hd, cfg.rope_dim, cfg.rope_type, cfg.rope_theta, table=m.rope_table)
+                    self.launches_per_pass += 1
+                ops.kv_append(qkv[:, qd:], qkv[:, qd + kvd:], self.k_cache[l], self.v_cache[l], self.positions[:T], self.page_rows[:T], m.kv_heads, hd)
             if pos0 is not None and shared_table and T >= self.flash_min_tokens and self.flash_ok and (L.o_in_off * 2) % 16 == 0:
                 ops.attn_prefill(self.qkv, self.attn_b[:, L.o_in_off:], self.k_cache[l], self.v_cache[l], page_table, T, pos0, m.heads, m.kv_heads, hd,
-                                 q_off=0, window=cfg.sliding_window or 0, pos0_dev=pos0_dev)       # bf16 result, read directly by the o_proj GEMM
+                                 q_off=0, window=cfg.sliding_window or 0, pos0_dev=pos0_dev, scratch=self.prefill_scratch)       # bf16 result, read directly by the o_proj GEMM
                 self.launches_per_pass += 3
             else:
                 ops.attn_decode_launch(ops.build_attn_decode_params(

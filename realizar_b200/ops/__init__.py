@@ -234,7 +234,8 @@ def device_error(clear: bool = True) -> int:
     """Error code recorded by a kernel whose bounded wait expired (0 = none)."""
     c = 1 if clear else 0
     return (int(lib().rlz_device_error(c)) or int(lib().rlz_gemv_slab_error(c)) or int(lib().rlz_gemm_error(c))
-            or int(lib().rlz_attn_decode_error(c)) or int(lib().rlz_attn_prefill_error(c)) or int(lib().rlz_index_error(c)))
+            or int(lib().rlz_attn_decode_error(c)) or int(lib().rlz_attn_prefill_error(c)) or int(lib().rlz_index_error(c))
+            or int(lib().rlz_q4_append_error(c)) or int(lib().rlz_attn_q4_error(c)))
 
 
 def gemv(w: DeviceWeight, x: torch.Tensor, bias=None, act=ACT_NONE, residual=None, norm=NORM_NONE, norm_w=None, norm_b=None,
@@ -253,8 +254,14 @@ def gemv(w: DeviceWeight, x: torch.Tensor, bias=None, act=ACT_NONE, residual=Non
 
 
 # ------------------------------------------------------------------------------ attention --
-def attn_decode_scratch(batch: int, n_heads: int, splits: int, head_dim: int, device):
-    partial = torch.empty(int(lib().rlz_attn_decode_partial_floats(batch, n_heads, splits, head_dim)), device=device, dtype=torch.float32)
+def attn_decode_scratch(batch: int, n_heads: int, splits: int, head_dim: int, device, kv_dtype: str = "bf16"):
+    """Workspace of the decode attention: partial results and arrival counters (zero between launches).  One to a stream: launches
+    that may run at the same time must not share it.  A 4-bit cache (``kv_dtype="q4"``) ignores ``splits``: its kernel divides the
+    cached tokens itself."""
+    floats = int(lib().rlz_attn_decode_partial_floats(batch, n_heads, splits, head_dim))
+    if kv_dtype == "q4":
+        floats = max(floats, int(lib().rlz_attn_q4_partial_floats(head_dim)))
+    partial = torch.empty(floats, device=device, dtype=torch.float32)
     counters = torch.zeros(int(lib().rlz_attn_decode_counter_ints(batch, n_heads)), device=device, dtype=torch.int32)
     return partial, counters
 
@@ -262,6 +269,22 @@ def attn_decode_scratch(batch: int, n_heads: int, splits: int, head_dim: int, de
 def build_attn_decode_params(qkv, out, k_cache, v_cache, positions, page_table, partial, counters, n_heads, n_kv_heads, head_dim,
                              splits, batch, rope_dim, rope_type, rope_theta, q_off, k_off, v_off, q_norm_w=None, k_norm_w=None,
                              eps=1e-6, ld_qkv=None, ld_out=None, shared_table=False, no_append=False, window=0, rope_table=None) -> S.AttnDecodeParams:
+    fmt = kv_format(k_cache, head_dim)
+    if fmt == KV_Q4:
+        _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, out, positions, page_table, partial, counters)
+        if batch < 1 or qkv.shape[0] < batch or out.shape[0] < batch or positions.numel() < batch or counters.numel() < batch * n_heads:
+            raise ValueError(f"batch {batch}: qkv, out, positions or counters hold fewer rows")
+        if not shared_table and page_table.dim() > 1 and page_table.shape[0] < batch:
+            raise ValueError(f"page_table has {page_table.shape[0]} rows for a batch of {batch}")
+        if qkv.dtype != torch.float32 or out.dtype != torch.float32 or qkv.stride(-1) != 1 or out.stride(-1) != 1 or page_table.stride(-1) != 1:
+            raise ValueError("qkv and out must be float32 with contiguous rows, page_table rows contiguous")
+        if positions.dtype != torch.int32 or page_table.dtype != torch.int32 or not positions.is_contiguous():
+            raise ValueError("positions and page_table must be contiguous int32")
+        if (q_norm_w is None) != (k_norm_w is None):
+            raise ValueError("q_norm_w and k_norm_w come together")
+        _check_current_device(k_cache)
+        if partial.numel() < int(lib().rlz_attn_q4_partial_floats(head_dim)):
+            raise ValueError("partial is too small for a 4-bit cache: take it from attn_decode_scratch(..., kv_dtype='q4')")
     p = S.AttnDecodeParams()
     p.qkv, p.out, p.k_cache, p.v_cache = qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     p.positions, p.page_table = positions.data_ptr(), page_table.data_ptr()
@@ -276,7 +299,7 @@ def build_attn_decode_params(qkv, out, k_cache, v_cache, positions, page_table, 
     p.pt_stride = 0 if shared_table else (page_table.stride(0) if page_table.dim() > 1 else page_table.shape[-1])
     p.no_append = 1 if no_append else 0
     p.window = int(window or 0)
-    p.kv_q8 = 1 if k_cache.dtype in (torch.uint8, torch.int8) else 0
+    p.kv_q8 = fmt
     p.num_pages = int(k_cache.shape[0]) if k_cache.dim() >= 4 else 0      # [pages, kv_heads, page, row]: page ids are checked on the device
     if rope_table is not None:
         if rope_table.dtype != torch.float32 or rope_table.dim() != 3 or rope_table.shape[1] != rope_dim // 2 or rope_table.shape[2] != 2 or not rope_table.is_contiguous():
@@ -302,17 +325,39 @@ def attn_prefill_supported(head_dim: int) -> bool:
 
 def attn_prefill(qkv: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, n_tokens: int,
                  pos0: int, n_heads: int, n_kv_heads: int, head_dim: int, q_off: int = 0, window: int = 0,
-                 pos0_dev: Optional[torch.Tensor] = None, impl: Optional[str] = None) -> None:
+                 pos0_dev: Optional[torch.Tensor] = None, impl: Optional[str] = None, scratch: Optional[torch.Tensor] = None) -> None:
     """Causal attention of chunk rows ``pos0 .. pos0+n_tokens-1`` of one sequence over its paged cache
     (tensor-core kernel; the chunk's own K/V rows must already be in the cache).  With ``pos0_dev`` (an int32 device
     tensor) the position of row 0 is read on the device, so a captured launch serves every chunk position.
-    ``impl``: "tc" (128-query tiles on tcgen05) or "mma" (16-query tiles on mma.sync); None = the launcher's choice."""
+    ``impl``: "tc" (128-query tiles on tcgen05) or "mma" (16-query tiles on mma.sync); None = the launcher's choice.
+    ``scratch`` (4-bit caches, from ``attn_prefill_scratch``, one to a stream): lets few rows over a long context be split over the keys."""
+    fmt = kv_format(k_cache, head_dim)
+    if fmt == KV_Q4:
+        if n_tokens < 1:
+            raise ValueError(f"n_tokens must be at least 1, got {n_tokens}")
+        _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, out, page_table, pos0_dev, scratch)
+        if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[0] < n_tokens or qkv.shape[1] < q_off + n_heads * head_dim:
+            raise ValueError("qkv must be float32 [>= n_tokens, >= q_off + n_heads * head_dim] with contiguous rows")
+        if out.dtype not in (torch.float32, torch.bfloat16) or out.dim() != 2 or out.stride(1) != 1 or out.shape[0] < n_tokens or out.shape[1] < n_heads * head_dim:
+            raise ValueError("out must be float32 or bfloat16 [>= n_tokens, >= n_heads * head_dim] with contiguous rows")
+        if page_table.dtype != torch.int32 or page_table.dim() != 1 or page_table.stride(0) != 1:
+            raise ValueError("page_table must be a contiguous int32 row")
+        if pos0 < 0 or window < 0 or (pos0_dev is None and pos0 + n_tokens > 16 * page_table.numel()):
+            raise ValueError(f"positions {pos0} .. {pos0 + n_tokens - 1} are not covered by {page_table.numel()} pages")
+        if pos0_dev is not None and pos0_dev.dtype != torch.int32:
+            raise ValueError("pos0_dev must be int32")
+        if scratch is not None and (scratch.dtype != torch.float32 or not scratch.is_contiguous()):
+            raise ValueError("scratch must be a contiguous float32 tensor from attn_prefill_scratch")
+        _check_current_device(k_cache)
     p = S.AttnPrefillParams()
     p.qkv, p.out, p.k_cache, p.v_cache, p.page_table = qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr()
     p.ld_qkv, p.ld_out = qkv.stride(0), out.stride(0)
     p.n_heads, p.n_kv_heads, p.head_dim, p.q_off = n_heads, n_kv_heads, head_dim, q_off
     p.n_tokens, p.pos0, p.window, p.scale = int(n_tokens), int(pos0), int(window or 0), head_dim ** -0.5
-    p.kv_q8 = 1 if k_cache.dtype in (torch.uint8, torch.int8) else 0
+    p.kv_q8 = fmt
+    if fmt == KV_Q4:
+        p.num_pages, p.pt_len = int(k_cache.shape[0]), int(page_table.shape[-1])
+        p.scratch, p.scratch_floats = ptr(scratch), 0 if scratch is None else scratch.numel()
     p.out_bf16 = 1 if out.dtype == torch.bfloat16 else 0          # bf16: written as the operand of the output-projection GEMM
     p.pos0_ptr = ptr(pos0_dev)
     check(lib().rlz_attn_prefill_impl(ctypes.byref(p), stream_ptr(), {None: -1, "tc": 0, "mma": 1}[impl]), "attn_prefill")
@@ -322,13 +367,61 @@ def attn_prefill_error(clear: bool = True) -> int:
     return int(lib().rlz_attn_prefill_error(1 if clear else 0))
 
 
+def attn_prefill_scratch(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Workspace with which ``attn_prefill`` splits chunks of up to ``n_tokens`` rows over a 4-bit cache along the keys when the rows
+    alone leave SMs idle.  One to a stream; it keeps nothing from one call for the next."""
+    return torch.zeros(int(lib().rlz_attn_prefill_q4_scratch_floats(int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim))), device=device, dtype=torch.float32)
+
+
+KV_BF16, KV_Q8, KV_Q4 = 0, 1, 2
+Q4_HEAD_DIMS = (64, 80, 96, 128)
+
+
+def kv_format(cache: torch.Tensor, head_dim: int) -> int:
+    """Row format of a cache tensor: its type, and for bytes the length of a row."""
+    if cache.dtype not in (torch.uint8, torch.int8):
+        return KV_BF16
+    return KV_Q4 if cache.shape[-1] == head_dim // 2 + 4 else KV_Q8
+
+
+def _check_q4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, n_kv_heads: int, head_dim: int, *others) -> None:
+    if head_dim not in Q4_HEAD_DIMS:
+        raise ValueError(f"4-bit caches serve head_dim {', '.join(map(str, Q4_HEAD_DIMS))}, got {head_dim}")
+    for t in (k_cache, v_cache):
+        if t.dtype != torch.uint8 or t.dim() != 4 or tuple(t.shape[1:]) != (n_kv_heads, 16, head_dim // 2 + 4) or t.shape[0] < 1 or not t.is_contiguous():
+            raise ValueError(f"a 4-bit cache is a contiguous uint8 [pages, {n_kv_heads}, 16, {head_dim // 2 + 4}] tensor, got {t.dtype} {tuple(t.shape)}")
+    if v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    for t in (v_cache, *others):
+        if t is not None and t.device != k_cache.device:
+            raise ValueError(f"tensors on {t.device} and {k_cache.device}: all of a call must be on one device")
+
+
+def _check_current_device(t: torch.Tensor) -> None:
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device}, which is not the current CUDA device")
+
+
+def kv_row_bytes(head_dim: int, dtype: str) -> int:
+    """Bytes of a cached key or value row of one kv head."""
+    if dtype not in ("bf16", "q8", "q4"):
+        raise ValueError(f"unknown KV cache dtype '{dtype}' (bf16 | q8 | q4)")
+    return {"bf16": 2 * head_dim, "q8": head_dim + 16, "q4": head_dim // 2 + 4}[dtype]
+
+
 def kv_cache_alloc(layers: int, pages: int, kv_heads: int, head_dim: int, device, dtype: str = "bf16", page: int = 16) -> torch.Tensor:
     """``[2 (k, v), layers, pages, kv_heads, page, row]``: bf16 rows of ``head_dim``, or with ``dtype="q8"`` uint8 rows of
-    ``head_dim + 16`` bytes (int8 codes, the fp32 scale of the row, padding)."""
+    ``head_dim + 16`` bytes (int8 codes, the fp32 scale of the row, padding).  With ``dtype="q4"`` a page is
+    ``16 * (head_dim / 2 + 4)`` bytes of 4-bit codes and of a bf16 scale and minimum to each row; inside a page the codes lie in
+    the order of the tensor-core operand (csrc/kernels/kv_q4.cuh), so only whole pages are to be copied."""
+    if dtype == "q4":
+        if head_dim not in Q4_HEAD_DIMS or page != 16:
+            raise ValueError(f"4-bit caches serve head_dim {', '.join(map(str, Q4_HEAD_DIMS))} in pages of 16, got {head_dim} and {page}")
+        return torch.zeros(2, layers, pages, kv_heads, page, head_dim // 2 + 4, device=device, dtype=torch.uint8)
     if dtype == "q8":
         return torch.zeros(2, layers, pages, kv_heads, page, head_dim + 16, device=device, dtype=torch.uint8)
     if dtype != "bf16":
-        raise ValueError(f"unknown KV cache dtype '{dtype}' (bf16 | q8)")
+        raise ValueError(f"unknown KV cache dtype '{dtype}' (bf16 | q8 | q4)")
     return torch.zeros(2, layers, pages, kv_heads, page, head_dim, device=device, dtype=torch.bfloat16)
 
 
@@ -336,9 +429,81 @@ def kv_rows_to_float(cache: torch.Tensor, head_dim: int) -> torch.Tensor:
     """Decode cache rows ``[..., row]`` (either layout) to fp32 ``[..., head_dim]`` (tests, snapshots, debugging)."""
     if cache.dtype == torch.bfloat16:
         return cache.float()
+    if kv_format(cache, head_dim) == KV_Q4:
+        raise ValueError("the rows of a 4-bit page are not contiguous: decode whole pages with kv_pages_to_float")
     codes = cache[..., :head_dim].contiguous().view(torch.int8).float()
     scale = cache[..., head_dim:head_dim + 4].contiguous().view(torch.float32)
     return codes * scale
+
+
+def _q4_byte_order(head_dim: int, values: bool, device) -> torch.Tensor:
+    """``[16, head_dim / 2]``: the byte of a 4-bit page that holds dims ``2b`` (low bits) and ``2b + 1`` of token ``t``."""
+    t, b = torch.arange(16, device=device)[:, None], torch.arange(head_dim // 2, device=device)[None, :]
+    ng = head_dim // 32
+    if not values:
+        w = b // 4
+        return t * (head_dim // 2) + torch.where(w < 4 * ng, (w % 4) * ng + w // 4, w) * 4 + b % 4
+    half, tq, odd, e = t // 8, (t % 8) // 2, t % 2, b // 2
+    main = (((half * 8 + e % 8) * 4 + tq) * ng + e // 8) * 4 + odd * 2 + b % 2
+    return torch.where(b < 16 * ng, main, 256 * ng + ((b - 16 * ng) * 4 + tq) * 4 + half * 2 + odd)
+
+
+def kv_pages_to_float(pages: torch.Tensor, head_dim: int, values: bool) -> torch.Tensor:
+    """Decode whole pages ``[..., 16, row]`` of any cache format to fp32 ``[..., 16, head_dim]`` (tests, snapshots, debugging).
+    ``values``: the pages come from the value cache (4-bit key and value pages are laid out differently)."""
+    if kv_format(pages, head_dim) != KV_Q4:
+        return kv_rows_to_float(pages, head_dim)
+    flat = pages.flatten(-2)
+    byte = flat[..., _q4_byte_order(head_dim, values, pages.device)]
+    codes = torch.stack([byte & 15, byte >> 4], -1).flatten(-2).float()
+    meta = flat[..., 8 * head_dim:].contiguous().view(torch.bfloat16).unflatten(-1, (16, 2)).float()
+    return codes * meta[..., :1] + meta[..., 1:]
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, page_rows: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_heads: int,
+                        n_kv_heads: int, head_dim: int, q_out: Optional[torch.Tensor] = None, q_norm_w: Optional[torch.Tensor] = None,
+                        k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6, rope_dim: int = 0, rope_type: int = 0,
+                        rope_table: Optional[torch.Tensor] = None, rope_theta: float = 10000.0) -> None:
+    """Rows ``qkv [n, >= (n_heads + 2 n_kv_heads) * head_dim]`` (fp32: q heads, k heads, v heads) in one launch: RMS norm of every q and
+    k head (when the weights are given), rotation of their first ``rope_dim`` values (``rope_type`` 2: split halves, else adjacent
+    pairs) by the table or, beyond it, by ``rope_theta``, the rotated queries to ``q_out`` (default: in place), and the k and v rows
+    into the 4-bit cache at ``positions[i]`` of page ``page_rows[i]``.  Rows with a position below 0 are left out altogether.  No two
+    rows of a call may name the same place.  Keys are normalised and rotated in 64 bits, so that the cached codes do not depend on
+    which kernel wrote them."""
+    if kv_format(k_cache, head_dim) != KV_Q4:
+        raise ValueError("qk_norm_rope_append writes 4-bit caches (kv_cache_alloc(dtype='q4')); other formats take head_rmsnorm_, rope_ and kv_append")
+    _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, positions, page_rows, q_out, q_norm_w, k_norm_w, rope_table)
+    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads:
+        raise ValueError(f"{n_heads} query heads do not divide over {n_kv_heads} kv heads")
+    if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
+        raise ValueError("qkv must be float32 [rows, >= (n_heads + 2 n_kv_heads) * head_dim] with contiguous rows")
+    n = qkv.shape[0]
+    q = qkv if q_out is None else q_out
+    if q.dtype != torch.float32 or q.dim() != 2 or q.stride(1) != 1 or q.shape[0] < n or q.shape[1] < n_heads * head_dim:
+        raise ValueError("q_out must be float32 [>= rows, >= n_heads * head_dim] with contiguous rows")
+    for name, t in (("positions", positions), ("page_rows", page_rows)):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < n:
+            raise ValueError(f"{name} must be a contiguous int32 vector of at least {n} entries")
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise ValueError("q_norm_w and k_norm_w come together")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != head_dim or not w.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous float32 of {head_dim} entries")
+    if rope_dim < 0 or rope_dim > head_dim or rope_dim % 2:
+        raise ValueError(f"rope_dim must be even and at most {head_dim}, got {rope_dim}")
+    if rope_table is not None and (rope_table.dtype != torch.float32 or rope_table.dim() != 3 or tuple(rope_table.shape[1:]) != (rope_dim // 2, 2)
+                                   or not rope_table.is_contiguous()):
+        raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim / 2, 2] (cos, sin) tensor")
+    _check_current_device(k_cache)
+    if n == 0:
+        return
+    p = S.QkAppendParams()
+    p.qkv, p.q_out, p.k_cache, p.v_cache = qkv.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    p.positions, p.page_rows, p.q_norm_w, p.k_norm_w, p.rope_table = positions.data_ptr(), page_rows.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), ptr(rope_table)
+    p.ld, p.ld_q, p.eps, p.rows, p.n_heads, p.n_kv_heads, p.head_dim = qkv.stride(0), q.stride(0), eps, n, n_heads, n_kv_heads, head_dim
+    p.rope_dim, p.rope_type, p.rope_theta, p.num_pages = rope_dim, rope_type, rope_theta, k_cache.shape[0]
+    p.rope_table_len = 0 if rope_table is None else rope_table.shape[0]
+    check(lib().rlz_qk_norm_rope_append(ctypes.byref(p), stream_ptr()), "qk_norm_rope_append")
 
 
 # ------------------------------------------------------------------------------ small ops --
@@ -404,6 +569,8 @@ def swiglu_bf16(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor, act=ACT
 
 def kv_append(k, v, k_cache, v_cache, positions, page_rows, n_kv_heads, d, page=16) -> None:
     """Write the rows of ``k`` / ``v`` at their positions into the paged cache (bf16 rows, or int8 rows with a per-row scale)."""
+    if kv_format(k_cache, d) == KV_Q4:
+        raise ValueError("4-bit caches are written by qk_norm_rope_append")
     fn = lib().rlz_kv_append_q8 if k_cache.dtype in (torch.uint8, torch.int8) else lib().rlz_kv_append
     check(fn(k.data_ptr(), v.data_ptr(), k.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
              page_rows.data_ptr(), k.shape[0], n_kv_heads, d, page, k_cache.shape[0], stream_ptr()), "kv_append")

@@ -3,7 +3,7 @@ exported launcher of ``librlz_cuda.so``."""
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, Structure, c_float, c_int, c_int32, c_int64, c_longlong, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_int32, c_int64, c_longlong, c_void_p
 
 GEMV_MAX_MATS = 4
 GEMV_MAX_X = 4
@@ -61,7 +61,16 @@ class AttnPrefillParams(Structure):
     _fields_ = [("qkv", c_void_p), ("out", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("page_table", c_void_p),
                 ("ld_qkv", c_int64), ("ld_out", c_int64), ("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32),
                 ("q_off", c_int32), ("n_tokens", c_int32), ("pos0", c_int32), ("window", c_int32), ("kv_q8", c_int32), ("scale", c_float),
-                ("out_bf16", c_int32), ("pos0_ptr", c_void_p)]
+                ("out_bf16", c_int32), ("pos0_ptr", c_void_p), ("num_pages", c_int32), ("pt_len", c_int32), ("scratch", c_void_p),
+                ("scratch_floats", c_int64)]
+
+
+class QkAppendParams(Structure):
+    _fields_ = [("qkv", c_void_p), ("q_out", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("positions", c_void_p),
+                ("page_rows", c_void_p), ("q_norm_w", c_void_p), ("k_norm_w", c_void_p), ("rope_table", c_void_p), ("ld", c_int64),
+                ("ld_q", c_int64), ("eps", c_double), ("rows", c_int32), ("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32),
+                ("rope_dim", c_int32), ("rope_type", c_int32), ("rope_table_len", c_int32), ("num_pages", c_int32), ("rope_theta", c_float),
+                ("_pad", c_int32)]
 
 
 class SampleParams(Structure):
@@ -167,6 +176,13 @@ def declare(lib: ctypes.CDLL) -> None:
     lib.rlz_attn_prefill_impl.argtypes = [POINTER(AttnPrefillParams), c_void_p, c_int]
     lib.rlz_attn_prefill_supported.argtypes = [c_int]
     lib.rlz_attn_prefill_error.argtypes = [c_int]
+    lib.rlz_qk_norm_rope_append.argtypes = [POINTER(QkAppendParams), c_void_p]
+    lib.rlz_q4_append_error.argtypes = [c_int]
+    lib.rlz_attn_q4_error.argtypes = [c_int]
+    lib.rlz_attn_q4_partial_floats.argtypes = [c_int]
+    lib.rlz_attn_q4_partial_floats.restype = c_longlong
+    lib.rlz_attn_prefill_q4_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
+    lib.rlz_attn_prefill_q4_scratch_floats.restype = c_longlong
     lib.rlz_ll_reduce.argtypes = [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p]
     lib.rlz_advance.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]
     lib.rlz_page_rows.argtypes = [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p]

@@ -51,7 +51,7 @@ class EngineConfig:
     gemm_decode_min_batch: int = 16        # decode batches at least this large run on the tensor-core GEMM path
     prefix_cache: bool = False             # share full KV pages between prompts with a common prefix
     parity_gate: bool = False              # at load: GPU vs CPU logits on the BOS token must agree (cosine >= 0.99)
-    kv_dtype: str = "bf16"                 # "q8": int8 KV rows with a per-(token, head) scale (half the cache memory)
+    kv_dtype: str = "bf16"                 # "q8": int8 KV rows with a per-(token, head) scale (half the cache memory); "q4": 4-bit rows (a quarter)
     resident_layers: Optional[int] = None  # layers whose matrices stay on the device; None = all if they fit, else as many as fit (the rest is streamed)
     canaries: bool = False                 # guard bands around every step buffer, inspected by check_health() (also RLZ_CANARIES=1)
     batch_buckets: Sequence[int] = ()      # graph buckets; default powers of two up to max_batch
@@ -104,7 +104,7 @@ class DecodeEngine:
             from .memory import StreamingMode, check_vram_sufficient
             wc, c0 = weights.config, self.cfg
             pages = c0.num_pages or c0.max_batch * -(-c0.max_seq_len // PAGE)
-            rowb = (wc.head_dim + 16) if c0.kv_dtype == "q8" else 2 * wc.head_dim
+            rowb = ops.kv_row_bytes(wc.head_dim, c0.kv_dtype)
             kv_est = 2 * wc.num_layers * pages * (wc.num_kv_heads // max(1, tp_size)) * PAGE * rowb
             free_bytes, _t = torch.cuda.mem_get_info(self.device)
             try:
@@ -127,14 +127,14 @@ class DecodeEngine:
         hd = self.mcfg.head_dim
         # [2 (k,v), layers, pages, kv_heads, PAGE, head_dim] bf16
         from .memory import check_vram_sufficient
-        row = (hd + 16) if c.kv_dtype == "q8" else 2 * hd
+        row = ops.kv_row_bytes(hd, c.kv_dtype)
         kv_bytes = 2 * self.mcfg.num_layers * self.num_pages * m.kv_heads * PAGE * row
         free_bytes, _total = torch.cuda.mem_get_info(self.device)
         try:                                                 # the weights are on the device already: what is left must hold the cache
             check_vram_sufficient(0, kv_bytes, free_bytes, self.mcfg.num_layers)
         except MemoryError:
             raise RuntimeError(f"KV cache of {kv_bytes / 2**30:.1f} GiB ({self.num_pages} pages) does not fit the {free_bytes / 2**30:.1f} GiB "
-                               f"left on {self.profile.name}: lower max_batch / max_seq_len / num_pages or use kv_dtype='q8'") from None
+                               f"left on {self.profile.name}: lower max_batch / max_seq_len / num_pages or use kv_dtype='q8' or 'q4'") from None
         self.kv = ops.kv_cache_alloc(self.mcfg.num_layers, self.num_pages, m.kv_heads, hd, dev, c.kv_dtype, PAGE)
         self.pages = PagedKvCache(self.num_pages, PAGE)
         self.splits = c.attn_splits or self._choose_splits(B)        # at the full batch; smaller buckets split the context further
@@ -155,7 +155,7 @@ class DecodeEngine:
             _n[0] += 1
             return self.guards.zeros(*s, dtype=dt, name=f"step buffer {_n[0]} {tuple(s)} {str(dt).split('.')[-1]}")
         self.buckets = sorted(set(c.batch_buckets or [b for b in (1, 2, 4, 8, 16, 32, 64, 128) if b < B] + [B]))
-        part, ctr = ops.attn_decode_scratch(max(b * self.splits_for(b) for b in self.buckets), m.heads, 1, hd, dev)
+        part, ctr = ops.attn_decode_scratch(max(b * self.splits_for(b) for b in self.buckets), m.heads, 1, hd, dev, c.kv_dtype)
         # tokens and positions are the two rows of one buffer (and of one pinned host buffer), so a step uploads both with one copy
         tok_pos = torch.zeros(2, B, device=dev, dtype=torch.int32)
         tok_pos[1].fill_(-1)
@@ -240,7 +240,7 @@ class DecodeEngine:
         want = self.cfg.persistent_step
         if want is None:
             want = os.environ.get("RLZ_PERSISTENT", "0") != "0"
-        return bool(want) and bucket == 1 and self.comm is None and self.cfg.kv_dtype != "q8"
+        return bool(want) and bucket == 1 and self.comm is None and self.cfg.kv_dtype == "bf16"
 
     def kernels_per_step(self, bucket: int) -> int:
         p = self.plan(bucket)
@@ -361,7 +361,7 @@ class DecodeEngine:
         bw = peaks()["hbm_gbs"]
         prof = self.profile_step(batch, steps)
         ctx = sum(max(0, s.position) for s in self.slots[:batch] if s.active)
-        kv_bytes = 2 * self.mcfg.num_layers * self.mcfg.num_kv_heads * self.mcfg.head_dim * ctx * (1 if self.cfg.kv_dtype == "q8" else 2)
+        kv_bytes = 2 * self.mcfg.num_layers * self.mcfg.num_kv_heads * ops.kv_row_bytes(self.mcfg.head_dim, self.cfg.kv_dtype) * ctx
         nbytes = {"gemv": self.model.weight_bytes(), "gemm": self.model.weight_bytes(), "attn": kv_bytes}
         bricks = []
         for kind, st in prof.items():

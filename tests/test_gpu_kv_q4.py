@@ -1,0 +1,480 @@
+"""4-bit KV cache on the GPU: the fused norm + rotation + append, decode attention and prompt attention, each against a plain
+computation in 64 bits, and the three together.
+
+Tolerances.  Cached rows are compared bit for bit: the definition is in 64 bits and the kernels follow it exactly.  Rotated
+queries go through about 3 roundings and a 7-level sum in 32 bits: 2e-6 of the norm covers 30 half-steps of 2^-24.  fp32
+attention: operands are held to 22 bits (2^-23 each, query and probability), scores of size 10 carry 10 x 2^-22 into the
+exponent, sums of up to some thousand terms add a few 2^-23: 1e-5 of the norm.  bf16 results add half a step of 2^-9 relative
+to each value (rms 2^-9 / sqrt(3) = 1.1e-3 .. 2^-8 / 2), operands in 16 bits (fp16, 2^-12 each) stay well below: 4e-3 of the norm."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+LIMIT = 32768.0
+
+
+def _rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm().clamp(min=1e-300))
+
+
+def _rope64(x, pos, table, rope_dim, rope_type):
+    """x [n, heads, d] float64, table float32 (cos, sin)"""
+    if not rope_dim:
+        return x
+    cs = table.double()[pos.clamp(min=0).long()][:, None]
+    c, s = cs[..., 0], cs[..., 1]
+    i = torch.arange(rope_dim // 2, device=x.device)
+    p, q = (i, i + rope_dim // 2) if rope_type == 2 else (2 * i, 2 * i + 1)
+    y = x.clone()
+    y[..., p], y[..., q] = x[..., p] * c - x[..., q] * s, x[..., p] * s + x[..., q] * c
+    return y
+
+
+def _head64(x, w, pos, table, rope_dim, rope_type, eps=1e-6):
+    x = x.double()
+    if w is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w.double()
+    return _rope64(x, pos, table, rope_dim, rope_type)
+
+
+def _quant64(x):
+    """What the cache returns for rows [..., d] (float32 arithmetic of the returned value, as kv_pages_to_float does it)."""
+    x = x.float().double()
+    x = torch.where(x.isnan(), 0.0, x).clamp(-LIMIT, LIMIT)
+    lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+    sc, mn = ((hi - lo).float().double() / 15).float().bfloat16(), lo.float().bfloat16()
+    code = torch.where(sc.double() > 0, ((x - mn.double()) / sc.double()).round().clamp(0, 15), 0.0)
+    return code.float() * sc.float() + mn.float()
+
+
+def _cache(n_pages, kvh, d, seed=0):
+    from realizar_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kv = ops.kv_cache_alloc(1, n_pages, kvh, d, "cuda", "q4")
+    kv.copy_(torch.randint(0, 256, kv.shape, generator=g, device="cuda", dtype=torch.uint8))
+    flat = kv.flatten(-2)
+    shape = (2, 1, n_pages, kvh, 16)
+    sc = 0.2 + 0.3 * torch.rand(shape, generator=g, device="cuda")
+    mn = sc * (-7.5 + torch.randn(shape, generator=g, device="cuda"))
+    flat[..., 8 * d:] = torch.stack([sc, mn], -1).bfloat16().view(torch.uint8).flatten(-2)
+    return kv[0, 0], kv[1, 0]
+
+
+def _gather(cache, pages, d, values, n):
+    from realizar_b200 import ops
+    return ops.kv_pages_to_float(cache[pages.long()], d, values).transpose(0, 1).flatten(1, 2)[:, :n].double()      # [kvh, n, d]
+
+
+def _attend64(q, k, v, lo):
+    """q [H, d], k / v [kvh, n, d]: attention to positions lo .. n-1"""
+    kvh = k.shape[0]
+    x = torch.einsum("hgd,hnd->hgn", q.view(kvh, -1, q.shape[-1]), k[:, lo:]) / math.sqrt(q.shape[-1])
+    return torch.einsum("hgn,hnd->hgd", torch.softmax(x, -1), v[:, lo:]).reshape(-1)
+
+
+# ------------------------------------------------------------------------------------------------ append
+@pytest.mark.parametrize("d, h, kvh", [(64, 14, 2), (80, 4, 4), (96, 6, 1), (128, 16, 2)])
+@pytest.mark.parametrize("rows, norm, rope_dim, rope_type, in_place", [(1, False, 32, 2, True), (37, True, -1, 2, False), (130, True, -1, 0, True), (19, False, 0, 0, False), (16, True, 50, 2, False)])
+def test_append_matches_the_definition(cuda_device, d, h, kvh, rows, norm, rope_dim, rope_type, in_place):
+    from realizar_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(rows + d)
+    rope_dim = d if rope_dim < 0 else rope_dim
+    n_pages = rows // 16 + 4
+    kc, vc = _cache(n_pages, kvh, d, seed=d)
+    k0, v0 = kc.clone(), vc.clone()
+    wide = torch.randn(rows, (h + 2 * kvh) * d + 24, generator=g, device="cuda") * 2                # row stride larger than the row
+    qkv = wide[:, : (h + 2 * kvh) * d]
+    first = 5                                                                                        # the rows start inside a page
+    pos = (torch.arange(rows, device="cuda", dtype=torch.int32) + first)
+    page_of = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32)
+    page_rows = page_of[(pos // 16).long()].contiguous()
+    if rows > 8:
+        pos[3] = -1; pos[rows - 2] = -1
+    qw, kw = (1 + 0.2 * torch.randn(2, d, generator=g, device="cuda")).unbind(0) if norm else (None, None)
+    table = ops.make_rope_table(rows + first, rope_dim, 1e4, "cuda") if rope_dim else None
+    before = wide.clone()
+    q_out = None if in_place else torch.full((rows, h * d), 7.0, device="cuda")
+    if norm:
+        qw, kw = qw.contiguous(), kw.contiguous()
+    ops.qk_norm_rope_append(qkv, pos, page_rows, kc, vc, h, kvh, d, q_out=q_out, q_norm_w=qw, k_norm_w=kw, eps=1e-6, rope_dim=rope_dim, rope_type=rope_type, rope_table=table)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    q, k, v = before[:, : (h + 2 * kvh) * d].split([h * d, kvh * d, kvh * d], -1)
+    live = pos >= 0
+    want_q = _head64(q.view(rows, h, d), qw, pos, table, rope_dim, rope_type).flatten(1)
+    got_q = wide[:, : h * d] if in_place else q_out
+    assert _rel(got_q[live], want_q[live]) < 2e-6
+    assert torch.equal(got_q[~live], (before[:, : h * d] if in_place else torch.full_like(got_q, 7.0))[~live])          # idle rows are left alone
+    assert torch.equal(wide[:, h * d:], before[:, h * d:])
+    if not in_place:
+        assert torch.equal(wide, before)
+    want_k, want_v = _quant64(_head64(k.view(rows, kvh, d), kw, pos, table, rope_dim, rope_type)), _quant64(v.reshape(rows, kvh, d).double())
+    for cache, old, want, values in ((kc, k0, want_k, False), (vc, v0, want_v, True)):
+        expect = ops.kv_pages_to_float(old, d, values)
+        expect[page_rows[live].long(), :, (pos[live] % 16).long()] = want[live]
+        assert torch.equal(ops.kv_pages_to_float(cache, d, values), expect)                             # every other row of the cache included
+
+
+def test_append_special_values(cuda_device):
+    """Constant rows, quotients that lie exactly on a border, NaN, infinities and values beyond the format's range."""
+    from realizar_b200 import ops
+    d, kvh = 64, 1
+    kc, vc = _cache(2, kvh, d)
+    rows = torch.zeros(8, 3 * d, device="cuda")
+    v = rows[:, 2 * d:]
+    v[0] = 3.25
+    v[1, :32] = torch.arange(32, device="cuda") * 0.5; v[1, 32:] = 15.0; v[1, 31] = 15.0               # 0, 0.5, 1, ...: ties go to the even code
+    v[2] = torch.randn(d, device="cuda"); v[2, 5] = float("nan")
+    v[3] = torch.randn(d, device="cuda"); v[3, 0] = float("inf"); v[3, 9] = float("-inf")
+    v[4] = torch.randn(d, device="cuda") * 1e30
+    v[5] = torch.randn(d, device="cuda") * 1e-39                                                        # the scale is a subnormal number or 0
+    v[6] = torch.randn(d, device="cuda") * 1e-3 + 100
+    v[7, 0] = -1.0
+    rows[:, d:2 * d] = v                                                                                # the same as keys, without norm and rotation
+    pos, pages = torch.arange(8, device="cuda", dtype=torch.int32), torch.ones(8, device="cuda", dtype=torch.int32)
+    ops.qk_norm_rope_append(rows, pos, pages, kc, vc, 1, kvh, d)
+    want = _quant64(v.double())
+    for cache, values in ((kc, False), (vc, True)):
+        got = ops.kv_pages_to_float(cache[1], d, values)[0, :8]
+        assert torch.equal(got, want)
+        assert bool(got.isfinite().all()) and float(got.abs().max()) < 65504
+
+
+def test_append_rejects_bad_pages_on_the_device(cuda_device):
+    """A page id outside the cache: nothing of the row is cached, the other rows are, and the status word tells."""
+    from realizar_b200 import ops
+    d, kvh, h = 128, 2, 4
+    kc, vc = _cache(3, kvh, d)
+    k0 = kc.clone()
+    qkv = torch.randn(3, (h + 2 * kvh) * d, device="cuda")
+    pos, pages = torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32), torch.tensor([3, 1, -1], device="cuda", dtype=torch.int32)
+    q = torch.zeros(3, h * d, device="cuda")
+    ops.device_error()
+    ops.qk_norm_rope_append(qkv, pos, pages, kc, vc, h, kvh, d, q_out=q)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 3405 and ops.device_error() == 0
+    assert torch.equal(q, qkv[:, : h * d])
+    assert torch.equal(kc[0], k0[0]) and torch.equal(kc[2], k0[2]) and not torch.equal(kc[1], k0[1])
+
+
+def test_append_positions_beyond_the_table_use_theta(cuda_device):
+    from realizar_b200 import ops
+    d, kvh, h, n = 64, 1, 2, 3
+    kc, vc = _cache(4, kvh, d)
+    qkv = torch.randn(n, (h + 2 * kvh) * d, device="cuda")
+    pos, pages = torch.tensor([2, 70_000, 1_000_003], device="cuda", dtype=torch.int32), torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32)
+    q = torch.zeros(n, h * d, device="cuda")
+    ops.qk_norm_rope_append(qkv, pos, pages, kc, vc, h, kvh, d, q_out=q, rope_dim=d, rope_type=2, rope_theta=5e5, rope_table=ops.make_rope_table(3, d, 5e5, "cuda"))
+    i = torch.arange(d // 2, dtype=torch.float64, device="cuda")
+    ang = pos.double()[:, None] * torch.pow(torch.tensor(5e5, dtype=torch.float64, device="cuda"), -2 * i / d)
+    c, s = ang.cos().float().double()[:, None], ang.sin().float().double()[:, None]
+    x = qkv[:, : h * d].double().view(n, h, d)
+    a, b = x[..., : d // 2], x[..., d // 2:]
+    assert _rel(q, torch.cat([a * c - b * s, a * s + b * c], -1).flatten(1)) < 2e-6
+
+
+# ------------------------------------------------------------------------------------------------ decode
+def _decode(h, kvh, d, lens, seed, norm=False, rope_dim=0, rope_type=2, window=0, no_append=False, shared_table=False, garbage=True, scale_q=1.0):
+    """One launch over sequences of the given lengths (new token included; 0: idle row) and what it should give."""
+    from realizar_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    B, per = len(lens), max(1, -(-max(lens) // 16)) + 1
+    n_pages = (1 if shared_table else B) * per + 2
+    kc, vc = _cache(n_pages, kvh, d, seed)
+    order = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32)
+    pt = order[:per].contiguous() if shared_table else order[: B * per].view(B, per).contiguous()
+    if garbage:          # rows behind the last token of every sequence and pages that no sequence uses: bytes that decode to NaN and infinity
+        for c in (kc, vc):
+            flat = c.flatten(-2)
+            for b, n in enumerate(lens):
+                row = pt if shared_table else pt[b]
+                last = max(lens) if shared_table else n
+                meta = flat[row.long()][..., 8 * d:].unflatten(-1, (16, 4)).transpose(1, 2).flatten(0, 1)
+                meta[last:] = 0xFF
+                flat[row.long()[:, None, None], torch.arange(kvh, device="cuda")[None, :, None], torch.arange(8 * d, 8 * d + 64, device="cuda")] = \
+                    meta.unflatten(0, (per, 16)).transpose(1, 2).flatten(-2)
+            flat[order[(per if shared_table else B * per):].long()] = 0xFF
+    qkv = torch.randn(B, (h + 2 * kvh) * d, generator=g, device="cuda")
+    qkv[:, : h * d] *= scale_q
+    pos = torch.tensor([n - 1 for n in lens], device="cuda", dtype=torch.int32)
+    out = torch.full((B, h * d), 9.0, device="cuda")
+    qw, kw = [w.contiguous() for w in (1 + 0.2 * torch.randn(2, d, generator=g, device="cuda")).unbind(0)] if norm else (None, None)
+    table = ops.make_rope_table(max(lens) + 1, rope_dim, 1e4, "cuda") if rope_dim else None
+    partial, counters = ops.attn_decode_scratch(B, h, 1, d, "cuda", kv_dtype="q4")
+    p = ops.build_attn_decode_params(qkv, out, kc, vc, pos, pt, partial, counters, h, kvh, d, 1, B, rope_dim, rope_type, 1e4, 0, h * d, (h + kvh) * d, qw, kw, 1e-6,
+                                     window=window, rope_table=table, no_append=no_append, shared_table=shared_table)
+    keep = (qkv, out, kc, vc, pos, pt, partial, counters, qw, kw, table)
+    k0, v0 = kc.clone(), vc.clone()
+
+    def check(launch=True):
+        if launch:
+            ops.attn_decode_launch(p)
+        torch.cuda.synchronize()
+        assert ops.device_error() == 0
+        q, k, v = qkv.split([h * d, kvh * d, kvh * d], -1)
+        q = _head64(q.view(B, h, d), qw, pos, table, rope_dim, rope_type)
+        k, v = _quant64(_head64(k.view(B, kvh, d), kw, pos, table, rope_dim, rope_type)), _quant64(v.reshape(B, kvh, d).double())
+        worst = 0.0
+        for b, p1 in enumerate(pos.tolist()):
+            if p1 < 0:
+                assert torch.equal(out[b], torch.full_like(out[b], 9.0))
+                continue
+            row = pt if shared_table else pt[b]
+            ks, vs = _gather(kc, row, d, False, p1 + 1), _gather(vc, row, d, True, p1 + 1)
+            if not no_append:
+                assert torch.equal(ks[:, p1].float(), k[b]) and torch.equal(vs[:, p1].float(), v[b])        # the appended rows, bit for bit
+            want = _attend64(q[b], ks, vs, max(0, p1 + 1 - window) if window else 0)
+            worst = max(worst, _rel(out[b], want))
+        touched = [(int((pt if shared_table else pt[b])[p1 // 16]), p1 % 16) for b, p1 in enumerate(pos.tolist()) if p1 >= 0 and not no_append]
+        for c, old in ((kc, k0), (vc, v0)):                                                                  # nothing else of the cache changed
+            same = (ops.kv_pages_to_float(c, d, c is vc).nan_to_num() == ops.kv_pages_to_float(old, d, c is vc).nan_to_num()).all(-1).all(1)
+            for pg, s in touched:
+                same[pg, s] = True
+            assert bool(same.all())
+        assert worst < 1e-5, worst
+    check.params, check.keep = p, keep
+    return check
+
+
+@pytest.mark.parametrize("h, kvh, d", [(8, 8, 80), (14, 2, 64), (6, 1, 96), (32, 8, 128), (12, 1, 64), (20, 1, 128), (1, 1, 80)])
+@pytest.mark.parametrize("lens", [[1], [17, 1, 16, 0, 300, 47], [1000]])
+def test_decode_attention(cuda_device, h, kvh, d, lens):
+    _decode(h, kvh, d, lens, seed=h + d + len(lens), norm=True, rope_dim=d, rope_type=2)()
+
+
+@pytest.mark.parametrize("kw", [dict(window=1), dict(window=16), dict(window=33, rope_dim=32, rope_type=0), dict(no_append=True), dict(no_append=True, shared_table=True),
+                                dict(norm=True), dict(scale_q=30.0), dict(scale_q=0.0), dict(window=5000, rope_dim=64)])
+def test_decode_attention_options(cuda_device, kw):
+    lens = [64, 31, 64, 5] if kw.get("shared_table") else [97, 1, 32, 700, 33]
+    _decode(8, 2, 128, lens, seed=5, **kw)()
+
+
+@pytest.mark.parametrize("B, n", [(1, 40000), (200, 70), (3, 5000), (600, 3)])
+def test_decode_attention_divides_any_batch(cuda_device, B, n):
+    _decode(8, 4, 64, [max(1, n - 13 * (b % 5)) for b in range(B)], seed=B, rope_dim=64)()
+
+
+def test_decode_wide_ranges_of_scales(cuda_device):
+    """Rows whose scales differ by many orders of magnitude, all-constant rows first, one row that takes all of the attention."""
+    from realizar_b200 import ops
+    h, kvh, d, n = 4, 1, 64, 200
+    for kind in ("constant first", "growing", "shrinking", "peaked"):
+        check = _decode(h, kvh, d, [n], seed=3, no_append=True)
+        qkv, out, kc, vc, pos, pt = check.keep[:6]
+        flat = vc.flatten(-2)
+        meta = torch.zeros(pt.numel() * 16, 2, device="cuda")
+        i = torch.arange(pt.numel() * 16, device="cuda").float()
+        meta[:, 0] = {"constant first": torch.where(i < 64, 0.0, 1e-6), "growing": torch.exp2(i / 8 - 20), "shrinking": torch.exp2(5 - i / 8), "peaked": 0.3 + 0 * i}[kind]
+        meta[:, 1] = -7.5 * meta[:, 0]
+        flat[pt[0].long(), 0, 8 * d:] = meta.bfloat16().view(torch.uint8).view(-1, 64)
+        if kind == "peaked":
+            kflat = kc.flatten(-2)
+            km = kflat[pt[0].long(), 0, 8 * d:].contiguous().view(torch.bfloat16).view(-1, 2)
+            km[150] *= 40
+            kflat[pt[0].long(), 0, 8 * d:] = km.view(torch.uint8).view(-1, 64)
+        ops.attn_decode_launch(check.params)
+        q = qkv[0, : h * d].double().view(h, d)
+        want = _attend64(q, _gather(kc, pt[0], d, False, n), _gather(vc, pt[0], d, True, n), 0)
+        assert _rel(out[0], want) < 1e-5, kind
+
+
+def test_decode_device_checks(cuda_device):
+    """A position beyond its page-table row and a page id outside the cache set the status word; the other sequences are right."""
+    from realizar_b200 import ops
+    check = _decode(8, 2, 64, [40, 50, 60], seed=1, rope_dim=64)
+    qkv, out, kc, vc, pos, pt = check.keep[:6]
+    keep = pos.clone()
+    pos[1] = pt.shape[1] * 16
+    ops.device_error()
+    ops.attn_decode_launch(check.params)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 3311 and bool((out[1] == 9.0).all()) and not bool((out[0] == 9.0).any())
+    pos.copy_(keep)
+    good = pt[1, 0].clone()
+    pt[1, 0] = kc.shape[0]
+    ops.attn_decode_launch(check.params)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 3312
+    pt[1, 0] = good
+    check()
+
+
+def test_decode_graph_replays_with_new_positions_and_shares_scratch(cuda_device):
+    """Two captured graphs with one workspace, replayed in turn while the sequences grow."""
+    a = _decode(8, 2, 128, [250, 3, 90], seed=2, rope_dim=128)
+    b = _decode(8, 2, 128, [60], seed=4, rope_dim=128)
+    b.params.partial, b.params.counters = a.params.partial, a.params.counters
+    from realizar_b200 import ops
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.attn_decode_launch(a.params); ops.attn_decode_launch(b.params)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for c in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.attn_decode_launch(c.params)
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    a(launch=False); b(launch=False)
+    first = a.keep[1].clone()
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a.keep[1], first)                       # the same bits every time
+    a.keep[4][1] = 1                                           # a shorter sequence in the same graph
+    graphs[0].replay(); graphs[1].replay()
+    torch.cuda.synchronize()
+    row, p1 = a.keep[5][1], 1
+    q = _head64(a.keep[0][1:2, : 8 * 128].view(1, 8, 128), None, a.keep[4][1:2], a.keep[10], 128, 2)[0]
+    want = _attend64(q, _gather(a.keep[2], row, 128, False, 2), _gather(a.keep[3], row, 128, True, 2), 0)
+    assert _rel(a.keep[1][1], want) < 1e-5
+
+
+# ------------------------------------------------------------------------------------------------ prompt
+def _prompt(h, kvh, d, rows, pos0, window=0, out_dtype=torch.bfloat16, with_scratch=True, dev_pos=False, tol=4e-3):
+    from realizar_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(rows + pos0 + d)
+    total = pos0 + rows
+    per = -(-total // 16) + 1
+    kc, vc = _cache(per + 2, kvh, d, seed=rows)
+    pt = torch.randperm(per + 2, generator=g, device="cuda").to(torch.int32)[:per].contiguous()
+    for c in (kc, vc):                                          # behind the last token: bytes that decode to NaN
+        flat = c.flatten(-2)
+        meta = flat[pt.long()][..., 8 * d:].unflatten(-1, (16, 4)).transpose(1, 2).flatten(0, 1)
+        meta[total:] = 0xFF
+        flat[pt.long()[:, None, None], torch.arange(kvh, device="cuda")[None, :, None], torch.arange(8 * d, 8 * d + 64, device="cuda")] = \
+            meta.unflatten(0, (per, 16)).transpose(1, 2).flatten(-2)
+    qkv = torch.randn(rows + 2, (h + 2 * kvh) * d, generator=g, device="cuda")
+    out = torch.full((rows + 2, h * d + 8), 9.0, device="cuda", dtype=out_dtype)
+    scratch = ops.attn_prefill_scratch(rows, h, kvh, d, "cuda") if with_scratch else None
+    pd = torch.tensor([pos0], device="cuda", dtype=torch.int32) if dev_pos else None
+    for _ in range(2):                                          # twice: the workspace keeps nothing
+        ops.attn_prefill(qkv, out[:, 8:], kc, vc, pt, rows, 0 if dev_pos else pos0, h, kvh, d, window=window, pos0_dev=pd, scratch=scratch)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    assert bool((out[:, :8] == 9.0).all()) and bool((out[rows:] == 9.0).all())
+    ks, vs = _gather(kc, pt, d, False, total), _gather(vc, pt, d, True, total)
+    at, pos = torch.arange(total, device="cuda"), pos0 + torch.arange(rows, device="cuda")[:, None]
+    seen = (at <= pos) & ((at > pos - window) if window else True)
+    q = qkv[:rows, : h * d].double().view(rows, kvh, h // kvh, d)
+    x = torch.where(seen[:, None, None], torch.einsum("rkgd,knd->rkgn", q, ks) / math.sqrt(d), -math.inf)
+    want = torch.einsum("rkgn,knd->rkgd", torch.softmax(x, -1), vs).reshape(rows, h * d)
+    got = out[:rows, 8:]
+    assert _rel(got, want) < tol, _rel(got, want)
+    per_row = ((got.double() - want).norm(dim=-1) / want.norm(dim=-1)).max()
+    assert float(per_row) < 3 * tol, float(per_row)
+
+
+@pytest.mark.parametrize("h, kvh, d", [(4, 4, 80), (14, 2, 64), (6, 1, 96), (16, 4, 128), (12, 1, 64), (5, 5, 128)])
+@pytest.mark.parametrize("rows, pos0", [(1, 0), (16, 0), (77, 1337), (130, 31), (300, 0)])
+def test_prompt_attention(cuda_device, h, kvh, d, rows, pos0):
+    _prompt(h, kvh, d, rows, pos0)
+
+
+@pytest.mark.parametrize("kw", [dict(window=1), dict(window=50), dict(window=300), dict(with_scratch=False), dict(dev_pos=True), dict(out_dtype=torch.float32)])
+def test_prompt_attention_options(cuda_device, kw):
+    _prompt(8, 2, 128, 150, 420, **kw)
+
+
+def test_prompt_attention_long(cuda_device):
+    _prompt(8, 2, 128, 40, 9000)
+    _prompt(8, 1, 64, 1100, 1500)
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_append_prompt_decode_as_a_serving_pass(cuda_device):
+    """A prompt in two chunks and then single tokens, all through the cache, against attention in 64 bits over the values the cache holds;
+    the rows a prompt pass writes and those a decode step writes are the same bits."""
+    from realizar_b200 import ops
+    h, kvh, d, n, steps = 8, 2, 128, 90, 5
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(n + steps, (h + 2 * kvh) * d, generator=g, device="cuda")
+    qw, kw = [w.contiguous() for w in (1 + 0.2 * torch.randn(2, d, generator=g, device="cuda")).unbind(0)]
+    table = ops.make_rope_table(256, d, 1e4, "cuda")
+    pt = torch.tensor([[5, 2, 7, 0, 3, 6]], device="cuda", dtype=torch.int32)
+    caches = [ops.kv_cache_alloc(1, 8, kvh, d, "cuda", "q4")[:, 0] for _ in range(2)]
+    kc, vc = caches[0]
+    pos = torch.arange(n + steps, device="cuda", dtype=torch.int32)
+    rows = pt[0, (pos // 16).long()].contiguous()
+    kw_args = dict(q_norm_w=qw, k_norm_w=kw, eps=1e-6, rope_dim=d, rope_type=2, rope_table=table)
+    ops.qk_norm_rope_append(x, pos, rows, caches[1][0], caches[1][1], h, kvh, d, q_out=torch.empty(n + steps, h * d, device="cuda"), **kw_args)
+    outs = []
+    scratch = ops.attn_prefill_scratch(64, h, kvh, d, "cuda")
+    for c0, c1 in ((0, 64), (64, n)):
+        chunk, out = x[c0:c1].clone(), torch.empty(c1 - c0, h * d, device="cuda", dtype=torch.bfloat16)
+        ops.qk_norm_rope_append(chunk, pos[c0:c1], rows[c0:c1], kc, vc, h, kvh, d, **kw_args)
+        ops.attn_prefill(chunk, out, kc, vc, pt[0], c1 - c0, c0, h, kvh, d, scratch=scratch)
+        outs.append(out.float())
+    partial, counters = ops.attn_decode_scratch(1, h, 1, d, "cuda", kv_dtype="q4")
+    for i in range(n, n + steps):
+        out = torch.empty(1, h * d, device="cuda")
+        p = ops.build_attn_decode_params(x[i:i + 1], out, kc, vc, pos[i:i + 1], pt, partial, counters, h, kvh, d, 1, 1, d, 2, 1e4, 0, h * d, (h + kvh) * d, qw, kw, 1e-6,
+                                         rope_table=table)
+        ops.attn_decode_launch(p)
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    assert torch.equal(caches[0], caches[1])
+    got = torch.cat(outs)
+    q = _head64(x[:, : h * d].view(-1, h, d), qw, pos, table, d, 2)
+    ks, vs = _gather(kc, pt[0], d, False, n + steps), _gather(vc, pt[0], d, True, n + steps)
+    for i in range(n + steps):
+        assert _rel(got[i], _attend64(q[i], ks[:, : i + 1], vs[:, : i + 1], 0)) < (4e-3 * 3 if i < n else 1e-5), i
+
+
+def test_two_streams_with_their_own_workspaces(cuda_device):
+    a, b = _decode(8, 2, 128, [2000, 900], seed=8, rope_dim=128), _decode(14, 2, 64, [1500], seed=9, rope_dim=64)
+    from realizar_b200 import ops
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for s, c in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                ops.attn_decode_launch(c.params)
+    a(launch=False); b(launch=False)
+
+
+@pytest.mark.parametrize("name", ["llama", "phi2"])
+def test_engine_serves_from_the_4_bit_cache(cuda_device, name):
+    """Prefill in chunks, decode steps, a batch and a snapshot over kv_dtype='q4': logits stay near those of the bf16 cache, the
+    cache takes (d / 2 + 4) / 2 d of the memory and results do not depend on the path that wrote it.
+
+    How near: a row of 64 or 80 normal values spans about 4.7 sigma, a step is 4.7 / 15 = 0.31 sigma, so every cached value is off by
+    0.31 / sqrt(12) = 0.09 sigma.  Scores q.k / sqrt(d) of these weights have a spread of about 1.3 and are off by 0.12, which moves the
+    weights by 12%; with the 9% of the values that is 15% to each attention output.  A gated layer (a product of two) doubles it and two
+    layers add up: at most 2 x 15% x sqrt(2) = 42% of the logits if nothing came past the attention, a cosine of 1 / sqrt(1 + 0.42^2) = 0.92."""
+    from test_gpu_engine import _cos, _kq_llama, small_phi2
+    from realizar_b200.models.weights import synthetic_weights
+    from realizar_b200.runtime.engine import DecodeEngine, EngineConfig
+    cfg = _kq_llama() if name == "llama" else small_phi2()
+    w = synthetic_weights(cfg, seed=21, std=0.05, **({} if name == "llama" else {"scheme": "Q4_K_M"}))
+    toks = [int(t) for t in np.random.default_rng(8).integers(0, cfg.vocab_size, 90)]
+    res = {}
+    for kd in ("bf16", "q4"):
+        eng = DecodeEngine(w, EngineConfig(max_batch=2, max_seq_len=160, greedy_only=True, kv_dtype=kd, prefill_chunk=64))
+        eng.open_slot(0, 128)
+        nxt = eng.prefill(0, toks)
+        logits = [eng.logits_of_last_step(0).float().cpu().numpy()]
+        for t in (5, 17, 3):
+            eng.feed({0: t})
+            logits.append(eng.logits_of_last_step(0).float().cpu().numpy())
+        res[kd] = (logits, eng.memory_report()["kv_bytes"])
+        if kd == "q4":
+            snap = eng.snapshot_kv(0)
+            eng.open_slot(1, 128)
+            eng.restore_kv(1, snap)
+            a, b = (eng.feed({s: 9}) is not None and eng.logits_of_last_step(s).float().cpu().numpy() for s in (0, 1))
+            assert _cos(a, b) > 0.99999
+            eng.check_health()
+        eng.close()
+    hd = cfg.head_dim
+    assert res["q4"][1] * 2 * hd == res["bf16"][1] * (hd // 2 + 4)
+    for a, b in zip(res["bf16"][0], res["q4"][0]):
+        assert _cos(a, b) > 0.9, _cos(a, b)
