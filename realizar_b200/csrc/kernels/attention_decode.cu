@@ -149,6 +149,8 @@ int rlz_attn_decode(const rlz::AttnDecodeParams* pp, void* stream) { return rlz:
 
 }  // extern "C"
 
+extern "C" long long rlz_attn_q4_partial_floats(int head_dim);      // attention_decode_q4.cu
+
 // ---- allocation-free variant: scratch lives in the library image (see attn_decode_static.h) -----
 namespace rlz {
 static __device__ __align__(256) float g_static_partial[RLZ_ATTN_STATIC_MAX_PARTIAL_FLOATS];
@@ -177,7 +179,7 @@ int rlz_attn_decode_static(const rlz::AttnDecodeParams* pp, void* stream) {
   if (p.n_kv_heads < 1 || p.n_heads % p.n_kv_heads || p.splits < 1 || p.batch < 1) return -2;
   if (p.rope_dim > p.head_dim || (p.rope_dim & 1)) return -3;
   if (((uintptr_t)p.k_cache & 15) || ((uintptr_t)p.v_cache & 15)) return -4;
-  const long long need_f = (long long)p.batch * p.n_heads * p.splits * (p.head_dim + 2);
+  const long long need_f = p.kv_q8 == 2 ? rlz_attn_q4_partial_floats(p.head_dim) : (long long)p.batch * p.n_heads * p.splits * (p.head_dim + 2);
   const long long need_c = (long long)p.batch * p.n_heads;
   if (need_f > RLZ_ATTN_STATIC_MAX_PARTIAL_FLOATS || need_c > RLZ_ATTN_STATIC_MAX_COUNTERS) return RLZ_STATIC_TOO_LARGE;
   int dev = -1;

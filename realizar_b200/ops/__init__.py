@@ -235,7 +235,7 @@ def device_error(clear: bool = True) -> int:
     c = 1 if clear else 0
     return (int(lib().rlz_device_error(c)) or int(lib().rlz_gemv_slab_error(c)) or int(lib().rlz_gemm_error(c))
             or int(lib().rlz_attn_decode_error(c)) or int(lib().rlz_attn_prefill_error(c)) or int(lib().rlz_index_error(c))
-            or int(lib().rlz_q4_append_error(c)) or int(lib().rlz_attn_q4_error(c)))
+            or int(lib().rlz_q4_append_error(c)) or int(lib().rlz_attn_q4_error(c)) or int(lib().rlz_attn_prefill_q4_error(c)))
 
 
 def gemv(w: DeviceWeight, x: torch.Tensor, bias=None, act=ACT_NONE, residual=None, norm=NORM_NONE, norm_w=None, norm_b=None,

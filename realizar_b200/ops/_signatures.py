@@ -179,6 +179,7 @@ def declare(lib: ctypes.CDLL) -> None:
     lib.rlz_qk_norm_rope_append.argtypes = [POINTER(QkAppendParams), c_void_p]
     lib.rlz_q4_append_error.argtypes = [c_int]
     lib.rlz_attn_q4_error.argtypes = [c_int]
+    lib.rlz_attn_prefill_q4_error.argtypes = [c_int]
     lib.rlz_attn_q4_partial_floats.argtypes = [c_int]
     lib.rlz_attn_q4_partial_floats.restype = c_longlong
     lib.rlz_attn_prefill_q4_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
