@@ -9,8 +9,10 @@
 //     lines products up by the exponent fields, so that a nibble left at the low bits, code x 2^-24 without the shift, costs the
 //     sum as many bits as stand empty above it: 2e-5 of the result where this gives 3e-7.)
 //   * The pages lie in fragment order, so a lane takes its operands with one wide shared-memory load and no shuffles.
-//   * The 16 rows of the instruction hold up to 8 query heads twice: rows 0..7 the fp16 head of q (then of p x scale'), rows 8..15
-//     what is left of it in fp16.  22 bits of the operands at the price of 11; with 8 heads a kv head's page is read once.
+//   * Keys (16 tokens) and values (16 dims) are the A operand and the heads the 8 columns of B: 4 heads, each as the fp16 head of
+//     its value and what that leaves, also fp16.  22 bits of q and of p x scale' at the price of 11, and the two products of a
+//     head meet in one lane.  Up to 4 heads take one such tile, up to 8 two, sharing the A operand.  (Heads as rows, 8 + 8 of
+//     16, took twice the instructions and registers for 4 heads: 46 us for every 65536 pages of 128, this STEP2.)
 //     q is scaled by a power of two so that its largest value lies in [2^13, 2^14), p x scale' by one that follows the scales.
 //   * The running maximum moves only when a score passes it by 2^8, so that the accumulators are rarely rescaled.
 // Each warp has a ring of whole pages (K and V) filled by bulk copies.
@@ -28,14 +30,17 @@ namespace rlz {
 // 3312: a page id outside the cache (read as page 0, not written)
 __device__ int g_attn_q4_error = 0;
 
-constexpr int QD_WARPS = 4, QD_THREADS = 32 * QD_WARPS, QD_STAGES = 4, QD_ROWS = 8, QD_CTAS_PER_SM = 3;
+constexpr int QD_WARPS = 4, QD_THREADS = 32 * QD_WARPS, QD_STAGES = 4;
 constexpr int QD_MAX_PARTS = 64;              // CTAs that share a tile: bounds the time of the last one, which joins their parts
-constexpr int QD_MAX_CTAS = 444;
+// query heads of a CTA (HN tiles of 4) and CTAs to an SM, by registers
+constexpr int qd_heads(int hn) { return 4 * hn; }
+constexpr int qd_occupancy(int hn) { return hn == 1 ? 4 : 3; }
+constexpr int QD_MAX_SMS = 148;
 
-template <int D> struct QdSmem {
-  float q[QD_ROWS][D];
-  float part[QD_WARPS][QD_ROWS][D + 4];       // per warp and head: sum, then maximum and weight
-  float qc[QD_ROWS], qx[QD_ROWS];             // 2^18 / f of a head whose fragments hold q f, and the sum of q
+template <int D, int HN> struct QdSmem {
+  float q[4 * HN][D];
+  float part[QD_WARPS][4 * HN][D + 4];         // per warp and head: sum, then maximum and weight
+  float qc[4 * HN], qx[4 * HN];               // 2^18 / f of a head whose fragments hold q f, and the sum of q
   uint8_t codes[2][D];                        // the new token's rows
   uint32_t meta[2];
   int wsum[QD_WARPS];
@@ -47,21 +52,25 @@ __device__ __forceinline__ int q4_page_id(int raw, int num_pages) {
   if (num_pages > 0 && (unsigned)raw >= (unsigned)num_pages) { atomicExch(&g_attn_q4_error, 3312); return 0; }
   return raw;
 }
-__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // nibble J of both halves of a word as fp16 subnormals: code x 2^-18
 template <int J> __device__ __forceinline__ uint32_t nib(uint32_t w) {
   return (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6) & 0x03C003C0u;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// fp16 head of two values, and of what the head leaves
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-  hi = *(const uint32_t*)&h; lo = *(const uint32_t*)&r;
+// fp16 head of a value (low half) and of what the head leaves (high half)
+__device__ __forceinline__ uint32_t split_f16(float x) {
+  const __half h = __float2half_rn(x);
+  const __half2 r = __halves2half2(h, __float2half_rn(x - __half2float(h)));
+  return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {       // of 16-bit values, row = lane / 4
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // 2^(e - exponent of x), at most 2^100; x > 0
 __device__ __forceinline__ float pow2_for(float x, int e) {
@@ -89,11 +98,12 @@ __device__ __forceinline__ QdSeq qd_seq(const AttnDecodeParams& p, int b) {
   return s;
 }
 
-template <int D>
-__global__ void __launch_bounds__(QD_THREADS, QD_CTAS_PER_SM) attn_decode_q4_kernel(const __grid_constant__ AttnDecodeParams p) {
-  constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, KS = 2 * NG + TAIL, NT = 4 * NG + 2 * TAIL, PB = q4_page_bytes(D), NP = HeadPairs<D>::NP;
+template <int D, int HN>
+__global__ void __launch_bounds__(QD_THREADS, qd_occupancy(HN)) attn_decode_q4_kernel(const __grid_constant__ AttnDecodeParams p) {
+  constexpr int QD_ROWS = 4 * HN;
+  constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, KS = 2 * NG + TAIL, NT = 2 * NG + TAIL, PB = q4_page_bytes(D), NP = HeadPairs<D>::NP;
   extern __shared__ __align__(128) uint8_t qd_ring[];
-  __shared__ __align__(16) QdSmem<D> sm;
+  __shared__ __align__(16) QdSmem<D, HN> sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
   if (tid < QD_WARPS * QD_STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(att_smem_u32(&sm.full[0][0] + tid)));
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -143,12 +153,14 @@ __global__ void __launch_bounds__(QD_THREADS, QD_CTAS_PER_SM) attn_decode_q4_ker
 
     // ---- first pages under way; lane i keeps the id of my i-th page of a group of 32, and of the next group -------------------
     int ids = lane < n_my ? q4_page_id(pt[QD_WARPS * lane], p.num_pages) : 0, ids_next = 0;
-    auto issue = [&](int i) {
-      if ((i & 31) == 0 && i > 0) ids = ids_next;
-      if ((i & 31) == 0) ids_next = i + 32 + lane < n_my ? q4_page_id(pt[QD_WARPS * (i + 32 + lane)], p.num_pages) : 0;
-      const int id = __shfl_sync(0xFFFFFFFFu, ids, i & 31);
-      if (lane == 0) {
-        const uint32_t slot = (taken + i) % QD_STAGES;
+    auto issue = [&](int i) {                                     // pages i and i + 1 (i even): lanes 0 and 1 take one each
+      if ((i & 31) == 0) {
+        if (i > 0) ids = ids_next;
+        ids_next = i + 32 + lane < n_my ? q4_page_id(pt[QD_WARPS * (i + 32 + lane)], p.num_pages) : 0;
+      }
+      const int id = __shfl_sync(0xFFFFFFFFu, ids, (i + lane) & 31);
+      if (lane < 2 && i + lane < n_my) {
+        const uint32_t slot = (taken + i + lane) % QD_STAGES;
         unsigned long long* bar = &sm.full[warp][slot];
         uint8_t* dst = my_ring + slot * (2 * PB);
         const int64_t off = ((int64_t)id * p.n_kv_heads + kvh) * PB;
@@ -157,7 +169,7 @@ __global__ void __launch_bounds__(QD_THREADS, QD_CTAS_PER_SM) attn_decode_q4_ker
         att_bulk_g2s(dst + PB, (const uint8_t*)p.v_cache + off, PB, bar);
       }
     };
-    for (int i = 0; i < min(QD_STAGES, n_my); ++i) issue(i);
+    for (int i = 0; i < min(QD_STAGES, n_my); i += 2) issue(i);
 
     // ---- the new token: queries of the group, and in the owner its key and value rows ------------------------------------------
     const float* row = p.qkv + (int64_t)b * p.ld_qkv;
@@ -208,115 +220,168 @@ __global__ void __launch_bounds__(QD_THREADS, QD_CTAS_PER_SM) attn_decode_q4_ker
     }
     __syncthreads();
 
-    // ---- query fragments: word tq of a group of 32 dims holds dims 8 tq .. + 7, its nibbles pair as (0, 4), (1, 5), (2, 6), (3, 7) ---
-    uint32_t qa[KS][4];
-    const bool has = gq < gn;
-    const float* qr = sm.q[has ? gq : 0];
-    auto frag = [&](uint32_t (&a)[4], int d0, int d1, int d2, int d3) {
-      split_f16(has ? qr[d0] : 0.f, has ? qr[d1] : 0.f, a[0], a[1]);
-      split_f16(has ? qr[d2] : 0.f, has ? qr[d3] : 0.f, a[2], a[3]);
-    };
+    // ---- query fragments: column gq is head gq / 2 of a tile, its head (even) or what that leaves (odd).  Word tq of a group of 32
+    // dims holds dims 8 tq .. + 7 and its nibbles pair as (0, 4), (1, 5), (2, 6), (3, 7) ----
+    uint32_t qb[HN][KS][2];
+    float qc[HN], qx[HN];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int d = 32 * g + 8 * tq;
-      frag(qa[2 * g], d, d + 4, d + 1, d + 5);
-      frag(qa[2 * g + 1], d + 2, d + 6, d + 3, d + 7);
-    }
-    if constexpr (TAIL) { const int d = 32 * NG + 4 * tq; frag(qa[2 * NG], d, d + 1, d + 2, d + 3); }
-    const float qc = has ? sm.qc[gq] : 0.f, qx = has ? sm.qx[gq] : 0.f;
-
-    float o[NT][4];
+    for (int h = 0; h < HN; ++h) {
+      const int head = 4 * h + (gq >> 1);
+      const bool has = head < gn;
+      const float* qr = sm.q[has ? head : 0];
+      const uint32_t sel = gq & 1 ? 0x7632u : 0x5410u;            // odd columns take the high halves of the two splits
+      auto frag = [&](int d0, int d1) { return has ? __byte_perm(split_f16(qr[d0]), split_f16(qr[d1]), sel) : 0u; };
 #pragma unroll
-    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float m = -INFINITY, l = 0.f, om = 0.f, vf = 0x1p100f;       // om: sum of p x min'; vf: power of two that p x scale' carries
-
-    for (int i = 0; i < n_my; ++i) {
-      const uint32_t slot = (taken + i) % QD_STAGES, parity = ((taken + i) / QD_STAGES) & 1u;
-      bool arrived = false;
-      const uint32_t limit = ok ? ATT_WAIT_LIMIT : 1024u;
-      for (uint32_t spin = 0; spin < limit; ++spin) if (att_try_wait(&sm.full[warp][slot], parity)) { arrived = true; break; }
-      if (!arrived) { ok = false; atomicExch(&g_attn_q4_error, 3211); }
-      uint8_t* kp = my_ring + slot * (2 * PB);
-      uint8_t* vp = kp + PB;
-      const int page = page0 + warp + QD_WARPS * i, t0 = page * Q4_PAGE;
-      if (owner && page == s.pages - 1) {                        // the copy may have passed the write of the new row
-        q4_store_k<D>(kp, s.pos % Q4_PAGE, sm.codes[0], sm.meta[0], lane);
-        q4_store_v<D>(vp, s.pos % Q4_PAGE, sm.codes[1], sm.meta[1], lane);
-        __syncwarp();
+      for (int g = 0; g < NG; ++g) {
+        const int d = 32 * g + 8 * tq;
+        qb[h][2 * g][0] = frag(d, d + 4); qb[h][2 * g][1] = frag(d + 1, d + 5);
+        qb[h][2 * g + 1][0] = frag(d + 2, d + 6); qb[h][2 * g + 1][1] = frag(d + 3, d + 7);
       }
-      // ---- scores of 16 tokens: lane has tokens 8 n + 2 tq + e of row gq ----
-      float sc[2][2], sv[2][2], mv[2][2];
+      if constexpr (TAIL) { const int d = 32 * NG + 4 * tq; qb[h][2 * NG][0] = frag(d, d + 1); qb[h][2 * NG][1] = frag(d + 2, d + 3); }
+      const bool mine_is = 4 * h + tq < gn;                      // the head whose scores this lane holds
+      qc[h] = mine_is ? sm.qc[4 * h + tq] : 0.f; qx[h] = mine_is ? sm.qx[4 * h + tq] : 0.f;
+    }
+
+    float o[HN][NT][4], m[HN], l[HN], om[HN];                    // om: sum of p x min'
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint8_t* kr = kp + (8 * n + gq) * (D / 2);
-        uint32_t w[NG];
-        load_words<NG>(kr + tq * NG * 4, w);
+    for (int h = 0; h < HN; ++h) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.f;
+      m[h] = -INFINITY; l[h] = om[h] = 0.f;
+    }
+    float vf = 0x1p100f;                                          // power of two that p x scale' carries
+
+    for (int i = 0; i < n_my; i += 2) {                           // two pages at a time (of an odd number, the last comes with a masked one)
+      uint8_t* kp[2];
+      int t0[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t slot = (taken + i + j) % QD_STAGES, parity = ((taken + i + j) / QD_STAGES) & 1u;
+        kp[j] = my_ring + slot * (2 * PB);
+        const int page = page0 + warp + QD_WARPS * (i + j);
+        t0[j] = page * Q4_PAGE;
+        if (i + j < n_my) {
+          bool arrived = false;
+          const uint32_t limit = ok ? ATT_WAIT_LIMIT : 1024u;
+          for (uint32_t spin = 0; spin < limit; ++spin) if (att_try_wait(&sm.full[warp][slot], parity)) { arrived = true; break; }
+          if (!arrived) { ok = false; atomicExch(&g_attn_q4_error, 3211); }
+          if (owner && page == s.pages - 1) {                    // the copy may have passed the write of the new row
+            q4_store_k<D>(kp[j], s.pos % Q4_PAGE, sm.codes[0], sm.meta[0], lane);
+            q4_store_v<D>(kp[j] + PB, s.pos % Q4_PAGE, sm.codes[1], sm.meta[1], lane);
+            __syncwarp();
+          }
+        }
+      }
+      // ---- scores: lane has tokens gq and gq + 8 of head tq of a tile ----
+      float acc[2][HN][4], sc[HN][2][2], sv[2][2], mv[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int h = 0; h < HN; ++h) acc[j][h][0] = acc[j][h][1] = acc[j][h][2] = acc[j][h][3] = 0.f;
+        uint32_t wa[NG], wb[NG];
+        load_words<NG>(kp[j] + gq * (D / 2) + tq * NG * 4, wa);
+        load_words<NG>(kp[j] + (gq + 8) * (D / 2) + tq * NG * 4, wb);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          mma_f16(acc, qa[2 * g], nib<0>(w[g]), nib<1>(w[g]));
-          mma_f16(acc, qa[2 * g + 1], nib<2>(w[g]), nib<3>(w[g]));
+          const uint32_t a0 = nib<0>(wa[g]), a1 = nib<0>(wb[g]), a2 = nib<1>(wa[g]), a3 = nib<1>(wb[g]);
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * g][0], qb[h][2 * g][1]);
+          const uint32_t b0 = nib<2>(wa[g]), b1 = nib<2>(wb[g]), b2 = nib<3>(wa[g]), b3 = nib<3>(wb[g]);
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], b0, b1, b2, b3, qb[h][2 * g + 1][0], qb[h][2 * g + 1][1]);
         }
         if constexpr (TAIL) {
-          const uint32_t r = (uint32_t)*(const uint16_t*)(kr + 16 * NG + 2 * tq) * 0x10001u;
-          mma_f16(acc, qa[2 * NG], (nib<0>(r) & 0xFFFFu) | (nib<1>(r) & 0xFFFF0000u), (nib<2>(r) & 0xFFFFu) | (nib<3>(r) & 0xFFFF0000u));
+          const uint8_t* kt = kp[j] + 16 * NG + 2 * tq;
+          const uint32_t ra = (uint32_t)*(const uint16_t*)(kt + gq * (D / 2)) * 0x10001u, rb = (uint32_t)*(const uint16_t*)(kt + (gq + 8) * (D / 2)) * 0x10001u;
+          const uint32_t a0 = (nib<0>(ra) & 0xFFFFu) | (nib<1>(ra) & 0xFFFF0000u), a1 = (nib<0>(rb) & 0xFFFFu) | (nib<1>(rb) & 0xFFFF0000u);
+          const uint32_t a2 = (nib<2>(ra) & 0xFFFFu) | (nib<3>(ra) & 0xFFFF0000u), a3 = (nib<2>(rb) & 0xFFFFu) | (nib<3>(rb) & 0xFFFF0000u);
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * NG][0], qb[h][2 * NG][1]);
         }
-        const uint2 km = *(const uint2*)(kp + 8 * D + (8 * n + 2 * tq) * 4), vm = *(const uint2*)(vp + 8 * D + (8 * n + 2 * tq) * 4);
-        sc[n][0] = fmaf((acc[0] + acc[2]) * qc, q4_scale(km.x), q4_min(km.x) * qx);
-        sc[n][1] = fmaf((acc[1] + acc[3]) * qc, q4_scale(km.y), q4_min(km.y) * qx);
-        sv[n][0] = q4_scale(vm.x); sv[n][1] = q4_scale(vm.y); mv[n][0] = q4_min(vm.x); mv[n][1] = q4_min(vm.y);
       }
-      if (t0 < s.lo || t0 + Q4_PAGE - 1 > s.pos) {               // rows outside the window or behind the last token hold anything
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int t = t0 + 8 * n + 2 * tq + e;
-            if (t < s.lo || t > s.pos) { sc[n][e] = -INFINITY; sv[n][e] = mv[n][e] = 0.f; }
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
+          sv[j][n] = q4_scale(vm); mv[j][n] = q4_min(vm);
+#pragma unroll
+          for (int h = 0; h < HN; ++h) sc[h][j][n] = fmaf((acc[j][h][2 * n] + acc[j][h][2 * n + 1]) * qc[h], q4_scale(km), q4_min(km) * qx[h]);
+        }
+        if (i + j >= n_my || t0[j] < s.lo || t0[j] + Q4_PAGE - 1 > s.pos) {      // rows outside the window or behind the last token hold anything
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int t = t0[j] + gq + 8 * n;
+            if (i + j >= n_my || t < s.lo || t > s.pos) {
+              sv[j][n] = mv[j][n] = 0.f;
+#pragma unroll
+              for (int h = 0; h < HN; ++h) sc[h][j][n] = -INFINITY;
+            }
           }
+        }
       }
       // ---- running maximum and scale: moved only where they fall behind by 2^8 and 2^2 ----
-      float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-      float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-      if (__any_sync(0xFFFFFFFFu, mx > m + 8.f || top * vf > 126.f)) {
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, mn = fmaxf(m, mx), corr = m == -INFINITY ? 0.f : ex2(m - mn), co = corr * (vn / vf);
+      float mx[HN], top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+      bool behind = top * vf > 126.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) { o[n][0] *= co; o[n][1] *= co; o[n][2] *= co; o[n][3] *= co; }
-        l *= corr; om *= corr; m = mn; vf = vn;
+      for (int h = 0; h < HN; ++h) {
+        mx[h] = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
+        behind |= mx[h] > m[h] + 8.f;
       }
-      uint32_t pa[4];
+      if (__any_sync(0xFFFFFFFFu, behind)) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float p0 = ex2(sc[n][0] - m), p1 = ex2(sc[n][1] - m);
-        l += p0 + p1;
-        om = fmaf(p0, mv[n][0], fmaf(p1, mv[n][1], om));
-        split_f16(p0 * (sv[n][0] * vf), p1 * (sv[n][1] * vf), pa[2 * n], pa[2 * n + 1]);
+        for (int k = 4; k < 32; k <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], k));
+        }
+        const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, vr = vn / vf;
+        vf = vn;
+#pragma unroll
+        for (int h = 0; h < HN; ++h) {
+          const float mn = fmaxf(m[h], mx[h]), corr = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn), co = corr * vr;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) { o[h][n][0] *= co; o[h][n][1] *= co; o[h][n][2] *= co; o[h][n][3] *= co; }
+          l[h] *= corr; om[h] *= corr; m[h] = mn;
+        }
       }
-      // ---- O += P V: column gq of tile 4 g + j is dim 32 g + 4 gq + j ----
-      {
+      // ---- O += P V: rows gq and gq + 8 of tile 2 g + k are dims 32 g + 4 gq + 2 k and + 1 ----
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t pb[HN][2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float f = sv[j][n] * vf;
+#pragma unroll
+          for (int h = 0; h < HN; ++h) {
+            const float e = ex2(sc[h][j][n] - m[h]);
+            l[h] += e;
+            om[h] = fmaf(e, mv[j][n], om[h]);
+            pb[h][n] = transpose_8x8(split_f16(e * f));
+          }
+        }
+        const uint8_t* vp = kp[j] + PB;
         uint32_t w0[NG], w1[NG];
         load_words<NG>(vp + lane * NG * 4, w0);
         load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          mma_f16(o[4 * g], pa, nib<0>(w0[g]), nib<0>(w1[g]));
-          mma_f16(o[4 * g + 1], pa, nib<1>(w0[g]), nib<1>(w1[g]));
-          mma_f16(o[4 * g + 2], pa, nib<2>(w0[g]), nib<2>(w1[g]));
-          mma_f16(o[4 * g + 3], pa, nib<3>(w0[g]), nib<3>(w1[g]));
+          const uint32_t a0 = nib<0>(w0[g]), a1 = nib<1>(w0[g]), a2 = nib<0>(w1[g]), a3 = nib<1>(w1[g]);
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g], a0, a1, a2, a3, pb[h][0], pb[h][1]);
+          const uint32_t b0 = nib<2>(w0[g]), b1 = nib<3>(w0[g]), b2 = nib<2>(w1[g]), b3 = nib<3>(w1[g]);
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g + 1], b0, b1, b2, b3, pb[h][0], pb[h][1]);
         }
         if constexpr (TAIL) {
           const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
           const uint32_t r0 = __byte_perm(w, 0u, 0x4140), r1 = __byte_perm(w, 0u, 0x4342);
-          mma_f16(o[4 * NG], pa, nib<0>(r0), nib<0>(r1));
-          mma_f16(o[4 * NG + 1], pa, nib<1>(r0), nib<1>(r1));
+#pragma unroll
+          for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], nib<0>(r0), nib<1>(r0), nib<0>(r1), nib<1>(r1), pb[h][0], pb[h][1]);
         }
       }
       if (i + QD_STAGES < n_my) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // this warp's reads of the slot come before the refill
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // this warp's reads of the slots come before the refill
         __syncwarp();
         issue(i + QD_STAGES);
       }
@@ -324,21 +389,19 @@ __global__ void __launch_bounds__(QD_THREADS, QD_CTAS_PER_SM) attn_decode_q4_ker
     taken += n_my;
 
     // ---- join the warps -----------------------------------------------------------------------------------------------------
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1); om += __shfl_xor_sync(0xFFFFFFFFu, om, 1);
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2); om += __shfl_xor_sync(0xFFFFFFFFu, om, 2);
-    if (has) {
-      float* dst = sm.part[warp][gq];
-      const float e0 = 262144.f / vf;
+    const float e0 = 262144.f / vf;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+    for (int h = 0; h < HN; ++h) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *(float4*)(dst + 32 * g + 8 * tq + 4 * k) = make_float4(fmaf(o[4 * g][k] + o[4 * g][k + 2], e0, om), fmaf(o[4 * g + 1][k] + o[4 * g + 1][k + 2], e0, om),
-                                                                   fmaf(o[4 * g + 2][k] + o[4 * g + 2][k + 2], e0, om), fmaf(o[4 * g + 3][k] + o[4 * g + 3][k + 2], e0, om));
-      if constexpr (TAIL)
-        *(float4*)(dst + 32 * NG + 4 * tq) = make_float4(fmaf(o[4 * NG][0] + o[4 * NG][2], e0, om), fmaf(o[4 * NG + 1][0] + o[4 * NG + 1][2], e0, om),
-                                                         fmaf(o[4 * NG][1] + o[4 * NG][3], e0, om), fmaf(o[4 * NG + 1][1] + o[4 * NG + 1][3], e0, om));
-      if (tq == 0) { dst[D] = m; dst[D + 1] = l; }
+      for (int k = 4; k < 32; k <<= 1) { l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], k); om[h] += __shfl_xor_sync(0xFFFFFFFFu, om[h], k); }
+      if (4 * h + tq < gn) {
+        float* dst = sm.part[warp][4 * h + tq];
+        auto val = [&](int n, int k) { return fmaf(o[h][n][2 * k] + o[h][n][2 * k + 1], e0, om[h]); };
+#pragma unroll
+        for (int g = 0; g < NG; ++g) *(float4*)(dst + 32 * g + 4 * gq) = make_float4(val(2 * g, 0), val(2 * g, 1), val(2 * g + 1, 0), val(2 * g + 1, 1));
+        if constexpr (TAIL) *(float2*)(dst + 32 * NG + 2 * gq) = make_float2(val(2 * NG, 0), val(2 * NG, 1));
+        if (gq == 0) { dst[D] = m[h]; dst[D + 1] = l[h]; }
+      }
     }
     __syncthreads();
     const bool whole = n_units == s.units;
@@ -419,17 +482,17 @@ __global__ void __launch_bounds__(QD_THREADS, QD_CTAS_PER_SM) attn_decode_q4_ker
   }
 }
 
-template <int D>
+template <int D, int HN>
 static int launch_decode_q4(const AttnDecodeParams& p, cudaStream_t st) {
-  int dev = 0, sms = 148;
+  int dev = 0, sms = QD_MAX_SMS;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int hgroups = (p.n_heads / p.n_kv_heads + QD_ROWS - 1) / QD_ROWS;
+  const int hgroups = (p.n_heads / p.n_kv_heads + qd_heads(HN) - 1) / qd_heads(HN);
   const long long tiles = (long long)p.batch * p.n_kv_heads * hgroups;
-  const int ctas = (int)std::min<long long>(std::min(sms * QD_CTAS_PER_SM, QD_MAX_CTAS), tiles * QD_MAX_PARTS);
+  const int ctas = (int)std::min<long long>(std::min(sms, QD_MAX_SMS) * qd_occupancy(HN), tiles * QD_MAX_PARTS);
   const size_t ring = (size_t)QD_WARPS * QD_STAGES * 2 * q4_page_bytes(D);
   static SmemOptIn opt;
-  if (cudaError_t e = opt.ensure(attn_decode_q4_kernel<D>, ring, 0); e != cudaSuccess) return (int)e;
-  return (int)launch(attn_decode_q4_kernel<D>, dim3(ctas), dim3(QD_THREADS), ring, st, p);
+  if (cudaError_t e = opt.ensure(attn_decode_q4_kernel<D, HN>, ring, 0); e != cudaSuccess) return (int)e;
+  return (int)launch(attn_decode_q4_kernel<D, HN>, dim3(ctas), dim3(QD_THREADS), ring, st, p);
 }
 
 int attn_decode_q4_dispatch(const AttnDecodeParams& p, cudaStream_t st) {
@@ -438,11 +501,12 @@ int attn_decode_q4_dispatch(const AttnDecodeParams& p, cudaStream_t st) {
   if (p.rope_dim < 0 || p.rope_dim > p.head_dim || (p.rope_dim & 1)) return -3;
   if (((uintptr_t)p.k_cache & 15) || ((uintptr_t)p.v_cache & 15) || ((uintptr_t)p.partial & 15)) return -4;
   if (p.window < 0) return -5;
+  const bool narrow = p.n_heads / p.n_kv_heads <= qd_heads(1);
   switch (p.head_dim) {
-    case 64: return launch_decode_q4<64>(p, st);
-    case 80: return launch_decode_q4<80>(p, st);
-    case 96: return launch_decode_q4<96>(p, st);
-    default: return launch_decode_q4<128>(p, st);
+    case 64: return narrow ? launch_decode_q4<64, 1>(p, st) : launch_decode_q4<64, 2>(p, st);
+    case 80: return narrow ? launch_decode_q4<80, 1>(p, st) : launch_decode_q4<80, 2>(p, st);
+    case 96: return narrow ? launch_decode_q4<96, 1>(p, st) : launch_decode_q4<96, 2>(p, st);
+    default: return narrow ? launch_decode_q4<128, 1>(p, st) : launch_decode_q4<128, 2>(p, st);
   }
 }
 
@@ -451,7 +515,10 @@ int attn_decode_q4_dispatch(const AttnDecodeParams& p, cudaStream_t st) {
 extern "C" {
 
 // floats of scratch (`partial`) that any launch over a 4-bit cache needs
-long long rlz_attn_q4_partial_floats(int head_dim) { return 2LL * rlz::QD_MAX_CTAS * rlz::QD_ROWS * (head_dim + 4); }
+long long rlz_attn_q4_partial_floats(int head_dim) { 
+  using namespace rlz;
+  return 2LL * QD_MAX_SMS * std::max(qd_occupancy(1) * qd_heads(1), qd_occupancy(2) * qd_heads(2)) * (head_dim + 4);
+}
 
 // 0 / 3211 / 3311 / 3312
 int rlz_attn_q4_error(int clear) {
