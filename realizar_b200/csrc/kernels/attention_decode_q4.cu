@@ -15,37 +15,43 @@
 //     16, took twice the instructions and registers for 4 heads: 46 us for every 65536 pages of 128, this STEP2.)
 //     q is scaled by a power of two so that its largest value lies in [2^13, 2^14), p x scale' by one that follows the scales.
 //   * The running maximum moves only when a score passes it by 2^8, so that the accumulators are rarely rescaled.
-// Each warp has a ring of whole pages (K and V) filled by bulk copies.
 //
-// Split: the pages of all (sequence, kv head, head group) tiles, in units of four, are divided evenly over one wave of CTAs,
-// whatever the lengths are; positions are read on the device, so a captured launch serves growing sequences.  A CTA whose units
-// do not cover a tile leaves its part in scratch, and the last of the tile's CTAs to arrive joins them in a fixed order.
+// One CTA to an SM.  The main warps do nothing but pages: each has a ring of page pairs (K and V) that its lanes fill by 16-byte
+// asynchronous copies, and its pages follow one another across tiles.  (Bulk copies need a dozen instructions each, and a warp that
+// issued them for all was too slow.)  Four helper warps prepare the next tile's query fragments (and the new token's rows) and join
+// and store the finished tile meanwhile, through two buffers each.
+// (With every warp doing its share of that between two tiles, a batch of 64 x 2048 tokens spent 28 of its 60 us there.)
+//
+// Split: the pages of all (sequence, kv head, head group) tiles are divided evenly over the CTAs, whatever the lengths are;
+// positions are read on the device, so a captured launch serves growing sequences.  A CTA that has only some pages of a tile
+// leaves its part in scratch, and the last of the tile's CTAs to arrive joins them in a fixed order.
 #include "attention_q4.cuh"
 #include "kv_q4.cuh"
 #include <algorithm>
 
 namespace rlz {
 
-// 3211: a page never arrived (bounded wait ran out); 3311: a position beyond the page-table row (the sequence is skipped);
+// 3211: a tile's helpers or main warps never answered (bounded wait ran out); 3311: a position beyond the page-table row (the sequence is skipped);
 // 3312: a page id outside the cache (read as page 0, not written)
 __device__ int g_attn_q4_error = 0;
 
-constexpr int QD_WARPS = 4, QD_THREADS = 32 * QD_WARPS, QD_STAGES = 4;
+constexpr int QD_STAGES = 3, QD_MAX_SMS = 148, QD_HELPERS = 128;
 constexpr int QD_MAX_PARTS = 64;              // CTAs that share a tile: bounds the time of the last one, which joins their parts
-// query heads of a CTA (HN tiles of 4) and CTAs to an SM, by registers
+// query heads of a CTA (HN tiles of 4) and its main warps: with the four others 16 warps of 128 registers, or 12 of 168
 constexpr int qd_heads(int hn) { return 4 * hn; }
-constexpr int qd_occupancy(int hn) { return hn == 1 ? 4 : 3; }
-constexpr int QD_MAX_SMS = 148;
+constexpr int qd_warps(int hn) { return hn == 1 ? 12 : 8; }
 
 template <int D, int HN> struct QdSmem {
-  float q[4 * HN][D];
-  float part[QD_WARPS][4 * HN][D + 4];         // per warp and head: sum, then maximum and weight
-  float qc[4 * HN], qx[4 * HN];               // 2^18 / f of a head whose fragments hold q f, and the sum of q
-  uint8_t codes[2][D];                        // the new token's rows
-  uint32_t meta[2];
-  int wsum[QD_WARPS];
-  int plan_b, plan_rem, last;
-  unsigned long long full[QD_WARPS][QD_STAGES];
+  static constexpr int KS = D / 16, ROWS = 4 * HN;
+  uint2 frag[2][HN][KS][32];                  // B fragments of the heads, as the main warps' lanes hold them
+  float part[2][qd_warps(HN)][ROWS][D + 4];   // per warp and head: sum, then maximum and weight
+  float q[ROWS][D];                           // helpers: normalised, rotated and scaled queries
+  float qc[2][ROWS], qx[2][ROWS];             // 2^18 / f of a head whose fragments hold q f, and the sum of q
+  uint8_t codes[2][2][D];                     // the new token's rows (key, value)
+  uint32_t meta[2][2];
+  struct { int n, tok, lo, pos, own; } tile[2];   // pages, first token, first and last visible position, place of the new token's page or -1
+  int last;
+  unsigned long long frag_full[2], part_full[2], part_empty[2];
 };
 
 __device__ __forceinline__ int q4_page_id(int raw, int num_pages) {
@@ -86,339 +92,409 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* src, 
   }
 }
 
-struct QdSeq { int pos, lo, first_page, pages, units; };      // units of QD_WARPS pages; 0: nothing to do
+struct QdSeq { int pos, lo, first_page, pages; };             // pages first_page .. first_page + pages - 1; 0 pages: nothing to do
 __device__ __forceinline__ QdSeq qd_seq(const AttnDecodeParams& p, int b) {
-  QdSeq s = {p.positions[b], 0, 0, 0, 0};
+  QdSeq s = {p.positions[b], 0, 0, 0};
   if (s.pos < 0) return s;
   if (s.pos / Q4_PAGE >= p.max_pages) { atomicExch(&g_attn_q4_error, 3311); return s; }
   s.lo = p.window > 0 ? max(0, s.pos + 1 - p.window) : 0;
   s.first_page = s.lo / Q4_PAGE;
-  s.pages = s.pos / Q4_PAGE + 1;
-  s.units = (s.pages - s.first_page + QD_WARPS - 1) / QD_WARPS;
+  s.pages = s.pos / Q4_PAGE + 1 - s.first_page;
   return s;
+}
+// the pages of one tile that a CTA has: `n` of them from the tile's page `skip` on
+struct QdTile { QdSeq s; int b, tile, skip, n; };
+// the tile that page `at` of sequence b's tiles (or the next sequence with any) lies in; the CTA has `left` more pages
+__device__ __forceinline__ QdTile qd_tile(const AttnDecodeParams& p, int b, int at, int left) {
+  QdTile t;
+  for (;; ++b, at = 0) { t.s = qd_seq(p, b); if (t.s.pages) break; }
+  t.b = b; t.tile = at / t.s.pages; t.skip = at - t.tile * t.s.pages; t.n = min(t.s.pages - t.skip, left);
+  return t;
+}
+__device__ __forceinline__ QdTile qd_next(const AttnDecodeParams& p, const QdTile& t, int tiles, int left) {
+  const bool new_seq = t.tile + 1 == tiles;
+  return qd_tile(p, new_seq ? t.b + 1 : t.b, new_seq ? 0 : (t.tile + 1) * t.s.pages, left);
+}
+// bounded: false (and the status word) when the barrier's phase does not end
+__device__ __forceinline__ bool qd_wait(unsigned long long* bar, uint32_t parity, bool patient) {
+  const uint32_t limit = patient ? ATT_WAIT_LIMIT : 1024u;
+  for (uint32_t spin = 0; spin < limit; ++spin) if (att_try_wait(bar, parity)) return true;
+  atomicExch(&g_attn_q4_error, 3211);
+  return false;
+}
+__device__ __forceinline__ void qd_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(att_smem_u32(bar)) : "memory");
 }
 
 template <int D, int HN>
-__global__ void __launch_bounds__(QD_THREADS, qd_occupancy(HN)) attn_decode_q4_kernel(const __grid_constant__ AttnDecodeParams p) {
-  constexpr int QD_ROWS = 4 * HN;
+__global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode_q4_kernel(const __grid_constant__ AttnDecodeParams p) {
+  constexpr int ROWS = 4 * HN, NW = qd_warps(HN);
   constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, KS = 2 * NG + TAIL, NT = 2 * NG + TAIL, PB = q4_page_bytes(D), NP = HeadPairs<D>::NP;
-  extern __shared__ __align__(128) uint8_t qd_ring[];
-  __shared__ __align__(16) QdSmem<D, HN> sm;
+  extern __shared__ __align__(128) uint8_t qd_smem[];
+  QdSmem<D, HN>& sm = *(QdSmem<D, HN>*)qd_smem;
+  uint8_t* qd_ring = qd_smem + (sizeof(QdSmem<D, HN>) + 127) / 128 * 128;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
-  if (tid < QD_WARPS * QD_STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(att_smem_u32(&sm.full[0][0] + tid)));
+  if (tid < 6) {
+    unsigned long long* bar = tid < 2 ? &sm.frag_full[tid] : tid < 4 ? &sm.part_full[tid - 2] : &sm.part_empty[tid - 4];
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(att_smem_u32(bar)), "r"(tid < 2 ? QD_HELPERS : tid < 4 ? NW : 1));
+  }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- my share of the units: [u, uend) of the sequence of all tiles' units -------------------------------------------------
-  const int G = p.n_heads / p.n_kv_heads, hgroups = (G + QD_ROWS - 1) / QD_ROWS, tiles = p.n_kv_heads * hgroups;
-  const int per = (p.batch + QD_THREADS - 1) / QD_THREADS, b_lo = min(tid * per, p.batch), b_hi = min(b_lo + per, p.batch);
-  int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += qd_seq(p, b).units * tiles;
+  // ---- my share: pages [x0, x1) of the sequence of all tiles' pages.  Every warp works it out, its lanes over the sequences -----
+  const int G = p.n_heads / p.n_kv_heads, hgroups = (G + ROWS - 1) / ROWS, tiles = p.n_kv_heads * hgroups;
+  const int per = (p.batch + 31) / 32, b_lo = min(lane * per, p.batch), b_hi = min(b_lo + per, p.batch);
+  int mine = 0, live = 0;
+  for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, b).pages; mine += n * tiles; live += n > 0; }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o); if (lane >= o) incl += v; }
-  if (lane == 31) sm.wsum[warp] = incl;
-  __syncthreads();
-  int total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < QD_WARPS; ++w) { if (w < warp) before += sm.wsum[w]; total += sm.wsum[w]; }
-  const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
+  const int total = __shfl_sync(0xFFFFFFFFu, incl, 31), before = incl - mine;
+  live = __reduce_add_sync(0xFFFFFFFFu, live);
+  // as many CTAs as there are tiles, and more as long as each warp of them has a page
+  const int ctas = min((int)gridDim.x, max(live * tiles, (total + NW - 1) / NW)), c = blockIdx.x;
   if (c >= ctas) return;
-  const int u0 = (int)((int64_t)c * total / ctas), uend = (int)((int64_t)(c + 1) * total / ctas);
-  if (mine > 0 && before <= u0 && u0 < before + mine) {
-    int b = b_lo, at = before;
-    for (;; ++b) { const int n = qd_seq(p, b).units * tiles; if (u0 < at + n) break; at += n; }
-    sm.plan_b = b; sm.plan_rem = u0 - at;
-  }
-  __syncthreads();
-
-  const RopeArgs rope = {p.rope_table, p.rope_table_len, p.rope_dim, p.rope_type, p.rope_theta};
-  const int half = p.rope_dim >> 1;
-  const float qscale = p.scale * 1.4426950408889634f;
-  uint8_t* my_ring = qd_ring + (size_t)warp * QD_STAGES * 2 * PB;
-  uint32_t taken = 0;                                          // pages this warp has been through: ring slot and parity
+  const int x0 = (int)((int64_t)c * total / ctas), x1 = (int)((int64_t)(c + 1) * total / ctas);
+  const bool holds = before <= x0 && x0 < incl;                  // one lane
+  int b0 = b_lo, at0 = x0 - before;
+  if (holds) for (;; ++b0) { const int n = qd_seq(p, b0).pages * tiles; if (at0 < n) break; at0 -= n; }
+  const int holder = __ffs(__ballot_sync(0xFFFFFFFFu, holds)) - 1;
+  b0 = __shfl_sync(0xFFFFFFFFu, b0, holder);
+  at0 = __shfl_sync(0xFFFFFFFFu, at0, holder);
+  // Page k of main warp w is page w + NW k of the CTA's share: the tiles' ends fall on all warps alike.  A warp's pages of a tile go
+  // through its ring two at a time, of an odd number the last alone.
+  auto first_k = [](int w, int x) { return x > w ? (x - w + NW - 1) / NW : 0; };        // first page of warp w at or behind place x of the share
   bool ok = true;
 
-  for (int u = u0, b = sm.plan_b, rem = sm.plan_rem; u < uend;) {
-    const QdSeq s = qd_seq(p, b);
-    if (s.units == 0) { ++b; rem = 0; continue; }
-    const int tile = rem / s.units, ub = rem - tile * s.units, n_units = min(s.units - ub, uend - u);
-    const int kvh = tile / hgroups, g0 = (tile - kvh * hgroups) * QD_ROWS, gn = min(QD_ROWS, G - g0);
-    const int tile_u0 = u - ub;
-    const int page0 = s.first_page + ub * QD_WARPS, page1 = min(s.pages, page0 + n_units * QD_WARPS);
-    const bool owner = !p.no_append && page1 == s.pages;         // the new token's page is mine
-    const int n_my = max(0, (page1 - page0 - warp + QD_WARPS - 1) / QD_WARPS);
-    const int32_t* pt = p.page_table + (int64_t)b * p.pt_stride + page0 + warp;
-
-    // ---- first pages under way; lane i keeps the id of my i-th page of a group of 32, and of the next group -------------------
-    int ids = lane < n_my ? q4_page_id(pt[QD_WARPS * lane], p.num_pages) : 0, ids_next = 0;
-    auto issue = [&](int i) {                                     // pages i and i + 1 (i even): lanes 0 and 1 take one each
-      if ((i & 31) == 0) {
-        if (i > 0) ids = ids_next;
-        ids_next = i + 32 + lane < n_my ? q4_page_id(pt[QD_WARPS * (i + 32 + lane)], p.num_pages) : 0;
+  if (warp < NW) {
+    // ================================ main warps ================================================================================
+    uint8_t* my_ring = qd_ring + (size_t)warp * QD_STAGES * 4 * PB;
+    // -- the copies: pair after pair of the stream, their page ids read one pair ahead
+    QdTile f = qd_tile(p, b0, at0, x1 - x0);
+    int f_at = 0, f_k = 0, f_k1 = first_k(warp, f.n), f_id[2], f_np = 0, f_kvh = f.tile / hgroups;
+    const int32_t* f_pt = p.page_table + (int64_t)f.b * p.pt_stride + f.s.first_page + f.skip + warp;
+    auto look_up = [&]() {
+      f_np = 0;
+      while (f_k >= f_k1) {                                          // none left in this tile
+        f_at += f.n;
+        if (f_at >= x1 - x0) return;
+        f = qd_next(p, f, tiles, x1 - x0 - f_at);
+        f_k1 = first_k(warp, f_at + f.n); f_kvh = f.tile / hgroups;
+        f_pt = p.page_table + (int64_t)f.b * p.pt_stride + f.s.first_page + f.skip + warp - f_at;
       }
-      const int id = __shfl_sync(0xFFFFFFFFu, ids, (i + lane) & 31);
-      if (lane < 2 && i + lane < n_my) {
-        const uint32_t slot = (taken + i + lane) % QD_STAGES;
-        unsigned long long* bar = &sm.full[warp][slot];
-        uint8_t* dst = my_ring + slot * (2 * PB);
-        const int64_t off = ((int64_t)id * p.n_kv_heads + kvh) * PB;
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(att_smem_u32(bar)), "r"((uint32_t)(2 * PB)) : "memory");
-        att_bulk_g2s(dst, (const uint8_t*)p.k_cache + off, PB, bar);
-        att_bulk_g2s(dst + PB, (const uint8_t*)p.v_cache + off, PB, bar);
-      }
+      f_np = min(2, f_k1 - f_k);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) f_id[j] = __ldg(f_pt + NW * (f_k + min(j, f_np - 1)));
+      f_k += f_np;
     };
-    for (int i = 0; i < min(QD_STAGES, n_my); i += 2) issue(i);
-
-    // ---- the new token: queries of the group, and in the owner its key and value rows ------------------------------------------
-    const float* row = p.qkv + (int64_t)b * p.ld_qkv;
-    float2 cs[NP];
-    load_rope<D>(rope, s.pos, lane, cs);
-    float x0[NP], x1[NP];
-    auto load = [&](const float* src, int hf, int type) {
+    auto copy_pair = [&](uint32_t to) {
+      if (f_np) {
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        const int i = lane + 32 * k;
-        x0[k] = x1[k] = 0.f;
-        if (i < D / 2) { const int2 at = pair_dims(i, hf, type); x0[k] = src[at.x]; x1[k] = src[at.y]; }
-      }
-    };
-    for (int g = warp; g < gn; g += QD_WARPS) {
-      load(row + p.q_off + (int64_t)(kvh * G + g0 + g) * D, half, p.rope_type);
-      norm_rope_f<D>(x0, x1, p.q_norm_w, p.eps, rope, cs, lane);
-      float top = 0.f, sum = 0.f;
+        for (int j = 0; j < 2; ++j) {
+          if (j < f_np) {
+            const int64_t off = ((int64_t)q4_page_id(f_id[j], p.num_pages) * p.n_kv_heads + f_kvh) * PB + 16 * lane;
+            const uint32_t dst = att_smem_u32(my_ring) + to * (4 * PB) + j * (2 * PB) + 16 * lane;
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        x0[k] *= qscale; x1[k] *= qscale;
-        top = fmaxf(top, fmaxf(fabsf(x0[k]), fabsf(x1[k]))); sum += x0[k] + x1[k];
-      }
-      top = warp_max(top); sum = warp_sum(sum);
-      const float f = top > 0.f ? pow2_for(top, 13) : 1.f;
+            for (int v = 0; v < 2; ++v) {
+              const uint8_t* src = (const uint8_t*)(v ? p.v_cache : p.k_cache) + off;
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        const int i = lane + 32 * k;
-        if (i < D / 2) { const int2 at = pair_dims(i, half, p.rope_type); sm.q[g][at.x] = x0[k] * f; sm.q[g][at.y] = x1[k] * f; }
-      }
-      if (lane == 0) { sm.qc[g] = 262144.f / f; sm.qx[g] = sum; }
-    }
-    if (owner && warp >= 2) {
-      const bool v = warp == 3;
-      load(row + (v ? p.v_off : p.k_off) + kvh * D, v ? 0 : half, v ? 0 : p.rope_type);
-      if (!v) norm_rope_d<D>(x0, x1, p.q_norm_w ? p.k_norm_w : nullptr, (double)p.eps, rope, cs, lane);
-      const uint32_t meta = q4_quantise<D>(x0, x1, v ? 0 : half, v ? 0 : p.rope_type, lane, sm.codes[v]);
-      __syncwarp();
-      if (lane == 0) sm.meta[v] = meta;
-      if (g0 == 0) {                                             // one head group writes the row
-        const int raw = p.page_table[(int64_t)b * p.pt_stride + s.pos / Q4_PAGE];
-        if (p.num_pages <= 0 || (unsigned)raw < (unsigned)p.num_pages) {
-          uint8_t* dst = (uint8_t*)(v ? p.v_cache : p.k_cache) + ((int64_t)raw * p.n_kv_heads + kvh) * PB;
-          if (v) q4_store_v<D>(dst, s.pos % Q4_PAGE, sm.codes[1], meta, lane);
-          else q4_store_k<D>(dst, s.pos % Q4_PAGE, sm.codes[0], meta, lane);
-        }
-      }
-    }
-    __syncthreads();
-
-    // ---- query fragments: column gq is head gq / 2 of a tile, its head (even) or what that leaves (odd).  Word tq of a group of 32
-    // dims holds dims 8 tq .. + 7 and its nibbles pair as (0, 4), (1, 5), (2, 6), (3, 7) ----
-    uint32_t qb[HN][KS][2];
-    float qc[HN], qx[HN];
-#pragma unroll
-    for (int h = 0; h < HN; ++h) {
-      const int head = 4 * h + (gq >> 1);
-      const bool has = head < gn;
-      const float* qr = sm.q[has ? head : 0];
-      const uint32_t sel = gq & 1 ? 0x7632u : 0x5410u;            // odd columns take the high halves of the two splits
-      auto frag = [&](int d0, int d1) { return has ? __byte_perm(split_f16(qr[d0]), split_f16(qr[d1]), sel) : 0u; };
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int d = 32 * g + 8 * tq;
-        qb[h][2 * g][0] = frag(d, d + 4); qb[h][2 * g][1] = frag(d + 1, d + 5);
-        qb[h][2 * g + 1][0] = frag(d + 2, d + 6); qb[h][2 * g + 1][1] = frag(d + 3, d + 7);
-      }
-      if constexpr (TAIL) { const int d = 32 * NG + 4 * tq; qb[h][2 * NG][0] = frag(d, d + 1); qb[h][2 * NG][1] = frag(d + 2, d + 3); }
-      const bool mine_is = 4 * h + tq < gn;                      // the head whose scores this lane holds
-      qc[h] = mine_is ? sm.qc[4 * h + tq] : 0.f; qx[h] = mine_is ? sm.qx[4 * h + tq] : 0.f;
-    }
-
-    float o[HN][NT][4], m[HN], l[HN], om[HN];                    // om: sum of p x min'
-#pragma unroll
-    for (int h = 0; h < HN; ++h) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.f;
-      m[h] = -INFINITY; l[h] = om[h] = 0.f;
-    }
-    float vf = 0x1p100f;                                          // power of two that p x scale' carries
-
-    for (int i = 0; i < n_my; i += 2) {                           // two pages at a time (of an odd number, the last comes with a masked one)
-      uint8_t* kp[2];
-      int t0[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t slot = (taken + i + j) % QD_STAGES, parity = ((taken + i + j) / QD_STAGES) & 1u;
-        kp[j] = my_ring + slot * (2 * PB);
-        const int page = page0 + warp + QD_WARPS * (i + j);
-        t0[j] = page * Q4_PAGE;
-        if (i + j < n_my) {
-          bool arrived = false;
-          const uint32_t limit = ok ? ATT_WAIT_LIMIT : 1024u;
-          for (uint32_t spin = 0; spin < limit; ++spin) if (att_try_wait(&sm.full[warp][slot], parity)) { arrived = true; break; }
-          if (!arrived) { ok = false; atomicExch(&g_attn_q4_error, 3211); }
-          if (owner && page == s.pages - 1) {                    // the copy may have passed the write of the new row
-            q4_store_k<D>(kp[j], s.pos % Q4_PAGE, sm.codes[0], sm.meta[0], lane);
-            q4_store_v<D>(kp[j] + PB, s.pos % Q4_PAGE, sm.codes[1], sm.meta[1], lane);
-            __syncwarp();
-          }
-        }
-      }
-      // ---- scores: lane has tokens gq and gq + 8 of head tq of a tile ----
-      float acc[2][HN][4], sc[HN][2][2], sv[2][2], mv[2][2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int h = 0; h < HN; ++h) acc[j][h][0] = acc[j][h][1] = acc[j][h][2] = acc[j][h][3] = 0.f;
-        uint32_t wa[NG], wb[NG];
-        load_words<NG>(kp[j] + gq * (D / 2) + tq * NG * 4, wa);
-        load_words<NG>(kp[j] + (gq + 8) * (D / 2) + tq * NG * 4, wb);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t a0 = nib<0>(wa[g]), a1 = nib<0>(wb[g]), a2 = nib<1>(wa[g]), a3 = nib<1>(wb[g]);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * g][0], qb[h][2 * g][1]);
-          const uint32_t b0 = nib<2>(wa[g]), b1 = nib<2>(wb[g]), b2 = nib<3>(wa[g]), b3 = nib<3>(wb[g]);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], b0, b1, b2, b3, qb[h][2 * g + 1][0], qb[h][2 * g + 1][1]);
-        }
-        if constexpr (TAIL) {
-          const uint8_t* kt = kp[j] + 16 * NG + 2 * tq;
-          const uint32_t ra = (uint32_t)*(const uint16_t*)(kt + gq * (D / 2)) * 0x10001u, rb = (uint32_t)*(const uint16_t*)(kt + (gq + 8) * (D / 2)) * 0x10001u;
-          const uint32_t a0 = (nib<0>(ra) & 0xFFFFu) | (nib<1>(ra) & 0xFFFF0000u), a1 = (nib<0>(rb) & 0xFFFFu) | (nib<1>(rb) & 0xFFFF0000u);
-          const uint32_t a2 = (nib<2>(ra) & 0xFFFFu) | (nib<3>(ra) & 0xFFFF0000u), a3 = (nib<2>(rb) & 0xFFFFu) | (nib<3>(rb) & 0xFFFF0000u);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * NG][0], qb[h][2 * NG][1]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
-          sv[j][n] = q4_scale(vm); mv[j][n] = q4_min(vm);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) sc[h][j][n] = fmaf((acc[j][h][2 * n] + acc[j][h][2 * n + 1]) * qc[h], q4_scale(km), q4_min(km) * qx[h]);
-        }
-        if (i + j >= n_my || t0[j] < s.lo || t0[j] + Q4_PAGE - 1 > s.pos) {      // rows outside the window or behind the last token hold anything
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int t = t0[j] + gq + 8 * n;
-            if (i + j >= n_my || t < s.lo || t > s.pos) {
-              sv[j][n] = mv[j][n] = 0.f;
-#pragma unroll
-              for (int h = 0; h < HN; ++h) sc[h][j][n] = -INFINITY;
+              for (int i = 0; i < (PB + 511) / 512; ++i)
+                if (512 * (i + 1) <= PB || 512 * i + 16 * lane < PB)
+                  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * PB + 512 * i), "l"(src + 512 * i) : "memory");
             }
           }
         }
       }
-      // ---- running maximum and scale: moved only where they fall behind by 2^8 and 2^2 ----
-      float mx[HN], top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-      bool behind = top * vf > 126.f;
-#pragma unroll
-      for (int h = 0; h < HN; ++h) {
-        mx[h] = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
-        behind |= mx[h] > m[h] + 8.f;
-      }
-      if (__any_sync(0xFFFFFFFFu, behind)) {
-#pragma unroll
-        for (int k = 4; k < 32; k <<= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], k));
-        }
-        const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, vr = vn / vf;
-        vf = vn;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    look_up();
+    for (int i = 0; i < QD_STAGES - 1; ++i) { copy_pair(i); look_up(); }
+    uint32_t slot = 0;
+    for (int it = 0, at = 0; at < x1 - x0; ++it) {
+      const int buf = it & 1;
+      const uint32_t phase = (uint32_t)(it >> 1) & 1u;
+      ok = qd_wait(&sm.frag_full[buf], phase, ok) && ok;
+      if (!ok) break;                                                // the tile's description never came
+      const auto s = sm.tile[buf];
+      const int end = at + s.n, k0 = first_k(warp, at), k1 = first_k(warp, end);
+      if (k0 < k1) {
+        const int own = s.own >= 0 && s.own % NW == warp ? s.own / NW : 1 << 30;        // my page that holds the new token
+        uint32_t qb[HN][KS][2];
+        float qc[HN], qx[HN];
 #pragma unroll
         for (int h = 0; h < HN; ++h) {
-          const float mn = fmaxf(m[h], mx[h]), corr = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn), co = corr * vr;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) { o[h][n][0] *= co; o[h][n][1] *= co; o[h][n][2] *= co; o[h][n][3] *= co; }
-          l[h] *= corr; om[h] *= corr; m[h] = mn;
+          for (int ks = 0; ks < KS; ++ks) { const uint2 f = sm.frag[buf][h][ks][lane]; qb[h][ks][0] = f.x; qb[h][ks][1] = f.y; }
+          qc[h] = sm.qc[buf][4 * h + tq]; qx[h] = sm.qx[buf][4 * h + tq];
         }
-      }
-      // ---- O += P V: rows gq and gq + 8 of tile 2 g + k are dims 32 g + 4 gq + 2 k and + 1 ----
+        float o[HN][NT][4], m[HN], l[HN], om[HN];                  // om: sum of p x min'
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t pb[HN][2];
+        for (int h = 0; h < HN; ++h) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float f = sv[j][n] * vf;
+          for (int n = 0; n < NT; ++n) o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.f;
+          m[h] = -INFINITY; l[h] = om[h] = 0.f;
+        }
+        float vf = 0x1p100f;                                        // power of two that p x scale' carries
+        int tok = s.tok + (warp + NW * k0 - at) * Q4_PAGE;           // first token of page k
+
+        for (int k = k0; k < k1; k += 2, tok += 2 * NW * Q4_PAGE) {   // two pages at a time (of an odd number, the last comes with a masked one)
+          copy_pair(slot == 0 ? QD_STAGES - 1 : slot - 1);            // into the slot that the pair before this one left
+          look_up();
+          asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
+          __syncwarp();
+          uint8_t* const kp[2] = {my_ring + slot * (4 * PB), my_ring + slot * (4 * PB) + 2 * PB};
+          if (own - k < 2 && own >= k) {                             // the copy may have passed the write of the new row
+            uint8_t* page = own == k ? kp[0] : kp[1];
+            q4_store_k<D>(page, s.pos % Q4_PAGE, sm.codes[buf][0], sm.meta[buf][0], lane);
+            q4_store_v<D>(page + PB, s.pos % Q4_PAGE, sm.codes[buf][1], sm.meta[buf][1], lane);
+            __syncwarp();
+          }
+          // ---- scores: lane has tokens gq and gq + 8 of head tq of a tile ----
+          float acc[2][HN][4], sc[HN][2][2], sv[2][2], mv[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int h = 0; h < HN; ++h) acc[j][h][0] = acc[j][h][1] = acc[j][h][2] = acc[j][h][3] = 0.f;
+            uint32_t wa[NG], wb[NG];
+            load_words<NG>(kp[j] + gq * (D / 2) + tq * NG * 4, wa);
+            load_words<NG>(kp[j] + (gq + 8) * (D / 2) + tq * NG * 4, wb);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const uint32_t a0 = nib<0>(wa[g]), a1 = nib<0>(wb[g]), a2 = nib<1>(wa[g]), a3 = nib<1>(wb[g]);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * g][0], qb[h][2 * g][1]);
+              const uint32_t b0 = nib<2>(wa[g]), b1 = nib<2>(wb[g]), b2 = nib<3>(wa[g]), b3 = nib<3>(wb[g]);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], b0, b1, b2, b3, qb[h][2 * g + 1][0], qb[h][2 * g + 1][1]);
+            }
+            if constexpr (TAIL) {
+              const uint8_t* kt = kp[j] + 16 * NG + 2 * tq;
+              const uint32_t ra = (uint32_t)*(const uint16_t*)(kt + gq * (D / 2)) * 0x10001u, rb = (uint32_t)*(const uint16_t*)(kt + (gq + 8) * (D / 2)) * 0x10001u;
+              const uint32_t a0 = (nib<0>(ra) & 0xFFFFu) | (nib<1>(ra) & 0xFFFF0000u), a1 = (nib<0>(rb) & 0xFFFFu) | (nib<1>(rb) & 0xFFFF0000u);
+              const uint32_t a2 = (nib<2>(ra) & 0xFFFFu) | (nib<3>(ra) & 0xFFFF0000u), a3 = (nib<2>(rb) & 0xFFFFu) | (nib<3>(rb) & 0xFFFF0000u);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * NG][0], qb[h][2 * NG][1]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
+              sv[j][n] = q4_scale(vm); mv[j][n] = q4_min(vm);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) sc[h][j][n] = fmaf((acc[j][h][2 * n] + acc[j][h][2 * n + 1]) * qc[h], q4_scale(km), q4_min(km) * qx[h]);
+            }
+          }
+          if (k + 1 >= k1 || tok < s.lo || tok + (NW + 1) * Q4_PAGE - 1 > s.pos) {       // rows outside the window or behind the last token hold anything
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const int t = tok + j * NW * Q4_PAGE + gq + 8 * n;
+                if (k + j >= k1 || t < s.lo || t > s.pos) {
+                  sv[j][n] = mv[j][n] = 0.f;
+#pragma unroll
+                  for (int h = 0; h < HN; ++h) sc[h][j][n] = -INFINITY;
+                }
+              }
+          }
+          // ---- running maximum and scale: moved only where they fall behind by 2^8 and 2^2 ----
+          float mx[HN], top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+          bool behind = top * vf > 126.f;
 #pragma unroll
           for (int h = 0; h < HN; ++h) {
-            const float e = ex2(sc[h][j][n] - m[h]);
-            l[h] += e;
-            om[h] = fmaf(e, mv[j][n], om[h]);
-            pb[h][n] = transpose_8x8(split_f16(e * f));
+            mx[h] = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
+            behind |= mx[h] > m[h] + 8.f;
           }
+          if (__any_sync(0xFFFFFFFFu, behind)) {
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], k));
+            }
+            const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, vr = vn / vf;
+            vf = vn;
+#pragma unroll
+            for (int h = 0; h < HN; ++h) {
+              const float mn = fmaxf(m[h], mx[h]), corr = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn), co = corr * vr;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) { o[h][n][0] *= co; o[h][n][1] *= co; o[h][n][2] *= co; o[h][n][3] *= co; }
+              l[h] *= corr; om[h] *= corr; m[h] = mn;
+            }
+          }
+          // ---- O += P V: rows gq and gq + 8 of tile 2 g + k are dims 32 g + 4 gq + 2 k and + 1 ----
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t pb[HN][2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const float f = sv[j][n] * vf;
+#pragma unroll
+              for (int h = 0; h < HN; ++h) {
+                const float e = ex2(sc[h][j][n] - m[h]);
+                l[h] += e;
+                om[h] = fmaf(e, mv[j][n], om[h]);
+                pb[h][n] = transpose_8x8(split_f16(e * f));
+              }
+            }
+            const uint8_t* vp = kp[j] + PB;
+            uint32_t w0[NG], w1[NG];
+            load_words<NG>(vp + lane * NG * 4, w0);
+            load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const uint32_t a0 = nib<0>(w0[g]), a1 = nib<1>(w0[g]), a2 = nib<0>(w1[g]), a3 = nib<1>(w1[g]);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g], a0, a1, a2, a3, pb[h][0], pb[h][1]);
+              const uint32_t b0 = nib<2>(w0[g]), b1 = nib<3>(w0[g]), b2 = nib<2>(w1[g]), b3 = nib<3>(w1[g]);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g + 1], b0, b1, b2, b3, pb[h][0], pb[h][1]);
+            }
+            if constexpr (TAIL) {
+              const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
+              const uint32_t r0 = __byte_perm(w, 0u, 0x4140), r1 = __byte_perm(w, 0u, 0x4342);
+#pragma unroll
+              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], nib<0>(r0), nib<1>(r0), nib<0>(r1), nib<1>(r1), pb[h][0], pb[h][1]);
+            }
+          }
+          __syncwarp();                                              // every lane has read the pair: its slot may be filled again
+          if (++slot == QD_STAGES) slot = 0;
         }
-        const uint8_t* vp = kp[j] + PB;
-        uint32_t w0[NG], w1[NG];
-        load_words<NG>(vp + lane * NG * 4, w0);
-        load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t a0 = nib<0>(w0[g]), a1 = nib<1>(w0[g]), a2 = nib<0>(w1[g]), a3 = nib<1>(w1[g]);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g], a0, a1, a2, a3, pb[h][0], pb[h][1]);
-          const uint32_t b0 = nib<2>(w0[g]), b1 = nib<3>(w0[g]), b2 = nib<2>(w1[g]), b3 = nib<3>(w1[g]);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g + 1], b0, b1, b2, b3, pb[h][0], pb[h][1]);
-        }
-        if constexpr (TAIL) {
-          const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
-          const uint32_t r0 = __byte_perm(w, 0u, 0x4140), r1 = __byte_perm(w, 0u, 0x4342);
-#pragma unroll
-          for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], nib<0>(r0), nib<1>(r0), nib<0>(r1), nib<1>(r1), pb[h][0], pb[h][1]);
-        }
-      }
-      if (i + QD_STAGES < n_my) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // this warp's reads of the slots come before the refill
-        __syncwarp();
-        issue(i + QD_STAGES);
-      }
-    }
-    taken += n_my;
 
-    // ---- join the warps -----------------------------------------------------------------------------------------------------
-    const float e0 = 262144.f / vf;
+        // ---- this warp's part of the tile ----
+        if (it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
+        const float e0 = 262144.f / vf;
 #pragma unroll
-    for (int h = 0; h < HN; ++h) {
+        for (int h = 0; h < HN; ++h) {
 #pragma unroll
-      for (int k = 4; k < 32; k <<= 1) { l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], k); om[h] += __shfl_xor_sync(0xFFFFFFFFu, om[h], k); }
-      if (4 * h + tq < gn) {
-        float* dst = sm.part[warp][4 * h + tq];
-        auto val = [&](int n, int k) { return fmaf(o[h][n][2 * k] + o[h][n][2 * k + 1], e0, om[h]); };
+          for (int k = 4; k < 32; k <<= 1) { l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], k); om[h] += __shfl_xor_sync(0xFFFFFFFFu, om[h], k); }
+          float* dst = sm.part[buf][warp][4 * h + tq];
+          auto val = [&](int n, int k) { return fmaf(o[h][n][2 * k] + o[h][n][2 * k + 1], e0, om[h]); };
 #pragma unroll
-        for (int g = 0; g < NG; ++g) *(float4*)(dst + 32 * g + 4 * gq) = make_float4(val(2 * g, 0), val(2 * g, 1), val(2 * g + 1, 0), val(2 * g + 1, 1));
-        if constexpr (TAIL) *(float2*)(dst + 32 * NG + 2 * gq) = make_float2(val(2 * NG, 0), val(2 * NG, 1));
-        if (gq == 0) { dst[D] = m[h]; dst[D + 1] = l[h]; }
+          for (int g = 0; g < NG; ++g) *(float4*)(dst + 32 * g + 4 * gq) = make_float4(val(2 * g, 0), val(2 * g, 1), val(2 * g + 1, 0), val(2 * g + 1, 1));
+          if constexpr (TAIL) *(float2*)(dst + 32 * NG + 2 * gq) = make_float2(val(2 * NG, 0), val(2 * NG, 1));
+          if (gq == 0) *(float2*)(dst + D) = make_float2(m[h], l[h]);
+        }
+      } else {                                                       // no page of this tile is mine
+        if (it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
+        if (lane < ROWS) *(float2*)(sm.part[buf][warp][lane] + D) = make_float2(-INFINITY, 0.f);
+      }
+      __syncwarp();
+      if (lane == 0) qd_arrive(&sm.part_full[buf]);
+      at = end;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+
+  QdTile now = qd_tile(p, b0, at0, x1 - x0);
+  // ================================== helper warps ================================================================================
+  const int hid = tid - 32 * NW, hw = hid >> 5;
+  const RopeArgs rope = {p.rope_table, p.rope_table_len, p.rope_dim, p.rope_type, p.rope_theta};
+  const int half = p.rope_dim >> 1;
+  const float qscale = p.scale * 1.4426950408889634f;
+  auto helpers_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(QD_HELPERS) : "memory"); };
+  // queries of a tile's heads (norm, rotation, split into fragments), and the new token's rows where its page is in my share
+  auto prepare = [&](const QdTile& t, int buf, int at) {
+    if (hid == 0)
+      sm.tile[buf] = {t.n, (t.s.first_page + t.skip) * Q4_PAGE, t.s.lo, t.s.pos, p.no_append || t.skip + t.n < t.s.pages ? -1 : at + t.n - 1};
+    const int kvh = t.tile / hgroups, g0 = (t.tile - kvh * hgroups) * ROWS, gn = min(ROWS, G - g0);
+    const float* row = p.qkv + (int64_t)t.b * p.ld_qkv;
+    float2 cs[NP];
+    load_rope<D>(rope, t.s.pos, lane, cs);
+    float xa[NP], xb[NP];
+    auto load = [&](const float* src, int hf, int type) {
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const int i = lane + 32 * k;
+        xa[k] = xb[k] = 0.f;
+        if (i < D / 2) { const int2 at = pair_dims(i, hf, type); xa[k] = src[at.x]; xb[k] = src[at.y]; }
+      }
+    };
+    for (int g = hw; g < ROWS; g += QD_HELPERS / 32) {
+      float f = 1.f, sum = 0.f;
+      if (g < gn) {
+        load(row + p.q_off + (int64_t)(kvh * G + g0 + g) * D, half, p.rope_type);
+        norm_rope_f<D>(xa, xb, p.q_norm_w, p.eps, rope, cs, lane);
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          xa[k] *= qscale; xb[k] *= qscale;
+          top = fmaxf(top, fmaxf(fabsf(xa[k]), fabsf(xb[k]))); sum += xa[k] + xb[k];
+        }
+        top = warp_max(top); sum = warp_sum(sum);
+        f = top > 0.f ? pow2_for(top, 13) : 1.f;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          const int i = lane + 32 * k;
+          if (i < D / 2) { const int2 at = pair_dims(i, half, p.rope_type); sm.q[g][at.x] = xa[k] * f; sm.q[g][at.y] = xb[k] * f; }
+        }
+      }
+      if (lane == 0) { sm.qc[buf][g] = g < gn ? 262144.f / f : 0.f; sm.qx[buf][g] = sum; }
+    }
+    if (!p.no_append && t.skip + t.n == t.s.pages && hw >= 2) {
+      const bool v = hw == 3;
+      load(row + (v ? p.v_off : p.k_off) + kvh * D, v ? 0 : half, v ? 0 : p.rope_type);
+      if (!v) norm_rope_d<D>(xa, xb, p.q_norm_w ? p.k_norm_w : nullptr, (double)p.eps, rope, cs, lane);
+      const uint32_t meta = q4_quantise<D>(xa, xb, v ? 0 : half, v ? 0 : p.rope_type, lane, sm.codes[buf][v]);
+      __syncwarp();
+      if (lane == 0) sm.meta[buf][v] = meta;
+      if (g0 == 0) {                                               // one head group writes the row
+        const int raw = p.page_table[(int64_t)t.b * p.pt_stride + t.s.pos / Q4_PAGE];
+        if (p.num_pages <= 0 || (unsigned)raw < (unsigned)p.num_pages) {
+          uint8_t* dst = (uint8_t*)(v ? p.v_cache : p.k_cache) + ((int64_t)raw * p.n_kv_heads + kvh) * PB;
+          if (v) q4_store_v<D>(dst, t.s.pos % Q4_PAGE, sm.codes[buf][1], meta, lane);
+          else q4_store_k<D>(dst, t.s.pos % Q4_PAGE, sm.codes[buf][0], meta, lane);
+        }
       }
     }
-    __syncthreads();
-    const bool whole = n_units == s.units;
-    float* out = p.out + (int64_t)b * p.ld_out + (int64_t)(kvh * G + g0) * D;
-    // slots of a CTA in scratch: 0 the tile its units begin in, 1 the one they end in
-    float* parts = p.partial + (int64_t)(2 * c + (u == u0 ? 0 : 1)) * QD_ROWS * (D + 4);
-    for (int it = tid; it < gn * (D / 4); it += QD_THREADS) {
-      const int g = it / (D / 4), j = 4 * (it - g * (D / 4));
+    helpers_sync();
+    // column gq is head gq / 2 of a tile, its fp16 head (even) or what that leaves (odd).  Word tq of a group of 32 dims holds dims
+    // 8 tq .. + 7 and its nibbles pair as (0, 4), (1, 5), (2, 6), (3, 7)
+    const uint32_t sel = gq & 1 ? 0x7632u : 0x5410u;
+    for (int f = hw; f < HN * KS; f += QD_HELPERS / 32) {
+      const int h = f / KS, ks = f - h * KS, head = 4 * h + (gq >> 1);
+      const float* qr = sm.q[head < gn ? head : 0];
+      auto frag = [&](int d0, int d1) { return head < gn ? __byte_perm(split_f16(qr[d0]), split_f16(qr[d1]), sel) : 0u; };
+      const int d = ks < 2 * NG ? 16 * (ks & ~1) + 8 * tq + 2 * (ks & 1) : 32 * NG + 4 * tq;
+      sm.frag[buf][h][ks][lane] = ks < 2 * NG ? make_uint2(frag(d, d + 4), frag(d + 1, d + 5)) : make_uint2(frag(d, d + 1), frag(d + 2, d + 3));
+    }
+    qd_arrive(&sm.frag_full[buf]);
+  };
+
+  prepare(now, 0, 0);
+  QdTile next;
+  for (int it = 0, at = 0; at < x1 - x0; ++it) {
+    const int end = at + now.n, buf = it & 1;
+    const bool more = end < x1 - x0;
+    if (more) {
+      next = qd_next(p, now, tiles, x1 - x0 - end);
+      helpers_sync();                                              // the fragments before are made: the staging rows are free
+      prepare(next, buf ^ 1, end);
+    }
+    ok = qd_wait(&sm.part_full[buf], (uint32_t)(it >> 1) & 1u, ok) && ok;
+    const int tile = now.tile, kvh = tile / hgroups, g0 = (tile - kvh * hgroups) * ROWS, gn = min(ROWS, G - g0);
+    const bool whole = now.n == now.s.pages;
+    float* out = p.out + (int64_t)now.b * p.ld_out + (int64_t)(kvh * G + g0) * D;
+    // slots of a CTA in scratch: 0 the tile its pages begin in, 1 the one they end in
+    float* parts = p.partial + (int64_t)(2 * c + (it == 0 ? 0 : 1)) * ROWS * (D + 4);
+    for (int i = hid; i < gn * (D / 4); i += QD_HELPERS) {
+      const int g = i / (D / 4), j = 4 * (i - g * (D / 4));
       float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < QD_WARPS; ++w) mm = fmaxf(mm, sm.part[w][g][D]);
+      for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sm.part[buf][w][g][D]);
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < QD_WARPS; ++w) {
-        const float mw = sm.part[w][g][D], e = mw == -INFINITY ? 0.f : ex2(mw - mm);
-        const float4 v = *(const float4*)&sm.part[w][g][j];
-        ll = fmaf(e, sm.part[w][g][D + 1], ll);
+      for (int w = 0; w < NW; ++w) {
+        const float2 st = *(const float2*)&sm.part[buf][w][g][D];
+        if (st.x == -INFINITY) continue;
+        const float e = ex2(st.x - mm);
+        const float4 v = *(const float4*)&sm.part[buf][w][g][j];
+        ll = fmaf(e, st.y, ll);
         a.x = fmaf(e, v.x, a.x); a.y = fmaf(e, v.y, a.y); a.z = fmaf(e, v.z, a.z); a.w = fmaf(e, v.w, a.w);
       }
       if (whole) {
@@ -427,34 +503,35 @@ __global__ void __launch_bounds__(QD_THREADS, qd_occupancy(HN)) attn_decode_q4_k
       } else {
         float* dst = parts + g * (D + 4);
         *(float4*)(dst + j) = a;
-        if (j == 0) { dst[D] = mm; dst[D + 1] = ll; }
+        if (j == 0) *(float2*)(dst + D) = make_float2(mm, ll);
       }
     }
+    helpers_sync();                                                // the parts are read, and what goes to scratch is written
+    if (hid == 0) qd_arrive(&sm.part_empty[buf]);
     if (!whole) {
-      // CTA that holds unit x: the largest c with c total / ctas <= x
-      const int c_lo = (int)(((int64_t)(tile_u0 + 1) * ctas - 1) / total), c_hi = (int)(((int64_t)(tile_u0 + s.units) * ctas - 1) / total);
-      __threadfence();
-      __syncthreads();
-      int32_t* ctr = p.counters + (int64_t)b * tiles + tile;
-      if (tid == 0) {
-        sm.last = atomicAdd(ctr, 1) == c_hi - c_lo;
-        if (sm.last) *ctr = 0;                                   // zero again for the next launch
-      }
-      __syncthreads();
-      if (sm.last) {
+      // CTA that has place x of the share of all: the largest c with c total / ctas <= x
+      const int t0 = x0 + at - now.skip;
+      const int c_lo = (int)(((int64_t)(t0 + 1) * ctas - 1) / total), c_hi = (int)(((int64_t)(t0 + now.s.pages) * ctas - 1) / total);
+      if (hid == 0) {
+        int32_t* ctr = p.counters + (int64_t)now.b * tiles + tile;
         __threadfence();
-        const int lead = (int)((int64_t)c_lo * total / ctas) == tile_u0 ? 0 : 1;
-        for (int it = tid; it < gn * (D / 4); it += QD_THREADS) {
-          const int g = it / (D / 4), j = 4 * (it - g * (D / 4));
+        sm.last = atomicAdd(ctr, 1) == c_hi - c_lo;
+        if (sm.last) { *ctr = 0; __threadfence(); }                // zero again for the next launch
+      }
+      helpers_sync();
+      if (sm.last) {
+        const int lead = (int)((int64_t)c_lo * total / ctas) == t0 ? 0 : 1;
+        for (int i = hid; i < gn * (D / 4); i += QD_HELPERS) {
+          const int g = i / (D / 4), j = 4 * (i - g * (D / 4));
           float mm = -INFINITY, ll = 0.f;
           float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int k0 = c_lo; k0 <= c_hi; k0 += 8) {
+          for (int q0 = c_lo; q0 <= c_hi; q0 += 8) {
             float2 st[8];
             float4 v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const int kc = min(k0 + k, c_hi);
-              const float* src = p.partial + ((int64_t)(2 * kc + (kc == c_lo ? lead : 0)) * QD_ROWS + g) * (D + 4);
+              const int kc = min(q0 + k, c_hi);
+              const float* src = p.partial + ((int64_t)(2 * kc + (kc == c_lo ? lead : 0)) * ROWS + g) * (D + 4);
               st[k] = __ldcg((const float2*)(src + D));
               v[k] = __ldcg((const float4*)(src + j));
             }
@@ -465,7 +542,7 @@ __global__ void __launch_bounds__(QD_THREADS, qd_occupancy(HN)) attn_decode_q4_k
             a.x *= c0; a.y *= c0; a.z *= c0; a.w *= c0; ll *= c0; mm = mn;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float e = k0 + k > c_hi || st[k].x == -INFINITY ? 0.f : ex2(st[k].x - mm);
+              const float e = q0 + k > c_hi || st[k].x == -INFINITY ? 0.f : ex2(st[k].x - mm);
               ll = fmaf(e, st[k].y, ll);
               a.x = fmaf(e, v[k].x, a.x); a.y = fmaf(e, v[k].y, a.y); a.z = fmaf(e, v[k].z, a.z); a.w = fmaf(e, v[k].w, a.w);
             }
@@ -475,10 +552,8 @@ __global__ void __launch_bounds__(QD_THREADS, qd_occupancy(HN)) attn_decode_q4_k
         }
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();                                             // the staging areas and the rings are free for the next tile
-    u += n_units; rem += n_units;
-    if (rem == s.units * tiles) { ++b; rem = 0; }
+    at = end;
+    if (more) now = next;
   }
 }
 
@@ -488,11 +563,11 @@ static int launch_decode_q4(const AttnDecodeParams& p, cudaStream_t st) {
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const int hgroups = (p.n_heads / p.n_kv_heads + qd_heads(HN) - 1) / qd_heads(HN);
   const long long tiles = (long long)p.batch * p.n_kv_heads * hgroups;
-  const int ctas = (int)std::min<long long>(std::min(sms, QD_MAX_SMS) * qd_occupancy(HN), tiles * QD_MAX_PARTS);
-  const size_t ring = (size_t)QD_WARPS * QD_STAGES * 2 * q4_page_bytes(D);
+  const int ctas = (int)std::min<long long>(std::min(sms, QD_MAX_SMS), tiles * QD_MAX_PARTS);
+  const size_t smem = (sizeof(QdSmem<D, HN>) + 127) / 128 * 128 + (size_t)qd_warps(HN) * QD_STAGES * 4 * q4_page_bytes(D);
   static SmemOptIn opt;
-  if (cudaError_t e = opt.ensure(attn_decode_q4_kernel<D, HN>, ring, 0); e != cudaSuccess) return (int)e;
-  return (int)launch(attn_decode_q4_kernel<D, HN>, dim3(ctas), dim3(QD_THREADS), ring, st, p);
+  if (cudaError_t e = opt.ensure(attn_decode_q4_kernel<D, HN>, smem, 0); e != cudaSuccess) return (int)e;
+  return (int)launch(attn_decode_q4_kernel<D, HN>, dim3(ctas), dim3(32 * qd_warps(HN) + QD_HELPERS), smem, st, p);
 }
 
 int attn_decode_q4_dispatch(const AttnDecodeParams& p, cudaStream_t st) {
@@ -517,7 +592,7 @@ extern "C" {
 // floats of scratch (`partial`) that any launch over a 4-bit cache needs
 long long rlz_attn_q4_partial_floats(int head_dim) { 
   using namespace rlz;
-  return 2LL * QD_MAX_SMS * std::max(qd_occupancy(1) * qd_heads(1), qd_occupancy(2) * qd_heads(2)) * (head_dim + 4);
+  return 2LL * QD_MAX_SMS * qd_heads(2) * (head_dim + 4);
 }
 
 // 0 / 3211 / 3311 / 3312
