@@ -22,9 +22,10 @@
 // and store the finished tile meanwhile, through two buffers each.
 // (With every warp doing its share of that between two tiles, a batch of 64 x 2048 tokens spent 28 of its 60 us there.)
 //
-// Split: the pages of all (sequence, kv head, head group) tiles are divided evenly over the CTAs, whatever the lengths are;
-// positions are read on the device, so a captured launch serves growing sequences.  A CTA that has only some pages of a tile
-// leaves its part in scratch, and the last of the tile's CTAs to arrive joins them in a fixed order.
+// Split, in pairs of pages: with more tiles (sequence, kv head, head group) than CTAs, the pairs of all tiles are divided evenly,
+// whatever the lengths are; with fewer, every tile gets the same number of CTAs, unless that leaves one of them with much more
+// than an even share.  Positions are read on the device, so a captured launch serves growing sequences.  A CTA that has only some
+// pairs of a tile leaves its part in scratch, and the last of the tile's CTAs to arrive joins them in a fixed order.
 #include "attention_q4.cuh"
 #include "kv_q4.cuh"
 #include <algorithm>
@@ -36,6 +37,8 @@ namespace rlz {
 __device__ int g_attn_q4_error = 0;
 
 constexpr int QD_STAGES = 3, QD_MAX_SMS = 148, QD_HELPERS = 128;
+constexpr int QD_PAIR = 2 * Q4_PAGE;          // tokens of a pair of pages
+constexpr int QD_TILE_COST = 40;              // a second tile costs a CTA about as much time as this many pairs
 constexpr int QD_MAX_PARTS = 64;              // CTAs that share a tile: bounds the time of the last one, which joins their parts
 // query heads of a CTA (HN tiles of 4) and its main warps: with the four others 16 warps of 128 registers, or 12 of 168
 constexpr int qd_heads(int hn) { return 4 * hn; }
@@ -49,7 +52,7 @@ template <int D, int HN> struct QdSmem {
   float qc[2][ROWS], qx[2][ROWS];             // 2^18 / f of a head whose fragments hold q f, and the sum of q
   uint8_t codes[2][2][D];                     // the new token's rows (key, value)
   uint32_t meta[2][2];
-  struct { int n, tok, lo, pos, own; } tile[2];   // pages, first token, first and last visible position, place of the new token's page or -1
+  struct { int n, tok, lo, pos, own; } tile[2];   // pairs, first token, first and last visible position, place of the new token's pair or -1
   int last;
   unsigned long long frag_full[2], part_full[2], part_empty[2];
 };
@@ -92,28 +95,28 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* src, 
   }
 }
 
-struct QdSeq { int pos, lo, first_page, pages; };             // pages first_page .. first_page + pages - 1; 0 pages: nothing to do
+struct QdSeq { int pos, lo, first_page, n; };                 // n pairs of pages from first_page on; 0: nothing to do
 __device__ __forceinline__ QdSeq qd_seq(const AttnDecodeParams& p, int b) {
   QdSeq s = {p.positions[b], 0, 0, 0};
   if (s.pos < 0) return s;
   if (s.pos / Q4_PAGE >= p.max_pages) { atomicExch(&g_attn_q4_error, 3311); return s; }
   s.lo = p.window > 0 ? max(0, s.pos + 1 - p.window) : 0;
   s.first_page = s.lo / Q4_PAGE;
-  s.pages = s.pos / Q4_PAGE + 1 - s.first_page;
+  s.n = (s.pos / Q4_PAGE - s.first_page) / 2 + 1;
   return s;
 }
-// the pages of one tile that a CTA has: `n` of them from the tile's page `skip` on
+// the pairs of one tile that a CTA has: `n` of them from the tile's pair `skip` on
 struct QdTile { QdSeq s; int b, tile, skip, n; };
-// the tile that page `at` of sequence b's tiles (or the next sequence with any) lies in; the CTA has `left` more pages
+// the tile that pair `at` of sequence b's tiles (or the next sequence with any) lies in; the CTA has `left` more pairs
 __device__ __forceinline__ QdTile qd_tile(const AttnDecodeParams& p, int b, int at, int left) {
   QdTile t;
-  for (;; ++b, at = 0) { t.s = qd_seq(p, b); if (t.s.pages) break; }
-  t.b = b; t.tile = at / t.s.pages; t.skip = at - t.tile * t.s.pages; t.n = min(t.s.pages - t.skip, left);
+  for (;; ++b, at = 0) { t.s = qd_seq(p, b); if (t.s.n) break; }
+  t.b = b; t.tile = at / t.s.n; t.skip = at - t.tile * t.s.n; t.n = min(t.s.n - t.skip, left);
   return t;
 }
 __device__ __forceinline__ QdTile qd_next(const AttnDecodeParams& p, const QdTile& t, int tiles, int left) {
   const bool new_seq = t.tile + 1 == tiles;
-  return qd_tile(p, new_seq ? t.b + 1 : t.b, new_seq ? 0 : (t.tile + 1) * t.s.pages, left);
+  return qd_tile(p, new_seq ? t.b + 1 : t.b, new_seq ? 0 : (t.tile + 1) * t.s.n, left);
 }
 // bounded: false (and the status word) when the barrier's phase does not end
 __device__ __forceinline__ bool qd_wait(unsigned long long* bar, uint32_t parity, bool patient) {
@@ -143,29 +146,45 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- my share: pages [x0, x1) of the sequence of all tiles' pages.  Every warp works it out, its lanes over the sequences -----
+  // ---- my share: pairs [x0, x1) of the sequence of all tiles' pairs.  Every warp works it out, its lanes over the sequences ------
   const int G = p.n_heads / p.n_kv_heads, hgroups = (G + ROWS - 1) / ROWS, tiles = p.n_kv_heads * hgroups;
   const int per = (p.batch + 31) / 32, b_lo = min(lane * per, p.batch), b_hi = min(b_lo + per, p.batch);
-  int mine = 0, live = 0;
-  for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, b).pages; mine += n * tiles; live += n > 0; }
-  int incl = mine;
+  int mine = 0, live = 0, longest = 0;
+  for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, b).n; mine += n; live += n > 0; longest = max(longest, n); }
+  int incl = mine, live_incl = live;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o); if (lane >= o) incl += v; }
-  const int total = __shfl_sync(0xFFFFFFFFu, incl, 31), before = incl - mine;
-  live = __reduce_add_sync(0xFFFFFFFFu, live);
-  // as many CTAs as there are tiles, and more as long as each warp of them has a page
-  const int ctas = min((int)gridDim.x, max(live * tiles, (total + NW - 1) / NW)), c = blockIdx.x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o), w = __shfl_up_sync(0xFFFFFFFFu, live_incl, o);
+    if (lane >= o) { incl += v; live_incl += w; }
+  }
+  const int total = __shfl_sync(0xFFFFFFFFu, incl, 31) * tiles, all_tiles = __shfl_sync(0xFFFFFFFFu, live_incl, 31) * tiles, c = blockIdx.x;
+  if (total == 0) return;
+  longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+  const int split = min((int)gridDim.x / all_tiles, longest);     // CTAs to a tile, 0: there are more tiles
+  const bool by_tile = split > 0 && (longest + split - 1) / split < total / (int)gridDim.x + QD_TILE_COST;
+  const int ctas = by_tile ? all_tiles * split : min((int)gridDim.x, total);
   if (c >= ctas) return;
-  const int x0 = (int)((int64_t)c * total / ctas), x1 = (int)((int64_t)(c + 1) * total / ctas);
-  const bool holds = before <= x0 && x0 < incl;                  // one lane
-  int b0 = b_lo, at0 = x0 - before;
-  if (holds) for (;; ++b0) { const int n = qd_seq(p, b0).pages * tiles; if (at0 < n) break; at0 -= n; }
+  int x0 = (int)((int64_t)c * total / ctas), x1 = (int)((int64_t)(c + 1) * total / ctas);
+  // the lane whose sequences hold place x0, or (by tile) live tile c / split
+  const int want = by_tile ? c / split : x0, first = by_tile ? (live_incl - live) * tiles : (incl - mine) * tiles;
+  const bool holds = first <= want && want < (by_tile ? live_incl : incl) * tiles;
+  int b0 = b_lo, at0 = want - first;
+  if (holds)
+    for (;; ++b0) {
+      const int n = qd_seq(p, b0).n, m = (by_tile ? n > 0 : n) * tiles;
+      if (at0 < m) { if (by_tile) at0 *= n; break; }
+      at0 -= m;
+    }
   const int holder = __ffs(__ballot_sync(0xFFFFFFFFu, holds)) - 1;
   b0 = __shfl_sync(0xFFFFFFFFu, b0, holder);
   at0 = __shfl_sync(0xFFFFFFFFu, at0, holder);
-  // Page k of main warp w is page w + NW k of the CTA's share: the tiles' ends fall on all warps alike.  A warp's pages of a tile go
-  // through its ring two at a time, of an odd number the last alone.
-  auto first_k = [](int w, int x) { return x > w ? (x - w + NW - 1) / NW : 0; };        // first page of warp w at or behind place x of the share
+  if (by_tile) {                                                   // places count from the tile's first pair
+    const int n = qd_seq(p, b0).n, parts = min(split, n), part = c % split;
+    if (part >= parts) return;
+    x0 = part * n / parts; x1 = (part + 1) * n / parts; at0 += x0;
+  }
+  // Pair k of main warp w is pair w + NW k of the CTA's share: the tiles' ends fall on all warps alike.
+  auto first_k = [](int w, int x) { return x > w ? (x - w + NW - 1) / NW : 0; };        // first pair of warp w at or behind place x of the share
   bool ok = true;
 
   if (warp < NW) {
@@ -174,7 +193,6 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     // -- the copies: pair after pair of the stream, their page ids read one pair ahead
     QdTile f = qd_tile(p, b0, at0, x1 - x0);
     int f_at = 0, f_k = 0, f_k1 = first_k(warp, f.n), f_id[2], f_np = 0, f_kvh = f.tile / hgroups;
-    const int32_t* f_pt = p.page_table + (int64_t)f.b * p.pt_stride + f.s.first_page + f.skip + warp;
     auto look_up = [&]() {
       f_np = 0;
       while (f_k >= f_k1) {                                          // none left in this tile
@@ -182,28 +200,26 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
         if (f_at >= x1 - x0) return;
         f = qd_next(p, f, tiles, x1 - x0 - f_at);
         f_k1 = first_k(warp, f_at + f.n); f_kvh = f.tile / hgroups;
-        f_pt = p.page_table + (int64_t)f.b * p.pt_stride + f.s.first_page + f.skip + warp - f_at;
       }
-      f_np = min(2, f_k1 - f_k);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) f_id[j] = __ldg(f_pt + NW * (f_k + min(j, f_np - 1)));
-      f_k += f_np;
+      const int page = f.s.first_page + 2 * (f.skip + warp + NW * f_k - f_at), last = f.s.pos / Q4_PAGE;
+      const int32_t* pt = p.page_table + (int64_t)f.b * p.pt_stride;
+      f_np = min(2, last - page + 1);
+      f_id[0] = __ldg(pt + page); f_id[1] = __ldg(pt + min(page + 1, last));
+      ++f_k;
     };
     auto copy_pair = [&](uint32_t to) {
-      if (f_np) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (j < f_np) {
-            const int64_t off = ((int64_t)q4_page_id(f_id[j], p.num_pages) * p.n_kv_heads + f_kvh) * PB + 16 * lane;
-            const uint32_t dst = att_smem_u32(my_ring) + to * (4 * PB) + j * (2 * PB) + 16 * lane;
+      for (int j = 0; j < 2; ++j) {
+        if (j < f_np) {
+          const int64_t off = ((int64_t)q4_page_id(f_id[j], p.num_pages) * p.n_kv_heads + f_kvh) * PB + 16 * lane;
+          const uint32_t dst = att_smem_u32(my_ring) + to * (4 * PB) + j * (2 * PB) + 16 * lane;
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              const uint8_t* src = (const uint8_t*)(v ? p.v_cache : p.k_cache) + off;
+          for (int v = 0; v < 2; ++v) {
+            const uint8_t* src = (const uint8_t*)(v ? p.v_cache : p.k_cache) + off;
 #pragma unroll
-              for (int i = 0; i < (PB + 511) / 512; ++i)
-                if (512 * (i + 1) <= PB || 512 * i + 16 * lane < PB)
-                  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * PB + 512 * i), "l"(src + 512 * i) : "memory");
-            }
+            for (int i = 0; i < (PB + 511) / 512; ++i)
+              if (512 * (i + 1) <= PB || 512 * i + 16 * lane < PB)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * PB + 512 * i), "l"(src + 512 * i) : "memory");
           }
         }
       }
@@ -220,7 +236,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       const auto s = sm.tile[buf];
       const int end = at + s.n, k0 = first_k(warp, at), k1 = first_k(warp, end);
       if (k0 < k1) {
-        const int own = s.own >= 0 && s.own % NW == warp ? s.own / NW : 1 << 30;        // my page that holds the new token
+        const int own = s.own >= 0 && s.own % NW == warp ? s.own / NW : -1;              // my pair that holds the new token
         uint32_t qb[HN][KS][2];
         float qc[HN], qx[HN];
 #pragma unroll
@@ -237,16 +253,16 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           m[h] = -INFINITY; l[h] = om[h] = 0.f;
         }
         float vf = 0x1p100f;                                        // power of two that p x scale' carries
-        int tok = s.tok + (warp + NW * k0 - at) * Q4_PAGE;           // first token of page k
+        int tok = s.tok + (warp + NW * k0 - at) * QD_PAIR;           // first token of pair k
 
-        for (int k = k0; k < k1; k += 2, tok += 2 * NW * Q4_PAGE) {   // two pages at a time (of an odd number, the last comes with a masked one)
+        for (int k = k0; k < k1; ++k, tok += NW * QD_PAIR) {          // (of an odd number of pages the last comes with a masked one)
           copy_pair(slot == 0 ? QD_STAGES - 1 : slot - 1);            // into the slot that the pair before this one left
           look_up();
           asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
           __syncwarp();
           uint8_t* const kp[2] = {my_ring + slot * (4 * PB), my_ring + slot * (4 * PB) + 2 * PB};
-          if (own - k < 2 && own >= k) {                             // the copy may have passed the write of the new row
-            uint8_t* page = own == k ? kp[0] : kp[1];
+          if (own == k) {                                            // the copy may have passed the write of the new row
+            uint8_t* page = s.pos - tok < Q4_PAGE ? kp[0] : kp[1];
             q4_store_k<D>(page, s.pos % Q4_PAGE, sm.codes[buf][0], sm.meta[buf][0], lane);
             q4_store_v<D>(page + PB, s.pos % Q4_PAGE, sm.codes[buf][1], sm.meta[buf][1], lane);
             __syncwarp();
@@ -288,13 +304,13 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
               for (int h = 0; h < HN; ++h) sc[h][j][n] = fmaf((acc[j][h][2 * n] + acc[j][h][2 * n + 1]) * qc[h], q4_scale(km), q4_min(km) * qx[h]);
             }
           }
-          if (k + 1 >= k1 || tok < s.lo || tok + (NW + 1) * Q4_PAGE - 1 > s.pos) {       // rows outside the window or behind the last token hold anything
+          if (tok < s.lo || tok + QD_PAIR - 1 > s.pos) {     // rows outside the window or behind the last token hold anything
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
-                const int t = tok + j * NW * Q4_PAGE + gq + 8 * n;
-                if (k + j >= k1 || t < s.lo || t > s.pos) {
+                const int t = tok + j * Q4_PAGE + gq + 8 * n;
+                if (t < s.lo || t > s.pos) {
                   sv[j][n] = mv[j][n] = 0.f;
 #pragma unroll
                   for (int h = 0; h < HN; ++h) sc[h][j][n] = -INFINITY;
@@ -401,7 +417,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   // queries of a tile's heads (norm, rotation, split into fragments), and the new token's rows where its page is in my share
   auto prepare = [&](const QdTile& t, int buf, int at) {
     if (hid == 0)
-      sm.tile[buf] = {t.n, (t.s.first_page + t.skip) * Q4_PAGE, t.s.lo, t.s.pos, p.no_append || t.skip + t.n < t.s.pages ? -1 : at + t.n - 1};
+      sm.tile[buf] = {t.n, (t.s.first_page + 2 * t.skip) * Q4_PAGE, t.s.lo, t.s.pos, p.no_append || t.skip + t.n < t.s.n ? -1 : at + t.n - 1};
     const int kvh = t.tile / hgroups, g0 = (t.tile - kvh * hgroups) * ROWS, gn = min(ROWS, G - g0);
     const float* row = p.qkv + (int64_t)t.b * p.ld_qkv;
     float2 cs[NP];
@@ -436,7 +452,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       }
       if (lane == 0) { sm.qc[buf][g] = g < gn ? 262144.f / f : 0.f; sm.qx[buf][g] = sum; }
     }
-    if (!p.no_append && t.skip + t.n == t.s.pages && hw >= 2) {
+    if (!p.no_append && t.skip + t.n == t.s.n && hw >= 2) {
       const bool v = hw == 3;
       load(row + (v ? p.v_off : p.k_off) + kvh * D, v ? 0 : half, v ? 0 : p.rope_type);
       if (!v) norm_rope_d<D>(xa, xb, p.q_norm_w ? p.k_norm_w : nullptr, (double)p.eps, rope, cs, lane);
@@ -478,9 +494,9 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     }
     ok = qd_wait(&sm.part_full[buf], (uint32_t)(it >> 1) & 1u, ok) && ok;
     const int tile = now.tile, kvh = tile / hgroups, g0 = (tile - kvh * hgroups) * ROWS, gn = min(ROWS, G - g0);
-    const bool whole = now.n == now.s.pages;
+    const bool whole = now.n == now.s.n;
     float* out = p.out + (int64_t)now.b * p.ld_out + (int64_t)(kvh * G + g0) * D;
-    // slots of a CTA in scratch: 0 the tile its pages begin in, 1 the one they end in
+    // slots of a CTA in scratch: 0 the tile its pairs begin in, 1 the one they end in
     float* parts = p.partial + (int64_t)(2 * c + (it == 0 ? 0 : 1)) * ROWS * (D + 4);
     for (int i = hid; i < gn * (D / 4); i += QD_HELPERS) {
       const int g = i / (D / 4), j = 4 * (i - g * (D / 4));
@@ -509,9 +525,10 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     helpers_sync();                                                // the parts are read, and what goes to scratch is written
     if (hid == 0) qd_arrive(&sm.part_empty[buf]);
     if (!whole) {
-      // CTA that has place x of the share of all: the largest c with c total / ctas <= x
+      // by tile, the CTAs are neighbours; else CTA that has place x of all: the largest c with c total / ctas <= x
       const int t0 = x0 + at - now.skip;
-      const int c_lo = (int)(((int64_t)(t0 + 1) * ctas - 1) / total), c_hi = (int)(((int64_t)(t0 + now.s.pages) * ctas - 1) / total);
+      const int c_lo = by_tile ? c - c % split : (int)(((int64_t)(t0 + 1) * ctas - 1) / total);
+      const int c_hi = by_tile ? c_lo + min(split, now.s.n) - 1 : (int)(((int64_t)(t0 + now.s.n) * ctas - 1) / total);
       if (hid == 0) {
         int32_t* ctr = p.counters + (int64_t)now.b * tiles + tile;
         __threadfence();
@@ -520,7 +537,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       }
       helpers_sync();
       if (sm.last) {
-        const int lead = (int)((int64_t)c_lo * total / ctas) == t0 ? 0 : 1;
+        const int lead = by_tile || (int)((int64_t)c_lo * total / ctas) == t0 ? 0 : 1;
         for (int i = hid; i < gn * (D / 4); i += QD_HELPERS) {
           const int g = i / (D / 4), j = 4 * (i - g * (D / 4));
           float mm = -INFINITY, ll = 0.f;
