@@ -4,16 +4,17 @@
 //   s_t = q . k_t = scale_t (q . code_t) + min_t sum(q)        o = sum_t p_t v_t = sum_t (p_t scale'_t) code'_t + sum_t p_t min'_t
 //
 // Bound by the bytes of the cache.  What a page costs besides them:
-//   * Codes are never turned into numbers.  A nibble moved to bits 6..9 of an fp16 is the subnormal code x 2^-18, and mma.sync
-//     multiplies subnormals exactly: a shift and an AND to two codes instead of a conversion and a multiply-add each.  (The unit
-//     lines products up by the exponent fields, so that a nibble left at the low bits, code x 2^-24 without the shift, costs the
-//     sum as many bits as stand empty above it: 2e-5 of the result where this gives 3e-7.)
-//   * The pages lie in fragment order, so a lane takes its operands with one wide shared-memory load and no shuffles.
-//   * Keys (16 tokens) and values (16 dims) are the A operand and the heads the 8 columns of B: 4 heads, each as the fp16 head of
-//     its value and what that leaves, also fp16.  22 bits of q and of p x scale' at the price of 11, and the two products of a
-//     head meet in one lane.  Up to 4 heads take one such tile, up to 8 two, sharing the A operand.  (Heads as rows, 8 + 8 of
-//     16, took twice the instructions and registers for 4 heads: 46 us for every 65536 pages of 128, this STEP2.)
-//     q is scaled by a power of two so that its largest value lies in [2^13, 2^14), p x scale' by one that follows the scales.
+// The arithmetic of the codes is what has to be cheap:
+//   * Keys: a masked word holds four codes as bytes, and the 8-bit integer product takes them as they are; q comes as three 8-bit
+//     digits of a 23-bit integer (its largest value in [2^21, 2^22)), so the sums over the dims are exact.
+//   * Values: a nibble moved to bits 6..9 of an fp16 is the subnormal code x 2^-18, which mma.sync multiplies exactly: a shift and an
+//     AND to two codes instead of a conversion and a multiply-add each.  (The unit lines products up by the exponent fields: a nibble
+//     left at the low bits, x 2^-24 without the shift, costs the sum as many bits as stand empty above it, 2e-5 of the result where
+//     this gives 3e-7.)  The right shifts are high halves of products, which leaves the busier integer pipe to the masks.
+//     p x scale' comes as its fp16 head and what that leaves, also fp16: 22 bits; its power of two follows the scales.
+//   * Tokens (keys) and dims (values) are the 16 rows of the instruction and 4 heads its 8 columns, two digits or halves each, so
+//     the parts of a head's sum meet in one lane.  Up to 8 heads take two such tiles and share the other operand.
+//   * The pages lie in fragment order: a lane takes its operands with one wide shared-memory load and no shuffles.
 //   * The running maximum moves only when a score passes it by 2^8, so that the accumulators are rarely rescaled.
 //
 // One CTA to an SM.  The main warps do nothing but pages: each has a ring of page pairs (K and V) that its lanes fill by 16-byte
@@ -45,11 +46,11 @@ constexpr int qd_heads(int hn) { return 4 * hn; }
 constexpr int qd_warps(int hn) { return hn == 1 ? 12 : 8; }
 
 template <int D, int HN> struct QdSmem {
-  static constexpr int KS = D / 16, ROWS = 4 * HN;
-  uint2 frag[2][HN][KS][32];                  // B fragments of the heads, as the main warps' lanes hold them
+  static constexpr int NF = D / 32 + (D % 32 ? 1 : 0), ROWS = 4 * HN;
+  uint4 frag[2][HN][NF][32];                  // digits 0 and 1 (x, y), 2 and none (z, w) of the heads, as the main warps' lanes hold them
   float part[2][qd_warps(HN)][ROWS][D + 4];   // per warp and head: sum, then maximum and weight
   float q[ROWS][D];                           // helpers: normalised, rotated and scaled queries
-  float qc[2][ROWS], qx[2][ROWS];             // 2^18 / f of a head whose fragments hold q f, and the sum of q
+  float qc[2][ROWS], qx[2][ROWS];             // 1 / f of a head whose fragments hold the integer q f, and the sum of q
   uint8_t codes[2][2][D];                     // the new token's rows (key, value)
   uint32_t meta[2][2];
   struct { int n, tok, lo, pos, own; } tile[2];   // pairs, first token, first and last visible position, place of the new token's pair or -1
@@ -65,9 +66,24 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// nibble J of both halves of a word as fp16 subnormals: code x 2^-18
-template <int J> __device__ __forceinline__ uint32_t nib(uint32_t w) {
-  return (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6) & 0x03C003C0u;
+// nibble J of both halves of a word as fp16 subnormals: code x 2^-18; one: the number 1, which the compiler must not know
+template <int J> __device__ __forceinline__ uint32_t nib(uint32_t w, uint32_t one) {
+  return (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? __umulhi(w, one << 30) : __umulhi(w, one << 26)) & 0x03C003C0u;
+}
+__device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_half(int* c, uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(b0));
+}
+// four codes of 16 bits as bytes
+__device__ __forceinline__ uint32_t nib_bytes(uint32_t h) { const uint32_t x = (h | h << 8) & 0x00FF00FFu; return (x | x << 4) & 0x0F0F0F0Fu; }
+// an integer below 2^22 as three signed bytes, the first in the low bits
+__device__ __forceinline__ uint32_t digits(int q) {
+  const int d2 = (int)(int8_t)(q & 255), q1 = (q - d2) >> 8, d1 = (int)(int8_t)(q1 & 255), d0 = (q1 - d1) >> 8;
+  return (uint32_t)(d0 & 255) | (uint32_t)(d1 & 255) << 8 | (uint32_t)(d2 & 255) << 16;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // fp16 head of a value (low half) and of what the head leaves (high half)
@@ -132,7 +148,7 @@ __device__ __forceinline__ void qd_arrive(unsigned long long* bar) {
 template <int D, int HN>
 __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode_q4_kernel(const __grid_constant__ AttnDecodeParams p) {
   constexpr int ROWS = 4 * HN, NW = qd_warps(HN);
-  constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, KS = 2 * NG + TAIL, NT = 2 * NG + TAIL, PB = q4_page_bytes(D), NP = HeadPairs<D>::NP;
+  constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, NF = NG + TAIL, NT = 2 * NG + TAIL, PB = q4_page_bytes(D), NP = HeadPairs<D>::NP;
   extern __shared__ __align__(128) uint8_t qd_smem[];
   QdSmem<D, HN>& sm = *(QdSmem<D, HN>*)qd_smem;
   uint8_t* qd_ring = qd_smem + (sizeof(QdSmem<D, HN>) + 127) / 128 * 128;
@@ -228,6 +244,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     look_up();
     for (int i = 0; i < QD_STAGES - 1; ++i) { copy_pair(i); look_up(); }
     uint32_t slot = 0;
+    const uint32_t one = gridDim.z;
     for (int it = 0, at = 0; at < x1 - x0; ++it) {
       const int buf = it & 1;
       const uint32_t phase = (uint32_t)(it >> 1) & 1u;
@@ -237,12 +254,12 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       const int end = at + s.n, k0 = first_k(warp, at), k1 = first_k(warp, end);
       if (k0 < k1) {
         const int own = s.own >= 0 && s.own % NW == warp ? s.own / NW : -1;              // my pair that holds the new token
-        uint32_t qb[HN][KS][2];
+        uint4 qb[HN][NF];
         float qc[HN], qx[HN];
 #pragma unroll
         for (int h = 0; h < HN; ++h) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) { const uint2 f = sm.frag[buf][h][ks][lane]; qb[h][ks][0] = f.x; qb[h][ks][1] = f.y; }
+          for (int f = 0; f < NF; ++f) qb[h][f] = sm.frag[buf][h][f][lane];
           qc[h] = sm.qc[buf][4 * h + tq]; qx[h] = sm.qx[buf][4 * h + tq];
         }
         float o[HN][NT][4], m[HN], l[HN], om[HN];                  // om: sum of p x min'
@@ -268,40 +285,37 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
             __syncwarp();
           }
           // ---- scores: lane has tokens gq and gq + 8 of head tq of a tile ----
-          float acc[2][HN][4], sc[HN][2][2], sv[2][2], mv[2][2];
+          float sc[HN][2][2], sv[2][2], mv[2][2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int h = 0; h < HN; ++h) acc[j][h][0] = acc[j][h][1] = acc[j][h][2] = acc[j][h][3] = 0.f;
+            int hi[HN][4] = {}, lo[HN][4] = {};                        // digits 0 and 1 of tokens gq and gq + 8, digit 2
             uint32_t wa[NG], wb[NG];
             load_words<NG>(kp[j] + gq * (D / 2) + tq * NG * 4, wa);
             load_words<NG>(kp[j] + (gq + 8) * (D / 2) + tq * NG * 4, wb);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              const uint32_t a0 = nib<0>(wa[g]), a1 = nib<0>(wb[g]), a2 = nib<1>(wa[g]), a3 = nib<1>(wb[g]);
+              const uint32_t a0 = wa[g] & 0x0F0F0F0Fu, a1 = wb[g] & 0x0F0F0F0Fu, a2 = wa[g] >> 4 & 0x0F0F0F0Fu, a3 = wb[g] >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * g][0], qb[h][2 * g][1]);
-              const uint32_t b0 = nib<2>(wa[g]), b1 = nib<2>(wb[g]), b2 = nib<3>(wa[g]), b3 = nib<3>(wb[g]);
-#pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], b0, b1, b2, b3, qb[h][2 * g + 1][0], qb[h][2 * g + 1][1]);
+              for (int h = 0; h < HN; ++h) {
+                mma_s8(hi[h], a0, a1, a2, a3, qb[h][g].x, qb[h][g].y);
+                mma_s8(lo[h], a0, a1, a2, a3, qb[h][g].z, qb[h][g].w);
+              }
             }
             if constexpr (TAIL) {
               const uint8_t* kt = kp[j] + 16 * NG + 2 * tq;
-              const uint32_t ra = (uint32_t)*(const uint16_t*)(kt + gq * (D / 2)) * 0x10001u, rb = (uint32_t)*(const uint16_t*)(kt + (gq + 8) * (D / 2)) * 0x10001u;
-              const uint32_t a0 = (nib<0>(ra) & 0xFFFFu) | (nib<1>(ra) & 0xFFFF0000u), a1 = (nib<0>(rb) & 0xFFFFu) | (nib<1>(rb) & 0xFFFF0000u);
-              const uint32_t a2 = (nib<2>(ra) & 0xFFFFu) | (nib<3>(ra) & 0xFFFF0000u), a3 = (nib<2>(rb) & 0xFFFFu) | (nib<3>(rb) & 0xFFFF0000u);
+              const uint32_t a0 = nib_bytes(*(const uint16_t*)(kt + gq * (D / 2))), a1 = nib_bytes(*(const uint16_t*)(kt + (gq + 8) * (D / 2)));
 #pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(acc[j][h], a0, a1, a2, a3, qb[h][2 * NG][0], qb[h][2 * NG][1]);
+              for (int h = 0; h < HN; ++h) { mma_s8_half(hi[h], a0, a1, qb[h][NG].x); mma_s8_half(lo[h], a0, a1, qb[h][NG].z); }
             }
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
               sv[j][n] = q4_scale(vm); mv[j][n] = q4_min(vm);
 #pragma unroll
-              for (int h = 0; h < HN; ++h) sc[h][j][n] = fmaf((acc[j][h][2 * n] + acc[j][h][2 * n + 1]) * qc[h], q4_scale(km), q4_min(km) * qx[h]);
+              for (int h = 0; h < HN; ++h) {
+                const float dot = fmaf((float)hi[h][2 * n], 65536.f, fmaf((float)hi[h][2 * n + 1], 256.f, (float)lo[h][2 * n]));
+                sc[h][j][n] = fmaf(dot * qc[h], q4_scale(km), q4_min(km) * qx[h]);
+              }
             }
           }
           if (tok < s.lo || tok + QD_PAIR - 1 > s.pos) {     // rows outside the window or behind the last token hold anything
@@ -363,10 +377,10 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
             load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              const uint32_t a0 = nib<0>(w0[g]), a1 = nib<1>(w0[g]), a2 = nib<0>(w1[g]), a3 = nib<1>(w1[g]);
+              const uint32_t a0 = nib<0>(w0[g], one), a1 = nib<1>(w0[g], one), a2 = nib<0>(w1[g], one), a3 = nib<1>(w1[g], one);
 #pragma unroll
               for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g], a0, a1, a2, a3, pb[h][0], pb[h][1]);
-              const uint32_t b0 = nib<2>(w0[g]), b1 = nib<3>(w0[g]), b2 = nib<2>(w1[g]), b3 = nib<3>(w1[g]);
+              const uint32_t b0 = nib<2>(w0[g], one), b1 = nib<3>(w0[g], one), b2 = nib<2>(w1[g], one), b3 = nib<3>(w1[g], one);
 #pragma unroll
               for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g + 1], b0, b1, b2, b3, pb[h][0], pb[h][1]);
             }
@@ -374,7 +388,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
               const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
               const uint32_t r0 = __byte_perm(w, 0u, 0x4140), r1 = __byte_perm(w, 0u, 0x4342);
 #pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], nib<0>(r0), nib<1>(r0), nib<0>(r1), nib<1>(r1), pb[h][0], pb[h][1]);
+              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], nib<0>(r0, one), nib<1>(r0, one), nib<0>(r1, one), nib<1>(r1, one), pb[h][0], pb[h][1]);
             }
           }
           __syncwarp();                                              // every lane has read the pair: its slot may be filled again
@@ -443,14 +457,14 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           top = fmaxf(top, fmaxf(fabsf(xa[k]), fabsf(xb[k]))); sum += xa[k] + xb[k];
         }
         top = warp_max(top); sum = warp_sum(sum);
-        f = top > 0.f ? pow2_for(top, 13) : 1.f;
+        f = top > 0.f ? pow2_for(top, 21) : 1.f;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
           const int i = lane + 32 * k;
           if (i < D / 2) { const int2 at = pair_dims(i, half, p.rope_type); sm.q[g][at.x] = xa[k] * f; sm.q[g][at.y] = xb[k] * f; }
         }
       }
-      if (lane == 0) { sm.qc[buf][g] = g < gn ? 262144.f / f : 0.f; sm.qx[buf][g] = sum; }
+      if (lane == 0) { sm.qc[buf][g] = g < gn ? 1.f / f : 0.f; sm.qx[buf][g] = sum; }
     }
     if (!p.no_append && t.skip + t.n == t.s.n && hw >= 2) {
       const bool v = hw == 3;
@@ -469,15 +483,21 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       }
     }
     helpers_sync();
-    // column gq is head gq / 2 of a tile, its fp16 head (even) or what that leaves (odd).  Word tq of a group of 32 dims holds dims
-    // 8 tq .. + 7 and its nibbles pair as (0, 4), (1, 5), (2, 6), (3, 7)
-    const uint32_t sel = gq & 1 ? 0x7632u : 0x5410u;
-    for (int f = hw; f < HN * KS; f += QD_HELPERS / 32) {
-      const int h = f / KS, ks = f - h * KS, head = 4 * h + (gq >> 1);
-      const float* qr = sm.q[head < gn ? head : 0];
-      auto frag = [&](int d0, int d1) { return head < gn ? __byte_perm(split_f16(qr[d0]), split_f16(qr[d1]), sel) : 0u; };
-      const int d = ks < 2 * NG ? 16 * (ks & ~1) + 8 * tq + 2 * (ks & 1) : 32 * NG + 4 * tq;
-      sm.frag[buf][h][ks][lane] = ks < 2 * NG ? make_uint2(frag(d, d + 4), frag(d + 1, d + 5)) : make_uint2(frag(d, d + 1), frag(d + 2, d + 3));
+    // column gq is head gq / 2 of a tile, its digits 0 (even) or 1 (odd), and in the second pair of registers digit 2 (even).  Word tq of
+    // a group of 32 dims holds dims 8 tq .. + 7: the low nibbles of its bytes are the even ones, the high nibbles the odd ones
+    for (int i = hw; i < HN * NF; i += QD_HELPERS / 32) {
+      const int h = i / NF, f = i - h * NF, head = 4 * h + (gq >> 1);
+      const float* qr = sm.q[head < gn ? head : 0] + 32 * f;
+      uint4 r = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t de = head < gn ? digits(__float2int_rn(f < NG ? qr[8 * tq + 2 * e] : qr[4 * tq + e])) : 0u;
+        const uint32_t od = head < gn && f < NG ? digits(__float2int_rn(qr[8 * tq + 2 * e + 1])) : 0u;
+        r.x |= (gq & 1 ? de >> 8 & 255u : de & 255u) << 8 * e;
+        r.y |= (gq & 1 ? od >> 8 & 255u : od & 255u) << 8 * e;
+        if (!(gq & 1)) { r.z |= (de >> 16) << 8 * e; r.w |= (od >> 16) << 8 * e; }
+      }
+      sm.frag[buf][h][f][lane] = r;
     }
     qd_arrive(&sm.frag_full[buf]);
   };
