@@ -1,76 +1,450 @@
-// Attention of the rows of a prompt chunk over the 4-bit paged cache (kv_q4.cuh).
+// Causal attention of the rows of a prompt chunk over the 4-bit paged cache (kv_q4.cuh), on the tcgen05 tensor cores.
+//
+// A CTA has 128 rows of one kv head, row = (token, query head of the group): the group's heads share the keys and values that the
+// CTA turns into fp16.  Per 128 keys:
+//   S = Q K^T      128 x 128 x D, accumulated in TMEM
+//   P = 2^(S - m)  one thread to a row; P goes back to TMEM as fp16, over the columns of S, and is the A operand of
+//   O += P V       128 x D x 128, accumulated in TMEM.  The running maximum moves only when a score passes it by 2^8, so that O is
+//                  rarely read, scaled and written back.
+// Warps 0..3 do the softmax, 4..7 decode keys and values (code x scale + minimum in fp16, rounded once) into the swizzled operand
+// tiles, warp 8 issues the products.  Two CTAs share an SM: the tensor cores work for one while the other is at its exponentials,
+// of which there are 128 to a row and tile: at 16 a clock and SM they take twice the time of the products and are what bounds this.
+//
+// Range: K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
+// softmax scale; V by one that changes only when a tile needs it, with O), q by one to a row.
+//
+// Few rows over many keys: the keys of a row tile are divided over several CTAs, which leave their parts in scratch; the last of
+// them to arrive joins them in order.
 #include "attention_q4.cuh"
 #include "kv_q4.cuh"
+#include "tcgen05_common.cuh"
+#include <algorithm>
 
 namespace rlz {
 
-// 3113: a page id outside the cache (read as page 0); 3114: a row beyond the page table (skipped)
+// 3113: a page id outside the cache (read as page 0); 3114: rows beyond the page table (not computed); 3115: a bounded wait ran out
 __device__ int g_prefill_q4_error = 0;
 
-__device__ __forceinline__ int q4_page_id(int raw, int num_pages) {
-  if (num_pages > 0 && (unsigned)raw >= (unsigned)num_pages) { atomicExch(&g_prefill_q4_error, 3113); return 0; }
-  return raw;
+constexpr int QP_THREADS = 288, QP_ROWS = 128, QP_KEYS = 128, QP_MAX_CTAS = 296, QP_MIN_TILES = 2;
+constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
+constexpr int QP_COUNTERS = 320;               // floats in front of the parts: arrival counters
+
+struct QpSmem {
+  unsigned long long q_full, k_full, k_empty, v_full, v_empty, s_full, p_full;
+  float kf[2], vf[2];                         // powers of two that the tile's K and V carry
+  float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
+  uint32_t tmem;
+  int last;
+};
+
+__device__ __forceinline__ float qp_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t qp_half2(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *(const uint32_t*)&h; }
+// 2^(e - exponent of x), x >= 0; 2^100 at most
+__device__ __forceinline__ float qp_pow2(float x, int e) {
+  const int k = e + 254 - (int)(__float_as_uint(x) >> 23);
+  return __uint_as_float((uint32_t)max(1, min(k, 227)) << 23);
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
+               ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+               "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ bool qp_wait(unsigned long long* bar, uint32_t parity) {
+  if (gm_wait((uint64_t*)bar, parity)) return true;
+  atomicExch(&g_prefill_q4_error, 3115);
+  return false;
 }
 
-// One warp to a (chunk row, query head)
+// true when it is for all 128 threads of a role (also their barrier)
+template <int BAR> __device__ __forceinline__ bool qp_agree(bool mine) {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.and.pred q, %2, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(r) : "r"((uint32_t)mine), "n"(BAR) : "memory");
+  return r != 0;
+}
+
+// eight codes of a word as fp16: pairs (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ void codes_f16(uint32_t w, __half2 (&c)[4]) {
+  const __half2 magic = __half2half2(__ushort_as_half(0x6400)), sixteenth = __half2half2(__ushort_as_half(0x2C00)), back = __half2half2(__ushort_as_half(0xD400));
+  const uint32_t h = w >> 8;                  // 0x6400 | code is 1024 + code, 0x6400 | 16 code is 1024 + 16 code: both come off exactly
+  const uint32_t r[4] = {(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x64006400u, (h & 0x000F000Fu) | 0x64006400u, (h & 0x00F000F0u) | 0x64006400u};
+  c[0] = __hsub2(*(const __half2*)&r[0], magic); c[1] = __hfma2(*(const __half2*)&r[1], sixteenth, back);
+  c[2] = __hsub2(*(const __half2*)&r[2], magic); c[3] = __hfma2(*(const __half2*)&r[3], sixteenth, back);
+}
+
+struct QpRange { int k0, tiles; };            // first key and number of key tiles of a CTA
+
 template <int D>
-__global__ void __launch_bounds__(128) attn_prefill_q4_simple_kernel(const __grid_constant__ AttnPrefillParams p) {
-  constexpr int NP = HeadPairs<D>::NP;
+__global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __grid_constant__ AttnPrefillParams p, const int nsplit) {
+  constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, NSLAB = (D + 63) / 64, PB = q4_page_bytes(D);
+  constexpr uint32_t TMEM_COLS = 256;         // S and P: columns 0..127, O: 128..
+  extern __shared__ __align__(1024) uint8_t qp_smem[];
+  __shared__ QpSmem sm;
+  uint8_t* Qs = (uint8_t*)(((uintptr_t)qp_smem + 1023) & ~(uintptr_t)1023);
+  uint8_t* Ks = Qs + NSLAB * QP_SLAB;
+  uint8_t* Vs = Ks + NSLAB * QP_SLAB;         // two slabs of [D rows x 64 keys]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G, kvh = blockIdx.y;
+  const int mtile = (int)(gridDim.x / nsplit) - 1 - (int)blockIdx.x / nsplit, part = (int)blockIdx.x % nsplit;      // the longest rows first
+  const int m0 = mtile * QP_ROWS;
+
+  if (tid == 0) {
+    unsigned long long* bars[7] = {&sm.q_full, &sm.k_full, &sm.k_empty, &sm.v_full, &sm.v_empty, &sm.s_full, &sm.p_full};
+    const int count[7] = {128, 128, 1, 128, 1, 1, 128};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(bars[i])), "r"(count[i]));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gm_smem_u32(&sm.tmem)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sm.tmem;
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y, r = blockIdx.x * 4 + warp;
-  if (r >= p.n_tokens) return;
-  const int kvh = head / (p.n_heads / p.n_kv_heads);
-  const int pos = (p.pos0_ptr ? *p.pos0_ptr : p.pos0) + r;
-  if (pos < 0 || pos / Q4_PAGE >= p.pt_len) { atomicExch(&g_prefill_q4_error, 3114); return; }
-  const int lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
-  const float* src = p.qkv + (int64_t)r * p.ld_qkv + p.q_off + (int64_t)head * D;
-  float q[NP][2] = {}, m = -INFINITY;
-  double l = 0.0, o[NP][2] = {};                      // a serial sum over tens of thousands of tokens
+
+  // ---- keys of this CTA: the rows' range, in tiles from a page boundary on, divided over the parts -----------------------------
+  const int pos0 = p.pos0_ptr ? *p.pos0_ptr : p.pos0;
+  const int tok0 = m0 / G, tok1 = min(p.n_tokens, (m0 + QP_ROWS - 1) / G + 1);            // tokens of the tile
+  const int kend = pos0 + tok1;
+  bool ok = pos0 >= 0 && (kend - 1) / Q4_PAGE < p.pt_len;
+  if (!ok && tid == 0) atomicExch(&g_prefill_q4_error, 3114);
+  const int klo = p.window > 0 ? max(0, pos0 + tok0 + 1 - p.window) / Q4_PAGE * Q4_PAGE : 0;
+  const int all = (kend - klo + QP_KEYS - 1) / QP_KEYS, parts = max(1, min(nsplit, all / QP_MIN_TILES));
+  const int j0 = part * all / parts, n_tiles = ok && part < parts ? (part + 1) * all / parts - j0 : 0;
+  const int kbeg = klo + j0 * QP_KEYS;
+
+  if (n_tiles > 0 && warp < 4) {
+    // ================================ softmax: one thread to a row ================================================================
+    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    const int row = m0 + tid, token = row / G, head = kvh * G + row - token * G;
+    const bool live = row < rows;
+    const int pos = pos0 + token;
+    float qs = 0.f;                                              // softmax scale of the row
+    {
+      const float* src = p.qkv + (int64_t)(live ? token : 0) * p.ld_qkv + p.q_off + (int64_t)(live ? head : 0) * D;
+      float top = 0.f;
+      if (live) for (int i = 0; i < D; ++i) top = fmaxf(top, fabsf(src[i]));
+      const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
+      qs = p.scale * 1.4426950408889634f / f;
+      for (int x = 0; x < NSLAB * 8; ++x) {                      // 8 dims in the order in which the keys' codes come out of a word
+        float v[8];
 #pragma unroll
-  for (int k = 0; k < NP; ++k) { const int i = lane + 32 * k; if (i < D / 2) { q[k][0] = src[2 * i] * p.scale; q[k][1] = src[2 * i + 1] * p.scale; } }
-  for (int t = lo; t <= pos; ++t) {
-    const int64_t at = ((int64_t)q4_page_id(p.page_table[t / Q4_PAGE], p.num_pages) * p.n_kv_heads + kvh) * q4_page_bytes(D);
-    const uint8_t *kp = (const uint8_t*)p.k_cache + at, *vp = (const uint8_t*)p.v_cache + at;
-    const int slot = t % Q4_PAGE;
-    const uint32_t km = *(const uint32_t*)(kp + 8 * D + 4 * slot), vm = *(const uint32_t*)(vp + 8 * D + 4 * slot);
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const int i = lane + 32 * k;
-      if (i >= D / 2) continue;
-      const int w = kp[q4_k_byte<D>(slot, i)];
-      s += q[k][0] * ((float)(w & 15) * q4_scale(km) + q4_min(km)) + q[k][1] * ((float)(w >> 4) * q4_scale(km) + q4_min(km));
+        for (int i = 0; i < 8; ++i) v[i] = live && 8 * x < D ? src[8 * x + i] * f : 0.f;
+        *(uint4*)(Qs + (x >> 3) * QP_SLAB + (tid >> 3) * 1024 + (tid & 7) * 128 + (((x & 7) ^ (tid & 7)) << 4)) =
+            make_uint4(qp_half2(v[0], v[4]), qp_half2(v[1], v[5]), qp_half2(v[2], v[6]), qp_half2(v[3], v[7]));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      gm_arrive((uint64_t*)&sm.q_full);
     }
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), corr = expf(m - mn), e = expf(s - mn);
-    l = l * corr + e; m = mn;
+    float m = -INFINITY, l = 0.f, vf = 1.f;
+    const int pos_first = pos0 + tok0, lo_last = p.window > 0 ? pos0 + tok1 - p.window : 0;     // masks are needed beyond these
+    for (int j = 0; ok && j < n_tiles; ++j) {
+      const int k0 = kbeg + j * QP_KEYS;
+      const uint32_t ph = (uint32_t)j & 1u;
+      ok = qp_wait(&sm.s_full, ph);                               // the scores, and with them the product before and the tile's powers of two
+      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+      tc_after();
+      const float sc = qs / sm.kf[ph], vn = sm.vf[ph];
+      const bool edge = k0 + QP_KEYS - 1 > pos_first || k0 < lo_last;
+      const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c0 = 0; c0 < QP_KEYS; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld32(t_lane + (uint32_t)c0, r);
+        if (edge) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const int i = lane + 32 * k;
-      if (i >= D / 2) continue;
-      const int w = vp[q4_v_byte<D>(slot, i)];
-      o[k][0] = o[k][0] * corr + e * ((float)(w & 15) * q4_scale(vm) + q4_min(vm));
-      o[k][1] = o[k][1] * corr + e * ((float)(w >> 4) * q4_scale(vm) + q4_min(vm));
+          for (int i = 0; i < 32; ++i) if (c0 + i < vis_hi && c0 + i >= vis_lo) top = fmaxf(top, __uint_as_float(r[i]));
+        } else {
+          float t0 = __uint_as_float(r[0]), t1 = __uint_as_float(r[1]);
+#pragma unroll
+          for (int i = 2; i < 32; i += 2) { t0 = fmaxf(t0, __uint_as_float(r[i])); t1 = fmaxf(t1, __uint_as_float(r[i + 1])); }
+          top = fmaxf(top, fmaxf(t0, t1));
+        }
+      }
+      top *= sc;
+      if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
+        const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
+        if (j > 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(t_lane + 128u + (uint32_t)c0, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * co);
+            tmem_st16(t_lane + 128u + (uint32_t)c0, r);
+          }
+        }
+        l *= corr; m = mn; vf = vn;
+      }
+      const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
+#pragma unroll 1
+      for (int c0 = 0; c0 < QP_KEYS; c0 += 32) {
+        uint32_t r[32], w[16];
+        tmem_ld32(t_lane + (uint32_t)c0, r);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float e0 = qp_ex2(fmaf(__uint_as_float(r[i]), sc, base)), e1 = qp_ex2(fmaf(__uint_as_float(r[i + 1]), sc, base));
+          if (edge) {
+            if (!(c0 + i < vis_hi && c0 + i >= vis_lo)) e0 = 0.f;
+            if (!(c0 + i + 1 < vis_hi && c0 + i + 1 >= vis_lo)) e1 = 0.f;
+          }
+          l += e0 + e1;
+          w[i >> 1] = qp_half2(e0, e1);
+        }
+        tmem_st16(t_lane + (uint32_t)(c0 >> 1), w);               // columns c0 / 2 ..: their scores have been read
+      }
+      tmem_wait_st();
+      tc_before();
+      gm_arrive((uint64_t*)&sm.p_full);
+    }
+    if (ok) ok = qp_wait(&sm.v_empty, (uint32_t)(n_tiles - 1) & 1u);       // the last product
+    if (qp_agree<1>(ok)) {
+      tc_after();
+      const float inv_vf = 1.f / vf;
+      auto store = [&](int c, const float* v) {                   // 16 finished values
+        const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
+        if (p.out_bf16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+          uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
+          dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      };
+      const int tile_id = kvh * (int)(gridDim.x / nsplit) + mtile;
+      float* slot = p.scratch + QP_COUNTERS + ((int64_t)tile_id * nsplit + part) * QP_ROWS * (D + 4) + (int64_t)tid * (D + 4);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(t_lane + 128u + (uint32_t)c, r);
+        float v[16];
+        const float f = parts == 1 ? inv_vf / l : inv_vf;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
+        if (parts == 1) { if (live) store(c, v); }
+        else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *(float4*)(slot + c + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      }
+      if (parts > 1) {
+        *(float2*)(slot + D) = make_float2(m, l);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (tid == 0) {
+          int32_t* ctr = (int32_t*)p.scratch + tile_id;
+          __threadfence();
+          sm.last = atomicAdd(ctr, 1) == parts - 1;
+          if (sm.last) { *ctr = 0; __threadfence(); }             // zero again for the next launch
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (sm.last && live) {
+          const float* src = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * QP_ROWS * (D + 4) + (int64_t)tid * (D + 4);
+          constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);
+          float mm = -INFINITY, ll = 0.f;
+          for (int i = 0; i < parts; ++i) mm = fmaxf(mm, __ldcg(src + i * step + D));
+          for (int i = 0; i < parts; ++i) { const float2 st = __ldcg((const float2*)(src + i * step + D)); if (st.x != -INFINITY) ll = fmaf(qp_ex2(st.x - mm), st.y, ll); }
+          const float inv = 1.f / ll;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float v[16] = {};
+            for (int i = 0; i < parts; ++i) {
+              const float mi = __ldcg(src + i * step + D), e = mi == -INFINITY ? 0.f : qp_ex2(mi - mm) * inv;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float4 x = __ldcg((const float4*)(src + i * step + c + 4 * q));
+                v[4 * q] = fmaf(e, x.x, v[4 * q]); v[4 * q + 1] = fmaf(e, x.y, v[4 * q + 1]); v[4 * q + 2] = fmaf(e, x.z, v[4 * q + 2]); v[4 * q + 3] = fmaf(e, x.w, v[4 * q + 3]);
+              }
+            }
+            store(c, v);
+          }
+        }
+      }
+    }
+  } else if (n_tiles > 0 && warp < 8) {
+    // ================================ decoding: a key row, and half a page of values, to a thread ===================================
+    const int t = tid - 128;
+    uint32_t kw[D / 8], vw[D / 8], km = 0u, vm[8];
+    auto row_of = [&](int key) {
+      int id = __ldg(p.page_table + key / Q4_PAGE);
+      if ((unsigned)id >= (unsigned)p.num_pages) { atomicExch(&g_prefill_q4_error, 3113); id = 0; }
+      return ((int64_t)id * p.n_kv_heads + kvh) * PB;
+    };
+    const int last_page = (kend - 1) / Q4_PAGE * Q4_PAGE;
+    auto load_k = [&](int k0) {
+      const int key = k0 + t;
+      const uint8_t* src = (const uint8_t*)p.k_cache + row_of(min(key, last_page));
+#pragma unroll
+      for (int i = 0; i < D / 8; i += 2) {
+        const uint2 v = __ldg((const uint2*)(src + (key % Q4_PAGE) * (D / 2) + 4 * i));
+        kw[i] = v.x; kw[i + 1] = v.y;
+      }
+      km = key < kend ? __ldg((const uint32_t*)(src + 8 * D + 4 * (key % Q4_PAGE))) : 0u;         // rows behind the last key count as 0
+    };
+    const int vh = (t >> 3) & 1, vg = t & 7;                       // page t / 16 of the tile, tokens 8 vh .. + 7, units vg of every 32 dims
+    auto load_v = [&](int k0) {
+      const int key = k0 + (t >> 4) * Q4_PAGE;
+      const uint8_t* src = (const uint8_t*)p.v_cache + row_of(min(key, last_page));
+      const uint32_t* w = (const uint32_t*)(src + (size_t)vh * 128 * NG + vg * 16 * NG);           // words [tq][g]
+#pragma unroll
+      for (int i = 0; i < 4 * NG; i += 4) { const uint4 v = __ldg((const uint4*)(w + i)); vw[i] = v.x; vw[i + 1] = v.y; vw[i + 2] = v.z; vw[i + 3] = v.w; }
+      if constexpr (TAIL) {                                        // bytes of both halves: mine of each word, as 16 bits
+        const uint4 v = __ldg((const uint4*)(src + 256 * NG + vg * 16));
+        vw[4 * NG] = __byte_perm(v.x, v.y, vh ? 0x7632 : 0x5410); vw[4 * NG + 1] = __byte_perm(v.z, v.w, vh ? 0x7632 : 0x5410);
+      }
+      const uint4 a = __ldg((const uint4*)(src + 8 * D + 32 * vh)), b = __ldg((const uint4*)(src + 8 * D + 32 * vh + 16));
+      const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vm[i] = key + 8 * vh + i < kend ? r[i] : 0u;
+    };
+    load_k(kbeg);
+    load_v(kbeg);
+    float vf = 0x1p100f;
+    for (int j = 0; j < n_tiles; ++j) {
+      const uint32_t ph = (uint32_t)j & 1u;
+      // powers of two for the tile: its largest value to [2^4, 2^5); the one of V stays as long as it keeps them below 2^12
+      auto largest = [](uint32_t meta) { return fmaxf(fabsf(q4_min(meta)), fabsf(fmaf(15.f, q4_scale(meta), q4_min(meta)))); };
+      float kt = largest(km), vt = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vt = fmaxf(vt, largest(vm[i]));
+      kt = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(kt)));
+      vt = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(vt)));
+      if (lane == 0) { sm.mag[ph][0][warp - 4] = kt; sm.mag[ph][1][warp - 4] = vt; }
+      if (!qp_agree<2>(ok)) break;
+      kt = fmaxf(fmaxf(sm.mag[ph][0][0], sm.mag[ph][0][1]), fmaxf(sm.mag[ph][0][2], sm.mag[ph][0][3]));
+      vt = fmaxf(fmaxf(sm.mag[ph][1][0], sm.mag[ph][1][1]), fmaxf(sm.mag[ph][1][2], sm.mag[ph][1][3]));
+      const float kf = qp_pow2(kt, 4);
+      if (vt * vf >= 4096.f) vf = qp_pow2(vt, 4);
+      if (t == 0) { sm.kf[ph] = kf; sm.vf[ph] = vf; }
+
+      if (j > 0) ok = qp_wait(&sm.k_empty, ph ^ 1u);
+      {
+        const __half2 s2 = __float2half2_rn(q4_scale(km) * kf), m2 = __float2half2_rn(q4_min(km) * kf);
+        uint8_t* base = Ks + (t >> 3) * 1024 + (t & 7) * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {                          // word i of the row: 8 dims from 8 x on
+          const int x = i < 4 * NG ? 4 * (i % NG) + i / NG : i;
+          __half2 c[4];
+          codes_f16(kw[i], c);
+          uint32_t o[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) { const __half2 v = __hfma2(c[q], s2, m2); o[q] = *(const uint32_t*)&v; }
+          *(uint4*)(base + (x >> 3) * QP_SLAB + (((x & 7) ^ (t & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      gm_arrive((uint64_t*)&sm.k_full);
+      if (j + 1 < n_tiles) load_k(kbeg + (j + 1) * QP_KEYS);
+
+      if (j > 0) ok = qp_wait(&sm.v_empty, ph ^ 1u) && ok;
+      {
+        __half2 s2[4], m2[4];                                      // of the token pairs
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s2[i] = __floats2half2_rn(q4_scale(vm[2 * i]) * vf, q4_scale(vm[2 * i + 1]) * vf);
+          m2[i] = __floats2half2_rn(q4_min(vm[2 * i]) * vf, q4_min(vm[2 * i + 1]) * vf);
+        }
+        const int chunk = (t >> 3) & 7;                            // eight keys of the 64 of a slab
+        uint8_t* base = Vs + (t >> 6) * (D * 128);
+        auto put = [&](int dim, const uint32_t* o) { *(uint4*)(base + (dim >> 3) * 1024 + (dim & 7) * 128 + ((chunk ^ (dim & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]); };
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          uint32_t o[4][4];                                        // [dim][token pair]
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            __half2 c[4];
+            codes_f16(vw[q * NG + g], c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) put(32 * g + 4 * vg + e, o[e]);
+        }
+        if constexpr (TAIL) {
+          uint32_t o[2][4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t two = vw[4 * NG + (q >> 1)] >> (16 * (q & 1));       // a byte to each token of the pair
+            __half2 c[4];
+            codes_f16((two & 0xFFu) | (two & 0xFF00u) << 8, c);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) put(32 * NG + 2 * vg + e, o[e]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      gm_arrive((uint64_t*)&sm.v_full);
+      if (j + 1 < n_tiles) load_v(kbeg + (j + 1) * QP_KEYS);
+    }
+  } else if (n_tiles > 0 && warp == 8 && lane == 0) {
+    // ================================ the products =================================================================================
+    const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_ROWS >> 4) << 24);      // fp16 operands, fp32 sums
+    const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_ROWS >> 4) << 24);
+    ok = qp_wait(&sm.q_full, 0u);
+    for (int j = 0; ok && j < n_tiles; ++j) {
+      const uint32_t ph = (uint32_t)j & 1u;
+      ok = qp_wait(&sm.k_full, ph) && (j == 0 || qp_wait(&sm.v_empty, ph ^ 1u));       // the scores go where the product before read P
+      if (!ok) break;
+      tc_after();
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        umma_bf16(tmem, make_sdesc_k_sw128(gm_smem_u32(Qs + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)),
+                  make_sdesc_k_sw128(gm_smem_u32(Ks + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)), id_s, kk > 0 ? 1u : 0u);
+      umma_commit((uint64_t*)&sm.s_full);
+      umma_commit((uint64_t*)&sm.k_empty);
+      ok = qp_wait(&sm.p_full, ph) && qp_wait(&sm.v_full, ph);
+      if (!ok) break;
+      tc_after();
+#pragma unroll
+      for (int kk = 0; kk < QP_KEYS / 16; ++kk)
+        umma_f16_ts(tmem + 128u, tmem + (uint32_t)(8 * kk), make_sdesc_k_sw128(gm_smem_u32(Vs + (kk >> 2) * (D * 128))) + (uint64_t)(2 * (kk & 3)), id_o,
+                    j > 0 || kk > 0 ? 1u : 0u);
+      umma_commit((uint64_t*)&sm.v_empty);
     }
   }
-#pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const int i = lane + 32 * k;
-    if (i >= D / 2) continue;
-    const int64_t at = (int64_t)r * p.ld_out + (int64_t)head * D + 2 * i;
-    if (p.out_bf16) *(__nv_bfloat162*)((__nv_bfloat16*)p.out + at) = __floats2bfloat162_rn((float)(o[k][0] / l), (float)(o[k][1] / l));
-    else { p.out[at] = (float)(o[k][0] / l); p.out[at + 1] = (float)(o[k][1] / l); }
-  }
+  tc_before();
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+template <int D>
+static int launch_prefill_q4(const AttnPrefillParams& p, cudaStream_t st) {
+  constexpr int NSLAB = (D + 63) / 64;
+  const size_t smem = (size_t)2 * NSLAB * QP_SLAB + 2 * D * 128 + 1024;
+  static SmemOptIn opt;
+  if (cudaError_t e = opt.ensure(attn_prefill_q4_kernel<D>, smem, 0); e != cudaSuccess) return (int)e;
+  const int64_t rows = (int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads);
+  const int mtiles = (int)((rows + QP_ROWS - 1) / QP_ROWS);
+  // parts of a row tile's keys: as many as fill two CTAs to an SM, if there is scratch for them
+  const bool room = p.scratch && p.scratch_floats >= (int64_t)QP_MAX_CTAS * QP_ROWS * (D + 4) + QP_COUNTERS;
+  const int nsplit = room ? std::max(1, std::min(32, QP_MAX_CTAS / (mtiles * p.n_kv_heads))) : 1;
+  return (int)launch(attn_prefill_q4_kernel<D>, dim3(mtiles * nsplit, p.n_kv_heads), dim3(QP_THREADS), smem, st, p, nsplit);
 }
 
 int attn_prefill_q4_dispatch(const AttnPrefillParams& p, cudaStream_t st) {
-  dim3 grid((p.n_tokens + 3) / 4, p.n_heads);
+  if (p.num_pages < 1 || p.pt_len < 1 || ((uintptr_t)p.scratch & 15)) return -6;
   switch (p.head_dim) {
-    case 64: return (int)launch(attn_prefill_q4_simple_kernel<64>, grid, dim3(128), 0, st, p);
-    case 80: return (int)launch(attn_prefill_q4_simple_kernel<80>, grid, dim3(128), 0, st, p);
-    case 96: return (int)launch(attn_prefill_q4_simple_kernel<96>, grid, dim3(128), 0, st, p);
-    case 128: return (int)launch(attn_prefill_q4_simple_kernel<128>, grid, dim3(128), 0, st, p);
+    case 64: return launch_prefill_q4<64>(p, st);
+    case 80: return launch_prefill_q4<80>(p, st);
+    case 96: return launch_prefill_q4<96>(p, st);
+    case 128: return launch_prefill_q4<128>(p, st);
     default: return -1;
   }
 }
@@ -79,10 +453,12 @@ int attn_prefill_q4_dispatch(const AttnPrefillParams& p, cudaStream_t st) {
 
 extern "C" {
 
-// floats of scratch that a chunk of up to n_tokens rows can use
-long long rlz_attn_prefill_q4_scratch_floats(int n_tokens, int n_heads, int n_kv_heads, int head_dim) { return 1; }
+// floats of scratch with which the keys can be split, whatever the number of rows is
+long long rlz_attn_prefill_q4_scratch_floats(int n_tokens, int n_heads, int n_kv_heads, int head_dim) {
+  return (long long)rlz::QP_MAX_CTAS * rlz::QP_ROWS * (head_dim + 4) + rlz::QP_COUNTERS;
+}
 
-// 0 / 3113 / 3114
+// 0 / 3113 / 3114 / 3115
 int rlz_attn_prefill_q4_error(int clear) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, rlz::g_prefill_q4_error, sizeof(int)) != cudaSuccess) return -1;
