@@ -7,10 +7,9 @@
 // The arithmetic of the codes is what has to be cheap:
 //   * Keys: a masked word holds four codes as bytes, and the 8-bit integer product takes them as they are; q comes as three 8-bit
 //     digits of a 23-bit integer (its largest value in [2^21, 2^22)), so the sums over the dims are exact.
-//   * Values: a nibble moved to bits 6..9 of an fp16 is the subnormal code x 2^-18, which mma.sync multiplies exactly: a shift and an
-//     AND to two codes instead of a conversion and a multiply-add each.  (The unit lines products up by the exponent fields: a nibble
-//     left at the low bits, x 2^-24 without the shift, costs the sum as many bits as stand empty above it, 2e-5 of the result where
-//     this gives 3e-7.)  The right shifts are high halves of products, which leaves the busier integer pipe to the masks.
+//   * Values: a nibble under the exponent of 1024 is the fp16 1024 + code (or 1024 + 16 code), which one subtraction (or
+//     multiply-add) turns into code - 8 exactly: 9 instructions to 8 codes.  The 8 goes into the minimum: without it, sum p scale code
+//     and sum p min cancel, over 131072 tokens to 1 / 900, and so do the digits of the result (2e-4 of it instead of 1e-6).
 //     p x scale' comes as its fp16 head and what that leaves, also fp16: 22 bits; its power of two follows the scales.
 //   * Tokens (keys) and dims (values) are the 16 rows of the instruction and 4 heads its 8 columns, two digits or halves each, so
 //     the parts of a head's sum meet in one lane.  Up to 8 heads take two such tiles and share the other operand.
@@ -66,9 +65,16 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// nibble J of both halves of a word as fp16 subnormals: code x 2^-18; one: the number 1, which the compiler must not know
-template <int J> __device__ __forceinline__ uint32_t nib(uint32_t w, uint32_t one) {
-  return (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? __umulhi(w, one << 30) : __umulhi(w, one << 26)) & 0x03C003C0u;
+// nibbles 0..3 of both halves of a word as fp16, less 8
+__device__ __forceinline__ void codes_less_8(uint32_t w, uint32_t (&c)[4]) {
+  const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k16th = __half2half2(__ushort_as_half(0x2C00)), k72 = __half2half2(__ushort_as_half(0xD480));
+  const uint32_t h = w >> 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = ((i ? h : w) & 0x000F000Fu) | 0x64006400u, y = ((i ? h : w) & 0x00F000F0u) | 0x64006400u;
+    const __half2 u = __hsub2(*(const __half2*)&x, k1032), v = __hfma2(*(const __half2*)&y, k16th, k72);
+    c[2 * i] = *(const uint32_t*)&u; c[2 * i + 1] = *(const uint32_t*)&v;
+  }
 }
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -206,45 +212,46 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   if (warp < NW) {
     // ================================ main warps ================================================================================
     uint8_t* my_ring = qd_ring + (size_t)warp * QD_STAGES * 4 * PB;
-    // -- the copies: pair after pair of the stream, their page ids read one pair ahead
+    // -- the copies, pair after pair of the stream.  Lane i keeps the (page, kv head) row of page i % 2 of the i / 2-th of 16 pairs; the
+    // ids of the 16 behind them are on their way
     QdTile f = qd_tile(p, b0, at0, x1 - x0);
-    int f_at = 0, f_k = 0, f_k1 = first_k(warp, f.n), f_id[2], f_np = 0, f_kvh = f.tile / hgroups;
-    auto look_up = [&]() {
-      f_np = 0;
-      while (f_k >= f_k1) {                                          // none left in this tile
-        f_at += f.n;
-        if (f_at >= x1 - x0) return;
-        f = qd_next(p, f, tiles, x1 - x0 - f_at);
-        f_k1 = first_k(warp, f_at + f.n); f_kvh = f.tile / hgroups;
+    int f_at = 0, row_now, id_next, kvh_next;
+    auto fetch = [&](int k) {                                        // ids of pairs k .. k + 15
+      while (f_at + f.n < x1 - x0 && warp + NW * k >= f_at + f.n) { f_at += f.n; f = qd_next(p, f, tiles, x1 - x0 - f_at); }
+      const int x = warp + NW * (k + (lane >> 1));
+      kvh_next = -1;
+      if (x < x1 - x0) {
+        QdTile t = f;
+        int t_at = f_at;
+        while (x >= t_at + t.n) { t_at += t.n; t = qd_next(p, t, tiles, x1 - x0 - t_at); }
+        const int page = t.s.first_page + 2 * (t.skip + x - t_at) + (lane & 1);
+        if (page <= t.s.pos / Q4_PAGE) { id_next = __ldg(p.page_table + (int64_t)t.b * p.pt_stride + page); kvh_next = t.tile / hgroups; }
       }
-      const int page = f.s.first_page + 2 * (f.skip + warp + NW * f_k - f_at), last = f.s.pos / Q4_PAGE;
-      const int32_t* pt = p.page_table + (int64_t)f.b * p.pt_stride;
-      f_np = min(2, last - page + 1);
-      f_id[0] = __ldg(pt + page); f_id[1] = __ldg(pt + min(page + 1, last));
-      ++f_k;
     };
-    auto copy_pair = [&](uint32_t to) {
+    auto turn = [&]() { row_now = kvh_next < 0 ? -1 : q4_page_id(id_next, p.num_pages) * p.n_kv_heads + kvh_next; };
+    const uint8_t* const my_k = (const uint8_t*)p.k_cache + 16 * lane;
+    const int64_t k_to_v = (const uint8_t*)p.v_cache - (const uint8_t*)p.k_cache;
+    auto copy_pair = [&](int k, uint32_t to) {
+      if ((k & 15) == 0) { turn(); fetch(k + 16); }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (j < f_np) {
-          const int64_t off = ((int64_t)q4_page_id(f_id[j], p.num_pages) * p.n_kv_heads + f_kvh) * PB + 16 * lane;
+        const int row = __shfl_sync(0xFFFFFFFFu, row_now, 2 * (k & 15) + j);
+        if (row >= 0) {
+          const uint8_t* src = my_k + (int64_t)row * PB;
           const uint32_t dst = att_smem_u32(my_ring) + to * (4 * PB) + j * (2 * PB) + 16 * lane;
 #pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            const uint8_t* src = (const uint8_t*)(v ? p.v_cache : p.k_cache) + off;
+          for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int i = 0; i < (PB + 511) / 512; ++i)
               if (512 * (i + 1) <= PB || 512 * i + 16 * lane < PB)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * PB + 512 * i), "l"(src + 512 * i) : "memory");
-          }
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * PB + 512 * i), "l"(src + (v ? k_to_v : 0) + 512 * i) : "memory");
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    look_up();
-    for (int i = 0; i < QD_STAGES - 1; ++i) { copy_pair(i); look_up(); }
+    fetch(0);
+    for (int k = 0; k < QD_STAGES - 1; ++k) copy_pair(k, k);
     uint32_t slot = 0;
-    const uint32_t one = gridDim.z;
     for (int it = 0, at = 0; at < x1 - x0; ++it) {
       const int buf = it & 1;
       const uint32_t phase = (uint32_t)(it >> 1) & 1u;
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           for (int f = 0; f < NF; ++f) qb[h][f] = sm.frag[buf][h][f][lane];
           qc[h] = sm.qc[buf][4 * h + tq]; qx[h] = sm.qx[buf][4 * h + tq];
         }
-        float o[HN][NT][4], m[HN], l[HN], om[HN];                  // om: sum of p x min'
+        float o[HN][NT][4], m[HN], l[HN], om[HN];                  // om: sum of p (min' + 8 scale')
 #pragma unroll
         for (int h = 0; h < HN; ++h) {
 #pragma unroll
@@ -273,8 +280,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
         int tok = s.tok + (warp + NW * k0 - at) * QD_PAIR;           // first token of pair k
 
         for (int k = k0; k < k1; ++k, tok += NW * QD_PAIR) {          // (of an odd number of pages the last comes with a masked one)
-          copy_pair(slot == 0 ? QD_STAGES - 1 : slot - 1);            // into the slot that the pair before this one left
-          look_up();
+          copy_pair(k + QD_STAGES - 1, slot == 0 ? QD_STAGES - 1 : slot - 1);       // into the slot that the pair before this one left
           asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
           __syncwarp();
           uint8_t* const kp[2] = {my_ring + slot * (4 * PB), my_ring + slot * (4 * PB) + 2 * PB};
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
-              sv[j][n] = q4_scale(vm); mv[j][n] = q4_min(vm);
+              sv[j][n] = q4_scale(vm); mv[j][n] = fmaf(8.f, sv[j][n], q4_min(vm));
 #pragma unroll
               for (int h = 0; h < HN; ++h) {
                 const float dot = fmaf((float)hi[h][2 * n], 65536.f, fmaf((float)hi[h][2 * n + 1], 256.f, (float)lo[h][2 * n]));
@@ -377,18 +383,22 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
             load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              const uint32_t a0 = nib<0>(w0[g], one), a1 = nib<1>(w0[g], one), a2 = nib<0>(w1[g], one), a3 = nib<1>(w1[g], one);
+              uint32_t a[4], c[4];
+              codes_less_8(w0[g], a);
+              codes_less_8(w1[g], c);
 #pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g], a0, a1, a2, a3, pb[h][0], pb[h][1]);
-              const uint32_t b0 = nib<2>(w0[g], one), b1 = nib<3>(w0[g], one), b2 = nib<2>(w1[g], one), b3 = nib<3>(w1[g], one);
-#pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * g + 1], b0, b1, b2, b3, pb[h][0], pb[h][1]);
+              for (int h = 0; h < HN; ++h) {
+                mma_f16(o[h][2 * g], a[0], a[1], c[0], c[1], pb[h][0], pb[h][1]);
+                mma_f16(o[h][2 * g + 1], a[2], a[3], c[2], c[3], pb[h][0], pb[h][1]);
+              }
             }
             if constexpr (TAIL) {
               const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
-              const uint32_t r0 = __byte_perm(w, 0u, 0x4140), r1 = __byte_perm(w, 0u, 0x4342);
+              uint32_t a[4], c[4];
+              codes_less_8(__byte_perm(w, 0u, 0x4140), a);
+              codes_less_8(__byte_perm(w, 0u, 0x4342), c);
 #pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], nib<0>(r0, one), nib<1>(r0, one), nib<0>(r1, one), nib<1>(r1, one), pb[h][0], pb[h][1]);
+              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], a[0], a[1], c[0], c[1], pb[h][0], pb[h][1]);
             }
           }
           __syncwarp();                                              // every lane has read the pair: its slot may be filled again
@@ -397,7 +407,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
 
         // ---- this warp's part of the tile ----
         if (it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
-        const float e0 = 262144.f / vf;
+        const float e0 = 1.f / vf;
 #pragma unroll
         for (int h = 0; h < HN; ++h) {
 #pragma unroll

@@ -252,7 +252,7 @@ def test_decode_attention_options(cuda_device, kw):
     _decode(8, 2, 128, lens, seed=5, **kw)()
 
 
-@pytest.mark.parametrize("B, n", [(1, 40000), (200, 70), (3, 5000), (600, 3)])
+@pytest.mark.parametrize("B, n", [(1, 40000), (1, 131072), (200, 70), (3, 5000), (600, 3)])
 def test_decode_attention_divides_any_batch(cuda_device, B, n):
     _decode(8, 4, 64, [max(1, n - 13 * (b % 5)) for b in range(B)], seed=B, rope_dim=64)()
 
