@@ -64,10 +64,18 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_min(float v) {
+// smallest and largest of a value over the warp
+__device__ __forceinline__ float redux_min(float v) { float r; asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float redux_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+
+// 1 / sqrt(x) in 64 bits: two Newton steps y (3 - x y^2) / 2 on the 32-bit result (2^-22 -> 2^-43 -> below 2^-52), a third of the
+// time of the square root and the division.  Where 32 bits do not hold x, those.
+__device__ __forceinline__ double rsqrt_d(double x) {
+  if (!(x > 1e-30 && x < 1e30)) return 1.0 / sqrt(x);
+  double y = (double)rsqrtf((float)x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  for (int i = 0; i < 2; ++i) y = y * fma(-0.5 * x * y, y, 1.5);
+  return y;
 }
 
 struct RopeArgs {
@@ -123,14 +131,14 @@ __device__ __forceinline__ void norm_rope_d(float (&a)[HeadPairs<D>::NP], float 
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < NP; ++k) ss += (double)a[k] * a[k] + (double)b[k] * b[k];
-    rs = 1.0 / sqrt(warp_sum_d(ss) / D + eps);
+    rs = rsqrt_d(warp_sum_d(ss) * (1.0 / D) + eps);
   }
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     const int i = lane + 32 * k;
     if (i >= D / 2) continue;
     double x = a[k], y = b[k];
-    if (w) { const int2 at = pair_dims(i, half, r.rope_type); x = x * rs * (double)__ldg(w + at.x); y = y * rs * (double)__ldg(w + at.y); }
+    if (w) { const int2 at = pair_dims(i, half, r.rope_type); x *= rs * (double)__ldg(w + at.x); y *= rs * (double)__ldg(w + at.y); }
     if (i < half) {
       const double c = cs[k].x, s = cs[k].y, t = x * c - y * s;
       y = x * s + y * c;
@@ -140,10 +148,21 @@ __device__ __forceinline__ void norm_rope_d(float (&a)[HeadPairs<D>::NP], float 
   }
 }
 
-// Codes of the lane's pairs into `codes` [D] (shared memory of this warp, one byte each); returns the row's meta word
+// the code of a value in 64 bits
+static __device__ __noinline__ float q4_code_64(float x, float mn, float sc) {
+  return sc > 0.f ? (float)fmin(fmax(rint(((double)x - (double)mn) / (double)sc), 0.0), 15.0) : 0.f;
+}
+// x / 15 rounded once: the product with 1 / 15 and one correction (checked for every 24-bit x; below 2^-100 the division itself)
+__device__ __forceinline__ float div_15(float x) {
+  if (x < 0x1p-100f) return __fdiv_rn(x, 15.f);
+  const float q = x * (1.f / 15.f);
+  return fmaf(fmaf(-15.f, q, x), 1.f / 15.f, q);
+}
+
+// Codes of the lane's pairs (low four bits of ca / cb); returns the row's meta word
 template <int D>
-__device__ __forceinline__ uint32_t q4_quantise(const float (&a)[HeadPairs<D>::NP], const float (&b)[HeadPairs<D>::NP], int half, int rope_type, int lane,
-                                                uint8_t* codes) {
+__device__ __forceinline__ uint32_t q4_codes(const float (&a)[HeadPairs<D>::NP], const float (&b)[HeadPairs<D>::NP], int lane, uint32_t (&ca)[HeadPairs<D>::NP],
+                                             uint32_t (&cb)[HeadPairs<D>::NP]) {
   constexpr int NP = HeadPairs<D>::NP;
   float lo = INFINITY, hi = -INFINITY;
   float x[NP][2];
@@ -153,25 +172,43 @@ __device__ __forceinline__ uint32_t q4_quantise(const float (&a)[HeadPairs<D>::N
     x[k][1] = b[k] == b[k] ? fminf(fmaxf(b[k], -Q4_LIMIT), Q4_LIMIT) : 0.f;
     if (lane + 32 * k < D / 2) { lo = fminf(lo, fminf(x[k][0], x[k][1])); hi = fmaxf(hi, fmaxf(x[k][0], x[k][1])); }
   }
-  lo = warp_min(lo); hi = warp_max(hi);
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f)), mb = __float2bfloat16_rn(lo);
+  lo = redux_min(lo); hi = redux_max(hi);
+  const __nv_bfloat16 sb = __float2bfloat16_rn(div_15(hi - lo)), mb = __float2bfloat16_rn(lo);
   const float sc = __bfloat162float(sb), mn = __bfloat162float(mb);
-  const float inv = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sc));       // infinite for scales of 0 and below 2^-126
+  // 32 bits settle a code unless the quotient lies within 2^-14 of a border (its error is below 16 x 2^-22: difference 2^-24,
+  // reciprocal 2^-23, product 2^-24); those divide in 64.
+  // y + 1.5 x 2^23 rounds y to an integer, ties to even, and leaves it in the low bits
+  float t[NP][2];
+  bool near = !(inv < 1e30f);
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const int i = lane + 32 * k;
-    if (i >= D / 2) continue;
-    const int2 at = pair_dims(i, half, rope_type);
+  for (int k = 0; k < NP; ++k)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      // 32 bits settle the code unless the quotient lies within 1/1024 of a border (its error is below 2^-17); the rest divide in 64
-      const float y = (x[k][e] - mn) * inv;
-      float q = rintf(y);
-      if (fabsf(y - q) > 0.5f - 0x1p-10f || !(inv < 1e30f)) q = sc > 0.f ? (float)rint(((double)x[k][e] - (double)mn) / (double)sc) : 0.f;
-      codes[e ? at.y : at.x] = (uint8_t)fminf(fmaxf(q, 0.f), 15.f);
+      const float y = fminf(fmaxf((x[k][e] - mn) * inv, 0.f), 15.f);
+      t[k][e] = y + 12582912.f;
+      near |= fabsf(y - (t[k][e] - 12582912.f)) > 0.5f - 0x1p-14f;
     }
+  if (near) {
+#pragma unroll
+    for (int k = 0; k < NP; ++k) { t[k][0] = q4_code_64(x[k][0], mn, sc) + 12582912.f; t[k][1] = q4_code_64(x[k][1], mn, sc) + 12582912.f; }
   }
+#pragma unroll
+  for (int k = 0; k < NP; ++k) { ca[k] = __float_as_uint(t[k][0]) & 15u; cb[k] = __float_as_uint(t[k][1]) & 15u; }
   return (uint32_t)__bfloat16_as_ushort(sb) | (uint32_t)__bfloat16_as_ushort(mb) << 16;
+}
+// the same as bytes in `codes` [D], shared memory of this warp
+template <int D>
+__device__ __forceinline__ uint32_t q4_quantise(const float (&a)[HeadPairs<D>::NP], const float (&b)[HeadPairs<D>::NP], int half, int rope_type, int lane,
+                                                uint8_t* codes) {
+  uint32_t ca[HeadPairs<D>::NP], cb[HeadPairs<D>::NP];
+  const uint32_t meta = q4_codes<D>(a, b, lane, ca, cb);
+#pragma unroll
+  for (int k = 0; k < HeadPairs<D>::NP; ++k) {
+    if (lane + 32 * k < D / 2) { const int2 at = pair_dims(lane + 32 * k, half, rope_type); codes[at.x] = (uint8_t)ca[k]; codes[at.y] = (uint8_t)cb[k]; }
+  }
+  return meta;
 }
 
 // Write a row of codes and its meta word into a page (global or shared memory); the warp calls together
