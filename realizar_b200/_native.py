@@ -69,6 +69,8 @@ def cuda_lib() -> ctypes.CDLL:
     """librlz_cuda.so: the sm_100a kernels.  Raises if the library cannot be built or loaded:
     GPU paths never fall back silently to another implementation."""
     global _cuda
+    if _cuda is not None:
+        return _cuda
     with _lock:
         if _cuda is None:
             path = cuda_lib_path()

@@ -1,14 +1,15 @@
 // Causal attention of the rows of a prompt chunk over the 4-bit paged cache (kv_q4.cuh), on the tcgen05 tensor cores.
 //
-// A CTA has 128 rows of one kv head, row = (token, query head of the group): the group's heads share the keys and values that the
-// CTA turns into fp16.  Per 128 keys:
+// A CTA has two groups of 128 rows of one kv head, row = (token, query head of the group): the group's heads share the keys and values
+// that the CTA turns into fp16.  Per group and 128 keys:
 //   S = Q K^T      128 x 128 x D, accumulated in TMEM
 //   P = 2^(S - m)  one thread to a row; P goes back to TMEM as fp16, over the columns of S, and is the A operand of
 //   O += P V       128 x D x 128, accumulated in TMEM.  The running maximum moves only when a score passes it by 2^8, so that O is
 //                  rarely read, scaled and written back.
-// Warps 0..3 do the softmax, 4..7 decode keys and values (code x scale + minimum in fp16, rounded once) into the swizzled operand
-// tiles, warp 8 issues the products.  Two CTAs share an SM: the tensor cores work for one while the other is at its exponentials,
-// of which there are 128 to a row and tile: at 16 a clock and SM they take twice the time of the products and are what bounds this.
+// Warps 0..7 do the softmax of the groups, 8..11 decode keys and 12..15 values (code x scale + minimum in fp16, rounded once) into two
+// buffers each of swizzled operand tiles, warp 16 issues the products: while one group is at its exponentials the tensor cores work
+// for the other.  Products (2048 clocks to 256 rows and 128 keys of 128 dims) and exponentials (16 a clock) take the same time.
+// Registers are moved from the decoding and issuing warps to the softmax.
 //
 // Range: K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
 // softmax scale; V by one that changes only when a tile needs it, with O), q by one to a row.
@@ -19,22 +20,25 @@
 #include "kv_q4.cuh"
 #include "tcgen05_common.cuh"
 #include <algorithm>
+#include <type_traits>
 
 namespace rlz {
 
 // 3113: a page id outside the cache (read as page 0); 3114: rows beyond the page table (not computed); 3115: a bounded wait ran out
 __device__ int g_prefill_q4_error = 0;
 
-constexpr int QP_THREADS = 288, QP_ROWS = 128, QP_KEYS = 128, QP_MAX_CTAS = 296, QP_MIN_TILES = 2;
+constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148, QP_MIN_TILES = 2;
+constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 88, QP_REGS_ISSUE = 40;      // 256, 256 and 128 threads: 60416 of the launch's 640 x 96
 constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
 constexpr int QP_COUNTERS = 320;               // floats in front of the parts: arrival counters
 
 struct QpSmem {
-  unsigned long long q_full, k_full, k_empty, v_full, v_empty, s_full, p_full;
-  float kf[2], vf[2];                         // powers of two that the tile's K and V carry
+  unsigned long long q_full[2], s_full[2], p_full[2], o_full[2];        // of the groups
+  unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];      // of the buffers
+  float kf[4], vf[2];                         // powers of two that the tiles carry (K's are read after the buffer is free again)
   float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
   uint32_t tmem;
-  int last;
+  int last[2];
 };
 
 __device__ __forceinline__ float qp_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -80,30 +84,56 @@ __device__ __forceinline__ void codes_f16(uint32_t w, __half2 (&c)[4]) {
   c[2] = __hsub2(*(const __half2*)&r[2], magic); c[3] = __hfma2(*(const __half2*)&r[3], sixteenth, back);
 }
 
-struct QpRange { int k0, tiles; };            // first key and number of key tiles of a CTA
+template <int R> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+}
+// the registers go through the wait, so that nothing that uses them can move in front of it
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :: "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*(uint64_t*)&d) : "l"(*(const uint64_t*)&a), "l"(*(const uint64_t*)&b), "l"(*(const uint64_t*)&c));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(uint64_t*)&d) : "l"(*(const uint64_t*)&a), "l"(*(const uint64_t*)&b));
+  return d;
+}
 
 template <int D>
-__global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __grid_constant__ AttnPrefillParams p, const int nsplit) {
+__global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __grid_constant__ AttnPrefillParams p, const int nsplit) {
   constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, NSLAB = (D + 63) / 64, PB = q4_page_bytes(D);
-  constexpr uint32_t TMEM_COLS = 256;         // S and P: columns 0..127, O: 128..
+  constexpr int Q_BYTES = NSLAB * QP_SLAB, K_BYTES = NSLAB * QP_SLAB, V_BYTES = 2 * D * 128;
+  constexpr uint32_t TMEM_COLS = 512;         // S and P of the groups: columns 0.. and 128.., O: 256.. and 384..
   extern __shared__ __align__(1024) uint8_t qp_smem[];
   __shared__ QpSmem sm;
   uint8_t* Qs = (uint8_t*)(((uintptr_t)qp_smem + 1023) & ~(uintptr_t)1023);
-  uint8_t* Ks = Qs + NSLAB * QP_SLAB;
-  uint8_t* Vs = Ks + NSLAB * QP_SLAB;         // two slabs of [D rows x 64 keys]
+  uint8_t* Ks = Qs + 2 * Q_BYTES;
+  uint8_t* Vs = Ks + 2 * K_BYTES;             // a tile is two slabs of [D rows x 64 keys]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G, kvh = blockIdx.y;
-  const int mtile = (int)(gridDim.x / nsplit) - 1 - (int)blockIdx.x / nsplit, part = (int)blockIdx.x % nsplit;      // the longest rows first
+  const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G, kvh = blockIdx.y, mtiles = (int)gridDim.x / nsplit;
+  const int mtile = mtiles - 1 - (int)blockIdx.x / nsplit, part = (int)blockIdx.x % nsplit;      // the longest rows first
   const int m0 = mtile * QP_ROWS;
 
-  if (tid == 0) {
-    unsigned long long* bars[7] = {&sm.q_full, &sm.k_full, &sm.k_empty, &sm.v_full, &sm.v_empty, &sm.s_full, &sm.p_full};
-    const int count[7] = {128, 128, 1, 128, 1, 1, 128};
-#pragma unroll
-    for (int i = 0; i < 7; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(bars[i])), "r"(count[i]));
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (tid < 16) {
+    const int count = tid < 2 || (tid >= 4 && tid < 6) ? QP_GROUP : tid >= 8 && (tid & 2) == 0 ? 128 : 1;     // q, p; k and v full | s, o; k and v empty
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(&sm.q_full[0] + tid)), "r"(count));
   }
-  if (warp == 8) {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gm_smem_u32(&sm.tmem)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -117,7 +147,7 @@ __global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __
   // ---- keys of this CTA: the rows' range, in tiles from a page boundary on, divided over the parts -----------------------------
   const int pos0 = p.pos0_ptr ? *p.pos0_ptr : p.pos0;
   const int tok0 = m0 / G, tok1 = min(p.n_tokens, (m0 + QP_ROWS - 1) / G + 1);            // tokens of the tile
-  const int kend = pos0 + tok1;
+  const int kend = pos0 + tok1, groups = rows - m0 > QP_GROUP ? 2 : 1;
   bool ok = pos0 >= 0 && (kend - 1) / Q4_PAGE < p.pt_len;
   if (!ok && tid == 0) atomicExch(&g_prefill_q4_error, 3114);
   const int klo = p.window > 0 ? max(0, pos0 + tok0 + 1 - p.window) / Q4_PAGE * Q4_PAGE : 0;
@@ -125,219 +155,240 @@ __global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __
   const int j0 = part * all / parts, n_tiles = ok && part < parts ? (part + 1) * all / parts - j0 : 0;
   const int kbeg = klo + j0 * QP_KEYS;
 
-  if (n_tiles > 0 && warp < 4) {
+  if (warp < 8) {
     // ================================ softmax: one thread to a row ================================================================
-    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
-    const int row = m0 + tid, token = row / G, head = kvh * G + row - token * G;
-    const bool live = row < rows;
-    const int pos = pos0 + token;
-    float qs = 0.f;                                              // softmax scale of the row
-    {
-      const float* src = p.qkv + (int64_t)(live ? token : 0) * p.ld_qkv + p.q_off + (int64_t)(live ? head : 0) * D;
-      float top = 0.f;
-      if (live) for (int i = 0; i < D; ++i) top = fmaxf(top, fabsf(src[i]));
-      const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
-      qs = p.scale * 1.4426950408889634f / f;
-      for (int x = 0; x < NSLAB * 8; ++x) {                      // 8 dims in the order in which the keys' codes come out of a word
-        float v[8];
+    regs_up<QP_REGS_SOFTMAX>();
+    const int grp = warp >> 2, t = tid & 127;
+    if (n_tiles > 0 && grp < groups) {
+      const uint32_t lane_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(128 * grp), lane_o = lane_s + 256u;
+      const int row = m0 + grp * QP_GROUP + t, token = row / G, head = kvh * G + row - token * G;
+      const bool live = row < rows;
+      const int pos = pos0 + token;
+      float qs = 0.f;                                              // softmax scale of my row
+      // ---- queries: the warp takes its 32 rows one after another, 4 dims to a lane, and stores them as fp16 in the order in which
+      // the keys' codes come out of a word: (0, 4), (1, 5), (2, 6), (3, 7) of every 8 dims
+      uint8_t* q_tile = Qs + grp * Q_BYTES;
+      const bool vec = (((uintptr_t)p.qkv | (uintptr_t)(4 * p.ld_qkv) | (uintptr_t)(4 * p.q_off)) & 15) == 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += 16) {                          // 16 rows in flight
+        float4 v[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = live && 8 * x < D ? src[8 * x + i] * f : 0.f;
-        *(uint4*)(Qs + (x >> 3) * QP_SLAB + (tid >> 3) * 1024 + (tid & 7) * 128 + (((x & 7) ^ (tid & 7)) << 4)) =
-            make_uint4(qp_half2(v[0], v[4]), qp_half2(v[1], v[5]), qp_half2(v[2], v[6]), qp_half2(v[3], v[7]));
+        for (int i = 0; i < 16; ++i) {
+          const int gr = m0 + grp * QP_GROUP + (warp & 3) * 32 + i0 + i, tk = gr / G;
+          v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (gr < rows && lane < D / 4) {
+            const float* src = p.qkv + (int64_t)tk * p.ld_qkv + p.q_off + (int64_t)(kvh * G + gr - tk * G) * D + 4 * lane;
+            v[i] = vec ? __ldg((const float4*)src) : make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = (warp & 3) * 32 + i0 + i;
+          const float top = redux_max(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+          const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
+          if (lane == i0 + i) qs = p.scale * 1.4426950408889634f / f;
+          const bool odd = lane & 1;
+          const float s0 = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[i].y : v[i].w, 1);
+          const uint2 w = odd ? make_uint2(qp_half2(s0 * f, v[i].z * f), qp_half2(s1 * f, v[i].w * f))
+                              : make_uint2(qp_half2(v[i].x * f, s0 * f), qp_half2(v[i].y * f, s1 * f));
+          const int x = lane >> 1;                                  // 8 dims from 8 x on
+          if (x < NSLAB * 8) *(uint2*)(q_tile + (x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4) + 8 * (lane & 1)) = w;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      gm_arrive((uint64_t*)&sm.q_full);
-    }
-    float m = -INFINITY, l = 0.f, vf = 1.f;
-    const int pos_first = pos0 + tok0, lo_last = p.window > 0 ? pos0 + tok1 - p.window : 0;     // masks are needed beyond these
-    for (int j = 0; ok && j < n_tiles; ++j) {
-      const int k0 = kbeg + j * QP_KEYS;
-      const uint32_t ph = (uint32_t)j & 1u;
-      ok = qp_wait(&sm.s_full, ph);                               // the scores, and with them the product before and the tile's powers of two
-      if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
-      tc_after();
-      const float sc = qs / sm.kf[ph], vn = sm.vf[ph];
-      const bool edge = k0 + QP_KEYS - 1 > pos_first || k0 < lo_last;
-      const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
-      float top = -INFINITY;
-#pragma unroll 1
-      for (int c0 = 0; c0 < QP_KEYS; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld32(t_lane + (uint32_t)c0, r);
-        if (edge) {
+      gm_arrive((uint64_t*)&sm.q_full[grp]);
+
+      float m = -INFINITY, vf = 1.f;
+      float2 l2 = make_float2(0.f, 0.f);
+      const int row_first = m0 + grp * QP_GROUP, row_last = min(rows, row_first + QP_GROUP) - 1;
+      const int pos_first = pos0 + row_first / G, lo_last = p.window > 0 ? pos0 + row_last / G + 1 - p.window : 0;     // masks are needed beyond these
+      for (int j = 0; ok && j < n_tiles; ++j) {
+        const int k0 = kbeg + j * QP_KEYS, buf = j & 1;
+        ok = qp_wait(&sm.s_full[grp], (uint32_t)j & 1u);              // the scores, and with them the tile's power of two of K
+        if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+        tc_after();
+        const float sc = qs / sm.kf[j & 3];
+        const bool edge = k0 + QP_KEYS - 1 > pos_first || k0 < lo_last;
+        const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
+        // EDGE: some entries are masked
+        auto tile = [&](auto edge_c) {
+          constexpr bool EDGE = decltype(edge_c)::value;
+          float top = -INFINITY, top1 = -INFINITY;
+          {
+            uint32_t r[2][32];
+            tmem_ld32_async(lane_s, r[0]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) if (c0 + i < vis_hi && c0 + i >= vis_lo) top = fmaxf(top, __uint_as_float(r[i]));
-        } else {
-          float t0 = __uint_as_float(r[0]), t1 = __uint_as_float(r[1]);
+            for (int c = 0; c < 4; ++c) {
+              tmem_wait_ld(r[c & 1]);
+              if (c < 3) tmem_ld32_async(lane_s + (uint32_t)(32 * (c + 1)), r[(c + 1) & 1]);
+              uint32_t (&x)[32] = r[c & 1];
 #pragma unroll
-          for (int i = 2; i < 32; i += 2) { t0 = fmaxf(t0, __uint_as_float(r[i])); t1 = fmaxf(t1, __uint_as_float(r[i + 1])); }
-          top = fmaxf(top, fmaxf(t0, t1));
-        }
-      }
-      top *= sc;
-      if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
-        const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
-        if (j > 0) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 16) {
-            uint32_t r[16];
-            tmem_ld16(t_lane + 128u + (uint32_t)c0, r);
+              for (int i = 0; i < 32; i += 4) {
+                float y[4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * co);
-            tmem_st16(t_lane + 128u + (uint32_t)c0, r);
-          }
-        }
-        l *= corr; m = mn; vf = vn;
-      }
-      const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
-#pragma unroll 1
-      for (int c0 = 0; c0 < QP_KEYS; c0 += 32) {
-        uint32_t r[32], w[16];
-        tmem_ld32(t_lane + (uint32_t)c0, r);
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float e0 = qp_ex2(fmaf(__uint_as_float(r[i]), sc, base)), e1 = qp_ex2(fmaf(__uint_as_float(r[i + 1]), sc, base));
-          if (edge) {
-            if (!(c0 + i < vis_hi && c0 + i >= vis_lo)) e0 = 0.f;
-            if (!(c0 + i + 1 < vis_hi && c0 + i + 1 >= vis_lo)) e1 = 0.f;
-          }
-          l += e0 + e1;
-          w[i >> 1] = qp_half2(e0, e1);
-        }
-        tmem_st16(t_lane + (uint32_t)(c0 >> 1), w);               // columns c0 / 2 ..: their scores have been read
-      }
-      tmem_wait_st();
-      tc_before();
-      gm_arrive((uint64_t*)&sm.p_full);
-    }
-    if (ok) ok = qp_wait(&sm.v_empty, (uint32_t)(n_tiles - 1) & 1u);       // the last product
-    if (qp_agree<1>(ok)) {
-      tc_after();
-      const float inv_vf = 1.f / vf;
-      auto store = [&](int c, const float* v) {                   // 16 finished values
-        const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
-        if (p.out_bf16) {
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-          uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
-          dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        }
-      };
-      const int tile_id = kvh * (int)(gridDim.x / nsplit) + mtile;
-      float* slot = p.scratch + QP_COUNTERS + ((int64_t)tile_id * nsplit + part) * QP_ROWS * (D + 4) + (int64_t)tid * (D + 4);
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(t_lane + 128u + (uint32_t)c, r);
-        float v[16];
-        const float f = parts == 1 ? inv_vf / l : inv_vf;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
-        if (parts == 1) { if (live) store(c, v); }
-        else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *(float4*)(slot + c + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        }
-      }
-      if (parts > 1) {
-        *(float2*)(slot + D) = make_float2(m, l);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (tid == 0) {
-          int32_t* ctr = (int32_t*)p.scratch + tile_id;
-          __threadfence();
-          sm.last = atomicAdd(ctr, 1) == parts - 1;
-          if (sm.last) { *ctr = 0; __threadfence(); }             // zero again for the next launch
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (sm.last && live) {
-          const float* src = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * QP_ROWS * (D + 4) + (int64_t)tid * (D + 4);
-          constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);
-          float mm = -INFINITY, ll = 0.f;
-          for (int i = 0; i < parts; ++i) mm = fmaxf(mm, __ldcg(src + i * step + D));
-          for (int i = 0; i < parts; ++i) { const float2 st = __ldcg((const float2*)(src + i * step + D)); if (st.x != -INFINITY) ll = fmaf(qp_ex2(st.x - mm), st.y, ll); }
-          const float inv = 1.f / ll;
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            float v[16] = {};
-            for (int i = 0; i < parts; ++i) {
-              const float mi = __ldcg(src + i * step + D), e = mi == -INFINITY ? 0.f : qp_ex2(mi - mm) * inv;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float4 x = __ldcg((const float4*)(src + i * step + c + 4 * q));
-                v[4 * q] = fmaf(e, x.x, v[4 * q]); v[4 * q + 1] = fmaf(e, x.y, v[4 * q + 1]); v[4 * q + 2] = fmaf(e, x.z, v[4 * q + 2]); v[4 * q + 3] = fmaf(e, x.w, v[4 * q + 3]);
+                for (int e = 0; e < 4; ++e)
+                  y[e] = EDGE && !(32 * c + i + e < vis_hi && 32 * c + i + e >= vis_lo) ? -INFINITY : __uint_as_float(x[i + e]);
+                top = max3(top, y[0], y[1]);
+                top1 = max3(top1, y[2], y[3]);
               }
             }
-            store(c, v);
+          }
+          top = fmaxf(top, top1) * sc;
+          ok = qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u);      // the tile's power of two of V
+          if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; return; }
+          const float vn = sm.vf[buf];
+          if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
+            const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
+            if (j > 0) {                                               // (the product before has ended: the issuing warp waits for it before it overwrites S)
+#pragma unroll 1
+              for (int c0 = 0; c0 < D; c0 += 16) {
+                uint32_t r[16];
+                tmem_ld16(lane_o + (uint32_t)c0, r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * co);
+                tmem_st16(lane_o + (uint32_t)c0, r);
+              }
+            }
+            l2.x *= corr; l2.y *= corr; m = mn; vf = vn;
+          }
+          const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
+          const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
+          uint32_t r[2][32];
+          tmem_ld32_async(lane_s, r[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld(r[c & 1]);
+            if (c < 3) tmem_ld32_async(lane_s + (uint32_t)(32 * (c + 1)), r[(c + 1) & 1]);
+            uint32_t (&x)[32] = r[c & 1];
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, b2);
+              float2 e = make_float2(qp_ex2(y.x), qp_ex2(y.y));
+              if (EDGE) {
+                if (!(32 * c + i < vis_hi && 32 * c + i >= vis_lo)) e.x = 0.f;
+                if (!(32 * c + i + 1 < vis_hi && 32 * c + i + 1 >= vis_lo)) e.y = 0.f;
+              }
+              l2 = add2(l2, e);
+              w[i >> 1] = qp_half2(e.x, e.y);
+            }
+            tmem_st16(lane_s + (uint32_t)(16 * c), w);                 // columns 16 c ..: their scores have been read, those on their way lie behind
+          }
+        };
+        if (edge) tile(std::true_type{}); else tile(std::false_type{});
+        if (!ok) break;
+        tmem_wait_st();
+        tc_before();
+        gm_arrive((uint64_t*)&sm.p_full[grp]);
+      }
+      if (ok) ok = qp_wait(&sm.o_full[grp], (uint32_t)(n_tiles - 1) & 1u);       // the last product
+      if (grp == 0 ? qp_agree<1>(ok) : qp_agree<2>(ok)) {
+        tc_after();
+        const float inv_vf = 1.f / vf, l = l2.x + l2.y;
+        auto store = [&](int c, const float* v) {                   // 16 finished values
+          const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
+          if (p.out_bf16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
+            dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        };
+        const int tile_id = kvh * mtiles + mtile;
+        constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);          // between the parts of a tile
+        const float* parts_of = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * step + (int64_t)(grp * QP_GROUP + t) * (D + 4);
+        float* slot = (float*)parts_of + part * step;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(lane_o + (uint32_t)c, r);
+          float v[16];
+          const float f = parts == 1 ? inv_vf / l : inv_vf;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
+          if (parts == 1) { if (live) store(c, v); }
+          else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(float4*)(slot + c + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+        if (parts > 1) {
+          *(float2*)(slot + D) = make_float2(m, l);
+          if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+          if (t == 0) {
+            int32_t* ctr = (int32_t*)p.scratch + 2 * tile_id + grp;
+            __threadfence();
+            sm.last[grp] = atomicAdd(ctr, 1) == parts - 1;
+            if (sm.last[grp]) { *ctr = 0; __threadfence(); }          // zero again for the next launch
+          }
+          if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+          if (sm.last[grp] && live) {
+            float mm = -INFINITY, ll = 0.f;
+            for (int i = 0; i < parts; ++i) mm = fmaxf(mm, __ldcg(parts_of + i * step + D));
+            for (int i = 0; i < parts; ++i) { const float2 st = __ldcg((const float2*)(parts_of + i * step + D)); if (st.x != -INFINITY) ll = fmaf(qp_ex2(st.x - mm), st.y, ll); }
+            const float inv = 1.f / ll;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float v[16] = {};
+              for (int i = 0; i < parts; ++i) {
+                const float mi = __ldcg(parts_of + i * step + D), e = mi == -INFINITY ? 0.f : qp_ex2(mi - mm) * inv;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const float4 x = __ldcg((const float4*)(parts_of + i * step + c + 4 * q));
+                  v[4 * q] = fmaf(e, x.x, v[4 * q]); v[4 * q + 1] = fmaf(e, x.y, v[4 * q + 1]); v[4 * q + 2] = fmaf(e, x.z, v[4 * q + 2]); v[4 * q + 3] = fmaf(e, x.w, v[4 * q + 3]);
+                }
+              }
+              store(c, v);
+            }
           }
         }
       }
     }
-  } else if (n_tiles > 0 && warp < 8) {
-    // ================================ decoding: a key row, and half a page of values, to a thread ===================================
-    const int t = tid - 128;
-    uint32_t kw[D / 8], vw[D / 8], km = 0u, vm[8];
-    auto row_of = [&](int key) {
-      int id = __ldg(p.page_table + key / Q4_PAGE);
+  } else if (warp < 16) {
+    // ================================ decoding ======================================================================================
+    regs_down<QP_REGS_DECODE>();
+    const int t = tid & 127;
+    const int last_page = (kend - 1) / Q4_PAGE * Q4_PAGE;
+    auto id_of = [&](int key) { return __ldg(p.page_table + min(key, last_page) / Q4_PAGE); };
+    auto row_of = [&](int id) {
       if ((unsigned)id >= (unsigned)p.num_pages) { atomicExch(&g_prefill_q4_error, 3113); id = 0; }
       return ((int64_t)id * p.n_kv_heads + kvh) * PB;
     };
-    const int last_page = (kend - 1) / Q4_PAGE * Q4_PAGE;
-    auto load_k = [&](int k0) {
-      const int key = k0 + t;
-      const uint8_t* src = (const uint8_t*)p.k_cache + row_of(min(key, last_page));
+    // largest magnitude that a row's codes can stand for; over all threads of the role
+    auto largest = [](uint32_t meta) { return fmaxf(fabsf(q4_min(meta)), fabsf(fmaf(15.f, q4_scale(meta), q4_min(meta)))); };
+    if (n_tiles > 0 && warp < 12) {
+      // -- keys: a token row to a thread
+      uint32_t kw[D / 8], km = 0u;
+      int id = id_of(kbeg + t);
+      auto load = [&](int k0) {
+        const int key = k0 + t;
+        const uint8_t* src = (const uint8_t*)p.k_cache + row_of(id);
 #pragma unroll
-      for (int i = 0; i < D / 8; i += 2) {
-        const uint2 v = __ldg((const uint2*)(src + (key % Q4_PAGE) * (D / 2) + 4 * i));
-        kw[i] = v.x; kw[i + 1] = v.y;
-      }
-      km = key < kend ? __ldg((const uint32_t*)(src + 8 * D + 4 * (key % Q4_PAGE))) : 0u;         // rows behind the last key count as 0
-    };
-    const int vh = (t >> 3) & 1, vg = t & 7;                       // page t / 16 of the tile, tokens 8 vh .. + 7, units vg of every 32 dims
-    auto load_v = [&](int k0) {
-      const int key = k0 + (t >> 4) * Q4_PAGE;
-      const uint8_t* src = (const uint8_t*)p.v_cache + row_of(min(key, last_page));
-      const uint32_t* w = (const uint32_t*)(src + (size_t)vh * 128 * NG + vg * 16 * NG);           // words [tq][g]
-#pragma unroll
-      for (int i = 0; i < 4 * NG; i += 4) { const uint4 v = __ldg((const uint4*)(w + i)); vw[i] = v.x; vw[i + 1] = v.y; vw[i + 2] = v.z; vw[i + 3] = v.w; }
-      if constexpr (TAIL) {                                        // bytes of both halves: mine of each word, as 16 bits
-        const uint4 v = __ldg((const uint4*)(src + 256 * NG + vg * 16));
-        vw[4 * NG] = __byte_perm(v.x, v.y, vh ? 0x7632 : 0x5410); vw[4 * NG + 1] = __byte_perm(v.z, v.w, vh ? 0x7632 : 0x5410);
-      }
-      const uint4 a = __ldg((const uint4*)(src + 8 * D + 32 * vh)), b = __ldg((const uint4*)(src + 8 * D + 32 * vh + 16));
-      const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vm[i] = key + 8 * vh + i < kend ? r[i] : 0u;
-    };
-    load_k(kbeg);
-    load_v(kbeg);
-    float vf = 0x1p100f;
-    for (int j = 0; j < n_tiles; ++j) {
-      const uint32_t ph = (uint32_t)j & 1u;
-      // powers of two for the tile: its largest value to [2^4, 2^5); the one of V stays as long as it keeps them below 2^12
-      auto largest = [](uint32_t meta) { return fmaxf(fabsf(q4_min(meta)), fabsf(fmaf(15.f, q4_scale(meta), q4_min(meta)))); };
-      float kt = largest(km), vt = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vt = fmaxf(vt, largest(vm[i]));
-      kt = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(kt)));
-      vt = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(vt)));
-      if (lane == 0) { sm.mag[ph][0][warp - 4] = kt; sm.mag[ph][1][warp - 4] = vt; }
-      if (!qp_agree<2>(ok)) break;
-      kt = fmaxf(fmaxf(sm.mag[ph][0][0], sm.mag[ph][0][1]), fmaxf(sm.mag[ph][0][2], sm.mag[ph][0][3]));
-      vt = fmaxf(fmaxf(sm.mag[ph][1][0], sm.mag[ph][1][1]), fmaxf(sm.mag[ph][1][2], sm.mag[ph][1][3]));
-      const float kf = qp_pow2(kt, 4);
-      if (vt * vf >= 4096.f) vf = qp_pow2(vt, 4);
-      if (t == 0) { sm.kf[ph] = kf; sm.vf[ph] = vf; }
-
-      if (j > 0) ok = qp_wait(&sm.k_empty, ph ^ 1u);
-      {
+        for (int i = 0; i < D / 8; i += 2) {
+          const uint2 v = __ldg((const uint2*)(src + (key % Q4_PAGE) * (D / 2) + 4 * i));
+          kw[i] = v.x; kw[i + 1] = v.y;
+        }
+        km = key < kend ? __ldg((const uint32_t*)(src + 8 * D + 4 * (key % Q4_PAGE))) : 0u;         // rows behind the last key count as 0
+        id = id_of(key + QP_KEYS);
+      };
+      load(kbeg);
+      for (int j = 0; j < n_tiles; ++j) {
+        const int buf = j & 1;
+        float top = redux_max(largest(km));
+        if (lane == 0) sm.mag[buf][0][warp & 3] = top;
+        if (!qp_agree<3>(ok)) break;
+        top = fmaxf(fmaxf(sm.mag[buf][0][0], sm.mag[buf][0][1]), fmaxf(sm.mag[buf][0][2], sm.mag[buf][0][3]));
+        const float kf = qp_pow2(top, 4);                              // the tile's largest value to [2^4, 2^5)
+        if (j >= 2) ok = qp_wait(&sm.k_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
+        if (t == 0) sm.kf[j & 3] = kf;
         const __half2 s2 = __float2half2_rn(q4_scale(km) * kf), m2 = __float2half2_rn(q4_min(km) * kf);
-        uint8_t* base = Ks + (t >> 3) * 1024 + (t & 7) * 128;
+        uint8_t* base = Ks + buf * K_BYTES + (t >> 3) * 1024 + (t & 7) * 128;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {                          // word i of the row: 8 dims from 8 x on
+        for (int i = 0; i < D / 8; ++i) {                              // word i of the row: 8 dims from 8 x on
           const int x = i < 4 * NG ? 4 * (i % NG) + i / NG : i;
           __half2 c[4];
           codes_f16(kw[i], c);
@@ -346,25 +397,57 @@ __global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __
           for (int q = 0; q < 4; ++q) { const __half2 v = __hfma2(c[q], s2, m2); o[q] = *(const uint32_t*)&v; }
           *(uint4*)(base + (x >> 3) * QP_SLAB + (((x & 7) ^ (t & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
+        if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        gm_arrive((uint64_t*)&sm.k_full[buf]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      gm_arrive((uint64_t*)&sm.k_full);
-      if (j + 1 < n_tiles) load_k(kbeg + (j + 1) * QP_KEYS);
-
-      if (j > 0) ok = qp_wait(&sm.v_empty, ph ^ 1u) && ok;
-      {
-        __half2 s2[4], m2[4];                                      // of the token pairs
+    } else if (n_tiles > 0) {
+      // -- values: half a page to a thread: page t / 16 of the tile, tokens 8 vh .. + 7, units vg of every 32 dims
+      uint32_t vw[D / 8], vm[8];
+      const int vh = (t >> 3) & 1, vg = t & 7;
+      int id = id_of(kbeg + (t >> 4) * Q4_PAGE);
+      auto load = [&](int k0) {
+        const int key = k0 + (t >> 4) * Q4_PAGE;
+        const uint8_t* src = (const uint8_t*)p.v_cache + row_of(id);
+        const uint32_t* w = (const uint32_t*)(src + (size_t)vh * 128 * NG + vg * 16 * NG);           // words [tq][g]
+#pragma unroll
+        for (int i = 0; i < 4 * NG; i += 4) { const uint4 v = __ldg((const uint4*)(w + i)); vw[i] = v.x; vw[i + 1] = v.y; vw[i + 2] = v.z; vw[i + 3] = v.w; }
+        if constexpr (TAIL) {                                          // bytes of both halves: mine of each word, as 16 bits
+          const uint4 v = __ldg((const uint4*)(src + 256 * NG + vg * 16));
+          vw[4 * NG] = __byte_perm(v.x, v.y, vh ? 0x7632 : 0x5410); vw[4 * NG + 1] = __byte_perm(v.z, v.w, vh ? 0x7632 : 0x5410);
+        }
+        const uint4 a = __ldg((const uint4*)(src + 8 * D + 32 * vh)), b = __ldg((const uint4*)(src + 8 * D + 32 * vh + 16));
+        const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vm[i] = key + 8 * vh + i < kend ? r[i] : 0u;
+        id = id_of(key + QP_KEYS);
+      };
+      load(kbeg);
+      float vf = 0x1p100f;
+      for (int j = 0; j < n_tiles; ++j) {
+        const int buf = j & 1;
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, largest(vm[i]));
+        top = redux_max(top);
+        if (lane == 0) sm.mag[buf][1][warp & 3] = top;
+        if (!qp_agree<4>(ok)) break;
+        top = fmaxf(fmaxf(sm.mag[buf][1][0], sm.mag[buf][1][1]), fmaxf(sm.mag[buf][1][2], sm.mag[buf][1][3]));
+        if (top * vf >= 4096.f) vf = qp_pow2(top, 4);                  // it stays as long as it keeps the values below 2^12
+        __half2 s2[4], m2[4];                                          // of the token pairs
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s2[i] = __floats2half2_rn(q4_scale(vm[2 * i]) * vf, q4_scale(vm[2 * i + 1]) * vf);
           m2[i] = __floats2half2_rn(q4_min(vm[2 * i]) * vf, q4_min(vm[2 * i + 1]) * vf);
         }
-        const int chunk = (t >> 3) & 7;                            // eight keys of the 64 of a slab
-        uint8_t* base = Vs + (t >> 6) * (D * 128);
+        if (j >= 2) ok = qp_wait(&sm.v_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
+        if (t == 0) sm.vf[buf] = vf;
+        const int chunk = (t >> 3) & 7;                                // eight keys of the 64 of a slab
+        uint8_t* base = Vs + buf * V_BYTES + (t >> 6) * (D * 128);
         auto put = [&](int dim, const uint32_t* o) { *(uint4*)(base + (dim >> 3) * 1024 + (dim & 7) * 128 + ((chunk ^ (dim & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]); };
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          uint32_t o[4][4];                                        // [dim][token pair]
+          uint32_t o[4][4];                                            // [dim][token pair]
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             __half2 c[4];
@@ -379,7 +462,7 @@ __global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __
           uint32_t o[2][4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const uint32_t two = vw[4 * NG + (q >> 1)] >> (16 * (q & 1));       // a byte to each token of the pair
+            const uint32_t two = vw[4 * NG + (q >> 1)] >> (16 * (q & 1));           // a byte to each token of the pair
             __half2 c[4];
             codes_f16((two & 0xFFu) | (two & 0xFF00u) << 8, c);
 #pragma unroll
@@ -388,51 +471,69 @@ __global__ void __launch_bounds__(QP_THREADS, 2) attn_prefill_q4_kernel(const __
 #pragma unroll
           for (int e = 0; e < 2; ++e) put(32 * NG + 2 * vg + e, o[e]);
         }
+        if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        gm_arrive((uint64_t*)&sm.v_full[buf]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      gm_arrive((uint64_t*)&sm.v_full);
-      if (j + 1 < n_tiles) load_v(kbeg + (j + 1) * QP_KEYS);
     }
-  } else if (n_tiles > 0 && warp == 8 && lane == 0) {
-    // ================================ the products =================================================================================
-    const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_ROWS >> 4) << 24);      // fp16 operands, fp32 sums
-    const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_ROWS >> 4) << 24);
-    ok = qp_wait(&sm.q_full, 0u);
-    for (int j = 0; ok && j < n_tiles; ++j) {
-      const uint32_t ph = (uint32_t)j & 1u;
-      ok = qp_wait(&sm.k_full, ph) && (j == 0 || qp_wait(&sm.v_empty, ph ^ 1u));       // the scores go where the product before read P
-      if (!ok) break;
-      tc_after();
+  } else {
+    regs_down<QP_REGS_ISSUE>();
+    if (n_tiles > 0 && warp == 16 && lane == 0) {
+      // ================================ the products ===============================================================================
+      const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
+      const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);
+      auto scores = [&](int g, int j) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        umma_bf16(tmem, make_sdesc_k_sw128(gm_smem_u32(Qs + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)),
-                  make_sdesc_k_sw128(gm_smem_u32(Ks + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)), id_s, kk > 0 ? 1u : 0u);
-      umma_commit((uint64_t*)&sm.s_full);
-      umma_commit((uint64_t*)&sm.k_empty);
-      ok = qp_wait(&sm.p_full, ph) && qp_wait(&sm.v_full, ph);
-      if (!ok) break;
-      tc_after();
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tmem + 128u * g, make_sdesc_k_sw128(gm_smem_u32(Qs + g * Q_BYTES + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)),
+                    make_sdesc_k_sw128(gm_smem_u32(Ks + (j & 1) * K_BYTES + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)), id_s, kk > 0 ? 1u : 0u);
+        umma_commit((uint64_t*)&sm.s_full[g]);
+        if (g == groups - 1) umma_commit((uint64_t*)&sm.k_empty[j & 1]);
+      };
+      ok = qp_wait(&sm.k_full[0], 0u);
+      for (int g = 0; ok && g < groups; ++g) { ok = qp_wait(&sm.q_full[g], 0u); if (ok) { tc_after(); scores(g, 0); } }
+      for (int j = 0; ok && j < n_tiles; ++j) {
+        const int buf = j & 1;
+        ok = qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u) && (j + 1 >= n_tiles || qp_wait(&sm.k_full[buf ^ 1], (uint32_t)((j + 1) >> 1) & 1u));
+        for (int g = 0; ok && g < groups; ++g) {
+          ok = qp_wait(&sm.p_full[g], (uint32_t)j & 1u);
+          if (!ok) break;
+          tc_after();
 #pragma unroll
-      for (int kk = 0; kk < QP_KEYS / 16; ++kk)
-        umma_f16_ts(tmem + 128u, tmem + (uint32_t)(8 * kk), make_sdesc_k_sw128(gm_smem_u32(Vs + (kk >> 2) * (D * 128))) + (uint64_t)(2 * (kk & 3)), id_o,
-                    j > 0 || kk > 0 ? 1u : 0u);
-      umma_commit((uint64_t*)&sm.v_empty);
+          for (int kk = 0; kk < QP_KEYS / 16; ++kk)
+            umma_f16_ts(tmem + 256u + 128u * g, tmem + 128u * g + (uint32_t)(8 * kk),
+                        make_sdesc_k_sw128(gm_smem_u32(Vs + buf * V_BYTES + (kk >> 2) * (D * 128))) + (uint64_t)(2 * (kk & 3)), id_o, j > 0 || kk > 0 ? 1u : 0u);
+          umma_commit((uint64_t*)&sm.o_full[g]);
+          if (g == groups - 1) umma_commit((uint64_t*)&sm.v_empty[buf]);
+          if (j + 1 < n_tiles) {
+            ok = qp_wait(&sm.o_full[g], (uint32_t)j & 1u);               // the new scores go where this product reads P
+            if (ok) { tc_after(); scores(g, j + 1); }
+          }
+        }
+      }
     }
   }
   tc_before();
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
 template <int D>
 static int launch_prefill_q4(const AttnPrefillParams& p, cudaStream_t st) {
   constexpr int NSLAB = (D + 63) / 64;
-  const size_t smem = (size_t)2 * NSLAB * QP_SLAB + 2 * D * 128 + 1024;
+  const size_t smem = (size_t)4 * NSLAB * QP_SLAB + 4 * D * 128 + 1024;
   static SmemOptIn opt;
   if (cudaError_t e = opt.ensure(attn_prefill_q4_kernel<D>, smem, 0); e != cudaSuccess) return (int)e;
+  // the roles' registers have to fit into what the launch brings, or the softmax would wait for them for good
+  static const bool regs_fit = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, attn_prefill_q4_kernel<D>) == cudaSuccess &&
+           a.numRegs * QP_THREADS >= 256 * (QP_REGS_SOFTMAX + QP_REGS_DECODE) + 128 * QP_REGS_ISSUE;
+  }();
+  if (!regs_fit) return -7;
   const int64_t rows = (int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads);
   const int mtiles = (int)((rows + QP_ROWS - 1) / QP_ROWS);
-  // parts of a row tile's keys: as many as fill two CTAs to an SM, if there is scratch for them
+  // parts of a row tile's keys: as many as fill the SMs, if there is scratch for them
   const bool room = p.scratch && p.scratch_floats >= (int64_t)QP_MAX_CTAS * QP_ROWS * (D + 4) + QP_COUNTERS;
   const int nsplit = room ? std::max(1, std::min(32, QP_MAX_CTAS / (mtiles * p.n_kv_heads))) : 1;
   return (int)launch(attn_prefill_q4_kernel<D>, dim3(mtiles * nsplit, p.n_kv_heads), dim3(QP_THREADS), smem, st, p, nsplit);

@@ -39,7 +39,7 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())      # current_stream().cuda_stream without the stream object (1 us)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -392,13 +392,14 @@ def _check_q4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, n_kv_heads: i
             raise ValueError(f"a 4-bit cache is a contiguous uint8 [pages, {n_kv_heads}, 16, {head_dim // 2 + 4}] tensor, got {t.dtype} {tuple(t.shape)}")
     if v_cache.shape != k_cache.shape:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    dev = k_cache.get_device()
     for t in (v_cache, *others):
-        if t is not None and t.device != k_cache.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on {t.device} and {k_cache.device}: all of a call must be on one device")
 
 
 def _check_current_device(t: torch.Tensor) -> None:
-    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"tensors on {t.device}, which is not the current CUDA device")
 
 
@@ -470,6 +471,33 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, page_rows: t
     into the 4-bit cache at ``positions[i]`` of page ``page_rows[i]``.  Rows with a position below 0 are left out altogether.  No two
     rows of a call may name the same place.  Keys are normalised and rotated in 64 bits, so that the cached codes do not depend on
     which kernel wrote them."""
+    n, d = qkv.shape[0], head_dim
+    q = qkv if q_out is None else q_out
+    shape, dev = k_cache.shape, k_cache.get_device()
+    ld, ld_q = qkv.stride(0), q.stride(0)
+    f32, i32 = torch.float32, torch.int32
+    # one test for a call that is in order (half of the time of the separate ones), which say what is wrong with another
+    if not (d in Q4_HEAD_DIMS and k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8 and shape[1:] == (n_kv_heads, 16, d // 2 + 4)
+            and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous() and n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0
+            and qkv.dtype is f32 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= (n_heads + 2 * n_kv_heads) * d
+            and (q_out is None or (q.dtype is f32 and q.dim() == 2 and q.stride(1) == 1 and q.shape[0] >= n and q.shape[1] >= n_heads * d and q.get_device() == dev))
+            and positions.dtype is i32 and positions.dim() == 1 and positions.is_contiguous() and positions.shape[0] >= n and positions.get_device() == dev
+            and page_rows.dtype is i32 and page_rows.dim() == 1 and page_rows.is_contiguous() and page_rows.shape[0] >= n and page_rows.get_device() == dev
+            and qkv.get_device() == dev and v_cache.get_device() == dev and 0 <= rope_dim <= d and rope_dim % 2 == 0 and (q_norm_w is None) == (k_norm_w is None)
+            and all(w is None or (w.dtype is f32 and w.numel() == d and w.is_contiguous() and w.get_device() == dev) for w in (q_norm_w, k_norm_w))
+            and (rope_table is None or (rope_table.dtype is f32 and rope_table.shape[1:] == (rope_dim // 2, 2) and rope_table.is_contiguous() and rope_table.get_device() == dev))
+            and ld % 2 == 0 and ld_q % 2 == 0 and qkv.data_ptr() % 8 == 0 and q.data_ptr() % 8 == 0
+            and dev >= 0 and dev == torch._C._cuda_getDevice()):
+        _refuse_append(qkv, positions, page_rows, k_cache, v_cache, n_heads, n_kv_heads, head_dim, q_out, q_norm_w, k_norm_w, rope_dim, rope_table)
+    if n == 0:
+        return
+    p = S.QkAppendParams(qkv.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), page_rows.data_ptr(), ptr(q_norm_w),
+                         ptr(k_norm_w), ptr(rope_table), ld, ld_q, eps, n, n_heads, n_kv_heads, d, rope_dim, rope_type,
+                         0 if rope_table is None else rope_table.shape[0], shape[0], rope_theta, 0)
+    check(lib().rlz_qk_norm_rope_append(ctypes.byref(p), stream_ptr()), "qk_norm_rope_append")
+
+
+def _refuse_append(qkv, positions, page_rows, k_cache, v_cache, n_heads, n_kv_heads, head_dim, q_out, q_norm_w, k_norm_w, rope_dim, rope_table) -> None:
     if kv_format(k_cache, head_dim) != KV_Q4:
         raise ValueError("qk_norm_rope_append writes 4-bit caches (kv_cache_alloc(dtype='q4')); other formats take head_rmsnorm_, rope_ and kv_append")
     _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, positions, page_rows, q_out, q_norm_w, k_norm_w, rope_table)
@@ -494,16 +522,10 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, page_rows: t
     if rope_table is not None and (rope_table.dtype != torch.float32 or rope_table.dim() != 3 or tuple(rope_table.shape[1:]) != (rope_dim // 2, 2)
                                    or not rope_table.is_contiguous()):
         raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim / 2, 2] (cos, sin) tensor")
+    if qkv.stride(0) % 2 or q.stride(0) % 2 or qkv.data_ptr() % 8 or q.data_ptr() % 8:
+        raise ValueError("rows of qkv and q_out must start on 8-byte boundaries")
     _check_current_device(k_cache)
-    if n == 0:
-        return
-    p = S.QkAppendParams()
-    p.qkv, p.q_out, p.k_cache, p.v_cache = qkv.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    p.positions, p.page_rows, p.q_norm_w, p.k_norm_w, p.rope_table = positions.data_ptr(), page_rows.data_ptr(), ptr(q_norm_w), ptr(k_norm_w), ptr(rope_table)
-    p.ld, p.ld_q, p.eps, p.rows, p.n_heads, p.n_kv_heads, p.head_dim = qkv.stride(0), q.stride(0), eps, n, n_heads, n_kv_heads, head_dim
-    p.rope_dim, p.rope_type, p.rope_theta, p.num_pages = rope_dim, rope_type, rope_theta, k_cache.shape[0]
-    p.rope_table_len = 0 if rope_table is None else rope_table.shape[0]
-    check(lib().rlz_qk_norm_rope_append(ctypes.byref(p), stream_ptr()), "qk_norm_rope_append")
+    raise ValueError("qk_norm_rope_append: invalid arguments")
 
 
 # ------------------------------------------------------------------------------ small ops --

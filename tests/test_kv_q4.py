@@ -48,7 +48,7 @@ def _append_args(d=64, n=4, h=4, kvh=2):
 @pytest.mark.parametrize("change, word", [
     (dict(qkv=torch.zeros(4, 100)), "qkv"), (dict(qkv=torch.zeros(4, 512).half()), "qkv"), (dict(qkv=torch.zeros(512, 4).t()), "qkv"),
     (dict(positions=torch.zeros(3, dtype=torch.int32)), "positions"), (dict(positions=torch.zeros(4, dtype=torch.int64)), "positions"),
-    (dict(page_rows=torch.zeros(8, dtype=torch.int32)[::2]), "page_rows"), (dict(q_out=torch.zeros(4, 100)), "q_out"), (dict(q_out=torch.zeros(3, 256)), "q_out"),
+    (dict(page_rows=torch.zeros(8, dtype=torch.int32)[::2]), "page_rows"), (dict(qkv=torch.zeros(4, 513)[:, 1:]), "8-byte"), (dict(q_out=torch.zeros(4, 257)[:, :256]), "8-byte"), (dict(q_out=torch.zeros(4, 100)), "q_out"), (dict(q_out=torch.zeros(3, 256)), "q_out"),
     (dict(q_norm_w=torch.ones(64)), "together"), (dict(q_norm_w=torch.ones(64), k_norm_w=torch.ones(32)), "norm weights"),
     (dict(rope_dim=33), "rope_dim"), (dict(rope_dim=66), "rope_dim"), (dict(rope_dim=-2), "rope_dim"),
     (dict(rope_dim=64, rope_table=torch.zeros(5, 16, 2)), "rope_table"), (dict(n_heads=3), "divide"), (dict(head_dim=48), "4-bit"), (dict(n_kv_heads=4, n_heads=4), "4-bit cache is"),
