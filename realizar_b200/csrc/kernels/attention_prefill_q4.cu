@@ -28,12 +28,13 @@ namespace rlz {
 __device__ int g_prefill_q4_error = 0;
 
 constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148, QP_MIN_TILES = 2;
-constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 88, QP_REGS_ISSUE = 40;      // 256, 256 and 128 threads: 60416 of the launch's 640 x 96
+constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 88, QP_REGS_ISSUE = 48;      // 256, 256 and 128 threads: the launch's 640 x 96
 constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
 constexpr int QP_COUNTERS = 320;               // floats in front of the parts: arrival counters
 
 struct QpSmem {
   unsigned long long q_full[2], s_full[2], p_full[2], o_full[2];        // of the groups
+  unsigned long long p_half[2], pad[2];                                 // the first half of P
   unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];      // of the buffers
   float kf[4], vf[2];                         // powers of two that the tiles carry (K's are read after the buffer is free again)
   float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
@@ -48,10 +49,24 @@ __device__ __forceinline__ float qp_pow2(float x, int e) {
   const int k = e + 254 - (int)(__float_as_uint(x) >> 23);
   return __uint_as_float((uint32_t)max(1, min(k, 227)) << 23);
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
-               ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+// Products and their commits, called by a whole warp with the same arguments: one elected lane issues.  (With the warp together the
+// descriptors stay in uniform registers; issued from a branch of one lane, a product cost 80 clocks of moves.)
+// Operand tiles are given by the low words of their descriptors; the high word is that of all K-major tiles with 128-byte swizzle
+constexpr uint32_t QP_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t qp_desc_lo(const void* tile) { return (gm_smem_u32(tile) >> 4 & 0x3FFFu) | 1u << 16; }
+__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint32_t lo_a, uint32_t lo_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
+               "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%5, %5, %5, %5}, p;\n\t}\n"
+               ::"r"(tmem_d), "r"(lo_a), "r"(lo_b), "r"(idesc), "r"(accumulate), "r"(0u), "n"(QP_DESC_HI) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t lo_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %6};\n\t"
+               "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%5, %5, %5, %5}, p;\n\t}\n"
+               ::"r"(tmem_d), "r"(tmem_a), "r"(lo_b), "r"(idesc), "r"(accumulate), "r"(0u), "n"(QP_DESC_HI) : "memory");
+}
+__device__ __forceinline__ void umma_commit_warp(unsigned long long* bar) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
+               ::"r"(gm_smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -66,6 +81,13 @@ __device__ __forceinline__ bool qp_wait(unsigned long long* bar, uint32_t parity
   if (gm_wait((uint64_t*)bar, parity)) return true;
   atomicExch(&g_prefill_q4_error, 3115);
   return false;
+}
+
+// has the phase ended (the warp asks together)
+__device__ __forceinline__ bool qp_test(unsigned long long* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(gm_smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xFFFFFFFFu, done != 0);
 }
 
 // true when it is for all 128 threads of a role (also their barrier)
@@ -123,13 +145,13 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
   uint8_t* Qs = (uint8_t*)(((uintptr_t)qp_smem + 1023) & ~(uintptr_t)1023);
   uint8_t* Ks = Qs + 2 * Q_BYTES;
   uint8_t* Vs = Ks + 2 * K_BYTES;             // a tile is two slabs of [D rows x 64 keys]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
   const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G, kvh = blockIdx.y, mtiles = (int)gridDim.x / nsplit;
   const int mtile = mtiles - 1 - (int)blockIdx.x / nsplit, part = (int)blockIdx.x % nsplit;      // the longest rows first
   const int m0 = mtile * QP_ROWS;
 
-  if (tid < 16) {
-    const int count = tid < 2 || (tid >= 4 && tid < 6) ? QP_GROUP : tid >= 8 && (tid & 2) == 0 ? 128 : 1;     // q, p; k and v full | s, o; k and v empty
+  if (tid < 20) {
+    const int count = tid < 2 || tid == 4 || tid == 5 || tid == 8 || tid == 9 ? QP_GROUP : tid == 12 || tid == 13 || tid == 16 || tid == 17 ? 128 : 1;
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(&sm.q_full[0] + tid)), "r"(count));
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -204,39 +226,39 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       const int pos_first = pos0 + row_first / G, lo_last = p.window > 0 ? pos0 + row_last / G + 1 - p.window : 0;     // masks are needed beyond these
       for (int j = 0; ok && j < n_tiles; ++j) {
         const int k0 = kbeg + j * QP_KEYS, buf = j & 1;
-        ok = qp_wait(&sm.s_full[grp], (uint32_t)j & 1u);              // the scores, and with them the tile's power of two of K
+        // the scores, and with them the tile's power of two of K; that of V
+        ok = qp_wait(&sm.s_full[grp], (uint32_t)j & 1u) && qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u);
         if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
         tc_after();
-        const float sc = qs / sm.kf[j & 3];
+        const float sc = qs / sm.kf[j & 3], vn = sm.vf[buf];
         const bool edge = k0 + QP_KEYS - 1 > pos_first || k0 < lo_last;
         const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
         // EDGE: some entries are masked
         auto tile = [&](auto edge_c) {
           constexpr bool EDGE = decltype(edge_c)::value;
           float top = -INFINITY, top1 = -INFINITY;
-          {
-            uint32_t r[2][32];
-            tmem_ld32_async(lane_s, r[0]);
+          uint32_t r[2][32];
+          auto seen = [&](int key) { return !EDGE || (key < vis_hi && key >= vis_lo); };
+          auto largest_of = [&](const uint32_t (&x)[32], int key) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              tmem_wait_ld(r[c & 1]);
-              if (c < 3) tmem_ld32_async(lane_s + (uint32_t)(32 * (c + 1)), r[(c + 1) & 1]);
-              uint32_t (&x)[32] = r[c & 1];
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  y[e] = EDGE && !(32 * c + i + e < vis_hi && 32 * c + i + e >= vis_lo) ? -INFINITY : __uint_as_float(x[i + e]);
-                top = max3(top, y[0], y[1]);
-                top1 = max3(top1, y[2], y[3]);
-              }
+            for (int i = 0; i < 32; i += 4) {
+              top = max3(top, seen(key + i) ? __uint_as_float(x[i]) : -INFINITY, seen(key + i + 1) ? __uint_as_float(x[i + 1]) : -INFINITY);
+              top1 = max3(top1, seen(key + i + 2) ? __uint_as_float(x[i + 2]) : -INFINITY, seen(key + i + 3) ? __uint_as_float(x[i + 3]) : -INFINITY);
             }
+          };
+          // two loads of 32 scores in turn.  Not unrolled, here and below: spread over the whole tile, the compiler's order of loads,
+          // exponentials and stores took a fifth more time
+          tmem_ld32_async(lane_s, r[0]);
+#pragma unroll 1
+          for (int c = 0; c < QP_KEYS; c += 64) {
+            tmem_wait_ld(r[0]);
+            tmem_ld32_async(lane_s + (uint32_t)(c + 32), r[1]);
+            largest_of(r[0], c);
+            tmem_wait_ld(r[1]);
+            tmem_ld32_async(lane_s + (uint32_t)(c == 0 ? 64 : 0), r[0]);         // the last one is the first of the second pass
+            largest_of(r[1], c + 32);
           }
           top = fmaxf(top, top1) * sc;
-          ok = qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u);      // the tile's power of two of V
-          if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; return; }
-          const float vn = sm.vf[buf];
           if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
             const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
             if (j > 0) {                                               // (the product before has ended: the issuing warp waits for it before it overwrites S)
@@ -253,33 +275,31 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           }
           const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
           const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
-          uint32_t r[2][32];
-          tmem_ld32_async(lane_s, r[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld(r[c & 1]);
-            if (c < 3) tmem_ld32_async(lane_s + (uint32_t)(32 * (c + 1)), r[(c + 1) & 1]);
-            uint32_t (&x)[32] = r[c & 1];
+          auto exponentials = [&](const uint32_t (&x)[32], int key) {
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const float2 y = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, b2);
-              float2 e = make_float2(qp_ex2(y.x), qp_ex2(y.y));
-              if (EDGE) {
-                if (!(32 * c + i < vis_hi && 32 * c + i >= vis_lo)) e.x = 0.f;
-                if (!(32 * c + i + 1 < vis_hi && 32 * c + i + 1 >= vis_lo)) e.y = 0.f;
-              }
+              const float2 e = make_float2(seen(key + i) ? qp_ex2(y.x) : 0.f, seen(key + i + 1) ? qp_ex2(y.y) : 0.f);
               l2 = add2(l2, e);
               w[i >> 1] = qp_half2(e.x, e.y);
             }
-            tmem_st16(lane_s + (uint32_t)(16 * c), w);                 // columns 16 c ..: their scores have been read, those on their way lie behind
+            tmem_st16(lane_s + (uint32_t)(key >> 1), w);               // columns key / 2 ..: their scores have been read, those on their way lie behind
+          };
+#pragma unroll 1
+          for (int c = 0; c < QP_KEYS; c += 64) {
+            tmem_wait_ld(r[0]);
+            tmem_ld32_async(lane_s + (uint32_t)(c + 32), r[1]);
+            exponentials(r[0], c);
+            tmem_wait_ld(r[1]);
+            if (c == 0) tmem_ld32_async(lane_s + 64u, r[0]);
+            exponentials(r[1], c + 32);
+            tmem_wait_st();
+            tc_before();
+            gm_arrive((uint64_t*)(c == 0 ? &sm.p_half[grp] : &sm.p_full[grp]));      // the product can begin with the first 64 keys
           }
         };
         if (edge) tile(std::true_type{}); else tile(std::false_type{});
-        if (!ok) break;
-        tmem_wait_st();
-        tc_before();
-        gm_arrive((uint64_t*)&sm.p_full[grp]);
       }
       if (ok) ok = qp_wait(&sm.o_full[grp], (uint32_t)(n_tiles - 1) & 1u);       // the last product
       if (grp == 0 ? qp_agree<1>(ok) : qp_agree<2>(ok)) {
@@ -478,38 +498,57 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
     }
   } else {
     regs_down<QP_REGS_ISSUE>();
-    if (n_tiles > 0 && warp == 16 && lane == 0) {
+    if (n_tiles > 0 && warp == 16) {
       // ================================ the products ===============================================================================
       const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
       const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);
+      const uint32_t q_lo = qp_desc_lo(Qs), k_lo = qp_desc_lo(Ks), v_lo = qp_desc_lo(Vs);
       auto scores = [&](int g, int j) {
+        uint32_t a = q_lo + (uint32_t)(g * (Q_BYTES >> 4)), b = k_lo + (uint32_t)((j & 1) * (K_BYTES >> 4));
+        asm volatile("" : "+r"(a), "+r"(b));                            // (or the sums below are all kept in registers, which do not suffice)
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem + 128u * g, make_sdesc_k_sw128(gm_smem_u32(Qs + g * Q_BYTES + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)),
-                    make_sdesc_k_sw128(gm_smem_u32(Ks + (j & 1) * K_BYTES + (kk >> 2) * QP_SLAB)) + (uint64_t)(2 * (kk & 3)), id_s, kk > 0 ? 1u : 0u);
-        umma_commit((uint64_t*)&sm.s_full[g]);
-        if (g == groups - 1) umma_commit((uint64_t*)&sm.k_empty[j & 1]);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (uint32_t)((kk >> 2) * (QP_SLAB >> 4) + 2 * (kk & 3));
+          umma_f16_ss(tmem + 128u * g, a + off, b + off, id_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit_warp(&sm.s_full[g]);
       };
-      ok = qp_wait(&sm.k_full[0], 0u);
-      for (int g = 0; ok && g < groups; ++g) { ok = qp_wait(&sm.q_full[g], 0u); if (ok) { tc_after(); scores(g, 0); } }
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        const int buf = j & 1;
-        ok = qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u) && (j + 1 >= n_tiles || qp_wait(&sm.k_full[buf ^ 1], (uint32_t)((j + 1) >> 1) & 1u));
-        for (int g = 0; ok && g < groups; ++g) {
-          ok = qp_wait(&sm.p_full[g], (uint32_t)j & 1u);
-          if (!ok) break;
-          tc_after();
+      auto values = [&](int g, int j, int half) {                       // O += P V over 64 keys
+        uint32_t pa = tmem + (uint32_t)(128 * g + 32 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
+        asm volatile("" : "+r"(pa), "+r"(b));
 #pragma unroll
-          for (int kk = 0; kk < QP_KEYS / 16; ++kk)
-            umma_f16_ts(tmem + 256u + 128u * g, tmem + 128u * g + (uint32_t)(8 * kk),
-                        make_sdesc_k_sw128(gm_smem_u32(Vs + buf * V_BYTES + (kk >> 2) * (D * 128))) + (uint64_t)(2 * (kk & 3)), id_o, j > 0 || kk > 0 ? 1u : 0u);
-          umma_commit((uint64_t*)&sm.o_full[g]);
-          if (g == groups - 1) umma_commit((uint64_t*)&sm.v_empty[buf]);
-          if (j + 1 < n_tiles) {
-            ok = qp_wait(&sm.o_full[g], (uint32_t)j & 1u);               // the new scores go where this product reads P
-            if (ok) { tc_after(); scores(g, j + 1); }
+        for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tmem + 256u + 128u * g, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, j > 0 || half + kk > 0 ? 1u : 0u);
+      };
+      // whatever a group is ready for goes out next: scores of tile js once the product of the tile before has ended (it reads P where
+      // they go), the two halves of the product of tile jp as P arrives.  While one group waits, the other's work is in the pipe
+      int js[2] = {0, groups > 1 ? 0 : n_tiles}, jp[2] = {0, js[1]}, half[2] = {0, 0};
+      uint32_t idle = 0;
+      while (js[0] < n_tiles || jp[0] < n_tiles || js[1] < n_tiles || jp[1] < n_tiles) {
+        bool moved = false;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (js[g] < n_tiles && js[g] == jp[g] && half[g] == 0 && qp_test(js[g] == 0 ? &sm.q_full[g] : &sm.o_full[g], js[g] == 0 ? 0u : (uint32_t)(js[g] - 1) & 1u) &&
+              qp_test(&sm.k_full[js[g] & 1], (uint32_t)(js[g] >> 1) & 1u)) {
+            tc_after();
+            scores(g, js[g]);
+            ++js[g];
+            if (js[g ^ 1] >= js[g]) umma_commit_warp(&sm.k_empty[(js[g] - 1) & 1]);        // both groups have used the keys
+            moved = true;
+          }
+          if (jp[g] < js[g] && jp[g] < n_tiles && qp_test(half[g] ? &sm.p_full[g] : &sm.p_half[g], (uint32_t)jp[g] & 1u)) {
+            tc_after();                                                 // (P comes after the softmax has seen that the values are there)
+            values(g, jp[g], half[g]);
+            if (half[g]) {
+              umma_commit_warp(&sm.o_full[g]);
+              ++jp[g];
+              if (jp[g ^ 1] >= jp[g]) umma_commit_warp(&sm.v_empty[(jp[g] - 1) & 1]);      // both groups have used the values
+            }
+            half[g] ^= 1;
+            moved = true;
           }
         }
+        if (moved) idle = 0;
+        else if (++idle > GM_WAIT_LIMIT) { if (lane == 0) atomicExch(&g_prefill_q4_error, 3115); break; }
       }
     }
   }
