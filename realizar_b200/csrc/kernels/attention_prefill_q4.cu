@@ -38,6 +38,7 @@ struct QpSmem {
   unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];      // of the buffers
   float kf[4], vf[2];                         // powers of two that the tiles carry (K's are read after the buffer is free again)
   float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
+  float qf[2][QP_GROUP];                      // powers of two of the query rows
   uint32_t tmem;
   int last[2];
 };
@@ -186,37 +187,45 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       const int row = m0 + grp * QP_GROUP + t, token = row / G, head = kvh * G + row - token * G;
       const bool live = row < rows;
       const int pos = pos0 + token;
-      float qs = 0.f;                                              // softmax scale of my row
-      // ---- queries: the warp takes its 32 rows one after another, 4 dims to a lane, and stores them as fp16 in the order in which
-      // the keys' codes come out of a word: (0, 4), (1, 5), (2, 6), (3, 7) of every 8 dims
+      // ---- queries: 8 dims to a lane, stored as fp16 in the order in which the keys' codes come out of a word: (0, 4), (1, 5), (2, 6),
+      // (3, 7) of every 8 dims.  A short loop: these instructions run once to a CTA, and fetching them takes longer than the loads
       uint8_t* q_tile = Qs + grp * Q_BYTES;
       const bool vec = (((uintptr_t)p.qkv | (uintptr_t)(4 * p.ld_qkv) | (uintptr_t)(4 * p.q_off)) & 15) == 0;
+      {
+        constexpr int LANES = D == 64 ? 8 : 16, STEP = 32 / LANES;     // lanes to a row, rows at once
+        const int x = lane % LANES, r0 = (warp & 3) * 32 + lane / LANES;
+        int gr = m0 + grp * QP_GROUP + r0, tk = gr / G, hd = gr - tk * G;
 #pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 16) {                          // 16 rows in flight
-        float4 v[16];
+        for (int r1 = r0; r1 < (warp & 3) * 32 + 32; r1 += 4 * STEP) {
+          float4 v[4][2];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int gr = m0 + grp * QP_GROUP + (warp & 3) * 32 + i0 + i, tk = gr / G;
-          v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (gr < rows && lane < D / 4) {
-            const float* src = p.qkv + (int64_t)tk * p.ld_qkv + p.q_off + (int64_t)(kvh * G + gr - tk * G) * D + 4 * lane;
-            v[i] = vec ? __ldg((const float4*)src) : make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3));
+          for (int i = 0; i < 4; ++i) {
+            v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (gr < rows && x < D / 8) {
+              const float* src = p.qkv + (int64_t)tk * p.ld_qkv + p.q_off + (int64_t)(kvh * G + hd) * D + 8 * x;
+              if (vec) { v[i][0] = __ldg((const float4*)src); v[i][1] = __ldg((const float4*)src + 1); }
+              else { v[i][0] = make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3)); v[i][1] = make_float4(__ldg(src + 4), __ldg(src + 5), __ldg(src + 6), __ldg(src + 7)); }
+            }
+            gr += STEP;
+            for (hd += STEP; hd >= G; hd -= G) ++tk;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = r1 + i * STEP;
+            const float4 a = v[i][0], b = v[i][1];
+            float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
+            if (x == 0) sm.qf[grp][r] = f;
+            if (x < NSLAB * 8)
+              *(uint4*)(q_tile + (x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(qp_half2(a.x * f, b.x * f), qp_half2(a.y * f, b.y * f), qp_half2(a.z * f, b.z * f), qp_half2(a.w * f, b.w * f));
           }
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = (warp & 3) * 32 + i0 + i;
-          const float top = redux_max(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
-          const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
-          if (lane == i0 + i) qs = p.scale * 1.4426950408889634f / f;
-          const bool odd = lane & 1;
-          const float s0 = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[i].y : v[i].w, 1);
-          const uint2 w = odd ? make_uint2(qp_half2(s0 * f, v[i].z * f), qp_half2(s1 * f, v[i].w * f))
-                              : make_uint2(qp_half2(v[i].x * f, s0 * f), qp_half2(v[i].y * f, s1 * f));
-          const int x = lane >> 1;                                  // 8 dims from 8 x on
-          if (x < NSLAB * 8) *(uint2*)(q_tile + (x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4) + 8 * (lane & 1)) = w;
-        }
       }
+      __syncwarp();
+      const float qs = p.scale * 1.4426950408889634f / sm.qf[grp][t];    // softmax scale of my row
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       gm_arrive((uint64_t*)&sm.q_full[grp]);
 
@@ -320,7 +329,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         };
         const int tile_id = kvh * mtiles + mtile;
         constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);          // between the parts of a tile
-        const float* parts_of = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * step + (int64_t)(grp * QP_GROUP + t) * (D + 4);
+        const float* parts_of = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * step + (int64_t)grp * QP_GROUP * (D + 4) + t;     // a column to 128 floats: a warp's rows lie together
         float* slot = (float*)parts_of + part * step;
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
@@ -333,11 +342,11 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           if (parts == 1) { if (live) store(c, v); }
           else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(float4*)(slot + c + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            for (int i = 0; i < 16; ++i) slot[(c + i) * QP_GROUP] = v[i];
           }
         }
         if (parts > 1) {
-          *(float2*)(slot + D) = make_float2(m, l);
+          slot[D * QP_GROUP] = m; slot[(D + 1) * QP_GROUP] = l;
           if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
           if (t == 0) {
             int32_t* ctr = (int32_t*)p.scratch + 2 * tile_id + grp;
@@ -348,19 +357,22 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
           if (sm.last[grp] && live) {
             float mm = -INFINITY, ll = 0.f;
-            for (int i = 0; i < parts; ++i) mm = fmaxf(mm, __ldcg(parts_of + i * step + D));
-            for (int i = 0; i < parts; ++i) { const float2 st = __ldcg((const float2*)(parts_of + i * step + D)); if (st.x != -INFINITY) ll = fmaf(qp_ex2(st.x - mm), st.y, ll); }
+#pragma unroll 4
+            for (int i = 0; i < parts; ++i) {
+              const float mi = __ldcg(parts_of + i * step + D * QP_GROUP), li = __ldcg(parts_of + i * step + (D + 1) * QP_GROUP), mn = fmaxf(mm, mi);
+              if (mn != -INFINITY) ll = fmaf(ll, qp_ex2(mm - mn), li * qp_ex2(mi - mn));
+              mm = mn;
+            }
             const float inv = 1.f / ll;
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               float v[16] = {};
+#pragma unroll 4
               for (int i = 0; i < parts; ++i) {
-                const float mi = __ldcg(parts_of + i * step + D), e = mi == -INFINITY ? 0.f : qp_ex2(mi - mm) * inv;
+                const float* part_i = parts_of + i * step;
+                const float e = qp_ex2(__ldcg(part_i + D * QP_GROUP) - mm) * inv;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const float4 x = __ldcg((const float4*)(parts_of + i * step + c + 4 * q));
-                  v[4 * q] = fmaf(e, x.x, v[4 * q]); v[4 * q + 1] = fmaf(e, x.y, v[4 * q + 1]); v[4 * q + 2] = fmaf(e, x.z, v[4 * q + 2]); v[4 * q + 3] = fmaf(e, x.w, v[4 * q + 3]);
-                }
+                for (int q = 0; q < 16; ++q) v[q] = fmaf(e, __ldcg(part_i + (c + q) * QP_GROUP), v[q]);
               }
               store(c, v);
             }
