@@ -35,7 +35,8 @@ constexpr int QP_COUNTERS = 320;               // floats in front of the parts: 
 struct QpSmem {
   unsigned long long q_full[2], s_full[2], p_full[2], o_full[2];        // of the groups
   unsigned long long p_half[2], pad[2];                                 // the first half of P
-  unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];      // of the buffers
+  unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];      // of the buffers (empty: an arrival from each group's products)
+  unsigned long long turn[2][4];                                        // a group's warps may do their exponentials
   float kf[4], vf[2];                         // powers of two that the tiles carry (K's are read after the buffer is free again)
   float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
   float qf[2][QP_GROUP];                      // powers of two of the query rows
@@ -149,10 +150,10 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
   const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G, kvh = blockIdx.y, mtiles = (int)gridDim.x / nsplit;
   const int mtile = mtiles - 1 - (int)blockIdx.x / nsplit, part = (int)blockIdx.x % nsplit;      // the longest rows first
-  const int m0 = mtile * QP_ROWS;
+  const int m0 = mtile * QP_ROWS, groups = rows - m0 > QP_GROUP ? 2 : 1;
 
-  if (tid < 20) {
-    const int count = tid < 2 || tid == 4 || tid == 5 || tid == 8 || tid == 9 ? QP_GROUP : tid == 12 || tid == 13 || tid == 16 || tid == 17 ? 128 : 1;
+  if (tid < 28) {
+    const int count = tid < 2 || tid == 4 || tid == 5 || tid == 8 || tid == 9 ? QP_GROUP : tid == 12 || tid == 13 || tid == 16 || tid == 17 ? 128 : tid >= 12 && tid < 20 ? groups : 1;
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(&sm.q_full[0] + tid)), "r"(count));
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
   // ---- keys of this CTA: the rows' range, in tiles from a page boundary on, divided over the parts -----------------------------
   const int pos0 = p.pos0_ptr ? *p.pos0_ptr : p.pos0;
   const int tok0 = m0 / G, tok1 = min(p.n_tokens, (m0 + QP_ROWS - 1) / G + 1);            // tokens of the tile
-  const int kend = pos0 + tok1, groups = rows - m0 > QP_GROUP ? 2 : 1;
+  const int kend = pos0 + tok1;
   bool ok = pos0 >= 0 && (kend - 1) / Q4_PAGE < p.pt_len;
   if (!ok && tid == 0) atomicExch(&g_prefill_q4_error, 3114);
   const int klo = p.window > 0 ? max(0, pos0 + tok0 + 1 - p.window) / Q4_PAGE * Q4_PAGE : 0;
@@ -192,14 +193,14 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       uint8_t* q_tile = Qs + grp * Q_BYTES;
       const bool vec = (((uintptr_t)p.qkv | (uintptr_t)(4 * p.ld_qkv) | (uintptr_t)(4 * p.q_off)) & 15) == 0;
       {
-        constexpr int LANES = D == 64 ? 8 : 16, STEP = 32 / LANES;     // lanes to a row, rows at once
+        constexpr int LANES = D == 64 ? 8 : 16, STEP = 32 / LANES, BATCH = 8;     // lanes to a row, rows at once and their loads in flight
         const int x = lane % LANES, r0 = (warp & 3) * 32 + lane / LANES;
         int gr = m0 + grp * QP_GROUP + r0, tk = gr / G, hd = gr - tk * G;
 #pragma unroll 1
-        for (int r1 = r0; r1 < (warp & 3) * 32 + 32; r1 += 4 * STEP) {
-          float4 v[4][2];
+        for (int r1 = r0; r1 < (warp & 3) * 32 + 32; r1 += BATCH * STEP) {
+          float4 v[BATCH][2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < BATCH; ++i) {
             v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (gr < rows && x < D / 8) {
               const float* src = p.qkv + (int64_t)tk * p.ld_qkv + p.q_off + (int64_t)(kvh * G + hd) * D + 8 * x;
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (hd += STEP; hd >= G; hd -= G) ++tk;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < BATCH; ++i) {
             const int r = r1 + i * STEP;
             const float4 a = v[i][0], b = v[i][1];
             float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
@@ -284,6 +285,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           }
           const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
           const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
+          // in turn with the other group's warp on the same scheduler: while one does its exponentials, the other waits for products or
+          // looks for its maxima
+          if (groups > 1 && grp + j > 0) ok = __all_sync(0xFFFFFFFFu, qp_wait(&sm.turn[grp][warp & 3], (uint32_t)(j + grp - 1) & 1u));
           auto exponentials = [&](const uint32_t (&x)[32], int key) {
             uint32_t w[16];
 #pragma unroll
@@ -303,6 +307,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             tmem_wait_ld(r[1]);
             if (c == 0) tmem_ld32_async(lane_s + 64u, r[0]);
             exponentials(r[1], c + 32);
+            if (c > 0 && groups > 1 && lane == 0) gm_arrive((uint64_t*)&sm.turn[grp ^ 1][warp & 3]);
             tmem_wait_st();
             tc_before();
             gm_arrive((uint64_t*)(c == 0 ? &sm.p_half[grp] : &sm.p_full[grp]));      // the product can begin with the first 64 keys
@@ -328,24 +333,29 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           }
         };
         const int tile_id = kvh * mtiles + mtile;
+        constexpr int COLS = D % 32 ? 16 : 32;
         constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);          // between the parts of a tile
         const float* parts_of = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * step + (int64_t)grp * QP_GROUP * (D + 4) + t;     // a column to 128 floats: a warp's rows lie together
         float* slot = (float*)parts_of + part * step;
+        if (parts == 1) {
+          const float f = inv_vf / l;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t r[16];
-          tmem_ld16(lane_o + (uint32_t)c, r);
-          float v[16];
-          const float f = parts == 1 ? inv_vf / l : inv_vf;
+          for (int c = 0; c < D; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(lane_o + (uint32_t)c, r);
+            float v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
-          if (parts == 1) { if (live) store(c, v); }
-          else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) slot[(c + i) * QP_GROUP] = v[i];
+            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
+            if (live) store(c, v);
           }
-        }
-        if (parts > 1) {
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(lane_o + (uint32_t)c, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) __stcg(slot + (c + i) * QP_GROUP, __uint_as_float(r[i]) * inv_vf);
+          }
           slot[D * QP_GROUP] = m; slot[(D + 1) * QP_GROUP] = l;
           if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
           if (t == 0) {
@@ -365,16 +375,17 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             }
             const float inv = 1.f / ll;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              float v[16] = {};
-#pragma unroll 4
+            for (int c = 0; c < D; c += COLS) {
+              float v[COLS] = {};
+#pragma unroll 2
               for (int i = 0; i < parts; ++i) {
                 const float* part_i = parts_of + i * step;
                 const float e = qp_ex2(__ldcg(part_i + D * QP_GROUP) - mm) * inv;
 #pragma unroll
-                for (int q = 0; q < 16; ++q) v[q] = fmaf(e, __ldcg(part_i + (c + q) * QP_GROUP), v[q]);
+                for (int q = 0; q < COLS; ++q) v[q] = fmaf(e, __ldcg(part_i + (c + q) * QP_GROUP), v[q]);
               }
-              store(c, v);
+#pragma unroll
+              for (int q = 0; q < COLS; q += 16) store(c + q, v + q);
             }
           }
         }
@@ -510,57 +521,37 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
     }
   } else {
     regs_down<QP_REGS_ISSUE>();
-    if (n_tiles > 0 && warp == 16) {
-      // ================================ the products ===============================================================================
+    if (warp < 16 + groups) {
+      // ================================ the products: a warp to a group, so that no group's waits hold up the other =====================
+      const int g = warp - 16;
       const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
       const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);
-      const uint32_t q_lo = qp_desc_lo(Qs), k_lo = qp_desc_lo(Ks), v_lo = qp_desc_lo(Vs);
-      auto scores = [&](int g, int j) {
-        uint32_t a = q_lo + (uint32_t)(g * (Q_BYTES >> 4)), b = k_lo + (uint32_t)((j & 1) * (K_BYTES >> 4));
-        asm volatile("" : "+r"(a), "+r"(b));                            // (or the sums below are all kept in registers, which do not suffice)
+      const uint32_t q_lo = qp_desc_lo(Qs + g * Q_BYTES), k_lo = qp_desc_lo(Ks), v_lo = qp_desc_lo(Vs), s_col = tmem + 128u * g, o_col = s_col + 256u;
+      auto both = [&](unsigned long long* bar, uint32_t parity) { const bool r = __all_sync(0xFFFFFFFFu, qp_wait(bar, parity)); tc_after(); return r; };
+      auto values = [&](int j, int half) {                              // O += P V over 64 keys
+        const uint32_t pa = s_col + (uint32_t)(32 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) umma_f16_ts(o_col, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, j > 0 || half + kk > 0 ? 1u : 0u);
+      };
+      for (int j = 0; j < n_tiles; ++j) {
+        const int buf = j & 1;
+        // scores, once the product of the tile before has ended (it reads P where they go)
+        if (!both(&sm.k_full[buf], (uint32_t)(j >> 1) & 1u) || !both(j == 0 ? &sm.q_full[g] : &sm.o_full[g], j == 0 ? 0u : (uint32_t)(j - 1) & 1u)) break;
+        const uint32_t b = k_lo + (uint32_t)(buf * (K_BYTES >> 4));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (uint32_t)((kk >> 2) * (QP_SLAB >> 4) + 2 * (kk & 3));
-          umma_f16_ss(tmem + 128u * g, a + off, b + off, id_s, kk > 0 ? 1u : 0u);
+          umma_f16_ss(s_col, q_lo + off, b + off, id_s, kk > 0 ? 1u : 0u);
         }
         umma_commit_warp(&sm.s_full[g]);
-      };
-      auto values = [&](int g, int j, int half) {                       // O += P V over 64 keys
-        uint32_t pa = tmem + (uint32_t)(128 * g + 32 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
-        asm volatile("" : "+r"(pa), "+r"(b));
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tmem + 256u + 128u * g, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, j > 0 || half + kk > 0 ? 1u : 0u);
-      };
-      // whatever a group is ready for goes out next: scores of tile js once the product of the tile before has ended (it reads P where
-      // they go), the two halves of the product of tile jp as P arrives.  While one group waits, the other's work is in the pipe
-      int js[2] = {0, groups > 1 ? 0 : n_tiles}, jp[2] = {0, js[1]}, half[2] = {0, 0};
-      uint32_t idle = 0;
-      while (js[0] < n_tiles || jp[0] < n_tiles || js[1] < n_tiles || jp[1] < n_tiles) {
-        bool moved = false;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (js[g] < n_tiles && js[g] == jp[g] && half[g] == 0 && qp_test(js[g] == 0 ? &sm.q_full[g] : &sm.o_full[g], js[g] == 0 ? 0u : (uint32_t)(js[g] - 1) & 1u) &&
-              qp_test(&sm.k_full[js[g] & 1], (uint32_t)(js[g] >> 1) & 1u)) {
-            tc_after();
-            scores(g, js[g]);
-            ++js[g];
-            if (js[g ^ 1] >= js[g]) umma_commit_warp(&sm.k_empty[(js[g] - 1) & 1]);        // both groups have used the keys
-            moved = true;
-          }
-          if (jp[g] < js[g] && jp[g] < n_tiles && qp_test(half[g] ? &sm.p_full[g] : &sm.p_half[g], (uint32_t)jp[g] & 1u)) {
-            tc_after();                                                 // (P comes after the softmax has seen that the values are there)
-            values(g, jp[g], half[g]);
-            if (half[g]) {
-              umma_commit_warp(&sm.o_full[g]);
-              ++jp[g];
-              if (jp[g ^ 1] >= jp[g]) umma_commit_warp(&sm.v_empty[(jp[g] - 1) & 1]);      // both groups have used the values
-            }
-            half[g] ^= 1;
-            moved = true;
-          }
-        }
-        if (moved) idle = 0;
-        else if (++idle > GM_WAIT_LIMIT) { if (lane == 0) atomicExch(&g_prefill_q4_error, 3115); break; }
+        if (j + 2 < n_tiles) umma_commit_warp(&sm.k_empty[buf]);
+        // the halves of the product as P arrives (it comes after the softmax has seen that the values are there)
+        if (!both(&sm.p_half[g], (uint32_t)j & 1u)) break;
+        values(j, 0);
+        if (!both(&sm.p_full[g], (uint32_t)j & 1u)) break;
+        values(j, 1);
+        umma_commit_warp(&sm.o_full[g]);
+        if (j + 2 < n_tiles) umma_commit_warp(&sm.v_empty[buf]);
       }
     }
   }
