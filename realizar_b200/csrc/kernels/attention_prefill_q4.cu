@@ -14,8 +14,10 @@
 // Range: K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
 // softmax scale; V by one that changes only when a tile needs it, with O), q by one to a row.
 //
-// Few rows over many keys: the keys of a row tile are divided over several CTAs, which leave their parts in scratch; the last of
-// them to arrive joins them in order.
+// Split, in tiles of 128 keys.  Few row tiles (256 rows of a kv head): to each the same number of CTAs, nsplit.  Many, or a number that
+// would leave SMs idle: one CTA to an SM, and the key tiles of all row tiles are divided evenly (nsplit = 0).  A CTA that has only some
+// keys of a row tile leaves its part in scratch, and the last of the tile's CTAs to arrive joins them in a fixed order.  Between two
+// row tiles a CTA starts over: all roles meet and the barriers are set up again.  Without scratch a CTA takes a row tile.
 #include "attention_q4.cuh"
 #include "kv_q4.cuh"
 #include "tcgen05_common.cuh"
@@ -27,10 +29,18 @@ namespace rlz {
 // 3113: a page id outside the cache (read as page 0); 3114: rows beyond the page table (not computed); 3115: a bounded wait ran out
 __device__ int g_prefill_q4_error = 0;
 
-constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148, QP_MIN_TILES = 2;
+constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148;
+constexpr int QP_MIN_TILES = 2, QP_SEG_COST = 5;      // least share of a CTA; what another row tile costs it, in key tiles (12 us)
 constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 88, QP_REGS_ISSUE = 48;      // 256, 256 and 128 threads: the launch's 640 x 96
 constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
-constexpr int QP_COUNTERS = 320;               // floats in front of the parts: arrival counters
+constexpr int QP_COUNTERS = 640;               // floats in front of the parts: arrival counters, one to each of a CTA's two slots and group
+
+// key tiles j0 .. j0 + n - 1 of the `all` of row tile mt of a kv head; the tiles' first key and the first key behind them
+struct QpSeg { int kvh, mt, j0, n, all, klo, kend; };
+struct QpShape { int G, rows, mtiles, pos0; };
+// how the key tiles are divided: `left` is the share of this CTA; of an even division, tiles to a CTA and how many have one more; else
+// (each = 0) parts of a row tile
+struct QpSched { int left, each, more, parts; QpShape z; };
 
 struct QpSmem {
   unsigned long long q_full[2], s_full[2], p_full[2], o_full[2];        // of the groups
@@ -42,6 +52,9 @@ struct QpSmem {
   float qf[2][QP_GROUP];                      // powers of two of the query rows
   uint32_t tmem;
   int last[2];
+  QpSched sched;
+  QpSeg seg;                                  // row tile that is worked on (n = 0: none is left)
+  int done, fail;                             // key tiles of my share in front of it; a wait has run out
 };
 
 __device__ __forceinline__ float qp_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -137,6 +150,61 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// a row tile's keys (all = 0: its rows lie beyond the page table)
+__device__ __forceinline__ QpSeg qp_rows(const AttnPrefillParams& p, const QpShape& z, int kvh, int mt) {
+  QpSeg s = {kvh, mt, 0, 0, 0, 0, 0};
+  const int tok0 = mt * QP_ROWS / z.G, tok1 = min(p.n_tokens, (mt * QP_ROWS + QP_ROWS - 1) / z.G + 1);
+  s.kend = z.pos0 + tok1;
+  if (z.pos0 < 0 || (s.kend - 1) / Q4_PAGE >= p.pt_len) { atomicExch(&g_prefill_q4_error, 3114); return s; }
+  s.klo = p.window > 0 ? max(0, z.pos0 + tok0 + 1 - p.window) / Q4_PAGE * Q4_PAGE : 0;
+  s.all = (s.kend - s.klo + QP_KEYS - 1) / QP_KEYS;
+  return s;
+}
+// the next row tile with keys, of which the CTA has at most `left` tiles (left > 0: there is one)
+__device__ __forceinline__ QpSeg qp_next(const AttnPrefillParams& p, const QpShape& z, int kvh, int mt, int left) {
+  for (;;) {
+    if (++mt == z.mtiles) { mt = 0; ++kvh; }
+    QpSeg s = qp_rows(p, z, kvh, mt);
+    if (s.all) { s.n = min(s.all, left); return s; }
+  }
+}
+
+// first key tile of CTA c when all are divided evenly, and the CTA that has a tile: the first `more` of them have one tile more
+__device__ __forceinline__ int qp_first(const QpSched& s, int c) { return c * s.each + min(c, s.more); }
+__device__ __forceinline__ int qp_owner(const QpSched& s, int t) {
+  const int edge = s.more * (s.each + 1);
+  return t < edge ? t / (s.each + 1) : s.more + (t - edge) / s.each;
+}
+// The share of this CTA when all key tiles are divided evenly: worked out by a warp, its lanes over the row tiles; true in the one lane
+// that has it
+__device__ __forceinline__ bool qp_share(const AttnPrefillParams& p, const QpShape& z, QpSched& out, QpSeg& s) {
+  const int lane = threadIdx.x & 31, c = blockIdx.x;
+  const int per = (z.mtiles + 31) / 32, mt_lo = min(lane * per, z.mtiles), mt_hi = min(mt_lo + per, z.mtiles);
+  int mine = 0;
+  for (int mt = mt_lo; mt < mt_hi; ++mt) { s = qp_rows(p, z, 0, mt); mine += s.all; }
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  const int per_head = __shfl_sync(0xFFFFFFFFu, incl, 31), total = per_head * p.n_kv_heads;
+  const int ctas = min((int)gridDim.x, max(1, total / QP_MIN_TILES));
+  out.z = z; out.parts = 0; out.each = total / ctas; out.more = total - out.each * ctas;
+  out.left = c < ctas ? out.each + (c < out.more ? 1 : 0) : 0;
+  if (out.left == 0) { s.n = 0; return lane == 0; }
+  const int x0 = qp_first(out, c), kvh = x0 / per_head, want = x0 - kvh * per_head, before = incl - mine;
+  if (want < before || want >= incl) return false;
+  int at = want - before;
+  for (int mt = mt_lo;; ++mt) {
+    if (per > 1) s = qp_rows(p, z, 0, mt);
+    if (at < s.all) break;
+    at -= s.all;
+  }
+  s.kvh = kvh; s.j0 = at; s.n = min(s.all - at, out.left);
+  return true;
+}
+
 template <int D>
 __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __grid_constant__ AttnPrefillParams p, const int nsplit) {
   constexpr int NG = D / 32, TAIL = D % 32 ? 1 : 0, NSLAB = (D + 63) / 64, PB = q4_page_bytes(D);
@@ -148,42 +216,73 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
   uint8_t* Ks = Qs + 2 * Q_BYTES;
   uint8_t* Vs = Ks + 2 * K_BYTES;             // a tile is two slabs of [D rows x 64 keys]
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
-  const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G, kvh = blockIdx.y, mtiles = (int)gridDim.x / nsplit;
-  const int mtile = mtiles - 1 - (int)blockIdx.x / nsplit, part = (int)blockIdx.x % nsplit;      // the longest rows first
-  const int m0 = mtile * QP_ROWS, groups = rows - m0 > QP_GROUP ? 2 : 1;
-
-  if (tid < 28) {
-    const int count = tid < 2 || tid == 4 || tid == 5 || tid == 8 || tid == 9 ? QP_GROUP : tid == 12 || tid == 13 || tid == 16 || tid == 17 ? 128 : tid >= 12 && tid < 20 ? groups : 1;
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(&sm.q_full[0] + tid)), "r"(count));
-  }
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G;
+  auto groups_of = [&](int mt) { return rows - mt * QP_ROWS > QP_GROUP ? 2 : 1; };
+  auto init_barriers = [&](int groups) {                          // by a warp
+    if (lane < 28) {
+      const int count = lane < 2 || lane == 4 || lane == 5 || lane == 8 || lane == 9 ? QP_GROUP : lane == 12 || lane == 13 || lane == 16 || lane == 17 ? 128 : lane >= 12 && lane < 20 ? groups : 1;
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(&sm.q_full[0] + lane)), "r"(count));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  };
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gm_smem_u32(&sm.tmem)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == 0) {
+    QpShape z = {G, rows, (rows + QP_ROWS - 1) / QP_ROWS, p.pos0_ptr ? *p.pos0_ptr : p.pos0};
+    QpSched d;
+    QpSeg s = {0, 0, 0, 0, 0, 0, 0};
+    bool have = lane == 0;
+    if (nsplit > 0) {
+      const int tile = blockIdx.x / nsplit, part = blockIdx.x - tile * nsplit, kvh = tile / z.mtiles;
+      s = qp_rows(p, z, kvh, z.mtiles - 1 - (tile - kvh * z.mtiles));                 // the longest rows first
+      d.z = z; d.each = d.more = 0; d.parts = max(1, min(nsplit, s.all / QP_MIN_TILES));
+      if (part < d.parts) { s.j0 = part * s.all / d.parts; s.n = (part + 1) * s.all / d.parts - s.j0; }
+      d.left = s.n;
+    } else have = qp_share(p, z, d, s);
+    if (have) { sm.sched = d; sm.seg = s; sm.done = 0; sm.fail = 0; }
+    __syncwarp();
+    init_barriers(groups_of(sm.seg.mt));
   }
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = sm.tmem;
-  pdl_launch_dependents();
-  pdl_wait();
-
-  // ---- keys of this CTA: the rows' range, in tiles from a page boundary on, divided over the parts -----------------------------
-  const int pos0 = p.pos0_ptr ? *p.pos0_ptr : p.pos0;
-  const int tok0 = m0 / G, tok1 = min(p.n_tokens, (m0 + QP_ROWS - 1) / G + 1);            // tokens of the tile
-  const int kend = pos0 + tok1;
-  bool ok = pos0 >= 0 && (kend - 1) / Q4_PAGE < p.pt_len;
-  if (!ok && tid == 0) atomicExch(&g_prefill_q4_error, 3114);
-  const int klo = p.window > 0 ? max(0, pos0 + tok0 + 1 - p.window) / Q4_PAGE * Q4_PAGE : 0;
-  const int all = (kend - klo + QP_KEYS - 1) / QP_KEYS, parts = max(1, min(nsplit, all / QP_MIN_TILES));
-  const int j0 = part * all / parts, n_tiles = ok && part < parts ? (part + 1) * all / parts - j0 : 0;
-  const int kbeg = klo + j0 * QP_KEYS;
+  // the CTA's next row tile, false: none is left; all threads come here, role 0 with warp 0
+  auto next_rows = [&](bool ok, auto role) {
+    if (!ok) sm.fail = 1;
+    tc_before();                                                   // O has been read
+    asm volatile("bar.sync 0, %0;" ::"n"(QP_THREADS) : "memory");
+    if (decltype(role)::value == 0 && warp == 0) {
+      if (lane == 0) {
+        const int done = sm.done + sm.seg.n;
+        sm.done = done;
+        if (done < sm.sched.left && !sm.fail) sm.seg = qp_next(p, sm.sched.z, sm.seg.kvh, sm.seg.mt, sm.sched.left - done); else sm.seg.n = 0;
+      }
+      __syncwarp();
+      if (sm.seg.n) {                                              // (every arrival of the tile before has been waited for)
+        if (lane < 28) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(gm_smem_u32(&sm.q_full[0] + lane)) : "memory");
+        init_barriers(groups_of(sm.seg.mt));
+      }
+    }
+    asm volatile("bar.sync 0, %0;" ::"n"(QP_THREADS) : "memory");
+    tc_after();
+    return sm.seg.n > 0;
+  };
+  const bool any = sm.seg.n > 0;
 
   if (warp < 8) {
     // ================================ softmax: one thread to a row ================================================================
     regs_up<QP_REGS_SOFTMAX>();
     const int grp = warp >> 2, t = tid & 127;
-    if (n_tiles > 0 && grp < groups) {
+    bool more = any;
+    while (more) {
+      const int m0 = sm.seg.mt * QP_ROWS, groups = groups_of(sm.seg.mt), kvh = sm.seg.kvh, n_tiles = sm.seg.n, kbeg = sm.seg.klo + sm.seg.j0 * QP_KEYS, pos0 = sm.sched.z.pos0;
+      bool ok = true;
+      if (grp < groups) {
       const uint32_t lane_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(128 * grp), lane_o = lane_s + 256u;
       const int row = m0 + grp * QP_GROUP + t, token = row / G, head = kvh * G + row - token * G;
       const bool live = row < rows;
@@ -332,12 +431,13 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         };
-        const int tile_id = kvh * mtiles + mtile;
+        const bool whole = n_tiles == sm.seg.all;
         constexpr int COLS = D % 32 ? 16 : 32;
-        constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);          // between the parts of a tile
-        const float* parts_of = p.scratch + QP_COUNTERS + (int64_t)tile_id * nsplit * step + (int64_t)grp * QP_GROUP * (D + 4) + t;     // a column to 128 floats: a warp's rows lie together
-        float* slot = (float*)parts_of + part * step;
-        if (parts == 1) {
+        // slots of a CTA in scratch: 0 the row tile that its share begins in, 1 the one that it ends in
+        constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);
+        float* const slots = p.scratch + QP_COUNTERS + (int64_t)grp * QP_GROUP * (D + 4) + t;     // a column to 128 floats: a warp's rows lie together
+        float* const slot = slots + (int64_t)(2 * blockIdx.x + (sm.done == 0 ? 0 : 1)) * step;
+        if (whole) {
           const float f = inv_vf / l;
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
@@ -357,19 +457,31 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (int i = 0; i < 16; ++i) __stcg(slot + (c + i) * QP_GROUP, __uint_as_float(r[i]) * inv_vf);
           }
           slot[D * QP_GROUP] = m; slot[(D + 1) * QP_GROUP] = l;
+          // the row tile's CTAs: neighbours by tile, else those that have its first and last place
+          int c_lo, c_hi, lead = 0;
+          {
+            const int c = blockIdx.x;
+            if (sm.sched.each == 0) { c_lo = c - c % nsplit; c_hi = c_lo + sm.sched.parts - 1; }
+            else {
+              const int t0 = qp_first(sm.sched, c) + sm.done - sm.seg.j0;
+              c_lo = qp_owner(sm.sched, t0); c_hi = qp_owner(sm.sched, t0 + sm.seg.all - 1);
+              lead = qp_first(sm.sched, c_lo) == t0 ? 0 : 1;
+            }
+          }
           if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
           if (t == 0) {
-            int32_t* ctr = (int32_t*)p.scratch + 2 * tile_id + grp;
+            int32_t* ctr = (int32_t*)p.scratch + 2 * (2 * c_lo + lead) + grp;
             __threadfence();
-            sm.last[grp] = atomicAdd(ctr, 1) == parts - 1;
+            sm.last[grp] = atomicAdd(ctr, 1) == c_hi - c_lo;
             if (sm.last[grp]) { *ctr = 0; __threadfence(); }          // zero again for the next launch
           }
           if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
           if (sm.last[grp] && live) {
+            auto part_of = [&](int k) { return slots + (int64_t)(2 * k + (k == c_lo ? lead : 0)) * step; };
             float mm = -INFINITY, ll = 0.f;
 #pragma unroll 4
-            for (int i = 0; i < parts; ++i) {
-              const float mi = __ldcg(parts_of + i * step + D * QP_GROUP), li = __ldcg(parts_of + i * step + (D + 1) * QP_GROUP), mn = fmaxf(mm, mi);
+            for (int k = c_lo; k <= c_hi; ++k) {
+              const float mi = __ldcg(part_of(k) + D * QP_GROUP), li = __ldcg(part_of(k) + (D + 1) * QP_GROUP), mn = fmaxf(mm, mi);
               if (mn != -INFINITY) ll = fmaf(ll, qp_ex2(mm - mn), li * qp_ex2(mi - mn));
               mm = mn;
             }
@@ -378,8 +490,8 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (int c = 0; c < D; c += COLS) {
               float v[COLS] = {};
 #pragma unroll 2
-              for (int i = 0; i < parts; ++i) {
-                const float* part_i = parts_of + i * step;
+              for (int k = c_lo; k <= c_hi; ++k) {
+                const float* part_i = part_of(k);
                 const float e = qp_ex2(__ldcg(part_i + D * QP_GROUP) - mm) * inv;
 #pragma unroll
                 for (int q = 0; q < COLS; ++q) v[q] = fmaf(e, __ldcg(part_i + (c + q) * QP_GROUP), v[q]);
@@ -390,11 +502,17 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           }
         }
       }
+      }
+      more = next_rows(ok, std::integral_constant<int, 0>{});
     }
   } else if (warp < 16) {
     // ================================ decoding ======================================================================================
     regs_down<QP_REGS_DECODE>();
     const int t = tid & 127;
+    bool more = any;
+    while (more) {
+    const int n_tiles = sm.seg.n, kbeg = sm.seg.klo + sm.seg.j0 * QP_KEYS, kend = sm.seg.kend, kvh = sm.seg.kvh;
+    bool ok = true;
     const int last_page = (kend - 1) / Q4_PAGE * Q4_PAGE;
     auto id_of = [&](int key) { return __ldg(p.page_table + min(key, last_page) / Q4_PAGE); };
     auto row_of = [&](int id) {
@@ -403,7 +521,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
     };
     // largest magnitude that a row's codes can stand for; over all threads of the role
     auto largest = [](uint32_t meta) { return fmaxf(fabsf(q4_min(meta)), fabsf(fmaf(15.f, q4_scale(meta), q4_min(meta)))); };
-    if (n_tiles > 0 && warp < 12) {
+    if (warp < 12) {
       // -- keys: a token row to a thread
       uint32_t kw[D / 8], km = 0u;
       int id = id_of(kbeg + t);
@@ -444,7 +562,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         gm_arrive((uint64_t*)&sm.k_full[buf]);
       }
-    } else if (n_tiles > 0) {
+    } else {
       // -- values: half a page to a thread: page t / 16 of the tile, tokens 8 vh .. + 7, units vg of every 32 dims
       uint32_t vw[D / 8], vm[8];
       const int vh = (t >> 3) & 1, vg = t & 7;
@@ -519,9 +637,15 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         gm_arrive((uint64_t*)&sm.v_full[buf]);
       }
     }
+    more = next_rows(ok, std::integral_constant<int, 1>{});
+    }
   } else {
     regs_down<QP_REGS_ISSUE>();
-    if (warp < 16 + groups) {
+    bool more = any;
+    while (more) {
+    const int n_tiles = sm.seg.n;
+    bool ok = true;
+    if (warp < 16 + groups_of(sm.seg.mt)) {
       // ================================ the products: a warp to a group, so that no group's waits hold up the other =====================
       const int g = warp - 16;
       const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
@@ -533,10 +657,10 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) umma_f16_ts(o_col, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, j > 0 || half + kk > 0 ? 1u : 0u);
       };
-      for (int j = 0; j < n_tiles; ++j) {
+      for (int j = 0; ok && j < n_tiles; ++j) {
         const int buf = j & 1;
         // scores, once the product of the tile before has ended (it reads P where they go)
-        if (!both(&sm.k_full[buf], (uint32_t)(j >> 1) & 1u) || !both(j == 0 ? &sm.q_full[g] : &sm.o_full[g], j == 0 ? 0u : (uint32_t)(j - 1) & 1u)) break;
+        if (!both(&sm.k_full[buf], (uint32_t)(j >> 1) & 1u) || !both(j == 0 ? &sm.q_full[g] : &sm.o_full[g], j == 0 ? 0u : (uint32_t)(j - 1) & 1u)) { ok = false; break; }
         const uint32_t b = k_lo + (uint32_t)(buf * (K_BYTES >> 4));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -546,13 +670,15 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         umma_commit_warp(&sm.s_full[g]);
         if (j + 2 < n_tiles) umma_commit_warp(&sm.k_empty[buf]);
         // the halves of the product as P arrives (it comes after the softmax has seen that the values are there)
-        if (!both(&sm.p_half[g], (uint32_t)j & 1u)) break;
+        if (!both(&sm.p_half[g], (uint32_t)j & 1u)) { ok = false; break; }
         values(j, 0);
-        if (!both(&sm.p_full[g], (uint32_t)j & 1u)) break;
+        if (!both(&sm.p_full[g], (uint32_t)j & 1u)) { ok = false; break; }
         values(j, 1);
         umma_commit_warp(&sm.o_full[g]);
         if (j + 2 < n_tiles) umma_commit_warp(&sm.v_empty[buf]);
       }
+    }
+    more = next_rows(ok, std::integral_constant<int, 1>{});
     }
   }
   tc_before();
@@ -573,16 +699,27 @@ static int launch_prefill_q4(const AttnPrefillParams& p, cudaStream_t st) {
            a.numRegs * QP_THREADS >= 256 * (QP_REGS_SOFTMAX + QP_REGS_DECODE) + 128 * QP_REGS_ISSUE;
   }();
   if (!regs_fit) return -7;
-  const int64_t rows = (int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads);
-  const int mtiles = (int)((rows + QP_ROWS - 1) / QP_ROWS);
-  // parts of a row tile's keys: as many as fill the SMs, if there is scratch for them
-  const bool room = p.scratch && p.scratch_floats >= (int64_t)QP_MAX_CTAS * QP_ROWS * (D + 4) + QP_COUNTERS;
-  const int nsplit = room ? std::max(1, std::min(32, QP_MAX_CTAS / (mtiles * p.n_kv_heads))) : 1;
-  return (int)launch(attn_prefill_q4_kernel<D>, dim3(mtiles * nsplit, p.n_kv_heads), dim3(QP_THREADS), smem, st, p, nsplit);
+  // row tiles, and key tiles to a row tile at most
+  const int tiles = (int)(((int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads) + QP_ROWS - 1) / QP_ROWS) * p.n_kv_heads;
+  const int64_t reach = p.pos0_ptr ? (int64_t)p.pt_len * Q4_PAGE : (int64_t)p.pos0 + p.n_tokens;
+  const int keys = (int)((p.window > 0 ? std::min<int64_t>(reach, p.window + QP_ROWS) : reach) / QP_KEYS) + 1;
+  int nsplit = 1, grid = tiles;
+  if (p.scratch && p.scratch_floats >= 2LL * QP_MAX_CTAS * QP_ROWS * (D + 4) + QP_COUNTERS) {
+    nsplit = std::min(std::max(QP_MAX_CTAS / tiles, 1), 32);
+    grid = tiles * nsplit;
+    // time in key tiles: of the longest CTA, or, of an even share, with the second row tile that it reaches into
+    const int waves = (grid + QP_MAX_CTAS - 1) / QP_MAX_CTAS, by_tile = waves * ((keys + nsplit - 1) / nsplit) + (waves - 1) * QP_SEG_COST;
+    const int even = (int)((int64_t)keys * tiles / QP_MAX_CTAS) + waves * QP_SEG_COST;
+    if (even < by_tile) { nsplit = 0; grid = QP_MAX_CTAS; }
+  }
+  return (int)launch(attn_prefill_q4_kernel<D>, dim3(grid), dim3(QP_THREADS), smem, st, p, nsplit);
 }
 
 int attn_prefill_q4_dispatch(const AttnPrefillParams& p, cudaStream_t st) {
   if (p.num_pages < 1 || p.pt_len < 1 || ((uintptr_t)p.scratch & 15)) return -6;
+  // row tiles x key tiles are counted in 32 bits
+  const int64_t mtiles = ((int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads) + QP_ROWS - 1) / QP_ROWS;
+  if (mtiles * p.n_kv_heads * ((int64_t)p.pt_len * Q4_PAGE / QP_KEYS + 2) > INT32_MAX) return -6;
   switch (p.head_dim) {
     case 64: return launch_prefill_q4<64>(p, st);
     case 80: return launch_prefill_q4<80>(p, st);
@@ -598,7 +735,7 @@ extern "C" {
 
 // floats of scratch with which the keys can be split, whatever the number of rows is
 long long rlz_attn_prefill_q4_scratch_floats(int n_tokens, int n_heads, int n_kv_heads, int head_dim) {
-  return (long long)rlz::QP_MAX_CTAS * rlz::QP_ROWS * (head_dim + 4) + rlz::QP_COUNTERS;
+  return 2LL * rlz::QP_MAX_CTAS * rlz::QP_ROWS * (head_dim + 4) + rlz::QP_COUNTERS;
 }
 
 // 0 / 3113 / 3114 / 3115
