@@ -3,8 +3,8 @@
 //
 //   s_t = q . k_t = scale_t (q . code_t) + min_t sum(q)        o = sum_t p_t v_t = sum_t (p_t scale'_t) code'_t + sum_t p_t min'_t
 //
-// Bound by the bytes of the cache.  What a page costs besides them:
-// The arithmetic of the codes is what has to be cheap:
+// Bound by the bytes of the cache as long as the arithmetic of the codes is cheap (96 sequences of 8192 tokens of 128 dims, 8 kv heads:
+// 130 us, 4.5 TB/s of the 6.6 that a copy reaches):
 //   * Keys: a masked word holds four codes as bytes, and the 8-bit integer product takes them as they are; q comes as three 8-bit
 //     digits of a 23-bit integer (its largest value in [2^21, 2^22)), so the sums over the dims are exact.
 //   * Values: a nibble under the exponent of 1024 is the fp16 1024 + code (or 1024 + 16 code), which one subtraction (or
@@ -39,6 +39,7 @@ __device__ int g_attn_q4_error = 0;
 constexpr int QD_STAGES = 3, QD_MAX_SMS = 148, QD_HELPERS = 128;
 constexpr int QD_PAIR = 2 * Q4_PAGE;          // tokens of a pair of pages
 constexpr int QD_TILE_COST = 40;              // a second tile costs a CTA about as much time as this many pairs
+constexpr int QD_POSITIONS = 512;
 constexpr int QD_MAX_PARTS = 64;              // CTAs that share a tile: bounds the time of the last one, which joins their parts
 // query heads of a CTA (HN tiles of 4) and its main warps: with the four others 16 warps of 128 registers, or 12 of 168
 constexpr int qd_heads(int hn) { return 4 * hn; }
@@ -54,7 +55,8 @@ template <int D, int HN> struct QdSmem {
   uint32_t meta[2][2];
   struct { int n, tok, lo, pos, own; } tile[2];   // pairs, first token, first and last visible position, place of the new token's pair or -1
   int last;
-  unsigned long long frag_full[2], part_full[2], part_empty[2];
+  int pos[QD_POSITIONS];                      // positions of the first sequences, which are asked for again and again
+  unsigned long long frag_full[2], part_full[2], part_empty[2], own_full[2];
 };
 
 __device__ __forceinline__ int q4_page_id(int raw, int num_pages) {
@@ -118,8 +120,8 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* src, 
 }
 
 struct QdSeq { int pos, lo, first_page, n; };                 // n pairs of pages from first_page on; 0: nothing to do
-__device__ __forceinline__ QdSeq qd_seq(const AttnDecodeParams& p, int b) {
-  QdSeq s = {p.positions[b], 0, 0, 0};
+__device__ __forceinline__ QdSeq qd_seq(const AttnDecodeParams& p, const int* cached, int b) {
+  QdSeq s = {b < QD_POSITIONS ? cached[b] : p.positions[b], 0, 0, 0};
   if (s.pos < 0) return s;
   if (s.pos / Q4_PAGE >= p.max_pages) { atomicExch(&g_attn_q4_error, 3311); return s; }
   s.lo = p.window > 0 ? max(0, s.pos + 1 - p.window) : 0;
@@ -130,15 +132,22 @@ __device__ __forceinline__ QdSeq qd_seq(const AttnDecodeParams& p, int b) {
 // the pairs of one tile that a CTA has: `n` of them from the tile's pair `skip` on
 struct QdTile { QdSeq s; int b, tile, skip, n; };
 // the tile that pair `at` of sequence b's tiles (or the next sequence with any) lies in; the CTA has `left` more pairs
-__device__ __forceinline__ QdTile qd_tile(const AttnDecodeParams& p, int b, int at, int left) {
+__device__ __forceinline__ QdTile qd_tile(const AttnDecodeParams& p, const int* cached, int b, int at, int left) {
   QdTile t;
-  for (;; ++b, at = 0) { t.s = qd_seq(p, b); if (t.s.n) break; }
+  for (;; ++b, at = 0) { t.s = qd_seq(p, cached, b); if (t.s.n) break; }
   t.b = b; t.tile = at / t.s.n; t.skip = at - t.tile * t.s.n; t.n = min(t.s.n - t.skip, left);
   return t;
 }
-__device__ __forceinline__ QdTile qd_next(const AttnDecodeParams& p, const QdTile& t, int tiles, int left) {
-  const bool new_seq = t.tile + 1 == tiles;
-  return qd_tile(p, new_seq ? t.b + 1 : t.b, new_seq ? 0 : (t.tile + 1) * t.s.n, left);
+__device__ __forceinline__ QdTile qd_next(const AttnDecodeParams& p, const int* cached, const QdTile& t, int tiles, int left) {
+  if (t.tile + 1 == tiles) return qd_tile(p, cached, t.b + 1, 0, left);
+  return {t.s, t.b, t.tile + 1, 0, min(t.s.n, left)};
+}
+// pairs divided evenly: the first one of CTA c (the first `more` have one more than `each`), and the CTA that has pair x
+struct QdShare { int each, more; };
+__device__ __forceinline__ int qd_first(const QdShare& s, int c) { return c * s.each + min(c, s.more); }
+__device__ __forceinline__ int qd_owner(const QdShare& s, int x) {
+  const int edge = s.more * (s.each + 1);
+  return x < edge ? x / (s.each + 1) : s.more + (x - edge) / s.each;
 }
 // bounded: false (and the status word) when the barrier's phase does not end
 __device__ __forceinline__ bool qd_wait(unsigned long long* bar, uint32_t parity, bool patient) {
@@ -159,20 +168,21 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   QdSmem<D, HN>& sm = *(QdSmem<D, HN>*)qd_smem;
   uint8_t* qd_ring = qd_smem + (sizeof(QdSmem<D, HN>) + 127) / 128 * 128;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
-  if (tid < 6) {
-    unsigned long long* bar = tid < 2 ? &sm.frag_full[tid] : tid < 4 ? &sm.part_full[tid - 2] : &sm.part_empty[tid - 4];
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(att_smem_u32(bar)), "r"(tid < 2 ? QD_HELPERS : tid < 4 ? NW : 1));
+  if (tid < 8) {
+    unsigned long long* bar = tid < 2 ? &sm.frag_full[tid] : tid < 4 ? &sm.part_full[tid - 2] : tid < 6 ? &sm.part_empty[tid - 4] : &sm.own_full[tid - 6];
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(att_smem_u32(bar)), "r"(tid < 2 ? QD_HELPERS : tid < 4 ? NW : tid < 6 ? 1 : 64));
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
+  for (int b = tid; b < min(p.batch, QD_POSITIONS); b += 32 * NW + QD_HELPERS) sm.pos[b] = __ldg(p.positions + b);
+  __syncthreads();
 
   // ---- my share: pairs [x0, x1) of the sequence of all tiles' pairs.  Every warp works it out, its lanes over the sequences ------
   const int G = p.n_heads / p.n_kv_heads, hgroups = (G + ROWS - 1) / ROWS, tiles = p.n_kv_heads * hgroups;
   const int per = (p.batch + 31) / 32, b_lo = min(lane * per, p.batch), b_hi = min(b_lo + per, p.batch);
   int mine = 0, live = 0, longest = 0;
-  for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, b).n; mine += n; live += n > 0; longest = max(longest, n); }
+  for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, sm.pos, b).n; mine += n; live += n > 0; longest = max(longest, n); }
   int incl = mine, live_incl = live;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -186,14 +196,15 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   const bool by_tile = split > 0 && (longest + split - 1) / split < total / (int)gridDim.x + QD_TILE_COST;
   const int ctas = by_tile ? all_tiles * split : min((int)gridDim.x, total);
   if (c >= ctas) return;
-  int x0 = (int)((int64_t)c * total / ctas), x1 = (int)((int64_t)(c + 1) * total / ctas);
+  const QdShare share = {total / ctas, total % ctas};
+  int x0 = qd_first(share, c), x1 = x0 + share.each + (c < share.more ? 1 : 0);
   // the lane whose sequences hold place x0, or (by tile) live tile c / split
   const int want = by_tile ? c / split : x0, first = by_tile ? (live_incl - live) * tiles : (incl - mine) * tiles;
   const bool holds = first <= want && want < (by_tile ? live_incl : incl) * tiles;
   int b0 = b_lo, at0 = want - first;
   if (holds)
     for (;; ++b0) {
-      const int n = qd_seq(p, b0).n, m = (by_tile ? n > 0 : n) * tiles;
+      const int n = qd_seq(p, sm.pos, b0).n, m = (by_tile ? n > 0 : n) * tiles;
       if (at0 < m) { if (by_tile) at0 *= n; break; }
       at0 -= m;
     }
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   b0 = __shfl_sync(0xFFFFFFFFu, b0, holder);
   at0 = __shfl_sync(0xFFFFFFFFu, at0, holder);
   if (by_tile) {                                                   // places count from the tile's first pair
-    const int n = qd_seq(p, b0).n, parts = min(split, n), part = c % split;
+    const int n = qd_seq(p, sm.pos, b0).n, parts = min(split, n), part = c % split;
     if (part >= parts) return;
     x0 = part * n / parts; x1 = (part + 1) * n / parts; at0 += x0;
   }
@@ -214,16 +225,16 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     uint8_t* my_ring = qd_ring + (size_t)warp * QD_STAGES * 4 * PB;
     // -- the copies, pair after pair of the stream.  Lane i keeps the (page, kv head) row of page i % 2 of the i / 2-th of 16 pairs; the
     // ids of the 16 behind them are on their way
-    QdTile f = qd_tile(p, b0, at0, x1 - x0);
+    QdTile f = qd_tile(p, sm.pos, b0, at0, x1 - x0);
     int f_at = 0, row_now, id_next, kvh_next;
     auto fetch = [&](int k) {                                        // ids of pairs k .. k + 15
-      while (f_at + f.n < x1 - x0 && warp + NW * k >= f_at + f.n) { f_at += f.n; f = qd_next(p, f, tiles, x1 - x0 - f_at); }
+      while (f_at + f.n < x1 - x0 && warp + NW * k >= f_at + f.n) { f_at += f.n; f = qd_next(p, sm.pos, f, tiles, x1 - x0 - f_at); }
       const int x = warp + NW * (k + (lane >> 1));
       kvh_next = -1;
       if (x < x1 - x0) {
         QdTile t = f;
         int t_at = f_at;
-        while (x >= t_at + t.n) { t_at += t.n; t = qd_next(p, t, tiles, x1 - x0 - t_at); }
+        while (x >= t_at + t.n) { t_at += t.n; t = qd_next(p, sm.pos, t, tiles, x1 - x0 - t_at); }
         const int page = t.s.first_page + 2 * (t.skip + x - t_at) + (lane & 1);
         if (page <= t.s.pos / Q4_PAGE) { id_next = __ldg(p.page_table + (int64_t)t.b * p.pt_stride + page); kvh_next = t.tile / hgroups; }
       }
@@ -285,6 +296,8 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           __syncwarp();
           uint8_t* const kp[2] = {my_ring + slot * (4 * PB), my_ring + slot * (4 * PB) + 2 * PB};
           if (own == k) {                                            // the copy may have passed the write of the new row
+            ok = qd_wait(&sm.own_full[buf], phase, ok) && ok;
+            __syncwarp();
             uint8_t* page = s.pos - tok < Q4_PAGE ? kp[0] : kp[1];
             q4_store_k<D>(page, s.pos % Q4_PAGE, sm.codes[buf][0], sm.meta[buf][0], lane);
             q4_store_v<D>(page + PB, s.pos % Q4_PAGE, sm.codes[buf][1], sm.meta[buf][1], lane);
@@ -431,7 +444,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     return;
   }
 
-  QdTile now = qd_tile(p, b0, at0, x1 - x0);
+  QdTile now = qd_tile(p, sm.pos, b0, at0, x1 - x0);
   // ================================== helper warps ================================================================================
   const int hid = tid - 32 * NW, hw = hid >> 5;
   const RopeArgs rope = {p.rope_table, p.rope_table_len, p.rope_dim, p.rope_type, p.rope_theta};
@@ -447,18 +460,21 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     float2 cs[NP];
     load_rope<D>(rope, t.s.pos, lane, cs);
     float xa[NP], xb[NP];
-    auto load = [&](const float* src, int hf, int type) {
+    auto load = [&](const float* src, int hf, int type, float (&a)[NP], float (&b)[NP]) {
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
         const int i = lane + 32 * k;
-        xa[k] = xb[k] = 0.f;
-        if (i < D / 2) { const int2 at = pair_dims(i, hf, type); xa[k] = src[at.x]; xb[k] = src[at.y]; }
+        a[k] = b[k] = 0.f;
+        if (i < D / 2) { const int2 at = pair_dims(i, hf, type); a[k] = src[at.x]; b[k] = src[at.y]; }
       }
     };
+    const bool own = !p.no_append && t.skip + t.n == t.s.n && hw >= 2, own_v = hw == 3;
+    float ra[NP], rb[NP];
+    if (own) load(row + (own_v ? p.v_off : p.k_off) + kvh * D, own_v ? 0 : half, own_v ? 0 : p.rope_type, ra, rb);
     for (int g = hw; g < ROWS; g += QD_HELPERS / 32) {
       float f = 1.f, sum = 0.f;
       if (g < gn) {
-        load(row + p.q_off + (int64_t)(kvh * G + g0 + g) * D, half, p.rope_type);
+        load(row + p.q_off + (int64_t)(kvh * G + g0 + g) * D, half, p.rope_type, xa, xb);
         norm_rope_f<D>(xa, xb, p.q_norm_w, p.eps, rope, cs, lane);
         float top = 0.f;
 #pragma unroll
@@ -475,22 +491,6 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
         }
       }
       if (lane == 0) { sm.qc[buf][g] = g < gn ? 1.f / f : 0.f; sm.qx[buf][g] = sum; }
-    }
-    if (!p.no_append && t.skip + t.n == t.s.n && hw >= 2) {
-      const bool v = hw == 3;
-      load(row + (v ? p.v_off : p.k_off) + kvh * D, v ? 0 : half, v ? 0 : p.rope_type);
-      if (!v) norm_rope_d<D>(xa, xb, p.q_norm_w ? p.k_norm_w : nullptr, (double)p.eps, rope, cs, lane);
-      const uint32_t meta = q4_quantise<D>(xa, xb, v ? 0 : half, v ? 0 : p.rope_type, lane, sm.codes[buf][v]);
-      __syncwarp();
-      if (lane == 0) sm.meta[buf][v] = meta;
-      if (g0 == 0) {                                               // one head group writes the row
-        const int raw = p.page_table[(int64_t)t.b * p.pt_stride + t.s.pos / Q4_PAGE];
-        if (p.num_pages <= 0 || (unsigned)raw < (unsigned)p.num_pages) {
-          uint8_t* dst = (uint8_t*)(v ? p.v_cache : p.k_cache) + ((int64_t)raw * p.n_kv_heads + kvh) * PB;
-          if (v) q4_store_v<D>(dst, t.s.pos % Q4_PAGE, sm.codes[buf][1], meta, lane);
-          else q4_store_k<D>(dst, t.s.pos % Q4_PAGE, sm.codes[buf][0], meta, lane);
-        }
-      }
     }
     helpers_sync();
     // column gq is head gq / 2 of a tile, its digits 0 (even) or 1 (odd), and in the second pair of registers digit 2 (even).  Word tq of
@@ -510,6 +510,23 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       sm.frag[buf][h][f][lane] = r;
     }
     qd_arrive(&sm.frag_full[buf]);
+    // the new token's rows, behind the fragments: only the warp that has its pair waits for them
+    if (own) {
+      const bool v = own_v;
+      if (!v) norm_rope_d<D>(ra, rb, p.q_norm_w ? p.k_norm_w : nullptr, (double)p.eps, rope, cs, lane);
+      const uint32_t meta = q4_quantise<D>(ra, rb, v ? 0 : half, v ? 0 : p.rope_type, lane, sm.codes[buf][v]);
+      __syncwarp();
+      if (lane == 0) sm.meta[buf][v] = meta;
+      if (g0 == 0) {                                               // one head group writes the row
+        const int raw = p.page_table[(int64_t)t.b * p.pt_stride + t.s.pos / Q4_PAGE];
+        if (p.num_pages <= 0 || (unsigned)raw < (unsigned)p.num_pages) {
+          uint8_t* dst = (uint8_t*)(v ? p.v_cache : p.k_cache) + ((int64_t)raw * p.n_kv_heads + kvh) * PB;
+          if (v) q4_store_v<D>(dst, t.s.pos % Q4_PAGE, sm.codes[buf][1], meta, lane);
+          else q4_store_k<D>(dst, t.s.pos % Q4_PAGE, sm.codes[buf][0], meta, lane);
+        }
+      }
+    }
+    if (hw >= 2) qd_arrive(&sm.own_full[buf]);
   };
 
   prepare(now, 0, 0);
@@ -518,7 +535,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     const int end = at + now.n, buf = it & 1;
     const bool more = end < x1 - x0;
     if (more) {
-      next = qd_next(p, now, tiles, x1 - x0 - end);
+      next = qd_next(p, sm.pos, now, tiles, x1 - x0 - end);
       helpers_sync();                                              // the fragments before are made: the staging rows are free
       prepare(next, buf ^ 1, end);
     }
@@ -555,10 +572,10 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     helpers_sync();                                                // the parts are read, and what goes to scratch is written
     if (hid == 0) qd_arrive(&sm.part_empty[buf]);
     if (!whole) {
-      // by tile, the CTAs are neighbours; else CTA that has place x of all: the largest c with c total / ctas <= x
+      // by tile, the CTAs are neighbours; else those that have its first and last pair
       const int t0 = x0 + at - now.skip;
-      const int c_lo = by_tile ? c - c % split : (int)(((int64_t)(t0 + 1) * ctas - 1) / total);
-      const int c_hi = by_tile ? c_lo + min(split, now.s.n) - 1 : (int)(((int64_t)(t0 + now.s.n) * ctas - 1) / total);
+      const int c_lo = by_tile ? c - c % split : qd_owner(share, t0);
+      const int c_hi = by_tile ? c_lo + min(split, now.s.n) - 1 : qd_owner(share, t0 + now.s.n - 1);
       if (hid == 0) {
         int32_t* ctr = p.counters + (int64_t)now.b * tiles + tile;
         __threadfence();
@@ -567,16 +584,17 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       }
       helpers_sync();
       if (sm.last) {
-        const int lead = by_tile || (int)((int64_t)c_lo * total / ctas) == t0 ? 0 : 1;
+        constexpr int BATCH = 8;                                    // parts on their way at once (16 took longer)
+        const int lead = by_tile || qd_first(share, c_lo) == t0 ? 0 : 1;
         for (int i = hid; i < gn * (D / 4); i += QD_HELPERS) {
           const int g = i / (D / 4), j = 4 * (i - g * (D / 4));
           float mm = -INFINITY, ll = 0.f;
           float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int q0 = c_lo; q0 <= c_hi; q0 += 8) {
-            float2 st[8];
-            float4 v[8];
+          for (int q0 = c_lo; q0 <= c_hi; q0 += BATCH) {
+            float2 st[BATCH];
+            float4 v[BATCH];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < BATCH; ++k) {
               const int kc = min(q0 + k, c_hi);
               const float* src = p.partial + ((int64_t)(2 * kc + (kc == c_lo ? lead : 0)) * ROWS + g) * (D + 4);
               st[k] = __ldcg((const float2*)(src + D));
@@ -584,11 +602,11 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
             }
             float mn = mm;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mn = fmaxf(mn, st[k].x);
+            for (int k = 0; k < BATCH; ++k) mn = fmaxf(mn, st[k].x);
             const float c0 = mm == -INFINITY ? 0.f : ex2(mm - mn);
             a.x *= c0; a.y *= c0; a.z *= c0; a.w *= c0; ll *= c0; mm = mn;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < BATCH; ++k) {
               const float e = q0 + k > c_hi || st[k].x == -INFINITY ? 0.f : ex2(st[k].x - mm);
               ll = fmaf(e, st[k].y, ll);
               a.x = fmaf(e, v[k].x, a.x); a.y = fmaf(e, v[k].y, a.y); a.z = fmaf(e, v[k].z, a.z); a.w = fmaf(e, v[k].w, a.w);
