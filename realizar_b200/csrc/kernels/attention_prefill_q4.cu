@@ -154,8 +154,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ QpSeg qp_rows(const AttnPrefillParams& p, const QpShape& z, int kvh, int mt) {
   QpSeg s = {kvh, mt, 0, 0, 0, 0, 0};
   const int tok0 = mt * QP_ROWS / z.G, tok1 = min(p.n_tokens, (mt * QP_ROWS + QP_ROWS - 1) / z.G + 1);
+  if (z.pos0 < 0 || z.pos0 + (int64_t)tok1 > (int64_t)p.pt_len * Q4_PAGE) { atomicExch(&g_prefill_q4_error, 3114); return s; }
   s.kend = z.pos0 + tok1;
-  if (z.pos0 < 0 || (s.kend - 1) / Q4_PAGE >= p.pt_len) { atomicExch(&g_prefill_q4_error, 3114); return s; }
   s.klo = p.window > 0 ? max(0, z.pos0 + tok0 + 1 - p.window) / Q4_PAGE * Q4_PAGE : 0;
   s.all = (s.kend - s.klo + QP_KEYS - 1) / QP_KEYS;
   return s;
@@ -715,8 +715,10 @@ static int launch_prefill_q4(const AttnPrefillParams& p, cudaStream_t st) {
   return (int)launch(attn_prefill_q4_kernel<D>, dim3(grid), dim3(QP_THREADS), smem, st, p, nsplit);
 }
 
-int attn_prefill_q4_dispatch(const AttnPrefillParams& p, cudaStream_t st) {
+int attn_prefill_q4_dispatch(const AttnPrefillParams& given, cudaStream_t st) {
+  AttnPrefillParams p = given;
   if (p.num_pages < 1 || p.pt_len < 1 || ((uintptr_t)p.scratch & 15)) return -6;
+  if (p.window >= (int64_t)p.pt_len * Q4_PAGE) p.window = 0;        // hides nothing, and differences of positions and a larger one could pass 32 bits
   // row tiles x key tiles are counted in 32 bits
   const int64_t mtiles = ((int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads) + QP_ROWS - 1) / QP_ROWS;
   if (mtiles * p.n_kv_heads * ((int64_t)p.pt_len * Q4_PAGE / QP_KEYS + 2) > INT32_MAX) return -6;

@@ -330,37 +330,68 @@ def attn_prefill(qkv: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     (tensor-core kernel; the chunk's own K/V rows must already be in the cache).  With ``pos0_dev`` (an int32 device
     tensor) the position of row 0 is read on the device, so a captured launch serves every chunk position.
     ``impl``: "tc" (128-query tiles on tcgen05) or "mma" (16-query tiles on mma.sync); None = the launcher's choice.
-    ``scratch`` (4-bit caches, from ``attn_prefill_scratch``, one to a stream): lets few rows over a long context be split over the keys."""
-    fmt = kv_format(k_cache, head_dim)
-    if fmt == KV_Q4:
-        if n_tokens < 1:
-            raise ValueError(f"n_tokens must be at least 1, got {n_tokens}")
-        _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, out, page_table, pos0_dev, scratch)
-        if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[0] < n_tokens or qkv.shape[1] < q_off + n_heads * head_dim:
-            raise ValueError("qkv must be float32 [>= n_tokens, >= q_off + n_heads * head_dim] with contiguous rows")
-        if out.dtype not in (torch.float32, torch.bfloat16) or out.dim() != 2 or out.stride(1) != 1 or out.shape[0] < n_tokens or out.shape[1] < n_heads * head_dim:
-            raise ValueError("out must be float32 or bfloat16 [>= n_tokens, >= n_heads * head_dim] with contiguous rows")
-        if page_table.dtype != torch.int32 or page_table.dim() != 1 or page_table.stride(0) != 1:
-            raise ValueError("page_table must be a contiguous int32 row")
-        if pos0 < 0 or window < 0 or (pos0_dev is None and pos0 + n_tokens > 16 * page_table.numel()):
-            raise ValueError(f"positions {pos0} .. {pos0 + n_tokens - 1} are not covered by {page_table.numel()} pages")
-        if pos0_dev is not None and pos0_dev.dtype != torch.int32:
-            raise ValueError("pos0_dev must be int32")
-        if scratch is not None and (scratch.dtype != torch.float32 or not scratch.is_contiguous()):
-            raise ValueError("scratch must be a contiguous float32 tensor from attn_prefill_scratch")
-        _check_current_device(k_cache)
+    ``scratch`` (4-bit caches, from ``attn_prefill_scratch``, one to a stream): lets the keys be divided over the SMs where the rows alone would
+    leave some idle.  Over a 4-bit cache, rows whose positions (read on the device) lie beyond the page table are not computed, nor are
+    those that share 256 (row, query head) pairs of a kv head with them, and the device status tells."""
+    if k_cache.dtype is torch.uint8 and k_cache.shape[-1] == head_dim // 2 + 4:
+        return _attn_prefill_q4(qkv, out, k_cache, v_cache, page_table, n_tokens, pos0, n_heads, n_kv_heads, head_dim, q_off, window or 0, pos0_dev, impl, scratch)
     p = S.AttnPrefillParams()
     p.qkv, p.out, p.k_cache, p.v_cache, p.page_table = qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr()
     p.ld_qkv, p.ld_out = qkv.stride(0), out.stride(0)
     p.n_heads, p.n_kv_heads, p.head_dim, p.q_off = n_heads, n_kv_heads, head_dim, q_off
     p.n_tokens, p.pos0, p.window, p.scale = int(n_tokens), int(pos0), int(window or 0), head_dim ** -0.5
-    p.kv_q8 = fmt
-    if fmt == KV_Q4:
-        p.num_pages, p.pt_len = int(k_cache.shape[0]), int(page_table.shape[-1])
-        p.scratch, p.scratch_floats = ptr(scratch), 0 if scratch is None else scratch.numel()
+    p.kv_q8 = kv_format(k_cache, head_dim)
     p.out_bf16 = 1 if out.dtype == torch.bfloat16 else 0          # bf16: written as the operand of the output-projection GEMM
     p.pos0_ptr = ptr(pos0_dev)
     check(lib().rlz_attn_prefill_impl(ctypes.byref(p), stream_ptr(), {None: -1, "tc": 0, "mma": 1}[impl]), "attn_prefill")
+
+
+def _attn_prefill_q4(qkv, out, k_cache, v_cache, page_table, n_tokens, pos0, n_heads, n_kv_heads, head_dim, q_off, window, pos0_dev, impl, scratch) -> None:
+    n, d, width, pages = int(n_tokens), head_dim, n_heads * head_dim, page_table.shape[-1]
+    shape, dev, ld, ld_out, bf16 = k_cache.shape, k_cache.get_device(), qkv.stride(0), out.stride(0), out.dtype is torch.bfloat16
+    f32, i32 = torch.float32, torch.int32
+    # one test for a call that is in order, as in qk_norm_rope_append
+    if not (n >= 1 and d in Q4_HEAD_DIMS and n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0 and impl != "mma"
+            and k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8 and shape[1:] == (n_kv_heads, 16, d // 2 + 4) and v_cache.shape == shape
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.get_device() == dev
+            and qkv.dtype is f32 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[0] >= n and q_off >= 0 and qkv.shape[1] >= q_off + width and qkv.get_device() == dev
+            and (bf16 or out.dtype is f32) and out.dim() == 2 and out.stride(1) == 1 and out.shape[0] >= n and out.shape[1] >= width and out.get_device() == dev
+            and ld_out % (8 if bf16 else 4) == 0 and out.data_ptr() % 16 == 0 and (ld_out >= width or n == 1)
+            and page_table.dtype is i32 and page_table.dim() == 1 and page_table.is_contiguous() and page_table.get_device() == dev
+            and pos0 >= 0 and window >= 0 and (pos0_dev is not None or pos0 + n <= 16 * pages)
+            and (pos0_dev is None or (pos0_dev.dtype is i32 and pos0_dev.numel() >= 1 and pos0_dev.get_device() == dev))
+            and (scratch is None or (scratch.dtype is f32 and scratch.is_contiguous() and scratch.get_device() == dev))
+            and dev >= 0 and dev == torch._C._cuda_getDevice()):
+        _refuse_prefill(qkv, out, k_cache, v_cache, page_table, n, pos0, n_heads, n_kv_heads, d, q_off, window, pos0_dev, impl, scratch)
+    p = S.AttnPrefillParams(qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), ld, ld_out, n_heads, n_kv_heads, d, q_off,
+                            n, int(pos0), int(window), KV_Q4, d ** -0.5, bf16, ptr(pos0_dev), shape[0], pages, ptr(scratch), 0 if scratch is None else scratch.numel())
+    check(lib().rlz_attn_prefill_impl(ctypes.byref(p), stream_ptr(), -1), "attn_prefill")
+
+
+def _refuse_prefill(qkv, out, k_cache, v_cache, page_table, n_tokens, pos0, n_heads, n_kv_heads, head_dim, q_off, window, pos0_dev, impl, scratch) -> None:
+    if n_tokens < 1:
+        raise ValueError(f"n_tokens must be at least 1, got {n_tokens}")
+    _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, out, page_table, pos0_dev, scratch)
+    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads:
+        raise ValueError(f"{n_heads} query heads do not divide over {n_kv_heads} kv heads")
+    if impl == "mma":
+        raise ValueError("impl='mma' serves bf16 caches only")
+    if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[0] < n_tokens or q_off < 0 or qkv.shape[1] < q_off + n_heads * head_dim:
+        raise ValueError("qkv must be float32 [>= n_tokens, >= q_off + n_heads * head_dim] with contiguous rows")
+    if out.dtype not in (torch.float32, torch.bfloat16) or out.dim() != 2 or out.stride(1) != 1 or out.shape[0] < n_tokens or out.shape[1] < n_heads * head_dim:
+        raise ValueError("out must be float32 or bfloat16 [>= n_tokens, >= n_heads * head_dim] with contiguous rows")
+    if out.data_ptr() % 16 or out.stride(0) * out.element_size() % 16 or (n_tokens > 1 and out.stride(0) < n_heads * head_dim):
+        raise ValueError("rows of out must start on 16-byte boundaries and not overlap")
+    if page_table.dtype != torch.int32 or page_table.dim() != 1 or not page_table.is_contiguous():
+        raise ValueError("page_table must be a contiguous int32 row")
+    if pos0 < 0 or window < 0 or (pos0_dev is None and pos0 + n_tokens > 16 * page_table.numel()):
+        raise ValueError(f"positions {pos0} .. {pos0 + n_tokens - 1} are not covered by {page_table.numel()} pages")
+    if pos0_dev is not None and (pos0_dev.dtype != torch.int32 or pos0_dev.numel() < 1):
+        raise ValueError("pos0_dev must be int32")
+    if scratch is not None and (scratch.dtype != torch.float32 or not scratch.is_contiguous()):
+        raise ValueError("scratch must be a contiguous float32 tensor from attn_prefill_scratch")
+    _check_current_device(k_cache)
+    raise ValueError("attn_prefill: invalid arguments")
 
 
 def attn_prefill_error(clear: bool = True) -> int:
@@ -368,8 +399,8 @@ def attn_prefill_error(clear: bool = True) -> int:
 
 
 def attn_prefill_scratch(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
-    """Workspace with which ``attn_prefill`` splits chunks of up to ``n_tokens`` rows over a 4-bit cache along the keys when the rows
-    alone leave SMs idle.  One to a stream; it keeps nothing from one call for the next."""
+    """Workspace with which ``attn_prefill`` divides chunks over a 4-bit cache along the keys when the rows alone leave SMs idle: the same
+    size for any number of rows.  One to a stream; it keeps nothing from one call for the next."""
     return torch.zeros(int(lib().rlz_attn_prefill_q4_scratch_floats(int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim))), device=device, dtype=torch.float32)
 
 
@@ -486,7 +517,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, page_rows: t
             and qkv.get_device() == dev and v_cache.get_device() == dev and 0 <= rope_dim <= d and rope_dim % 2 == 0 and (q_norm_w is None) == (k_norm_w is None)
             and all(w is None or (w.dtype is f32 and w.numel() == d and w.is_contiguous() and w.get_device() == dev) for w in (q_norm_w, k_norm_w))
             and (rope_table is None or (rope_table.dtype is f32 and rope_table.shape[1:] == (rope_dim // 2, 2) and rope_table.is_contiguous() and rope_table.get_device() == dev))
-            and ld % 2 == 0 and ld_q % 2 == 0 and qkv.data_ptr() % 8 == 0 and q.data_ptr() % 8 == 0
+            and ld % 2 == 0 and ld_q % 2 == 0 and (ld_q >= n_heads * d or n < 2) and qkv.data_ptr() % 8 == 0 and q.data_ptr() % 8 == 0
             and dev >= 0 and dev == torch._C._cuda_getDevice()):
         _refuse_append(qkv, positions, page_rows, k_cache, v_cache, n_heads, n_kv_heads, head_dim, q_out, q_norm_w, k_norm_w, rope_dim, rope_table)
     if n == 0:
@@ -524,6 +555,8 @@ def _refuse_append(qkv, positions, page_rows, k_cache, v_cache, n_heads, n_kv_he
         raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim / 2, 2] (cos, sin) tensor")
     if qkv.stride(0) % 2 or q.stride(0) % 2 or qkv.data_ptr() % 8 or q.data_ptr() % 8:
         raise ValueError("rows of qkv and q_out must start on 8-byte boundaries")
+    if n > 1 and q.stride(0) < n_heads * head_dim:
+        raise ValueError("rows of q_out overlap")
     _check_current_device(k_cache)
     raise ValueError("qk_norm_rope_append: invalid arguments")
 

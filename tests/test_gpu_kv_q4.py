@@ -388,7 +388,175 @@ def test_prompt_attention_long(cuda_device):
     _prompt(8, 1, 64, 1100, 1500)
 
 
+@pytest.mark.parametrize("h, kvh, d, rows, pos0, kw", [
+    (8, 4, 64, 4999, 0, dict(window=2000)), (16, 16, 80, 1700, 5995, {}), (8, 8, 96, 3600, 700, dict(dev_pos=True, window=900)), (24, 8, 128, 1501, 3333, dict(out_dtype=torch.float32))])
+def test_prompt_attention_divided_evenly(cuda_device, h, kvh, d, rows, pos0, kw):
+    """More row tiles than SMs, or a number that leaves many idle: shares that begin and end inside row tiles, tiles with one group of rows."""
+    _prompt(h, kvh, d, rows, pos0, **kw)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 600])
+def test_prompt_attention_window_beyond_the_positions(cuda_device, window):
+    _prompt(4, 2, 64, 90, 500, window=window)
+
+
+def test_prompt_attention_rows_on_odd_addresses(cuda_device):
+    """Query rows that start on 4-byte boundaries only."""
+    from realizar_b200 import ops
+    h, kvh, d, n = 6, 2, 80, 70
+    kc, vc = _cache(6, kvh, d)
+    pt = torch.arange(6, device="cuda", dtype=torch.int32)
+    qkv = torch.randn(n, (h + 2 * kvh) * d, device="cuda")
+    odd = torch.zeros(n, (h + 2 * kvh) * d + 3, device="cuda")[:, 1:]
+    odd[:, :qkv.shape[1]] = qkv
+    a, b = torch.empty(2, n, h * d, device="cuda")
+    ops.attn_prefill(qkv, a, kc, vc, pt, n, 5, h, kvh, d)
+    ops.attn_prefill(odd, b, kc, vc, pt, n, 5, h, kvh, d)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["constant first", "growing", "shrinking"])
+def test_prompt_wide_ranges_of_scales(cuda_device, kind):
+    """Values whose scales differ by many orders of magnitude: the operands' power of two moves with them."""
+    from realizar_b200 import ops
+    h, kvh, d, n, rows = 4, 1, 64, 400, 60
+    kc, vc = _cache(26, kvh, d)
+    pt = torch.randperm(26, device="cuda").to(torch.int32)[:25].contiguous()
+    i = torch.arange(400, device="cuda").float()
+    sc = {"constant first": torch.where(i < 200, 0.0, 1e-6), "growing": torch.exp2(i / 16 - 20), "shrinking": torch.exp2(5 - i / 16)}[kind]
+    vc.flatten(-2)[pt.long(), 0, 8 * d:] = torch.stack([sc, -7.5 * sc], -1).bfloat16().view(torch.uint8).view(-1, 64)
+    qkv = torch.randn(rows, (h + 2 * kvh) * d, device="cuda")
+    ks, vs = _gather(kc, pt, d, False, n), _gather(vc, pt, d, True, n)
+    for scratch in (None, ops.attn_prefill_scratch(rows, h, kvh, d, "cuda")):
+        out = torch.empty(rows, h * d, device="cuda")
+        ops.attn_prefill(qkv, out, kc, vc, pt, rows, n - rows, h, kvh, d, scratch=scratch)
+        for r in range(0, rows, 7):
+            p1 = n - rows + r + 1
+            assert _rel(out[r], _attend64(qkv[r, : h * d].double().view(h, d), ks[:, :p1], vs[:, :p1], 0)) < 4e-3, r
+
+
+def test_prompt_device_checks(cuda_device):
+    """Rows beyond the page table are left alone, a page id outside the cache reads page 0; the status word tells of both."""
+    from realizar_b200 import ops
+    h, kvh, d, n = 8, 2, 128, 40
+    kc, vc = _cache(5, kvh, d)
+    pt = torch.tensor([3, 0, 2, 1], device="cuda", dtype=torch.int32)
+    qkv, out = torch.randn(n, (h + 2 * kvh) * d, device="cuda"), torch.full((n, h * d), 9.0, device="cuda")
+    ops.device_error()
+    for first in (25, -1, 2 ** 31 - 8):
+        ops.attn_prefill(qkv, out, kc, vc, pt, n, 0, h, kvh, d, pos0_dev=torch.tensor([first], device="cuda", dtype=torch.int32))
+        torch.cuda.synchronize()
+        assert ops.device_error() == 3114 and ops.device_error() == 0 and bool((out == 9.0).all())
+    ops.attn_prefill(qkv, out, kc, vc, pt, n, 0, h, kvh, d, pos0_dev=torch.tensor([24], device="cuda", dtype=torch.int32))
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    for bad in (5, -3):
+        ops.attn_prefill(qkv, out, kc, vc, torch.tensor([3, bad, 2, 1], device="cuda", dtype=torch.int32), n, 24, h, kvh, d)
+        torch.cuda.synchronize()
+        want = torch.empty_like(out)
+        assert ops.device_error() == 3113
+        ops.attn_prefill(qkv, want, kc, vc, pt, n, 24, h, kvh, d)
+        assert torch.equal(out, want)
+
+
+def test_prompt_scratch_of_other_sizes(cuda_device):
+    """A workspace that is too small is not used, a larger one is; both leave it as it was for the next call."""
+    from realizar_b200 import ops
+    small, large = ops.attn_prefill_scratch(64, 4, 1, 64, "cuda"), ops.attn_prefill_scratch(64, 4, 1, 128, "cuda")
+    res = []
+    for d in (128, 64, 128):
+        kc, vc = _cache(60, 1, d, seed=1)
+        pt, qkv = torch.arange(60, device="cuda", dtype=torch.int32), torch.randn(64, 6 * d, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+        outs = [torch.empty(64, 4 * d, device="cuda") for _ in range(3)]
+        for o, s in zip(outs, (None, small, large)):
+            ops.attn_prefill(qkv, o, kc, vc, pt, 64, 800, 4, 1, d, scratch=s)
+        assert ops.device_error() == 0
+        assert _rel(outs[1], outs[0]) < 1e-3 and _rel(outs[2], outs[0]) < 1e-3          # P is rounded to fp16 (2^-12) against the maximum of other parts
+        res.append(outs)
+    assert torch.equal(res[0][2], res[2][2])
+
+
 # ------------------------------------------------------------------------------------------------ together
+def test_captured_append_and_prompt_replay_at_other_positions(cuda_device):
+    """A chunk's append and attention in one graph: positions, pages and the first position are read on the device.  Two graphs share a workspace."""
+    from realizar_b200 import ops
+    h, kvh, d, n = 8, 2, 128, 32
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(96, (h + 2 * kvh) * d, generator=g, device="cuda")
+    table, pt = ops.make_rope_table(128, d, 1e4, "cuda"), torch.tensor([4, 1, 6, 0, 5, 2], device="cuda", dtype=torch.int32)
+    scratch = ops.attn_prefill_scratch(n, h, kvh, d, "cuda")
+    caches = [ops.kv_cache_alloc(1, 7, kvh, d, "cuda", "q4")[:, 0] for _ in range(3)]
+
+    def chunk(c, first, qkv, pos, pages, p0, out):
+        qkv.copy_(x[first:first + n])
+        pos.copy_(torch.arange(first, first + n, dtype=torch.int32)); pages.copy_(pt[(pos // 16).long()]); p0.fill_(first)
+
+    def launches(c, qkv, pos, pages, p0, out):
+        ops.qk_norm_rope_append(qkv, pos, pages, caches[c][0], caches[c][1], h, kvh, d, rope_dim=d, rope_type=2, rope_table=table)
+        ops.attn_prefill(qkv, out, caches[c][0], caches[c][1], pt, n, 0, h, kvh, d, pos0_dev=p0, scratch=scratch)
+
+    bufs = [(torch.empty(n, x.shape[1], device="cuda"), torch.empty(n, device="cuda", dtype=torch.int32), torch.empty(n, device="cuda", dtype=torch.int32),
+             torch.zeros(1, device="cuda", dtype=torch.int32), torch.empty(n, h * d, device="cuda", dtype=torch.bfloat16)) for _ in range(3)]
+    graphs = []
+    for c in (0, 1):
+        chunk(c, 0, *bufs[c])
+        launches(c, *bufs[c])
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[c]):
+            launches(c, *bufs[c])
+    for c in range(3):
+        caches[c].zero_()
+    for first in (0, 32, 64):
+        for c in range(3):
+            chunk(c, first, *bufs[c])
+        for c in (0, 1):
+            graphs[c].replay()
+        launches(2, *bufs[2])
+        torch.cuda.synchronize()
+        assert ops.device_error() == 0
+        for c in (0, 1):
+            assert torch.equal(bufs[c][4], bufs[2][4]) and torch.equal(caches[c], caches[2])
+
+
+def test_prompts_on_two_streams_with_their_own_workspaces(cuda_device):
+    from realizar_b200 import ops
+    h, kvh, d = 8, 2, 64
+    jobs = []
+    for i, (n, first) in enumerate(((50, 900), (300, 700))):
+        kc, vc = _cache(64, kvh, d, seed=i)
+        qkv = torch.randn(n, (h + 2 * kvh) * d, device="cuda")
+        a = (kc, vc, torch.randperm(64, device="cuda").to(torch.int32), n, first, h, kvh, d)
+        want, scratch = torch.empty(n, h * d, device="cuda"), ops.attn_prefill_scratch(n, h, kvh, d, "cuda")
+        ops.attn_prefill(qkv, want, *a, scratch=scratch)
+        jobs.append((qkv, torch.empty_like(want), a, scratch, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for qkv, out, a, scratch, _, stream in jobs:
+            with torch.cuda.stream(stream):
+                ops.attn_prefill(qkv, out, *a, scratch=scratch)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    for _, out, _, _, want, _ in jobs:
+        assert torch.equal(out, want)
+
+
+def test_decode_static_entry_point(cuda_device):
+    """The entry point with built-in scratch takes 4-bit caches too, twice in a row."""
+    import ctypes
+    from realizar_b200 import ops
+    fn = ops.lib().rlz_attn_decode_static
+    fn.argtypes, fn.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
+    check = _decode(8, 2, 128, [3000, 17], seed=6, rope_dim=128)
+    check()
+    want = check.keep[1].clone()
+    for _ in range(2):
+        check.keep[1].fill_(9.0)
+        assert fn(ctypes.addressof(check.params), torch.cuda.current_stream().cuda_stream) == 0
+        check(launch=False)
+        assert torch.equal(check.keep[1], want)
+
+
 def test_append_prompt_decode_as_a_serving_pass(cuda_device):
     """A prompt in two chunks and then single tokens, all through the cache, against attention in 64 bits over the values the cache holds;
     the rows a prompt pass writes and those a decode step writes are the same bits."""

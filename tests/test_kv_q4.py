@@ -93,6 +93,22 @@ def test_prefill_refuses(change, word):
         ops.attn_prefill(**{**a, **change})
 
 
+@pytest.mark.parametrize("change, word", [
+    (dict(out=torch.zeros(4, 258)[:, 2:]), "16-byte"), (dict(out=torch.zeros(4, 259)[:, :256]), "16-byte"), (dict(out=torch.zeros(1, 256).expand(4, 256)), "overlap"),
+    (dict(impl="mma"), "mma"), (dict(n_heads=3), "divide"), (dict(q_off=-64), "qkv"), (dict(page_table=torch.zeros(4, dtype=torch.int32)[::2]), "page_table")])
+def test_prefill_refuses_layouts(change, word):
+    kv = ops.kv_cache_alloc(1, 3, 2, 64, "cpu", "q4")
+    a = dict(qkv=torch.zeros(4, 512), out=torch.zeros(4, 256), k_cache=kv[0, 0], v_cache=kv[1, 0], page_table=torch.zeros(2, dtype=torch.int32), n_tokens=4, pos0=0,
+             n_heads=4, n_kv_heads=2, head_dim=64)
+    with pytest.raises(ValueError, match=word):
+        ops.attn_prefill(**{**a, **change})
+
+
+def test_append_refuses_overlapping_results():
+    with pytest.raises(ValueError, match="overlap"):
+        ops.qk_norm_rope_append(**_append_args(), q_out=torch.zeros(1, 256).expand(4, 256))
+
+
 def test_cli_offers_the_format():
     from realizar_b200.cli import build_parser
     assert build_parser().parse_args(["run", "m.gguf", "hi", "--kv-dtype", "q4"]).kv_dtype == "q4"
