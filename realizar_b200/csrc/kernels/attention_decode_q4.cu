@@ -6,7 +6,8 @@
 // Bound by the bytes of the cache as long as the arithmetic of the codes is cheap (96 sequences of 8192 tokens of 128 dims, 8 kv heads:
 // 130 us, 4.5 TB/s of the 6.6 that a copy reaches):
 //   * Keys: a masked word holds four codes as bytes, and the 8-bit integer product takes them as they are; q comes as three 8-bit
-//     digits of a 23-bit integer (its largest value in [2^21, 2^22)), so the sums over the dims are exact.
+//     digits of a 24-bit integer (its largest value in [2^22, 2^23) x 127 / 128), so the sums over the dims are exact; sum(q) is that of
+//     the integers.
 //   * Values: a nibble under the exponent of 1024 is the fp16 1024 + code (or 1024 + 16 code), which one subtraction (or
 //     multiply-add) turns into code - 8 exactly: 9 instructions to 8 codes.  The 8 goes into the minimum: without it, sum p scale code
 //     and sum p min cancel, over 131072 tokens to 1 / 900, and so do the digits of the result (2e-4 of it instead of 1e-6).
@@ -88,7 +89,7 @@ __device__ __forceinline__ void mma_s8_half(int* c, uint32_t a0, uint32_t a1, ui
 }
 // four codes of 16 bits as bytes
 __device__ __forceinline__ uint32_t nib_bytes(uint32_t h) { const uint32_t x = (h | h << 8) & 0x00FF00FFu; return (x | x << 4) & 0x0F0F0F0Fu; }
-// an integer below 2^22 as three signed bytes, the first in the low bits
+// an integer below 2^23 x 127 / 128 as three signed bytes, the first in the low bits
 __device__ __forceinline__ uint32_t digits(int q) {
   const int d2 = (int)(int8_t)(q & 255), q1 = (q - d2) >> 8, d1 = (int)(int8_t)(q1 & 255), d0 = (q1 - d1) >> 8;
   return (uint32_t)(d0 & 255) | (uint32_t)(d1 & 255) << 8 | (uint32_t)(d2 & 255) << 16;
@@ -473,6 +474,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     if (own) load(row + (own_v ? p.v_off : p.k_off) + kvh * D, own_v ? 0 : half, own_v ? 0 : p.rope_type, ra, rb);
     for (int g = hw; g < ROWS; g += QD_HELPERS / 32) {
       float f = 1.f, sum = 0.f;
+      int isum = 0;
       if (g < gn) {
         load(row + p.q_off + (int64_t)(kvh * G + g0 + g) * D, half, p.rope_type, xa, xb);
         norm_rope_f<D>(xa, xb, p.q_norm_w, p.eps, rope, cs, lane);
@@ -483,14 +485,21 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           top = fmaxf(top, fmaxf(fabsf(xa[k]), fabsf(xb[k]))); sum += xa[k] + xb[k];
         }
         top = warp_max(top); sum = warp_sum(sum);
-        f = top > 0.f ? pow2_for(top, 21) : 1.f;
+        f = top > 0.f ? pow2_for(top, 22) * (127.f / 128.f) : 1.f;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
           const int i = lane + 32 * k;
-          if (i < D / 2) { const int2 at = pair_dims(i, half, p.rope_type); sm.q[g][at.x] = xa[k] * f; sm.q[g][at.y] = xb[k] * f; }
+          if (i < D / 2) {
+            const int2 at = pair_dims(i, half, p.rope_type);
+            const int ia = __float2int_rn(xa[k] * f), ib = __float2int_rn(xb[k] * f);
+            sm.q[g][at.x] = (float)ia; sm.q[g][at.y] = (float)ib;
+            isum += ia + ib;
+          }
         }
+        isum = __reduce_add_sync(0xFFFFFFFFu, isum);
       }
-      if (lane == 0) { sm.qc[buf][g] = g < gn ? 1.f / f : 0.f; sm.qx[buf][g] = sum; }
+      // the sum of the integers, so that their roundings meet centred keys (NaN and infinite queries stay what they are by the other sum)
+      if (lane == 0) { const float qc = g < gn ? 1.f / f : 0.f; sm.qc[buf][g] = qc; sm.qx[buf][g] = fmaf((float)isum, qc, sum * 0.f); }
     }
     helpers_sync();
     // column gq is head gq / 2 of a tile, its digits 0 (even) or 1 (odd), and in the second pair of registers digit 2 (even).  Word tq of
