@@ -1,15 +1,20 @@
 // Causal attention of the rows of a prompt chunk over the 4-bit paged cache (kv_q4.cuh), on the tcgen05 tensor cores.
 //
 // A CTA has two groups of 128 rows of one kv head, row = (token, query head of the group): the group's heads share the keys and values
-// that the CTA turns into fp16.  Per group and 128 keys:
-//   S = Q K^T      128 x 128 x D, accumulated in TMEM
+// that the CTA turns into fp16, 128 keys at a time.  Per group and half a tile (64 keys):
+//   S = Q K^T      128 x 64 x D, accumulated in TMEM
 //   P = 2^(S - m)  one thread to a row; P goes back to TMEM as fp16, over the columns of S, and is the A operand of
-//   O += P V       128 x D x 128, accumulated in TMEM.  The running maximum moves only when a score passes it by 2^8, so that O is
+//   O += P V       128 x D x 64, accumulated in TMEM.  The running maximum moves only when a score passes it by 2^8, so that O is
 //                  rarely read, scaled and written back.
 // Warps 0..7 do the softmax of the groups, 8..11 decode keys and 12..15 values (code x scale + minimum in fp16, rounded once) into two
-// buffers each of swizzled operand tiles, warp 16 issues the products: while one group is at its exponentials the tensor cores work
-// for the other.  Products (2048 clocks to 256 rows and 128 keys of 128 dims) and exponentials (16 a clock) take the same time.
-// Registers are moved from the decoding and issuing warps to the softmax.
+// buffers each of swizzled operand tiles, warps 16 and 17 issue the products of a group each.  The scores of one half are computed while
+// the softmax is at the other (whole tiles, whose scores have to wait for the product that reads P in their place: 280 instead of
+// 266 us for 2048 rows behind 6144 keys, 32 query and 8 kv heads of 128).  Registers are moved from the decoding and issuing warps to
+// the softmax.
+//
+// Bound, for 256 rows and 128 keys of 128 dims, by the chain of product, softmax and product, about 4000 clocks: of them the tensor
+// cores work 2560 (products of 64 keys read the queries from shared memory twice as often: 384 instead of 256 clocks), the exponentials
+// take 2048 (16 a clock) and the decoding 9% of the issue slots' time.
 //
 // Range: K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
 // softmax scale; V by one that changes only when a tile needs it, with O), q by one to a row.
@@ -30,8 +35,8 @@ namespace rlz {
 __device__ int g_prefill_q4_error = 0;
 
 constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148;
-constexpr int QP_MIN_TILES = 2, QP_SEG_COST = 5;      // least share of a CTA; what another row tile costs it, in key tiles (12 us)
-constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 88, QP_REGS_ISSUE = 48;      // 256, 256 and 128 threads: the launch's 640 x 96
+constexpr int QP_MIN_TILES = 2, QP_SEG_COST = 5;      // least share of a CTA; what another row tile costs it, in key tiles
+constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 96, QP_REGS_ISSUE = 32;      // 256, 256 and 128 threads: the launch's 640 x 96
 constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
 constexpr int QP_COUNTERS = 640;               // floats in front of the parts: arrival counters, one to each of a CTA's two slots and group
 
@@ -43,11 +48,9 @@ struct QpShape { int G, rows, mtiles, pos0; };
 struct QpSched { int left, each, more, parts; QpShape z; };
 
 struct QpSmem {
-  unsigned long long q_full[2], s_full[2], p_full[2], o_full[2];        // of the groups
-  unsigned long long p_half[2], pad[2];                                 // the first half of P
+  unsigned long long q_full[2], s_full[2][2], p_full[2][2], o_full[2][2];        // of the groups, and of the tile's halves (64 keys each)
   unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];      // of the buffers (empty: an arrival from each group's products)
-  unsigned long long turn[2][4];                                        // a group's warps may do their exponentials
-  float kf[4], vf[2];                         // powers of two that the tiles carry (K's are read after the buffer is free again)
+  float kf[4], vf[2];                         // powers of two that the tiles carry (of K the inverse, read after the buffer is free again)
   float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
   float qf[2][QP_GROUP];                      // powers of two of the query rows
   uint32_t tmem;
@@ -68,7 +71,7 @@ __device__ __forceinline__ float qp_pow2(float x, int e) {
 // descriptors stay in uniform registers; issued from a branch of one lane, a product cost 80 clocks of moves.)
 // Operand tiles are given by the low words of their descriptors; the high word is that of all K-major tiles with 128-byte swizzle
 constexpr uint32_t QP_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ uint32_t qp_desc_lo(const void* tile) { return (gm_smem_u32(tile) >> 4 & 0x3FFFu) | 1u << 16; }
+__device__ __forceinline__ uint32_t qp_desc_lo(uint32_t tile) { return (tile >> 4 & 0x3FFFu) | 1u << 16; }
 __device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint32_t lo_a, uint32_t lo_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
                "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%5, %5, %5, %5}, p;\n\t}\n"
@@ -87,6 +90,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// (the tiles are reached by their 32-bit shared addresses: a generic store takes 64-bit sums for each address)
+__device__ __forceinline__ void st_shared(uint32_t at, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -212,15 +219,13 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
   constexpr uint32_t TMEM_COLS = 512;         // S and P of the groups: columns 0.. and 128.., O: 256.. and 384..
   extern __shared__ __align__(1024) uint8_t qp_smem[];
   __shared__ QpSmem sm;
-  uint8_t* Qs = (uint8_t*)(((uintptr_t)qp_smem + 1023) & ~(uintptr_t)1023);
-  uint8_t* Ks = Qs + 2 * Q_BYTES;
-  uint8_t* Vs = Ks + 2 * K_BYTES;             // a tile is two slabs of [D rows x 64 keys]
+  const uint32_t Qs = (gm_smem_u32(qp_smem) + 1023u) & ~1023u, Ks = Qs + 2 * Q_BYTES, Vs = Ks + 2 * K_BYTES;             // a tile is two slabs of [D rows x 64 keys]
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;      // (the same in all lanes, for the compiler too)
   const int G = p.n_heads / p.n_kv_heads, rows = p.n_tokens * G;
   auto groups_of = [&](int mt) { return rows - mt * QP_ROWS > QP_GROUP ? 2 : 1; };
   auto init_barriers = [&](int groups) {                          // by a warp
-    if (lane < 28) {
-      const int count = lane < 2 || lane == 4 || lane == 5 || lane == 8 || lane == 9 ? QP_GROUP : lane == 12 || lane == 13 || lane == 16 || lane == 17 ? 128 : lane >= 12 && lane < 20 ? groups : 1;
+    if (lane < 22) {
+      const int count = lane < 2 || (lane >= 6 && lane < 10) || lane == 14 || lane == 15 || lane == 18 || lane == 19 ? 128 : lane >= 16 ? groups : 1;
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(gm_smem_u32(&sm.q_full[0] + lane)), "r"(count));
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       }
       __syncwarp();
       if (sm.seg.n) {                                              // (every arrival of the tile before has been waited for)
-        if (lane < 28) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(gm_smem_u32(&sm.q_full[0] + lane)) : "memory");
+        if (lane < 22) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(gm_smem_u32(&sm.q_full[0] + lane)) : "memory");
         init_barriers(groups_of(sm.seg.mt));
       }
     }
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       const int pos = pos0 + token;
       // ---- queries: 8 dims to a lane, stored as fp16 in the order in which the keys' codes come out of a word: (0, 4), (1, 5), (2, 6),
       // (3, 7) of every 8 dims.  A short loop: these instructions run once to a CTA, and fetching them takes longer than the loads
-      uint8_t* q_tile = Qs + grp * Q_BYTES;
+      const uint32_t q_tile = Qs + (uint32_t)(grp * Q_BYTES);
       const bool vec = (((uintptr_t)p.qkv | (uintptr_t)(4 * p.ld_qkv) | (uintptr_t)(4 * p.q_off)) & 15) == 0;
       {
         constexpr int LANES = D == 64 ? 8 : 16, STEP = 32 / LANES, BATCH = 8;     // lanes to a row, rows at once and their loads in flight
@@ -318,9 +323,10 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
             const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
             if (x == 0) sm.qf[grp][r] = f;
-            if (x < NSLAB * 8)
-              *(uint4*)(q_tile + (x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4)) =
-                  make_uint4(qp_half2(a.x * f, b.x * f), qp_half2(a.y * f, b.y * f), qp_half2(a.z * f, b.z * f), qp_half2(a.w * f, b.w * f));
+            if (x < NSLAB * 8) {
+              const uint32_t w[4] = {qp_half2(a.x * f, b.x * f), qp_half2(a.y * f, b.y * f), qp_half2(a.z * f, b.z * f), qp_half2(a.w * f, b.w * f)};
+              st_shared(q_tile + (uint32_t)((x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4)), w);
+            }
           }
         }
       }
@@ -333,88 +339,70 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       float2 l2 = make_float2(0.f, 0.f);
       const int row_first = m0 + grp * QP_GROUP, row_last = min(rows, row_first + QP_GROUP) - 1;
       const int pos_first = pos0 + row_first / G, lo_last = p.window > 0 ? pos0 + row_last / G + 1 - p.window : 0;     // masks are needed beyond these
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        const int k0 = kbeg + j * QP_KEYS, buf = j & 1;
+      for (int i = 0; ok && i < 2 * n_tiles; ++i) {
+        const int j = i >> 1, half = i & 1, k0 = kbeg + 64 * i, buf = j & 1;
+        const uint32_t s_at = lane_s + (uint32_t)(64 * half);
         // the scores, and with them the tile's power of two of K; that of V
-        ok = qp_wait(&sm.s_full[grp], (uint32_t)j & 1u) && qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u);
+        ok = qp_wait(&sm.s_full[grp][half], (uint32_t)j & 1u) && (half || qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u));
         if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
         tc_after();
-        const float sc = qs / sm.kf[j & 3], vn = sm.vf[buf];
-        const bool edge = k0 + QP_KEYS - 1 > pos_first || k0 < lo_last;
+        const float sc = qs * sm.kf[j & 3], vn = sm.vf[buf];
+        const bool edge = k0 + 63 > pos_first || k0 < lo_last;
         const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
         // EDGE: some entries are masked
-        auto tile = [&](auto edge_c) {
+        auto part = [&](auto edge_c) {
           constexpr bool EDGE = decltype(edge_c)::value;
-          float top = -INFINITY, top1 = -INFINITY;
           uint32_t r[2][32];
+          tmem_ld32_async(s_at, r[0]);
+          tmem_ld32_async(s_at + 32u, r[1]);
+          tmem_wait_ld(r[0]);
+          tmem_wait_ld(r[1]);
           auto seen = [&](int key) { return !EDGE || (key < vis_hi && key >= vis_lo); };
-          auto largest_of = [&](const uint32_t (&x)[32], int key) {
+          float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              top = max3(top, seen(key + i) ? __uint_as_float(x[i]) : -INFINITY, seen(key + i + 1) ? __uint_as_float(x[i + 1]) : -INFINITY);
-              top1 = max3(top1, seen(key + i + 2) ? __uint_as_float(x[i + 2]) : -INFINITY, seen(key + i + 3) ? __uint_as_float(x[i + 3]) : -INFINITY);
-            }
-          };
-          // two loads of 32 scores in turn.  Not unrolled, here and below: spread over the whole tile, the compiler's order of loads,
-          // exponentials and stores took a fifth more time
-          tmem_ld32_async(lane_s, r[0]);
-#pragma unroll 1
-          for (int c = 0; c < QP_KEYS; c += 64) {
-            tmem_wait_ld(r[0]);
-            tmem_ld32_async(lane_s + (uint32_t)(c + 32), r[1]);
-            largest_of(r[0], c);
-            tmem_wait_ld(r[1]);
-            tmem_ld32_async(lane_s + (uint32_t)(c == 0 ? 64 : 0), r[0]);         // the last one is the first of the second pass
-            largest_of(r[1], c + 32);
+          for (int k = 0; k < 64; k += 4) {
+            auto score = [&](int key) { return seen(key) ? __uint_as_float(r[key >> 5][key & 31]) : -INFINITY; };
+            top = max3(top, score(k), score(k + 1));
+            top1 = max3(top1, score(k + 2), score(k + 3));
           }
           top = fmaxf(top, top1) * sc;
           if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
             const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
-            if (j > 0) {                                               // (the product before has ended: the issuing warp waits for it before it overwrites S)
+            if (i > 0) {
+              ok = __all_sync(0xFFFFFFFFu, qp_wait(&sm.o_full[grp][half ^ 1], (uint32_t)((i - 1) >> 1) & 1u));      // the product before has ended
+              tc_after();
 #pragma unroll 1
               for (int c0 = 0; c0 < D; c0 += 16) {
-                uint32_t r[16];
-                tmem_ld16(lane_o + (uint32_t)c0, r);
+                uint32_t o[16];
+                tmem_ld16(lane_o + (uint32_t)c0, o);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * co);
-                tmem_st16(lane_o + (uint32_t)c0, r);
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * co);
+                tmem_st16(lane_o + (uint32_t)c0, o);
               }
             }
             l2.x *= corr; l2.y *= corr; m = mn; vf = vn;
           }
           const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
           const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
-          // in turn with the other group's warp on the same scheduler: while one does its exponentials, the other waits for products or
-          // looks for its maxima
-          if (groups > 1 && grp + j > 0) ok = __all_sync(0xFFFFFFFFu, qp_wait(&sm.turn[grp][warp & 3], (uint32_t)(j + grp - 1) & 1u));
-          auto exponentials = [&](const uint32_t (&x)[32], int key) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, b2);
-              const float2 e = make_float2(seen(key + i) ? qp_ex2(y.x) : 0.f, seen(key + i + 1) ? qp_ex2(y.y) : 0.f);
+            for (int k = 0; k < 32; k += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), sc2, b2);
+              const float2 e = make_float2(seen(32 * c + k) ? qp_ex2(y.x) : 0.f, seen(32 * c + k + 1) ? qp_ex2(y.y) : 0.f);
               l2 = add2(l2, e);
-              w[i >> 1] = qp_half2(e.x, e.y);
+              w[k >> 1] = qp_half2(e.x, e.y);
             }
-            tmem_st16(lane_s + (uint32_t)(key >> 1), w);               // columns key / 2 ..: their scores have been read, those on their way lie behind
-          };
-#pragma unroll 1
-          for (int c = 0; c < QP_KEYS; c += 64) {
-            tmem_wait_ld(r[0]);
-            tmem_ld32_async(lane_s + (uint32_t)(c + 32), r[1]);
-            exponentials(r[0], c);
-            tmem_wait_ld(r[1]);
-            if (c == 0) tmem_ld32_async(lane_s + 64u, r[0]);
-            exponentials(r[1], c + 32);
-            if (c > 0 && groups > 1 && lane == 0) gm_arrive((uint64_t*)&sm.turn[grp ^ 1][warp & 3]);
-            tmem_wait_st();
-            tc_before();
-            gm_arrive((uint64_t*)(c == 0 ? &sm.p_half[grp] : &sm.p_full[grp]));      // the product can begin with the first 64 keys
+            tmem_st16(s_at + (uint32_t)(16 * c), w);                   // over the scores
           }
+          tmem_wait_st();
+          tc_before();
+          gm_arrive((uint64_t*)&sm.p_full[grp][half]);
         };
-        if (edge) tile(std::true_type{}); else tile(std::false_type{});
+        if (edge) part(std::true_type{}); else part(std::false_type{});
       }
-      if (ok) ok = qp_wait(&sm.o_full[grp], (uint32_t)(n_tiles - 1) & 1u);       // the last product
+      if (ok) ok = qp_wait(&sm.o_full[grp][0], (uint32_t)(n_tiles - 1) & 1u) && qp_wait(&sm.o_full[grp][1], (uint32_t)(n_tiles - 1) & 1u);       // the last products
       if (grp == 0 ? qp_agree<1>(ok) : qp_agree<2>(ok)) {
         tc_after();
         const float inv_vf = 1.f / vf, l = l2.x + l2.y;
@@ -545,9 +533,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         top = fmaxf(fmaxf(sm.mag[buf][0][0], sm.mag[buf][0][1]), fmaxf(sm.mag[buf][0][2], sm.mag[buf][0][3]));
         const float kf = qp_pow2(top, 4);                              // the tile's largest value to [2^4, 2^5)
         if (j >= 2) ok = qp_wait(&sm.k_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
-        if (t == 0) sm.kf[j & 3] = kf;
+        if (t == 0) sm.kf[j & 3] = 1.f / kf;
         const __half2 s2 = __float2half2_rn(q4_scale(km) * kf), m2 = __float2half2_rn(q4_min(km) * kf);
-        uint8_t* base = Ks + buf * K_BYTES + (t >> 3) * 1024 + (t & 7) * 128;
+        const uint32_t base = Ks + (uint32_t)(buf * K_BYTES + (t >> 3) * 1024 + (t & 7) * (128 + 16));       // 16-byte piece x of a row lies at x ^ (row % 8)
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {                              // word i of the row: 8 dims from 8 x on
           const int x = i < 4 * NG ? 4 * (i % NG) + i / NG : i;
@@ -556,7 +544,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
           uint32_t o[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) { const __half2 v = __hfma2(c[q], s2, m2); o[q] = *(const uint32_t*)&v; }
-          *(uint4*)(base + (x >> 3) * QP_SLAB + (((x & 7) ^ (t & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          st_shared((base ^ (uint32_t)((x & 7) << 4)) + (uint32_t)((x >> 3) * QP_SLAB), o);
         }
         if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -604,8 +592,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         if (j >= 2) ok = qp_wait(&sm.v_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
         if (t == 0) sm.vf[buf] = vf;
         const int chunk = (t >> 3) & 7;                                // eight keys of the 64 of a slab
-        uint8_t* base = Vs + buf * V_BYTES + (t >> 6) * (D * 128);
-        auto put = [&](int dim, const uint32_t* o) { *(uint4*)(base + (dim >> 3) * 1024 + (dim & 7) * 128 + ((chunk ^ (dim & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]); };
+        // dim 32 g + 4 vg + e is row 4 (vg % 2) + e of the eight of row group 4 g + vg / 2; its keys lie at chunk ^ row
+        const uint32_t slab = Vs + (uint32_t)(buf * V_BYTES + (t >> 6) * (D * 128));
+        const uint32_t base = slab + (uint32_t)((vg >> 1) * 1024 + (vg & 1) * 512 + ((chunk ^ (vg & 1) << 2) << 4));
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           uint32_t o[4][4];                                            // [dim][token pair]
@@ -617,7 +606,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (int e = 0; e < 4; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) put(32 * g + 4 * vg + e, o[e]);
+          for (int e = 0; e < 4; ++e) st_shared((base ^ (uint32_t)(e << 4)) + (uint32_t)(g * 4096 + e * 128), o[e]);
         }
         if constexpr (TAIL) {
           uint32_t o[2][4];
@@ -630,7 +619,10 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
             for (int e = 0; e < 2; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
           }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) put(32 * NG + 2 * vg + e, o[e]);
+          for (int e = 0; e < 2; ++e) {
+            const int dim = 2 * vg + e;
+            st_shared(slab + (uint32_t)(NG * 4096 + (dim >> 3) * 1024 + (dim & 7) * 128 + ((chunk ^ (dim & 7)) << 4)), o[e]);
+          }
         }
         if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -648,34 +640,39 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
     if (warp < 16 + groups_of(sm.seg.mt)) {
       // ================================ the products: a warp to a group, so that no group's waits hold up the other =====================
       const int g = warp - 16;
-      const uint32_t id_s = (1u << 4) | ((uint32_t)(QP_KEYS >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
+      const uint32_t id_s = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
       const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);
       const uint32_t q_lo = qp_desc_lo(Qs + g * Q_BYTES), k_lo = qp_desc_lo(Ks), v_lo = qp_desc_lo(Vs), s_col = tmem + 128u * g, o_col = s_col + 256u;
-      auto both = [&](unsigned long long* bar, uint32_t parity) { const bool r = __all_sync(0xFFFFFFFFu, qp_wait(bar, parity)); tc_after(); return r; };
-      auto values = [&](int j, int half) {                              // O += P V over 64 keys
-        const uint32_t pa = s_col + (uint32_t)(32 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_f16_ts(o_col, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, j > 0 || half + kk > 0 ? 1u : 0u);
-      };
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        const int buf = j & 1;
-        // scores, once the product of the tile before has ended (it reads P where they go)
-        if (!both(&sm.k_full[buf], (uint32_t)(j >> 1) & 1u) || !both(j == 0 ? &sm.q_full[g] : &sm.o_full[g], j == 0 ? 0u : (uint32_t)(j - 1) & 1u)) { ok = false; break; }
-        const uint32_t b = k_lo + (uint32_t)(buf * (K_BYTES >> 4));
+      auto both = [&](unsigned long long* bar, uint32_t parity) { if (ok) { ok = __all_sync(0xFFFFFFFFu, qp_wait(bar, parity)); tc_after(); } };
+      // half i of the key tiles: S = Q K^T
+      auto scores = [&](int i) {
+        const int j = i >> 1, half = i & 1;
+        if (half == 0) both(&sm.k_full[j & 1], (uint32_t)(j >> 1) & 1u);
+        if (!ok) return;
+        const uint32_t b = k_lo + (uint32_t)((j & 1) * (K_BYTES >> 4) + half * (64 * 128 >> 4));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (uint32_t)((kk >> 2) * (QP_SLAB >> 4) + 2 * (kk & 3));
-          umma_f16_ss(s_col, q_lo + off, b + off, id_s, kk > 0 ? 1u : 0u);
+          umma_f16_ss(s_col + 64u * half, q_lo + off, b + off, id_s, kk > 0 ? 1u : 0u);
         }
-        umma_commit_warp(&sm.s_full[g]);
-        if (j + 2 < n_tiles) umma_commit_warp(&sm.k_empty[buf]);
-        // the halves of the product as P arrives (it comes after the softmax has seen that the values are there)
-        if (!both(&sm.p_half[g], (uint32_t)j & 1u)) { ok = false; break; }
-        values(j, 0);
-        if (!both(&sm.p_full[g], (uint32_t)j & 1u)) { ok = false; break; }
-        values(j, 1);
-        umma_commit_warp(&sm.o_full[g]);
-        if (j + 2 < n_tiles) umma_commit_warp(&sm.v_empty[buf]);
+        umma_commit_warp(&sm.s_full[g][half]);
+        if (half && j + 2 < n_tiles) umma_commit_warp(&sm.k_empty[j & 1]);
+      };
+      both(&sm.q_full[g], 0u);
+      scores(0);
+      scores(1);
+      for (int i = 0; ok && i < 2 * n_tiles; ++i) {
+        const int j = i >> 1, half = i & 1;
+        // O += P V, as P arrives (it comes after the softmax has seen that the values are there)
+        both(&sm.p_full[g][half], (uint32_t)j & 1u);
+        if (!ok) break;
+        const uint32_t pa = s_col + (uint32_t)(64 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) umma_f16_ts(o_col, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, i > 0 || kk > 0 ? 1u : 0u);
+        umma_commit_warp(&sm.o_full[g][half]);
+        if (half && j + 2 < n_tiles) umma_commit_warp(&sm.v_empty[j & 1]);
+        // the scores that go where P lay, once the product has ended: while the softmax works on the other half
+        if (i + 2 < 2 * n_tiles) { both(&sm.o_full[g][half], (uint32_t)j & 1u); scores(i + 2); }
       }
     }
     more = next_rows(ok, std::integral_constant<int, 1>{});
