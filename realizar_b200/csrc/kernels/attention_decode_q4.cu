@@ -40,6 +40,7 @@ __device__ int g_attn_q4_error = 0;
 constexpr int QD_STAGES = 3, QD_MAX_SMS = 148, QD_HELPERS = 128;
 constexpr int QD_PAIR = 2 * Q4_PAGE;          // tokens of a pair of pages
 constexpr int QD_TILE_COST = 40;              // a second tile costs a CTA about as much time as this many pairs
+constexpr int QD_FLUSH = 8;                   // pairs whose values a warp adds up in the tensor core's accumulators, a power of two
 constexpr int QD_POSITIONS = 512;
 constexpr int QD_MAX_PARTS = 64;              // CTAs that share a tile: bounds the time of the last one, which joins their parts
 // query heads of a CTA (HN tiles of 4) and its main warps: with the four others 16 warps of 128 registers, or 12 of 168
@@ -111,6 +112,7 @@ __device__ __forceinline__ float pow2_for(float x, int e) {
   const int k = e + 254 - (int)(__float_as_uint(x) >> 23);
   return __uint_as_float((uint32_t)max(1, min(k, 227)) << 23);
 }
+__device__ __forceinline__ float inverse_pow2(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }      // x a power of two from pow2_for
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* src, uint32_t (&w)[N]) {
   if constexpr (N == 4) { const uint4 v = *(const uint4*)src; w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
   else if constexpr (N == 2) { const uint2 v = *(const uint2*)src; w[0] = v.x; w[1] = v.y; }
@@ -289,150 +291,186 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           m[h] = -INFINITY; l[h] = om[h] = 0.f;
         }
         float vf = 0x1p100f;                                        // power of two that p x scale' carries
-        int tok = s.tok + (warp + NW * k0 - at) * QD_PAIR;           // first token of pair k
-
-        for (int k = k0; k < k1; ++k, tok += NW * QD_PAIR) {          // (of an odd number of pages the last comes with a masked one)
-          copy_pair(k + QD_STAGES - 1, slot == 0 ? QD_STAGES - 1 : slot - 1);       // into the slot that the pair before this one left
-          asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
-          __syncwarp();
-          uint8_t* const kp[2] = {my_ring + slot * (4 * PB), my_ring + slot * (4 * PB) + 2 * PB};
-          if (own == k) {                                            // the copy may have passed the write of the new row
-            ok = qd_wait(&sm.own_full[buf], phase, ok) && ok;
-            __syncwarp();
-            uint8_t* page = s.pos - tok < Q4_PAGE ? kp[0] : kp[1];
-            q4_store_k<D>(page, s.pos % Q4_PAGE, sm.codes[buf][0], sm.meta[buf][0], lane);
-            q4_store_v<D>(page + PB, s.pos % Q4_PAGE, sm.codes[buf][1], sm.meta[buf][1], lane);
-            __syncwarp();
-          }
-          // ---- scores: lane has tokens gq and gq + 8 of head tq of a tile ----
-          float sc[HN][2][2], sv[2][2], mv[2][2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            int hi[HN][4] = {}, lo[HN][4] = {};                        // digits 0 and 1 of tokens gq and gq + 8, digit 2
-            uint32_t wa[NG], wb[NG];
-            load_words<NG>(kp[j] + gq * (D / 2) + tq * NG * 4, wa);
-            load_words<NG>(kp[j] + (gq + 8) * (D / 2) + tq * NG * 4, wb);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              const uint32_t a0 = wa[g] & 0x0F0F0F0Fu, a1 = wb[g] & 0x0F0F0F0Fu, a2 = wa[g] >> 4 & 0x0F0F0F0Fu, a3 = wb[g] >> 4 & 0x0F0F0F0Fu;
-#pragma unroll
-              for (int h = 0; h < HN; ++h) {
-                mma_s8(hi[h], a0, a1, a2, a3, qb[h][g].x, qb[h][g].y);
-                mma_s8(lo[h], a0, a1, a2, a3, qb[h][g].z, qb[h][g].w);
-              }
-            }
-            if constexpr (TAIL) {
-              const uint8_t* kt = kp[j] + 16 * NG + 2 * tq;
-              const uint32_t a0 = nib_bytes(*(const uint16_t*)(kt + gq * (D / 2))), a1 = nib_bytes(*(const uint16_t*)(kt + (gq + 8) * (D / 2)));
-#pragma unroll
-              for (int h = 0; h < HN; ++h) { mma_s8_half(hi[h], a0, a1, qb[h][NG].x); mma_s8_half(lo[h], a0, a1, qb[h][NG].z); }
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
-              sv[j][n] = q4_scale(vm); mv[j][n] = fmaf(8.f, sv[j][n], q4_min(vm));
-#pragma unroll
-              for (int h = 0; h < HN; ++h) {
-                const float dot = fmaf((float)hi[h][2 * n], 65536.f, fmaf((float)hi[h][2 * n + 1], 256.f, (float)lo[h][2 * n]));
-                sc[h][j][n] = fmaf(dot * qc[h], q4_scale(km), q4_min(km) * qx[h]);
-              }
-            }
-          }
-          if (tok < s.lo || tok + QD_PAIR - 1 > s.pos) {     // rows outside the window or behind the last token hold anything
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const int t = tok + j * Q4_PAGE + gq + 8 * n;
-                if (t < s.lo || t > s.pos) {
-                  sv[j][n] = mv[j][n] = 0.f;
-#pragma unroll
-                  for (int h = 0; h < HN; ++h) sc[h][j][n] = -INFINITY;
-                }
-              }
-          }
-          // ---- running maximum and scale: moved only where they fall behind by 2^8 and 2^2 ----
-          float mx[HN], top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-          bool behind = top * vf > 126.f;
+        // Every QD_FLUSH pairs the sums go to the warp's part in shared memory: the tensor core cuts off what its 32-bit accumulators do
+        // not hold, always towards zero, so that the error of one long sum grows with its length (131072 tokens: 1.2e-6 of the result)
+        auto part_at = [&](int h) { return sm.part[buf][warp][4 * h + tq] + 4 * gq; };
+        auto for_part = [&](auto f) {                                // f(h, n, k, place in shared memory) for the lane's values
 #pragma unroll
           for (int h = 0; h < HN; ++h) {
-            mx[h] = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
-            behind |= mx[h] > m[h] + 8.f;
-          }
-          if (__any_sync(0xFFFFFFFFu, behind)) {
-#pragma unroll
-            for (int k = 4; k < 32; k <<= 1) {
-              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
-#pragma unroll
-              for (int h = 0; h < HN; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], k));
-            }
-            const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, vr = vn / vf;
-            vf = vn;
-#pragma unroll
-            for (int h = 0; h < HN; ++h) {
-              const float mn = fmaxf(m[h], mx[h]), corr = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn), co = corr * vr;
-#pragma unroll
-              for (int n = 0; n < NT; ++n) { o[h][n][0] *= co; o[h][n][1] *= co; o[h][n][2] *= co; o[h][n][3] *= co; }
-              l[h] *= corr; om[h] *= corr; m[h] = mn;
-            }
-          }
-          // ---- O += P V: rows gq and gq + 8 of tile 2 g + k are dims 32 g + 4 gq + 2 k and + 1 ----
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t pb[HN][2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const float f = sv[j][n] * vf;
-#pragma unroll
-              for (int h = 0; h < HN; ++h) {
-                const float e = ex2(sc[h][j][n] - m[h]);
-                l[h] += e;
-                om[h] = fmaf(e, mv[j][n], om[h]);
-                pb[h][n] = transpose_8x8(split_f16(e * f));
-              }
-            }
-            const uint8_t* vp = kp[j] + PB;
-            uint32_t w0[NG], w1[NG];
-            load_words<NG>(vp + lane * NG * 4, w0);
-            load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-              uint32_t a[4], c[4];
-              codes_less_8(w0[g], a);
-              codes_less_8(w1[g], c);
-#pragma unroll
-              for (int h = 0; h < HN; ++h) {
-                mma_f16(o[h][2 * g], a[0], a[1], c[0], c[1], pb[h][0], pb[h][1]);
-                mma_f16(o[h][2 * g + 1], a[2], a[3], c[2], c[3], pb[h][0], pb[h][1]);
-              }
+              float4* at4 = (float4*)(part_at(h) + 32 * g);
+              float4 v = *at4;
+              v.x = f(h, 2 * g, 0, v.x); v.y = f(h, 2 * g, 1, v.y); v.z = f(h, 2 * g + 1, 0, v.z); v.w = f(h, 2 * g + 1, 1, v.w);
+              *at4 = v;
             }
             if constexpr (TAIL) {
-              const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
-              uint32_t a[4], c[4];
-              codes_less_8(__byte_perm(w, 0u, 0x4140), a);
-              codes_less_8(__byte_perm(w, 0u, 0x4342), c);
-#pragma unroll
-              for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], a[0], a[1], c[0], c[1], pb[h][0], pb[h][1]);
+              float2* at2 = (float2*)(sm.part[buf][warp][4 * h + tq] + 32 * NG + 2 * gq);
+              float2 v = *at2;
+              v.x = f(h, 2 * NG, 0, v.x); v.y = f(h, 2 * NG, 1, v.y);
+              *at2 = v;
             }
           }
-          __syncwarp();                                              // every lane has read the pair: its slot may be filled again
-          if (++slot == QD_STAGES) slot = 0;
+        };
+        int tok = s.tok + (warp + NW * k0 - at) * QD_PAIR;           // first token of pair k
+
+        int kb = k0;                                                // first pair of the sums in the accumulators
+        for (;;) {
+          const int ke = min(kb + QD_FLUSH, k1);
+          for (int k = kb; k < ke; ++k, tok += NW * QD_PAIR) {          // (of an odd number of pages the last comes with a masked one)
+            copy_pair(k + QD_STAGES - 1, slot == 0 ? QD_STAGES - 1 : slot - 1);       // into the slot that the pair before this one left
+            asm volatile("cp.async.wait_group %0;" ::"n"(QD_STAGES - 1) : "memory");
+            __syncwarp();
+            uint8_t* const kp[2] = {my_ring + slot * (4 * PB), my_ring + slot * (4 * PB) + 2 * PB};
+            if (own == k) {                                            // the copy may have passed the write of the new row
+              ok = qd_wait(&sm.own_full[buf], phase, ok) && ok;
+              __syncwarp();
+              uint8_t* page = s.pos - tok < Q4_PAGE ? kp[0] : kp[1];
+              q4_store_k<D>(page, s.pos % Q4_PAGE, sm.codes[buf][0], sm.meta[buf][0], lane);
+              q4_store_v<D>(page + PB, s.pos % Q4_PAGE, sm.codes[buf][1], sm.meta[buf][1], lane);
+              __syncwarp();
+            }
+            // ---- scores: lane has tokens gq and gq + 8 of head tq of a tile ----
+            float sc[HN][2][2], sv[2][2], mv[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              int hi[HN][4] = {}, lo[HN][4] = {};                        // digits 0 and 1 of tokens gq and gq + 8, digit 2
+              uint32_t wa[NG], wb[NG];
+              load_words<NG>(kp[j] + gq * (D / 2) + tq * NG * 4, wa);
+              load_words<NG>(kp[j] + (gq + 8) * (D / 2) + tq * NG * 4, wb);
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                const uint32_t a0 = wa[g] & 0x0F0F0F0Fu, a1 = wb[g] & 0x0F0F0F0Fu, a2 = wa[g] >> 4 & 0x0F0F0F0Fu, a3 = wb[g] >> 4 & 0x0F0F0F0Fu;
+#pragma unroll
+                for (int h = 0; h < HN; ++h) {
+                  mma_s8(hi[h], a0, a1, a2, a3, qb[h][g].x, qb[h][g].y);
+                  mma_s8(lo[h], a0, a1, a2, a3, qb[h][g].z, qb[h][g].w);
+                }
+              }
+              if constexpr (TAIL) {
+                const uint8_t* kt = kp[j] + 16 * NG + 2 * tq;
+                const uint32_t a0 = nib_bytes(*(const uint16_t*)(kt + gq * (D / 2))), a1 = nib_bytes(*(const uint16_t*)(kt + (gq + 8) * (D / 2)));
+#pragma unroll
+                for (int h = 0; h < HN; ++h) { mma_s8_half(hi[h], a0, a1, qb[h][NG].x); mma_s8_half(lo[h], a0, a1, qb[h][NG].z); }
+              }
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const uint32_t km = *(const uint32_t*)(kp[j] + 8 * D + (gq + 8 * n) * 4), vm = *(const uint32_t*)(kp[j] + PB + 8 * D + (gq + 8 * n) * 4);
+                sv[j][n] = q4_scale(vm); mv[j][n] = fmaf(8.f, sv[j][n], q4_min(vm));
+#pragma unroll
+                for (int h = 0; h < HN; ++h) {
+                  const float dot = fmaf((float)hi[h][2 * n], 65536.f, fmaf((float)hi[h][2 * n + 1], 256.f, (float)lo[h][2 * n]));
+                  sc[h][j][n] = fmaf(dot * qc[h], q4_scale(km), q4_min(km) * qx[h]);
+                }
+              }
+            }
+            if (tok < s.lo || tok + QD_PAIR - 1 > s.pos) {     // rows outside the window or behind the last token hold anything
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                  const int t = tok + j * Q4_PAGE + gq + 8 * n;
+                  if (t < s.lo || t > s.pos) {
+                    sv[j][n] = mv[j][n] = 0.f;
+#pragma unroll
+                    for (int h = 0; h < HN; ++h) sc[h][j][n] = -INFINITY;
+                  }
+                }
+            }
+            // ---- running maximum and scale: moved only where they fall behind by 2^8 and 2^2 ----
+            float mx[HN], top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+            bool behind = top * vf > 126.f;
+#pragma unroll
+            for (int h = 0; h < HN; ++h) {
+              mx[h] = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
+              behind |= mx[h] > m[h] + 8.f;
+            }
+            if (__any_sync(0xFFFFFFFFu, behind)) {
+#pragma unroll
+              for (int k = 4; k < 32; k <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+#pragma unroll
+                for (int h = 0; h < HN; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], k));
+              }
+              const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, vr = vn / vf;
+              vf = vn;
+#pragma unroll
+              for (int h = 0; h < HN; ++h) {
+                const float mn = fmaxf(m[h], mx[h]), corr = m[h] == -INFINITY ? 0.f : ex2(m[h] - mn), co = corr * vr;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) { o[h][n][0] *= co; o[h][n][1] *= co; o[h][n][2] *= co; o[h][n][3] *= co; }
+                l[h] *= corr; om[h] *= corr; m[h] = mn;
+                mx[h] = corr;
+              }
+              if (kb > k0) for_part([&](int h, int, int, float v) { return v * mx[h]; });
+            }
+            // ---- O += P V: rows gq and gq + 8 of tile 2 g + k are dims 32 g + 4 gq + 2 k and + 1 ----
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t pb[HN][2];
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const float f = sv[j][n] * vf;
+#pragma unroll
+                for (int h = 0; h < HN; ++h) {
+                  const float e = ex2(sc[h][j][n] - m[h]);
+                  l[h] += e;
+                  om[h] = fmaf(e, mv[j][n], om[h]);
+                  pb[h][n] = transpose_8x8(split_f16(e * f));
+                }
+              }
+              const uint8_t* vp = kp[j] + PB;
+              uint32_t w0[NG], w1[NG];
+              load_words<NG>(vp + lane * NG * 4, w0);
+              load_words<NG>(vp + 128 * NG + lane * NG * 4, w1);
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                uint32_t a[4], c[4];
+                codes_less_8(w0[g], a);
+                codes_less_8(w1[g], c);
+#pragma unroll
+                for (int h = 0; h < HN; ++h) {
+                  mma_f16(o[h][2 * g], a[0], a[1], c[0], c[1], pb[h][0], pb[h][1]);
+                  mma_f16(o[h][2 * g + 1], a[2], a[3], c[2], c[3], pb[h][0], pb[h][1]);
+                }
+              }
+              if constexpr (TAIL) {
+                const uint32_t w = *(const uint32_t*)(vp + 256 * NG + lane * 4);
+                uint32_t a[4], c[4];
+                codes_less_8(__byte_perm(w, 0u, 0x4140), a);
+                codes_less_8(__byte_perm(w, 0u, 0x4342), c);
+#pragma unroll
+                for (int h = 0; h < HN; ++h) mma_f16(o[h][2 * NG], a[0], a[1], c[0], c[1], pb[h][0], pb[h][1]);
+              }
+            }
+            __syncwarp();                                              // every lane has read the pair: its slot may be filled again
+            if (++slot == QD_STAGES) slot = 0;
+          }
+          if (ke == k1) break;
+          if (kb == k0 && it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
+          const float e0 = inverse_pow2(vf);
+          for_part([&](int h, int n, int i, float v) {
+            const float add = (o[h][n][2 * i] + o[h][n][2 * i + 1]) * e0;
+            o[h][n][2 * i] = o[h][n][2 * i + 1] = 0.f;
+            return kb == k0 ? add : v + add;
+          });
+          kb = ke;
         }
 
         // ---- this warp's part of the tile ----
-        if (it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
-        const float e0 = 1.f / vf;
+        const bool begun = kb > k0;
+        if (!begun && it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
+        const float e0 = inverse_pow2(vf);
 #pragma unroll
-        for (int h = 0; h < HN; ++h) {
+        for (int h = 0; h < HN; ++h)
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) { l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], k); om[h] += __shfl_xor_sync(0xFFFFFFFFu, om[h], k); }
-          float* dst = sm.part[buf][warp][4 * h + tq];
-          auto val = [&](int n, int k) { return fmaf(o[h][n][2 * k] + o[h][n][2 * k + 1], e0, om[h]); };
+        for_part([&](int h, int n, int i, float v) {
+          const float add = fmaf(o[h][n][2 * i] + o[h][n][2 * i + 1], e0, om[h]);
+          return begun ? v + add : add;
+        });
 #pragma unroll
-          for (int g = 0; g < NG; ++g) *(float4*)(dst + 32 * g + 4 * gq) = make_float4(val(2 * g, 0), val(2 * g, 1), val(2 * g + 1, 0), val(2 * g + 1, 1));
-          if constexpr (TAIL) *(float2*)(dst + 32 * NG + 2 * gq) = make_float2(val(2 * NG, 0), val(2 * NG, 1));
-          if (gq == 0) *(float2*)(dst + D) = make_float2(m[h], l[h]);
-        }
+        for (int h = 0; h < HN; ++h) if (gq == 0) *(float2*)(sm.part[buf][warp][4 * h + tq] + D) = make_float2(m[h], l[h]);
       } else {                                                       // no page of this tile is mine
         if (it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
         if (lane < ROWS) *(float2*)(sm.part[buf][warp][lane] + D) = make_float2(-INFINITY, 0.f);

@@ -105,13 +105,6 @@ __device__ __forceinline__ bool qp_wait(unsigned long long* bar, uint32_t parity
   return false;
 }
 
-// has the phase ended (the warp asks together)
-__device__ __forceinline__ bool qp_test(unsigned long long* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(gm_smem_u32(bar)), "r"(parity) : "memory");
-  return __all_sync(0xFFFFFFFFu, done != 0);
-}
-
 // true when it is for all 128 threads of a role (also their barrier)
 template <int BAR> __device__ __forceinline__ bool qp_agree(bool mine) {
   uint32_t r;
@@ -288,208 +281,209 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       const int m0 = sm.seg.mt * QP_ROWS, groups = groups_of(sm.seg.mt), kvh = sm.seg.kvh, n_tiles = sm.seg.n, kbeg = sm.seg.klo + sm.seg.j0 * QP_KEYS, pos0 = sm.sched.z.pos0;
       bool ok = true;
       if (grp < groups) {
-      const uint32_t lane_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(128 * grp), lane_o = lane_s + 256u;
-      const int row = m0 + grp * QP_GROUP + t, token = row / G, head = kvh * G + row - token * G;
-      const bool live = row < rows;
-      const int pos = pos0 + token;
-      // ---- queries: 8 dims to a lane, stored as fp16 in the order in which the keys' codes come out of a word: (0, 4), (1, 5), (2, 6),
-      // (3, 7) of every 8 dims.  A short loop: these instructions run once to a CTA, and fetching them takes longer than the loads
-      const uint32_t q_tile = Qs + (uint32_t)(grp * Q_BYTES);
-      const bool vec = (((uintptr_t)p.qkv | (uintptr_t)(4 * p.ld_qkv) | (uintptr_t)(4 * p.q_off)) & 15) == 0;
-      {
-        constexpr int LANES = D == 64 ? 8 : 16, STEP = 32 / LANES, BATCH = 8;     // lanes to a row, rows at once and their loads in flight
-        const int x = lane % LANES, r0 = (warp & 3) * 32 + lane / LANES;
-        int gr = m0 + grp * QP_GROUP + r0, tk = gr / G, hd = gr - tk * G;
+        const uint32_t lane_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(128 * grp), lane_o = lane_s + 256u;
+        const int row = m0 + grp * QP_GROUP + t, token = row / G, head = kvh * G + row - token * G;
+        const bool live = row < rows;
+        const int pos = pos0 + token;
+        // ---- queries: 8 dims to a lane, stored as fp16 in the order in which the keys' codes come out of a word: (0, 4), (1, 5), (2, 6),
+        // (3, 7) of every 8 dims.  Not unrolled further: 16 rows at
+        // once took 11 us instead of 6 (the instructions run once to a CTA and have to be fetched)
+        const uint32_t q_tile = Qs + (uint32_t)(grp * Q_BYTES);
+        const bool vec = (((uintptr_t)p.qkv | (uintptr_t)(4 * p.ld_qkv) | (uintptr_t)(4 * p.q_off)) & 15) == 0;
+        {
+          constexpr int LANES = D == 64 ? 8 : 16, STEP = 32 / LANES, BATCH = 8;     // lanes to a row, rows at once and their loads in flight
+          const int x = lane % LANES, r0 = (warp & 3) * 32 + lane / LANES;
+          int gr = m0 + grp * QP_GROUP + r0, tk = gr / G, hd = gr - tk * G;
 #pragma unroll 1
-        for (int r1 = r0; r1 < (warp & 3) * 32 + 32; r1 += BATCH * STEP) {
-          float4 v[BATCH][2];
+          for (int r1 = r0; r1 < (warp & 3) * 32 + 32; r1 += BATCH * STEP) {
+            float4 v[BATCH][2];
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (gr < rows && x < D / 8) {
-              const float* src = p.qkv + (int64_t)tk * p.ld_qkv + p.q_off + (int64_t)(kvh * G + hd) * D + 8 * x;
-              if (vec) { v[i][0] = __ldg((const float4*)src); v[i][1] = __ldg((const float4*)src + 1); }
-              else { v[i][0] = make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3)); v[i][1] = make_float4(__ldg(src + 4), __ldg(src + 5), __ldg(src + 6), __ldg(src + 7)); }
+            for (int i = 0; i < BATCH; ++i) {
+              v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (gr < rows && x < D / 8) {
+                const float* src = p.qkv + (int64_t)tk * p.ld_qkv + p.q_off + (int64_t)(kvh * G + hd) * D + 8 * x;
+                if (vec) { v[i][0] = __ldg((const float4*)src); v[i][1] = __ldg((const float4*)src + 1); }
+                else { v[i][0] = make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3)); v[i][1] = make_float4(__ldg(src + 4), __ldg(src + 5), __ldg(src + 6), __ldg(src + 7)); }
+              }
+              gr += STEP;
+              for (hd += STEP; hd >= G; hd -= G) ++tk;
             }
-            gr += STEP;
-            for (hd += STEP; hd >= G; hd -= G) ++tk;
-          }
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int r = r1 + i * STEP;
-            const float4 a = v[i][0], b = v[i][1];
-            float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+            for (int i = 0; i < BATCH; ++i) {
+              const int r = r1 + i * STEP;
+              const float4 a = v[i][0], b = v[i][1];
+              float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
-            if (x == 0) sm.qf[grp][r] = f;
-            if (x < NSLAB * 8) {
-              const uint32_t w[4] = {qp_half2(a.x * f, b.x * f), qp_half2(a.y * f, b.y * f), qp_half2(a.z * f, b.z * f), qp_half2(a.w * f, b.w * f)};
-              st_shared(q_tile + (uint32_t)((x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4)), w);
+              for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+              const float f = top > 0.f ? qp_pow2(top, 4) : 1.f;
+              if (x == 0) sm.qf[grp][r] = f;
+              if (x < NSLAB * 8) {
+                const uint32_t w[4] = {qp_half2(a.x * f, b.x * f), qp_half2(a.y * f, b.y * f), qp_half2(a.z * f, b.z * f), qp_half2(a.w * f, b.w * f)};
+                st_shared(q_tile + (uint32_t)((x >> 3) * QP_SLAB + (r >> 3) * 1024 + (r & 7) * 128 + (((x & 7) ^ (r & 7)) << 4)), w);
+              }
             }
           }
         }
-      }
-      __syncwarp();
-      const float qs = p.scale * 1.4426950408889634f / sm.qf[grp][t];    // softmax scale of my row
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      gm_arrive((uint64_t*)&sm.q_full[grp]);
+        __syncwarp();
+        const float qs = p.scale * 1.4426950408889634f / sm.qf[grp][t];    // softmax scale of my row
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        gm_arrive((uint64_t*)&sm.q_full[grp]);
 
-      float m = -INFINITY, vf = 1.f;
-      float2 l2 = make_float2(0.f, 0.f);
-      const int row_first = m0 + grp * QP_GROUP, row_last = min(rows, row_first + QP_GROUP) - 1;
-      const int pos_first = pos0 + row_first / G, lo_last = p.window > 0 ? pos0 + row_last / G + 1 - p.window : 0;     // masks are needed beyond these
-      for (int i = 0; ok && i < 2 * n_tiles; ++i) {
-        const int j = i >> 1, half = i & 1, k0 = kbeg + 64 * i, buf = j & 1;
-        const uint32_t s_at = lane_s + (uint32_t)(64 * half);
-        // the scores, and with them the tile's power of two of K; that of V
-        ok = qp_wait(&sm.s_full[grp][half], (uint32_t)j & 1u) && (half || qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u));
-        if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
-        tc_after();
-        const float sc = qs * sm.kf[j & 3], vn = sm.vf[buf];
-        const bool edge = k0 + 63 > pos_first || k0 < lo_last;
-        const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
-        // EDGE: some entries are masked
-        auto part = [&](auto edge_c) {
-          constexpr bool EDGE = decltype(edge_c)::value;
-          uint32_t r[2][32];
-          tmem_ld32_async(s_at, r[0]);
-          tmem_ld32_async(s_at + 32u, r[1]);
-          tmem_wait_ld(r[0]);
-          tmem_wait_ld(r[1]);
-          auto seen = [&](int key) { return !EDGE || (key < vis_hi && key >= vis_lo); };
-          float top = -INFINITY, top1 = -INFINITY;
+        float m = -INFINITY, vf = 1.f;
+        float2 l2 = make_float2(0.f, 0.f);
+        const int row_first = m0 + grp * QP_GROUP, row_last = min(rows, row_first + QP_GROUP) - 1;
+        const int pos_first = pos0 + row_first / G, lo_last = p.window > 0 ? pos0 + row_last / G + 1 - p.window : 0;     // masks are needed beyond these
+        for (int i = 0; ok && i < 2 * n_tiles; ++i) {
+          const int j = i >> 1, half = i & 1, k0 = kbeg + 64 * i, buf = j & 1;
+          const uint32_t s_at = lane_s + (uint32_t)(64 * half);
+          // the scores, and with them the tile's power of two of K; that of V
+          ok = qp_wait(&sm.s_full[grp][half], (uint32_t)j & 1u) && (half || qp_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1u));
+          if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+          tc_after();
+          const float sc = qs * sm.kf[j & 3], vn = sm.vf[buf];
+          const bool edge = k0 + 63 > pos_first || k0 < lo_last;
+          const int vis_hi = live ? pos + 1 - k0 : 0, vis_lo = p.window > 0 ? pos + 1 - p.window - k0 : 0;
+          // EDGE: some entries are masked
+          auto part = [&](auto edge_c) {
+            constexpr bool EDGE = decltype(edge_c)::value;
+            uint32_t r[2][32];
+            tmem_ld32_async(s_at, r[0]);
+            tmem_ld32_async(s_at + 32u, r[1]);
+            tmem_wait_ld(r[0]);
+            tmem_wait_ld(r[1]);
+            auto seen = [&](int key) { return !EDGE || (key < vis_hi && key >= vis_lo); };
+            float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < 64; k += 4) {
-            auto score = [&](int key) { return seen(key) ? __uint_as_float(r[key >> 5][key & 31]) : -INFINITY; };
-            top = max3(top, score(k), score(k + 1));
-            top1 = max3(top1, score(k + 2), score(k + 3));
-          }
-          top = fmaxf(top, top1) * sc;
-          if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
-            const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
-            if (i > 0) {
-              ok = __all_sync(0xFFFFFFFFu, qp_wait(&sm.o_full[grp][half ^ 1], (uint32_t)((i - 1) >> 1) & 1u));      // the product before has ended
-              tc_after();
+            for (int k = 0; k < 64; k += 4) {
+              auto score = [&](int key) { return seen(key) ? __uint_as_float(r[key >> 5][key & 31]) : -INFINITY; };
+              top = max3(top, score(k), score(k + 1));
+              top1 = max3(top1, score(k + 2), score(k + 3));
+            }
+            top = fmaxf(top, top1) * sc;
+            if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
+              const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
+              if (i > 0) {
+                ok = __all_sync(0xFFFFFFFFu, qp_wait(&sm.o_full[grp][half ^ 1], (uint32_t)((i - 1) >> 1) & 1u));      // the product before has ended
+                tc_after();
 #pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 16) {
-                uint32_t o[16];
-                tmem_ld16(lane_o + (uint32_t)c0, o);
+                for (int c0 = 0; c0 < D; c0 += 16) {
+                  uint32_t o[16];
+                  tmem_ld16(lane_o + (uint32_t)c0, o);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * co);
-                tmem_st16(lane_o + (uint32_t)c0, o);
+                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * co);
+                  tmem_st16(lane_o + (uint32_t)c0, o);
+                }
               }
+              l2.x *= corr; l2.y *= corr; m = mn; vf = vn;
             }
-            l2.x *= corr; l2.y *= corr; m = mn; vf = vn;
-          }
-          const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
-          const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
+            const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
+            const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t w[16];
+            for (int c = 0; c < 2; ++c) {
+              uint32_t w[16];
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), sc2, b2);
-              const float2 e = make_float2(seen(32 * c + k) ? qp_ex2(y.x) : 0.f, seen(32 * c + k + 1) ? qp_ex2(y.y) : 0.f);
-              l2 = add2(l2, e);
-              w[k >> 1] = qp_half2(e.x, e.y);
+              for (int k = 0; k < 32; k += 2) {
+                const float2 y = fma2(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), sc2, b2);
+                const float2 e = make_float2(seen(32 * c + k) ? qp_ex2(y.x) : 0.f, seen(32 * c + k + 1) ? qp_ex2(y.y) : 0.f);
+                l2 = add2(l2, e);
+                w[k >> 1] = qp_half2(e.x, e.y);
+              }
+              tmem_st16(s_at + (uint32_t)(16 * c), w);                   // over the scores
             }
-            tmem_st16(s_at + (uint32_t)(16 * c), w);                   // over the scores
-          }
-          tmem_wait_st();
-          tc_before();
-          gm_arrive((uint64_t*)&sm.p_full[grp][half]);
-        };
-        if (edge) part(std::true_type{}); else part(std::false_type{});
-      }
-      if (ok) ok = qp_wait(&sm.o_full[grp][0], (uint32_t)(n_tiles - 1) & 1u) && qp_wait(&sm.o_full[grp][1], (uint32_t)(n_tiles - 1) & 1u);       // the last products
-      if (grp == 0 ? qp_agree<1>(ok) : qp_agree<2>(ok)) {
-        tc_after();
-        const float inv_vf = 1.f / vf, l = l2.x + l2.y;
-        auto store = [&](int c, const float* v) {                   // 16 finished values
-          const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
-          if (p.out_bf16) {
-            uint32_t w[8];
+            tmem_wait_st();
+            tc_before();
+            gm_arrive((uint64_t*)&sm.p_full[grp][half]);
+          };
+          if (edge) part(std::true_type{}); else part(std::false_type{});
+        }
+        if (ok) ok = qp_wait(&sm.o_full[grp][0], (uint32_t)(n_tiles - 1) & 1u) && qp_wait(&sm.o_full[grp][1], (uint32_t)(n_tiles - 1) & 1u);       // the last products
+        if (grp == 0 ? qp_agree<1>(ok) : qp_agree<2>(ok)) {
+          tc_after();
+          const float inv_vf = 1.f / vf, l = l2.x + l2.y;
+          auto store = [&](int c, const float* v) {                   // 16 finished values
+            const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
+            if (p.out_bf16) {
+              uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-            uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
-            dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+              for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+              uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
+              dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
+          };
+          const bool whole = n_tiles == sm.seg.all;
+          constexpr int COLS = D % 32 ? 16 : 32;
+          // slots of a CTA in scratch: 0 the row tile that its share begins in, 1 the one that it ends in
+          constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);
+          float* const slots = p.scratch + QP_COUNTERS + (int64_t)grp * QP_GROUP * (D + 4) + t;     // a column to 128 floats: a warp's rows lie together
+          float* const slot = slots + (int64_t)(2 * blockIdx.x + (sm.done == 0 ? 0 : 1)) * step;
+          if (whole) {
+            const float f = inv_vf / l;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t r[16];
+              tmem_ld16(lane_o + (uint32_t)c, r);
+              float v[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
+              if (live) store(c, v);
+            }
           } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          }
-        };
-        const bool whole = n_tiles == sm.seg.all;
-        constexpr int COLS = D % 32 ? 16 : 32;
-        // slots of a CTA in scratch: 0 the row tile that its share begins in, 1 the one that it ends in
-        constexpr int64_t step = (int64_t)QP_ROWS * (D + 4);
-        float* const slots = p.scratch + QP_COUNTERS + (int64_t)grp * QP_GROUP * (D + 4) + t;     // a column to 128 floats: a warp's rows lie together
-        float* const slot = slots + (int64_t)(2 * blockIdx.x + (sm.done == 0 ? 0 : 1)) * step;
-        if (whole) {
-          const float f = inv_vf / l;
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t r[16];
-            tmem_ld16(lane_o + (uint32_t)c, r);
-            float v[16];
+            for (int c = 0; c < D; c += 16) {
+              uint32_t r[16];
+              tmem_ld16(lane_o + (uint32_t)c, r);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
-            if (live) store(c, v);
-          }
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t r[16];
-            tmem_ld16(lane_o + (uint32_t)c, r);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) __stcg(slot + (c + i) * QP_GROUP, __uint_as_float(r[i]) * inv_vf);
-          }
-          slot[D * QP_GROUP] = m; slot[(D + 1) * QP_GROUP] = l;
-          // the row tile's CTAs: neighbours by tile, else those that have its first and last place
-          int c_lo, c_hi, lead = 0;
-          {
-            const int c = blockIdx.x;
-            if (sm.sched.each == 0) { c_lo = c - c % nsplit; c_hi = c_lo + sm.sched.parts - 1; }
-            else {
-              const int t0 = qp_first(sm.sched, c) + sm.done - sm.seg.j0;
-              c_lo = qp_owner(sm.sched, t0); c_hi = qp_owner(sm.sched, t0 + sm.seg.all - 1);
-              lead = qp_first(sm.sched, c_lo) == t0 ? 0 : 1;
+              for (int i = 0; i < 16; ++i) __stcg(slot + (c + i) * QP_GROUP, __uint_as_float(r[i]) * inv_vf);
             }
-          }
-          if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
-          if (t == 0) {
-            int32_t* ctr = (int32_t*)p.scratch + 2 * (2 * c_lo + lead) + grp;
-            __threadfence();
-            sm.last[grp] = atomicAdd(ctr, 1) == c_hi - c_lo;
-            if (sm.last[grp]) { *ctr = 0; __threadfence(); }          // zero again for the next launch
-          }
-          if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
-          if (sm.last[grp] && live) {
-            auto part_of = [&](int k) { return slots + (int64_t)(2 * k + (k == c_lo ? lead : 0)) * step; };
-            float mm = -INFINITY, ll = 0.f;
-#pragma unroll 4
-            for (int k = c_lo; k <= c_hi; ++k) {
-              const float mi = __ldcg(part_of(k) + D * QP_GROUP), li = __ldcg(part_of(k) + (D + 1) * QP_GROUP), mn = fmaxf(mm, mi);
-              if (mn != -INFINITY) ll = fmaf(ll, qp_ex2(mm - mn), li * qp_ex2(mi - mn));
-              mm = mn;
-            }
-            const float inv = 1.f / ll;
-#pragma unroll 1
-            for (int c = 0; c < D; c += COLS) {
-              float v[COLS] = {};
-#pragma unroll 2
-              for (int k = c_lo; k <= c_hi; ++k) {
-                const float* part_i = part_of(k);
-                const float e = qp_ex2(__ldcg(part_i + D * QP_GROUP) - mm) * inv;
-#pragma unroll
-                for (int q = 0; q < COLS; ++q) v[q] = fmaf(e, __ldcg(part_i + (c + q) * QP_GROUP), v[q]);
+            slot[D * QP_GROUP] = m; slot[(D + 1) * QP_GROUP] = l;
+            // the row tile's CTAs: neighbours by tile, else those that have its first and last place
+            int c_lo, c_hi, lead = 0;
+            {
+              const int c = blockIdx.x;
+              if (sm.sched.each == 0) { c_lo = c - c % nsplit; c_hi = c_lo + sm.sched.parts - 1; }
+              else {
+                const int t0 = qp_first(sm.sched, c) + sm.done - sm.seg.j0;
+                c_lo = qp_owner(sm.sched, t0); c_hi = qp_owner(sm.sched, t0 + sm.seg.all - 1);
+                lead = qp_first(sm.sched, c_lo) == t0 ? 0 : 1;
               }
+            }
+            if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+            if (t == 0) {
+              int32_t* ctr = (int32_t*)p.scratch + 2 * (2 * c_lo + lead) + grp;
+              __threadfence();
+              sm.last[grp] = atomicAdd(ctr, 1) == c_hi - c_lo;
+              if (sm.last[grp]) { *ctr = 0; __threadfence(); }          // zero again for the next launch
+            }
+            if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+            if (sm.last[grp] && live) {
+              auto part_of = [&](int k) { return slots + (int64_t)(2 * k + (k == c_lo ? lead : 0)) * step; };
+              float mm = -INFINITY, ll = 0.f;
+#pragma unroll 4
+              for (int k = c_lo; k <= c_hi; ++k) {
+                const float mi = __ldcg(part_of(k) + D * QP_GROUP), li = __ldcg(part_of(k) + (D + 1) * QP_GROUP), mn = fmaxf(mm, mi);
+                if (mn != -INFINITY) ll = fmaf(ll, qp_ex2(mm - mn), li * qp_ex2(mi - mn));
+                mm = mn;
+              }
+              const float inv = 1.f / ll;
+#pragma unroll 1
+              for (int c = 0; c < D; c += COLS) {
+                float v[COLS] = {};
+#pragma unroll 2
+                for (int k = c_lo; k <= c_hi; ++k) {
+                  const float* part_i = part_of(k);
+                  const float e = qp_ex2(__ldcg(part_i + D * QP_GROUP) - mm) * inv;
 #pragma unroll
-              for (int q = 0; q < COLS; q += 16) store(c + q, v + q);
+                  for (int q = 0; q < COLS; ++q) v[q] = fmaf(e, __ldcg(part_i + (c + q) * QP_GROUP), v[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < COLS; q += 16) store(c + q, v + q);
+              }
             }
           }
         }
-      }
       }
       more = next_rows(ok, std::integral_constant<int, 0>{});
     }
@@ -499,183 +493,183 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
     const int t = tid & 127;
     bool more = any;
     while (more) {
-    const int n_tiles = sm.seg.n, kbeg = sm.seg.klo + sm.seg.j0 * QP_KEYS, kend = sm.seg.kend, kvh = sm.seg.kvh;
-    bool ok = true;
-    const int last_page = (kend - 1) / Q4_PAGE * Q4_PAGE;
-    auto id_of = [&](int key) { return __ldg(p.page_table + min(key, last_page) / Q4_PAGE); };
-    auto row_of = [&](int id) {
-      if ((unsigned)id >= (unsigned)p.num_pages) { atomicExch(&g_prefill_q4_error, 3113); id = 0; }
-      return ((int64_t)id * p.n_kv_heads + kvh) * PB;
-    };
-    // largest magnitude that a row's codes can stand for; over all threads of the role
-    auto largest = [](uint32_t meta) { return fmaxf(fabsf(q4_min(meta)), fabsf(fmaf(15.f, q4_scale(meta), q4_min(meta)))); };
-    if (warp < 12) {
-      // -- keys: a token row to a thread
-      uint32_t kw[D / 8], km = 0u;
-      int id = id_of(kbeg + t);
-      auto load = [&](int k0) {
-        const int key = k0 + t;
-        const uint8_t* src = (const uint8_t*)p.k_cache + row_of(id);
-#pragma unroll
-        for (int i = 0; i < D / 8; i += 2) {
-          const uint2 v = __ldg((const uint2*)(src + (key % Q4_PAGE) * (D / 2) + 4 * i));
-          kw[i] = v.x; kw[i + 1] = v.y;
-        }
-        km = key < kend ? __ldg((const uint32_t*)(src + 8 * D + 4 * (key % Q4_PAGE))) : 0u;         // rows behind the last key count as 0
-        id = id_of(key + QP_KEYS);
+      const int n_tiles = sm.seg.n, kbeg = sm.seg.klo + sm.seg.j0 * QP_KEYS, kend = sm.seg.kend, kvh = sm.seg.kvh;
+      bool ok = true;
+      const int last_page = (kend - 1) / Q4_PAGE * Q4_PAGE;
+      auto id_of = [&](int key) { return __ldg(p.page_table + min(key, last_page) / Q4_PAGE); };
+      auto row_of = [&](int id) {
+        if ((unsigned)id >= (unsigned)p.num_pages) { atomicExch(&g_prefill_q4_error, 3113); id = 0; }
+        return ((int64_t)id * p.n_kv_heads + kvh) * PB;
       };
-      load(kbeg);
-      for (int j = 0; j < n_tiles; ++j) {
-        const int buf = j & 1;
-        float top = redux_max(largest(km));
-        if (lane == 0) sm.mag[buf][0][warp & 3] = top;
-        if (!qp_agree<3>(ok)) break;
-        top = fmaxf(fmaxf(sm.mag[buf][0][0], sm.mag[buf][0][1]), fmaxf(sm.mag[buf][0][2], sm.mag[buf][0][3]));
-        const float kf = qp_pow2(top, 4);                              // the tile's largest value to [2^4, 2^5)
-        if (j >= 2) ok = qp_wait(&sm.k_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
-        if (t == 0) sm.kf[j & 3] = 1.f / kf;
-        const __half2 s2 = __float2half2_rn(q4_scale(km) * kf), m2 = __float2half2_rn(q4_min(km) * kf);
-        const uint32_t base = Ks + (uint32_t)(buf * K_BYTES + (t >> 3) * 1024 + (t & 7) * (128 + 16));       // 16-byte piece x of a row lies at x ^ (row % 8)
+      // largest magnitude that a row's codes can stand for; over all threads of the role
+      auto largest = [](uint32_t meta) { return fmaxf(fabsf(q4_min(meta)), fabsf(fmaf(15.f, q4_scale(meta), q4_min(meta)))); };
+      if (warp < 12) {
+        // -- keys: a token row to a thread
+        uint32_t kw[D / 8], km = 0u;
+        int id = id_of(kbeg + t);
+        auto load = [&](int k0) {
+          const int key = k0 + t;
+          const uint8_t* src = (const uint8_t*)p.k_cache + row_of(id);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {                              // word i of the row: 8 dims from 8 x on
-          const int x = i < 4 * NG ? 4 * (i % NG) + i / NG : i;
-          __half2 c[4];
-          codes_f16(kw[i], c);
-          uint32_t o[4];
+          for (int i = 0; i < D / 8; i += 2) {
+            const uint2 v = __ldg((const uint2*)(src + (key % Q4_PAGE) * (D / 2) + 4 * i));
+            kw[i] = v.x; kw[i + 1] = v.y;
+          }
+          km = key < kend ? __ldg((const uint32_t*)(src + 8 * D + 4 * (key % Q4_PAGE))) : 0u;         // rows behind the last key count as 0
+          id = id_of(key + QP_KEYS);
+        };
+        load(kbeg);
+        for (int j = 0; j < n_tiles; ++j) {
+          const int buf = j & 1;
+          float top = redux_max(largest(km));
+          if (lane == 0) sm.mag[buf][0][warp & 3] = top;
+          if (!qp_agree<3>(ok)) break;
+          top = fmaxf(fmaxf(sm.mag[buf][0][0], sm.mag[buf][0][1]), fmaxf(sm.mag[buf][0][2], sm.mag[buf][0][3]));
+          const float kf = qp_pow2(top, 4);                              // the tile's largest value to [2^4, 2^5)
+          if (j >= 2) ok = qp_wait(&sm.k_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
+          if (t == 0) sm.kf[j & 3] = 1.f / kf;
+          const __half2 s2 = __float2half2_rn(q4_scale(km) * kf), m2 = __float2half2_rn(q4_min(km) * kf);
+          const uint32_t base = Ks + (uint32_t)(buf * K_BYTES + (t >> 3) * 1024 + (t & 7) * (128 + 16));       // 16-byte piece x of a row lies at x ^ (row % 8)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) { const __half2 v = __hfma2(c[q], s2, m2); o[q] = *(const uint32_t*)&v; }
-          st_shared((base ^ (uint32_t)((x & 7) << 4)) + (uint32_t)((x >> 3) * QP_SLAB), o);
-        }
-        if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        gm_arrive((uint64_t*)&sm.k_full[buf]);
-      }
-    } else {
-      // -- values: half a page to a thread: page t / 16 of the tile, tokens 8 vh .. + 7, units vg of every 32 dims
-      uint32_t vw[D / 8], vm[8];
-      const int vh = (t >> 3) & 1, vg = t & 7;
-      int id = id_of(kbeg + (t >> 4) * Q4_PAGE);
-      auto load = [&](int k0) {
-        const int key = k0 + (t >> 4) * Q4_PAGE;
-        const uint8_t* src = (const uint8_t*)p.v_cache + row_of(id);
-        const uint32_t* w = (const uint32_t*)(src + (size_t)vh * 128 * NG + vg * 16 * NG);           // words [tq][g]
-#pragma unroll
-        for (int i = 0; i < 4 * NG; i += 4) { const uint4 v = __ldg((const uint4*)(w + i)); vw[i] = v.x; vw[i + 1] = v.y; vw[i + 2] = v.z; vw[i + 3] = v.w; }
-        if constexpr (TAIL) {                                          // bytes of both halves: mine of each word, as 16 bits
-          const uint4 v = __ldg((const uint4*)(src + 256 * NG + vg * 16));
-          vw[4 * NG] = __byte_perm(v.x, v.y, vh ? 0x7632 : 0x5410); vw[4 * NG + 1] = __byte_perm(v.z, v.w, vh ? 0x7632 : 0x5410);
-        }
-        const uint4 a = __ldg((const uint4*)(src + 8 * D + 32 * vh)), b = __ldg((const uint4*)(src + 8 * D + 32 * vh + 16));
-        const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vm[i] = key + 8 * vh + i < kend ? r[i] : 0u;
-        id = id_of(key + QP_KEYS);
-      };
-      load(kbeg);
-      float vf = 0x1p100f;
-      for (int j = 0; j < n_tiles; ++j) {
-        const int buf = j & 1;
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, largest(vm[i]));
-        top = redux_max(top);
-        if (lane == 0) sm.mag[buf][1][warp & 3] = top;
-        if (!qp_agree<4>(ok)) break;
-        top = fmaxf(fmaxf(sm.mag[buf][1][0], sm.mag[buf][1][1]), fmaxf(sm.mag[buf][1][2], sm.mag[buf][1][3]));
-        if (top * vf >= 4096.f) vf = qp_pow2(top, 4);                  // it stays as long as it keeps the values below 2^12
-        __half2 s2[4], m2[4];                                          // of the token pairs
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s2[i] = __floats2half2_rn(q4_scale(vm[2 * i]) * vf, q4_scale(vm[2 * i + 1]) * vf);
-          m2[i] = __floats2half2_rn(q4_min(vm[2 * i]) * vf, q4_min(vm[2 * i + 1]) * vf);
-        }
-        if (j >= 2) ok = qp_wait(&sm.v_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
-        if (t == 0) sm.vf[buf] = vf;
-        const int chunk = (t >> 3) & 7;                                // eight keys of the 64 of a slab
-        // dim 32 g + 4 vg + e is row 4 (vg % 2) + e of the eight of row group 4 g + vg / 2; its keys lie at chunk ^ row
-        const uint32_t slab = Vs + (uint32_t)(buf * V_BYTES + (t >> 6) * (D * 128));
-        const uint32_t base = slab + (uint32_t)((vg >> 1) * 1024 + (vg & 1) * 512 + ((chunk ^ (vg & 1) << 2) << 4));
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          uint32_t o[4][4];                                            // [dim][token pair]
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int i = 0; i < D / 8; ++i) {                              // word i of the row: 8 dims from 8 x on
+            const int x = i < 4 * NG ? 4 * (i % NG) + i / NG : i;
             __half2 c[4];
-            codes_f16(vw[q * NG + g], c);
+            codes_f16(kw[i], c);
+            uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
+            for (int q = 0; q < 4; ++q) { const __half2 v = __hfma2(c[q], s2, m2); o[q] = *(const uint32_t*)&v; }
+            st_shared((base ^ (uint32_t)((x & 7) << 4)) + (uint32_t)((x >> 3) * QP_SLAB), o);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) st_shared((base ^ (uint32_t)(e << 4)) + (uint32_t)(g * 4096 + e * 128), o[e]);
+          if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          gm_arrive((uint64_t*)&sm.k_full[buf]);
         }
-        if constexpr (TAIL) {
-          uint32_t o[2][4];
+      } else {
+        // -- values: half a page to a thread: page t / 16 of the tile, tokens 8 vh .. + 7, units vg of every 32 dims
+        uint32_t vw[D / 8], vm[8];
+        const int vh = (t >> 3) & 1, vg = t & 7;
+        int id = id_of(kbeg + (t >> 4) * Q4_PAGE);
+        auto load = [&](int k0) {
+          const int key = k0 + (t >> 4) * Q4_PAGE;
+          const uint8_t* src = (const uint8_t*)p.v_cache + row_of(id);
+          const uint32_t* w = (const uint32_t*)(src + (size_t)vh * 128 * NG + vg * 16 * NG);           // words [tq][g]
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t two = vw[4 * NG + (q >> 1)] >> (16 * (q & 1));           // a byte to each token of the pair
-            __half2 c[4];
-            codes_f16((two & 0xFFu) | (two & 0xFF00u) << 8, c);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
+          for (int i = 0; i < 4 * NG; i += 4) { const uint4 v = __ldg((const uint4*)(w + i)); vw[i] = v.x; vw[i + 1] = v.y; vw[i + 2] = v.z; vw[i + 3] = v.w; }
+          if constexpr (TAIL) {                                          // bytes of both halves: mine of each word, as 16 bits
+            const uint4 v = __ldg((const uint4*)(src + 256 * NG + vg * 16));
+            vw[4 * NG] = __byte_perm(v.x, v.y, vh ? 0x7632 : 0x5410); vw[4 * NG + 1] = __byte_perm(v.z, v.w, vh ? 0x7632 : 0x5410);
           }
+          const uint4 a = __ldg((const uint4*)(src + 8 * D + 32 * vh)), b = __ldg((const uint4*)(src + 8 * D + 32 * vh + 16));
+          const uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int dim = 2 * vg + e;
-            st_shared(slab + (uint32_t)(NG * 4096 + (dim >> 3) * 1024 + (dim & 7) * 128 + ((chunk ^ (dim & 7)) << 4)), o[e]);
+          for (int i = 0; i < 8; ++i) vm[i] = key + 8 * vh + i < kend ? r[i] : 0u;
+          id = id_of(key + QP_KEYS);
+        };
+        load(kbeg);
+        float vf = 0x1p100f;
+        for (int j = 0; j < n_tiles; ++j) {
+          const int buf = j & 1;
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, largest(vm[i]));
+          top = redux_max(top);
+          if (lane == 0) sm.mag[buf][1][warp & 3] = top;
+          if (!qp_agree<4>(ok)) break;
+          top = fmaxf(fmaxf(sm.mag[buf][1][0], sm.mag[buf][1][1]), fmaxf(sm.mag[buf][1][2], sm.mag[buf][1][3]));
+          if (top * vf >= 4096.f) vf = qp_pow2(top, 4);                  // it stays as long as it keeps the values below 2^12
+          __half2 s2[4], m2[4];                                          // of the token pairs
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s2[i] = __floats2half2_rn(q4_scale(vm[2 * i]) * vf, q4_scale(vm[2 * i + 1]) * vf);
+            m2[i] = __floats2half2_rn(q4_min(vm[2 * i]) * vf, q4_min(vm[2 * i + 1]) * vf);
           }
+          if (j >= 2) ok = qp_wait(&sm.v_empty[buf], (uint32_t)((j >> 1) - 1) & 1u);
+          if (t == 0) sm.vf[buf] = vf;
+          const int chunk = (t >> 3) & 7;                                // eight keys of the 64 of a slab
+          // dim 32 g + 4 vg + e is row 4 (vg % 2) + e of the eight of row group 4 g + vg / 2; its keys lie at chunk ^ row
+          const uint32_t slab = Vs + (uint32_t)(buf * V_BYTES + (t >> 6) * (D * 128));
+          const uint32_t base = slab + (uint32_t)((vg >> 1) * 1024 + (vg & 1) * 512 + ((chunk ^ (vg & 1) << 2) << 4));
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            uint32_t o[4][4];                                            // [dim][token pair]
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              __half2 c[4];
+              codes_f16(vw[q * NG + g], c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st_shared((base ^ (uint32_t)(e << 4)) + (uint32_t)(g * 4096 + e * 128), o[e]);
+          }
+          if constexpr (TAIL) {
+            uint32_t o[2][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t two = vw[4 * NG + (q >> 1)] >> (16 * (q & 1));           // a byte to each token of the pair
+              __half2 c[4];
+              codes_f16((two & 0xFFu) | (two & 0xFF00u) << 8, c);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) { const __half2 v = __hfma2(c[e], s2[q], m2[q]); o[e][q] = *(const uint32_t*)&v; }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int dim = 2 * vg + e;
+              st_shared(slab + (uint32_t)(NG * 4096 + (dim >> 3) * 1024 + (dim & 7) * 128 + ((chunk ^ (dim & 7)) << 4)), o[e]);
+            }
+          }
+          if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          gm_arrive((uint64_t*)&sm.v_full[buf]);
         }
-        if (j + 1 < n_tiles) load(kbeg + (j + 1) * QP_KEYS);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        gm_arrive((uint64_t*)&sm.v_full[buf]);
       }
-    }
-    more = next_rows(ok, std::integral_constant<int, 1>{});
+      more = next_rows(ok, std::integral_constant<int, 1>{});
     }
   } else {
     regs_down<QP_REGS_ISSUE>();
     bool more = any;
     while (more) {
-    const int n_tiles = sm.seg.n;
-    bool ok = true;
-    if (warp < 16 + groups_of(sm.seg.mt)) {
-      // ================================ the products: a warp to a group, so that no group's waits hold up the other =====================
-      const int g = warp - 16;
-      const uint32_t id_s = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
-      const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);
-      const uint32_t q_lo = qp_desc_lo(Qs + g * Q_BYTES), k_lo = qp_desc_lo(Ks), v_lo = qp_desc_lo(Vs), s_col = tmem + 128u * g, o_col = s_col + 256u;
-      auto both = [&](unsigned long long* bar, uint32_t parity) { if (ok) { ok = __all_sync(0xFFFFFFFFu, qp_wait(bar, parity)); tc_after(); } };
-      // half i of the key tiles: S = Q K^T
-      auto scores = [&](int i) {
-        const int j = i >> 1, half = i & 1;
-        if (half == 0) both(&sm.k_full[j & 1], (uint32_t)(j >> 1) & 1u);
-        if (!ok) return;
-        const uint32_t b = k_lo + (uint32_t)((j & 1) * (K_BYTES >> 4) + half * (64 * 128 >> 4));
+      const int n_tiles = sm.seg.n;
+      bool ok = true;
+      if (warp < 16 + groups_of(sm.seg.mt)) {
+        // ================================ the products: a warp to a group, so that no group's waits hold up the other =====================
+        const int g = warp - 16;
+        const uint32_t id_s = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);      // fp16 operands, fp32 sums
+        const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(QP_GROUP >> 4) << 24);
+        const uint32_t q_lo = qp_desc_lo(Qs + g * Q_BYTES), k_lo = qp_desc_lo(Ks), v_lo = qp_desc_lo(Vs), s_col = tmem + 128u * g, o_col = s_col + 256u;
+        auto both = [&](unsigned long long* bar, uint32_t parity) { if (ok) { ok = __all_sync(0xFFFFFFFFu, qp_wait(bar, parity)); tc_after(); } };
+        // half i of the key tiles: S = Q K^T
+        auto scores = [&](int i) {
+          const int j = i >> 1, half = i & 1;
+          if (half == 0) both(&sm.k_full[j & 1], (uint32_t)(j >> 1) & 1u);
+          if (!ok) return;
+          const uint32_t b = k_lo + (uint32_t)((j & 1) * (K_BYTES >> 4) + half * (64 * 128 >> 4));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (uint32_t)((kk >> 2) * (QP_SLAB >> 4) + 2 * (kk & 3));
-          umma_f16_ss(s_col + 64u * half, q_lo + off, b + off, id_s, kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (uint32_t)((kk >> 2) * (QP_SLAB >> 4) + 2 * (kk & 3));
+            umma_f16_ss(s_col + 64u * half, q_lo + off, b + off, id_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit_warp(&sm.s_full[g][half]);
+          if (half && j + 2 < n_tiles) umma_commit_warp(&sm.k_empty[j & 1]);
+        };
+        both(&sm.q_full[g], 0u);
+        scores(0);
+        scores(1);
+        for (int i = 0; ok && i < 2 * n_tiles; ++i) {
+          const int j = i >> 1, half = i & 1;
+          // O += P V, as P arrives (it comes after the softmax has seen that the values are there)
+          both(&sm.p_full[g][half], (uint32_t)j & 1u);
+          if (!ok) break;
+          const uint32_t pa = s_col + (uint32_t)(64 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) umma_f16_ts(o_col, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, i > 0 || kk > 0 ? 1u : 0u);
+          umma_commit_warp(&sm.o_full[g][half]);
+          if (half && j + 2 < n_tiles) umma_commit_warp(&sm.v_empty[j & 1]);
+          // the scores that go where P lay, once the product has ended: while the softmax works on the other half
+          if (i + 2 < 2 * n_tiles) { both(&sm.o_full[g][half], (uint32_t)j & 1u); scores(i + 2); }
         }
-        umma_commit_warp(&sm.s_full[g][half]);
-        if (half && j + 2 < n_tiles) umma_commit_warp(&sm.k_empty[j & 1]);
-      };
-      both(&sm.q_full[g], 0u);
-      scores(0);
-      scores(1);
-      for (int i = 0; ok && i < 2 * n_tiles; ++i) {
-        const int j = i >> 1, half = i & 1;
-        // O += P V, as P arrives (it comes after the softmax has seen that the values are there)
-        both(&sm.p_full[g][half], (uint32_t)j & 1u);
-        if (!ok) break;
-        const uint32_t pa = s_col + (uint32_t)(64 * half), b = v_lo + (uint32_t)((j & 1) * (V_BYTES >> 4) + half * (D * 128 >> 4));
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_f16_ts(o_col, pa + (uint32_t)(8 * kk), b + (uint32_t)(2 * kk), id_o, i > 0 || kk > 0 ? 1u : 0u);
-        umma_commit_warp(&sm.o_full[g][half]);
-        if (half && j + 2 < n_tiles) umma_commit_warp(&sm.v_empty[j & 1]);
-        // the scores that go where P lay, once the product has ended: while the softmax works on the other half
-        if (i + 2 < 2 * n_tiles) { both(&sm.o_full[g][half], (uint32_t)j & 1u); scores(i + 2); }
       }
-    }
-    more = next_rows(ok, std::integral_constant<int, 1>{});
+      more = next_rows(ok, std::integral_constant<int, 1>{});
     }
   }
   tc_before();
