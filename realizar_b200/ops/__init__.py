@@ -500,7 +500,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, page_rows: t
     k head (when the weights are given), rotation of their first ``rope_dim`` values (``rope_type`` 2: split halves, else adjacent
     pairs) by the table or, beyond it, by ``rope_theta``, the rotated queries to ``q_out`` (default: in place), and the k and v rows
     into the 4-bit cache at ``positions[i]`` of page ``page_rows[i]``.  Rows with a position below 0 are left out altogether.  No two
-    rows of a call may name the same place.  Keys are normalised and rotated in 64 bits, so that the cached codes do not depend on
+    rows of a call may name the same place, and ``q_out`` shares no memory with the key and value heads of ``qkv``.  Keys are normalised and rotated in 64 bits, so that the cached codes do not depend on
     which kernel wrote them."""
     n, d = qkv.shape[0], head_dim
     q = qkv if q_out is None else q_out
