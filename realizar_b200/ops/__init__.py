@@ -502,30 +502,30 @@ def qk_norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, page_rows: t
     into the 4-bit cache at ``positions[i]`` of page ``page_rows[i]``.  Rows with a position below 0 are left out altogether.  No two
     rows of a call may name the same place, and ``q_out`` shares no memory with the key and value heads of ``qkv``.  Keys are normalised and rotated in 64 bits, so that the cached codes do not depend on
     which kernel wrote them."""
-    n, d = qkv.shape[0], head_dim
-    q = qkv if q_out is None else q_out
-    shape, dev = k_cache.shape, k_cache.get_device()
-    ld, ld_q = qkv.stride(0), q.stride(0)
-    f32, i32 = torch.float32, torch.int32
+    d, q = head_dim, qkv if q_out is None else q_out
+    shape, dev, size, size_q, stride, stride_q = k_cache.shape, k_cache.get_device(), qkv.shape, q.shape, qkv.stride(), q.stride()
+    n, u8, f32, i32, p_qkv, p_q = size[0] if size else 0, torch.uint8, torch.float32, torch.int32, qkv.data_ptr(), q.data_ptr()
     # one test for a call that is in order (half of the time of the separate ones), which say what is wrong with another
-    if not (d in Q4_HEAD_DIMS and k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8 and shape[1:] == (n_kv_heads, 16, d // 2 + 4)
-            and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous() and n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0
-            and qkv.dtype is f32 and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= (n_heads + 2 * n_kv_heads) * d
-            and (q_out is None or (q.dtype is f32 and q.dim() == 2 and q.stride(1) == 1 and q.shape[0] >= n and q.shape[1] >= n_heads * d and q.get_device() == dev))
-            and positions.dtype is i32 and positions.dim() == 1 and positions.is_contiguous() and positions.shape[0] >= n and positions.get_device() == dev
-            and page_rows.dtype is i32 and page_rows.dim() == 1 and page_rows.is_contiguous() and page_rows.shape[0] >= n and page_rows.get_device() == dev
-            and qkv.get_device() == dev and v_cache.get_device() == dev and 0 <= rope_dim <= d and rope_dim % 2 == 0 and (q_norm_w is None) == (k_norm_w is None)
-            and all(w is None or (w.dtype is f32 and w.numel() == d and w.is_contiguous() and w.get_device() == dev) for w in (q_norm_w, k_norm_w))
+    if not (d in Q4_HEAD_DIMS and k_cache.dtype is u8 and v_cache.dtype is u8 and shape[1:] == (n_kv_heads, 16, d // 2 + 4) and v_cache.shape == shape
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0
+            and qkv.dtype is f32 and len(size) == 2 and stride[1] == 1 and size[1] >= (n_heads + 2 * n_kv_heads) * d
+            and (q is qkv or (q.dtype is f32 and len(size_q) == 2 and stride_q[1] == 1 and size_q[0] >= n and size_q[1] >= n_heads * d and q.get_device() == dev))
+            and positions.dtype is i32 and positions.dim() == 1 and positions.is_contiguous() and positions.numel() >= n and positions.get_device() == dev
+            and page_rows.dtype is i32 and page_rows.dim() == 1 and page_rows.is_contiguous() and page_rows.numel() >= n and page_rows.get_device() == dev
+            and qkv.get_device() == dev and v_cache.get_device() == dev and 0 <= rope_dim <= d and rope_dim % 2 == 0
+            and ((q_norm_w is None and k_norm_w is None) or (q_norm_w is not None and k_norm_w is not None and
+                 all(w.dtype is f32 and w.numel() == d and w.is_contiguous() and w.get_device() == dev for w in (q_norm_w, k_norm_w))))
             and (rope_table is None or (rope_table.dtype is f32 and rope_table.shape[1:] == (rope_dim // 2, 2) and rope_table.is_contiguous() and rope_table.get_device() == dev))
-            and ld % 2 == 0 and ld_q % 2 == 0 and (ld_q >= n_heads * d or n < 2) and qkv.data_ptr() % 8 == 0 and q.data_ptr() % 8 == 0
+            and stride[0] % 2 == 0 and stride_q[0] % 2 == 0 and (stride_q[0] >= n_heads * d or n < 2) and p_qkv % 8 == 0 and p_q % 8 == 0
             and dev >= 0 and dev == torch._C._cuda_getDevice()):
         _refuse_append(qkv, positions, page_rows, k_cache, v_cache, n_heads, n_kv_heads, head_dim, q_out, q_norm_w, k_norm_w, rope_dim, rope_table)
     if n == 0:
         return
-    p = S.QkAppendParams(qkv.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), page_rows.data_ptr(), ptr(q_norm_w),
-                         ptr(k_norm_w), ptr(rope_table), ld, ld_q, eps, n, n_heads, n_kv_heads, d, rope_dim, rope_type,
+    p = S.pack_qk_append(p_qkv, p_q, k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), page_rows.data_ptr(),
+                         0 if q_norm_w is None else q_norm_w.data_ptr(), 0 if k_norm_w is None else k_norm_w.data_ptr(),
+                         0 if rope_table is None else rope_table.data_ptr(), stride[0], stride_q[0], eps, n, n_heads, n_kv_heads, d, rope_dim, rope_type,
                          0 if rope_table is None else rope_table.shape[0], shape[0], rope_theta, 0)
-    check(lib().rlz_qk_norm_rope_append(ctypes.byref(p), stream_ptr()), "qk_norm_rope_append")
+    check(lib().rlz_qk_norm_rope_append(p, torch._C._cuda_getCurrentRawStream(dev)), "qk_norm_rope_append")
 
 
 def _refuse_append(qkv, positions, page_rows, k_cache, v_cache, n_heads, n_kv_heads, head_dim, q_out, q_norm_w, k_norm_w, rope_dim, rope_table) -> None:

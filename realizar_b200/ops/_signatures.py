@@ -3,6 +3,7 @@ exported launcher of ``librlz_cuda.so``."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, Structure, c_double, c_float, c_int, c_int32, c_int64, c_longlong, c_void_p
 
 GEMV_MAX_MATS = 4
@@ -71,6 +72,10 @@ class QkAppendParams(Structure):
                 ("ld_q", c_int64), ("eps", c_double), ("rows", c_int32), ("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32),
                 ("rope_dim", c_int32), ("rope_type", c_int32), ("rope_table_len", c_int32), ("num_pages", c_int32), ("rope_theta", c_float),
                 ("_pad", c_int32)]
+
+
+# the bytes of a QkAppendParams from its fields in order (a fifth of the time that the structure takes)
+pack_qk_append = struct.Struct("@" + "".join({c_void_p: "P", c_int64: "q", c_double: "d", c_int32: "i", c_float: "f"}[t] for _, t in QkAppendParams._fields_)).pack
 
 
 class SampleParams(Structure):
@@ -176,7 +181,7 @@ def declare(lib: ctypes.CDLL) -> None:
     lib.rlz_attn_prefill_impl.argtypes = [POINTER(AttnPrefillParams), c_void_p, c_int]
     lib.rlz_attn_prefill_supported.argtypes = [c_int]
     lib.rlz_attn_prefill_error.argtypes = [c_int]
-    lib.rlz_qk_norm_rope_append.argtypes = [POINTER(QkAppendParams), c_void_p]
+    lib.rlz_qk_norm_rope_append.argtypes = [c_void_p, c_void_p]            # a QkAppendParams or the bytes of one
     lib.rlz_q4_append_error.argtypes = [c_int]
     lib.rlz_attn_q4_error.argtypes = [c_int]
     lib.rlz_attn_prefill_q4_error.argtypes = [c_int]

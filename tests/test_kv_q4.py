@@ -112,3 +112,11 @@ def test_append_refuses_overlapping_results():
 def test_cli_offers_the_format():
     from realizar_b200.cli import build_parser
     assert build_parser().parse_args(["run", "m.gguf", "hi", "--kv-dtype", "q4"]).kv_dtype == "q4"
+
+
+def test_append_parameters_are_packed_as_the_structure_lies():
+    import ctypes
+    from realizar_b200.ops import _signatures as S
+    values = [11 * (i + 1) for i in range(11)] + [1e-6] + list(range(1, 9)) + [5e5, 0]
+    assert bytes(S.QkAppendParams(*values)) == S.pack_qk_append(*values)
+    assert len(S.pack_qk_append(*values)) == ctypes.sizeof(S.QkAppendParams)
