@@ -181,43 +181,59 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
   for (int b = tid; b < min(p.batch, QD_POSITIONS); b += 32 * NW + QD_HELPERS) sm.pos[b] = __ldg(p.positions + b);
   __syncthreads();
 
-  // ---- my share: pairs [x0, x1) of the sequence of all tiles' pairs.  Every warp works it out, its lanes over the sequences ------
-  const int G = p.n_heads / p.n_kv_heads, hgroups = (G + ROWS - 1) / ROWS, tiles = p.n_kv_heads * hgroups;
-  const int per = (p.batch + 31) / 32, b_lo = min(lane * per, p.batch), b_hi = min(b_lo + per, p.batch);
-  int mine = 0, live = 0, longest = 0;
-  for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, sm.pos, b).n; mine += n; live += n > 0; longest = max(longest, n); }
-  int incl = mine, live_incl = live;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o), w = __shfl_up_sync(0xFFFFFFFFu, live_incl, o);
-    if (lane >= o) { incl += v; live_incl += w; }
+  // ---- my share: pairs [x0, x1) of the sequence of all tiles' pairs.  Every warp works it out, its lanes over the sequences.  (Integer
+  // quotients by variables take 100 clocks each, one after another: as few as there can be) ------------------------------------------
+  const int G = p.n_heads / p.n_kv_heads, hgroups = (G + ROWS - 1) / ROWS, tiles = p.n_kv_heads * hgroups, c = blockIdx.x;
+  int mine = 0, live = 0, longest = 0, b_lo = 0;
+  if (p.batch == 1) { mine = longest = qd_seq(p, sm.pos, 0).n; live = mine > 0; }
+  else {
+    const int per = (p.batch + 31) / 32, b_hi = min((lane + 1) * per, p.batch);
+    b_lo = min(lane * per, p.batch);
+    for (int b = b_lo; b < b_hi; ++b) { const int n = qd_seq(p, sm.pos, b).n; mine += n; live += n > 0; longest = max(longest, n); }
   }
-  const int total = __shfl_sync(0xFFFFFFFFu, incl, 31) * tiles, all_tiles = __shfl_sync(0xFFFFFFFFu, live_incl, 31) * tiles, c = blockIdx.x;
+  int incl = mine, live_incl = live, total = mine, all_tiles = live;
+  if (p.batch > 1) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o), w = __shfl_up_sync(0xFFFFFFFFu, live_incl, o);
+      if (lane >= o) { incl += v; live_incl += w; }
+    }
+    total = __shfl_sync(0xFFFFFFFFu, incl, 31); all_tiles = __shfl_sync(0xFFFFFFFFu, live_incl, 31);
+    longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+  }
+  total *= tiles; all_tiles *= tiles;
   if (total == 0) return;
-  longest = __reduce_max_sync(0xFFFFFFFFu, longest);
   const int split = min((int)gridDim.x / all_tiles, longest);     // CTAs to a tile, 0: there are more tiles
-  const bool by_tile = split > 0 && (longest + split - 1) / split < total / (int)gridDim.x + QD_TILE_COST;
+  const bool by_tile = split > 0 && __fdividef((float)longest, (float)split) < __fdividef((float)total, (float)gridDim.x) + QD_TILE_COST;
   const int ctas = by_tile ? all_tiles * split : min((int)gridDim.x, total);
   if (c >= ctas) return;
-  const QdShare share = {total / ctas, total % ctas};
+  const int my_tile = by_tile ? c / split : 0;
+  QdShare share = {0, 0};
+  if (!by_tile) { share.each = total / ctas; share.more = total - share.each * ctas; }
   int x0 = qd_first(share, c), x1 = x0 + share.each + (c < share.more ? 1 : 0);
   // the lane whose sequences hold place x0, or (by tile) live tile c / split
-  const int want = by_tile ? c / split : x0, first = by_tile ? (live_incl - live) * tiles : (incl - mine) * tiles;
-  const bool holds = first <= want && want < (by_tile ? live_incl : incl) * tiles;
-  int b0 = b_lo, at0 = want - first;
-  if (holds)
-    for (;; ++b0) {
-      const int n = qd_seq(p, sm.pos, b0).n, m = (by_tile ? n > 0 : n) * tiles;
-      if (at0 < m) { if (by_tile) at0 *= n; break; }
-      at0 -= m;
-    }
-  const int holder = __ffs(__ballot_sync(0xFFFFFFFFu, holds)) - 1;
-  b0 = __shfl_sync(0xFFFFFFFFu, b0, holder);
-  at0 = __shfl_sync(0xFFFFFFFFu, at0, holder);
+  const int want = by_tile ? my_tile : x0;
+  int b0 = b_lo, at0 = want;
+  if (p.batch == 1) { if (by_tile) at0 *= mine; }
+  else {
+    const int first = by_tile ? (live_incl - live) * tiles : (incl - mine) * tiles;
+    const bool holds = first <= want && want < (by_tile ? live_incl : incl) * tiles;
+    at0 -= first;
+    if (holds)
+      for (;; ++b0) {
+        const int n = qd_seq(p, sm.pos, b0).n, m = (by_tile ? n > 0 : n) * tiles;
+        if (at0 < m) { if (by_tile) at0 *= n; break; }
+        at0 -= m;
+      }
+    const int holder = __ffs(__ballot_sync(0xFFFFFFFFu, holds)) - 1;
+    b0 = __shfl_sync(0xFFFFFFFFu, b0, holder);
+    at0 = __shfl_sync(0xFFFFFFFFu, at0, holder);
+  }
   if (by_tile) {                                                   // places count from the tile's first pair
-    const int n = qd_seq(p, sm.pos, b0).n, parts = min(split, n), part = c % split;
+    const int n = qd_seq(p, sm.pos, b0).n, parts = min(split, n), part = c - my_tile * split;
     if (part >= parts) return;
-    x0 = part * n / parts; x1 = (part + 1) * n / parts; at0 += x0;
+    const QdShare in_tile = {n / parts, n % parts};
+    x0 = qd_first(in_tile, part); x1 = x0 + in_tile.each + (part < in_tile.more ? 1 : 0); at0 += x0;
   }
   // Pair k of main warp w is pair w + NW k of the CTA's share: the tiles' ends fall on all warps alike.
   auto first_k = [](int w, int x) { return x > w ? (x - w + NW - 1) / NW : 0; };        // first pair of warp w at or behind place x of the share
