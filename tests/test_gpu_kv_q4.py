@@ -281,6 +281,32 @@ def test_decode_wide_ranges_of_scales(cuda_device):
         assert _rel(out[0], want) < 1e-5, kind
 
 
+@pytest.mark.parametrize("h, kvh, d, grow", [(8, 2, 64, True), (14, 2, 80, True), (4, 2, 96, False), (6, 1, 128, True), (16, 2, 128, False)])
+def test_decode_long_shares(cuda_device, h, kvh, d, grow):
+    """Many rows over the same long context, so that a warp goes through dozens of pages: its sums leave the registers on the way.  With
+    ``grow``, scores and values grow along the context: the running maximum and the values' power of two move after that.
+
+    Scores reach 20 in powers of two and are rounded some three times: 3 x 20 x 2^-24 x ln 2 = 2.5e-6, and the sums add less than 2e-6."""
+    from realizar_b200 import ops
+    B, n = 64 if kvh == 2 else 128, 6000
+    check = _decode(h, kvh, d, [n - 7 * (b % 3) for b in range(B)], seed=d + h, no_append=True, shared_table=True, garbage=False)
+    qkv, out, kc, vc, pos, pt = check.keep[:6]
+    if grow:
+        i = torch.arange(pt.numel() * 16, device="cuda").float()[:, None]
+        for c, factor in ((kc, torch.exp2(i / n)), (vc, torch.exp2(i / 400 - 8))):
+            flat = c.flatten(-2)
+            for k in range(kvh):
+                meta = flat[pt.long(), k, 8 * d:].contiguous().view(torch.bfloat16).view(-1, 2).float()
+                flat[pt.long(), k, 8 * d:] = (meta * factor).bfloat16().view(torch.uint8).view(-1, 64)
+    ops.attn_decode_launch(check.params)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    ks, vs = _gather(kc, pt, d, False, n), _gather(vc, pt, d, True, n)
+    for b in range(0, B, 5):
+        p1 = int(pos[b]) + 1
+        assert _rel(out[b], _attend64(qkv[b, : h * d].double().view(h, d), ks[:, :p1], vs[:, :p1], 0)) < 1e-5, b
+
+
 def test_decode_device_checks(cuda_device):
     """A position beyond its page-table row and a page id outside the cache set the status word; the other sequences are right."""
     from realizar_b200 import ops
