@@ -19,10 +19,12 @@
 // Range: K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
 // softmax scale; V by one that changes only when a tile needs it, with O), q by one to a row.
 //
-// Split, in tiles of 128 keys.  Few row tiles (256 rows of a kv head): to each the same number of CTAs, nsplit.  Many, or a number that
-// would leave SMs idle: one CTA to an SM, and the key tiles of all row tiles are divided evenly (nsplit = 0).  A CTA that has only some
-// keys of a row tile leaves its part in scratch, and the last of the tile's CTAs to arrive joins them in a fixed order.  Between two
-// row tiles a CTA starts over: all roles meet and the barriers are set up again.  Without scratch a CTA takes a row tile.
+// Split, in tiles of 128 keys.  Few row tiles (256 rows of a kv head): to each a cluster of nsplit CTAs, which take the keys in parts
+// and join them out of one another's shared memory, every CTA some of the rows (by way of global memory, written by all and read by the
+// last to arrive, 512 rows behind 1536 keys took 38 us).  Many, or a number that would leave SMs idle: one CTA to an SM, and the key
+// tiles of all row tiles are divided evenly (nsplit = 0).  There a CTA that has only some keys of a row tile leaves its part in scratch,
+// and the last of the tile's CTAs to arrive joins them in a fixed order.  Between two row tiles a CTA starts over: all roles meet and
+// the barriers are set up again.  Without scratch and for too many row tiles for clusters, a CTA takes a row tile.
 #include "attention_q4.cuh"
 #include "kv_q4.cuh"
 #include "tcgen05_common.cuh"
@@ -35,6 +37,7 @@ namespace rlz {
 __device__ int g_prefill_q4_error = 0;
 
 constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148;
+constexpr int QP_MAX_SPLIT = 8;                // CTAs to a cluster
 constexpr int QP_MIN_TILES = 2, QP_SEG_COST = 5;      // least share of a CTA; what another row tile costs it, in key tiles
 constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 96, QP_REGS_ISSUE = 32;      // 256, 256 and 128 threads: the launch's 640 x 96
 constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
@@ -53,6 +56,7 @@ struct QpSmem {
   float kf[4], vf[2];                         // powers of two that the tiles carry (of K the inverse, read after the buffer is free again)
   float mag[2][2][4];                         // largest magnitudes of K and V seen by the decoding warps, for even and odd tiles
   float qf[2][QP_GROUP];                      // powers of two of the query rows
+  float2 ml[2][QP_GROUP];                     // maxima and weights of a part's rows
   uint32_t tmem;
   int last[2];
   QpSched sched;
@@ -120,6 +124,11 @@ __device__ __forceinline__ void codes_f16(uint32_t w, __half2 (&c)[4]) {
   c[0] = __hsub2(*(const __half2*)&r[0], magic); c[1] = __hfma2(*(const __half2*)&r[1], sixteenth, back);
   c[2] = __hsub2(*(const __half2*)&r[2], magic); c[3] = __hfma2(*(const __half2*)&r[3], sixteenth, back);
 }
+
+// shared memory of another CTA of the cluster; the cluster's barrier
+__device__ __forceinline__ uint32_t qp_peer(uint32_t at, int rank) { uint32_t r; asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank)); return r; }
+__device__ __forceinline__ float qp_ld_peer(uint32_t at) { float v; asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory"); return v; }
+__device__ __forceinline__ void qp_cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 
 template <int R> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
@@ -276,6 +285,20 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
     // ================================ softmax: one thread to a row ================================================================
     regs_up<QP_REGS_SOFTMAX>();
     const int grp = warp >> 2, t = tid & 127;
+    auto store_at = [&](int token, int head, int c, const float* v) {      // 16 finished values
+      const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
+      if (p.out_bf16) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
+        dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
+    };
+    float part_f = 0.f;                                              // of a part of my row that waits in TMEM: 1 / vf
     bool more = any;
     while (more) {
       const int m0 = sm.seg.mt * QP_ROWS, groups = groups_of(sm.seg.mt), kvh = sm.seg.kvh, n_tiles = sm.seg.n, kbeg = sm.seg.klo + sm.seg.j0 * QP_KEYS, pos0 = sm.sched.z.pos0;
@@ -400,19 +423,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         if (grp == 0 ? qp_agree<1>(ok) : qp_agree<2>(ok)) {
           tc_after();
           const float inv_vf = 1.f / vf, l = l2.x + l2.y;
-          auto store = [&](int c, const float* v) {                   // 16 finished values
-            const int64_t at = (int64_t)token * p.ld_out + (int64_t)head * D + c;
-            if (p.out_bf16) {
-              uint32_t w[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-              uint4* dst = (uint4*)((__nv_bfloat16*)p.out + at);
-              dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) *(float4*)(p.out + at + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            }
-          };
+          auto store = [&](int c, const float* v) { store_at(token, head, c, v); };
           const bool whole = n_tiles == sm.seg.all;
           constexpr int COLS = D % 32 ? 16 : 32;
           // slots of a CTA in scratch: 0 the row tile that its share begins in, 1 the one that it ends in
@@ -430,6 +441,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
               for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * f;
               if (live) store(c, v);
             }
+          } else if (nsplit > 0) {
+            sm.ml[grp][t] = make_float2(m, l);
+            part_f = inv_vf;
           } else {
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -439,17 +453,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
               for (int i = 0; i < 16; ++i) __stcg(slot + (c + i) * QP_GROUP, __uint_as_float(r[i]) * inv_vf);
             }
             slot[D * QP_GROUP] = m; slot[(D + 1) * QP_GROUP] = l;
-            // the row tile's CTAs: neighbours by tile, else those that have its first and last place
-            int c_lo, c_hi, lead = 0;
-            {
-              const int c = blockIdx.x;
-              if (sm.sched.each == 0) { c_lo = c - c % nsplit; c_hi = c_lo + sm.sched.parts - 1; }
-              else {
-                const int t0 = qp_first(sm.sched, c) + sm.done - sm.seg.j0;
-                c_lo = qp_owner(sm.sched, t0); c_hi = qp_owner(sm.sched, t0 + sm.seg.all - 1);
-                lead = qp_first(sm.sched, c_lo) == t0 ? 0 : 1;
-              }
-            }
+            // the row tile's CTAs: those that have its first and last key tile
+            const int t0 = qp_first(sm.sched, blockIdx.x) + sm.done - sm.seg.j0;
+            const int c_lo = qp_owner(sm.sched, t0), c_hi = qp_owner(sm.sched, t0 + sm.seg.all - 1), lead = qp_first(sm.sched, c_lo) == t0 ? 0 : 1;
             if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
             if (t == 0) {
               int32_t* ctr = (int32_t*)p.scratch + 2 * (2 * c_lo + lead) + grp;
@@ -486,6 +492,49 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
         }
       }
       more = next_rows(ok, std::integral_constant<int, 0>{});
+    }
+    if (nsplit > 1) {
+      // ---- the cluster's parts; the last meeting of the roles has freed the operand tiles: sums by columns of 128 rows
+      const int parts = sm.sched.parts, rank = (int)blockIdx.x % nsplit, m0 = sm.seg.mt * QP_ROWS, kvh = sm.seg.kvh;
+      if (parts > 1 && rank < parts && grp < groups_of(sm.seg.mt)) {
+        const uint32_t lane_o = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(128 * grp) + 256u;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(lane_o + (uint32_t)c, r);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(Qs + (uint32_t)(((grp * D + c + i) * QP_GROUP + t) * 4)), "f"(__uint_as_float(r[i]) * part_f) : "memory");
+        }
+      }
+      qp_cluster_sync();
+      if (parts > 1) {
+        const int n = min(QP_ROWS, rows - m0), r0 = rank * n / nsplit, mine = (rank + 1) * n / nsplit - r0;        // my rows
+        for (int i = tid; i < mine * (D / 16); i += 256) {
+          const int c = i / mine, row = r0 + i - c * mine, g = row >> 7, tr = row & 127;
+          float m[QP_MAX_SPLIT], l[QP_MAX_SPLIT], mm = -INFINITY, ll = 0.f, v[16] = {};
+#pragma unroll
+          for (int k = 0; k < QP_MAX_SPLIT; ++k) {
+            const uint32_t at = qp_peer(gm_smem_u32(&sm.ml[g][tr]), min(k, parts - 1));
+            m[k] = k < parts ? qp_ld_peer(at) : -INFINITY; l[k] = k < parts ? qp_ld_peer(at + 4u) : 0.f;
+            mm = fmaxf(mm, m[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < QP_MAX_SPLIT; ++k) { m[k] = m[k] == -INFINITY ? 0.f : qp_ex2(m[k] - mm); ll = fmaf(m[k], l[k], ll); }
+          const float inv = 1.f / ll;
+#pragma unroll
+          for (int k = 0; k < QP_MAX_SPLIT; ++k) {
+            if (k >= parts) break;
+            const uint32_t at = qp_peer(Qs + (uint32_t)(((g * D + 16 * c) * QP_GROUP + tr) * 4), k);
+            const float e = m[k] * inv;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = fmaf(e, qp_ld_peer(at + (uint32_t)(q * QP_GROUP * 4)), v[q]);
+          }
+          const int token = (m0 + row) / G;
+          store_at(token, kvh * G + m0 + row - token * G, 16 * c, v);
+        }
+      }
+      qp_cluster_sync();                                             // the others have read my part
     }
   } else if (warp < 16) {
     // ================================ decoding ======================================================================================
@@ -625,6 +674,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       }
       more = next_rows(ok, std::integral_constant<int, 1>{});
     }
+    if (nsplit > 1) { qp_cluster_sync(); qp_cluster_sync(); }
   } else {
     regs_down<QP_REGS_ISSUE>();
     bool more = any;
@@ -671,6 +721,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
       }
       more = next_rows(ok, std::integral_constant<int, 1>{});
     }
+    if (nsplit > 1) { qp_cluster_sync(); qp_cluster_sync(); }
   }
   tc_before();
   __syncthreads();
@@ -694,16 +745,33 @@ static int launch_prefill_q4(const AttnPrefillParams& p, cudaStream_t st) {
   const int tiles = (int)(((int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads) + QP_ROWS - 1) / QP_ROWS) * p.n_kv_heads;
   const int64_t reach = p.pos0_ptr ? (int64_t)p.pt_len * Q4_PAGE : (int64_t)p.pos0 + p.n_tokens;
   const int keys = (int)((p.window > 0 ? std::min<int64_t>(reach, p.window + QP_ROWS) : reach) / QP_KEYS) + 1;
-  int nsplit = 1, grid = tiles;
+  // as many CTAs to a row tile as fit, in clusters, onto the SMs at once
+  static int fits[64][QP_MAX_SPLIT + 1] = {};                        // clusters of a size that a device holds, and one
+  int dev = 0, nsplit = 1;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return (int)e;
+  for (int n = std::min(QP_MAX_SPLIT, QP_MAX_CTAS / tiles); n > 1 && nsplit == 1; --n) {
+    int& f = fits[dev & 63][n];
+    if (f == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      cfg.gridDim = dim3(n); cfg.blockDim = dim3(QP_THREADS); cfg.dynamicSmemBytes = smem;
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = n; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = 1;
+      int active = 0;
+      if (cudaError_t e = cudaOccupancyMaxActiveClusters(&active, attn_prefill_q4_kernel<D>, &cfg); e != cudaSuccess) return (int)e;
+      f = active + 1;
+    }
+    if (tiles < f) nsplit = n;
+  }
+  int grid = tiles * nsplit;
   if (p.scratch && p.scratch_floats >= 2LL * QP_MAX_CTAS * QP_ROWS * (D + 4) + QP_COUNTERS) {
-    nsplit = std::min(std::max(QP_MAX_CTAS / tiles, 1), 32);
-    grid = tiles * nsplit;
     // time in key tiles: of the longest CTA, or, of an even share, with the second row tile that it reaches into
     const int waves = (grid + QP_MAX_CTAS - 1) / QP_MAX_CTAS, by_tile = waves * ((keys + nsplit - 1) / nsplit) + (waves - 1) * QP_SEG_COST;
     const int even = (int)((int64_t)keys * tiles / QP_MAX_CTAS) + waves * QP_SEG_COST;
     if (even < by_tile) { nsplit = 0; grid = QP_MAX_CTAS; }
   }
-  return (int)launch(attn_prefill_q4_kernel<D>, dim3(grid), dim3(QP_THREADS), smem, st, p, nsplit);
+  return (int)launch_cluster(attn_prefill_q4_kernel<D>, dim3(grid), dim3(QP_THREADS), dim3(std::max(nsplit, 1)), smem, st, p, nsplit);
 }
 
 int attn_prefill_q4_dispatch(const AttnPrefillParams& given, cudaStream_t st) {

@@ -330,8 +330,8 @@ def attn_prefill(qkv: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     (tensor-core kernel; the chunk's own K/V rows must already be in the cache).  With ``pos0_dev`` (an int32 device
     tensor) the position of row 0 is read on the device, so a captured launch serves every chunk position.
     ``impl``: "tc" (128-query tiles on tcgen05) or "mma" (16-query tiles on mma.sync); None = the launcher's choice.
-    ``scratch`` (4-bit caches, from ``attn_prefill_scratch``, one to a stream): lets the keys be divided over the SMs where the rows alone would
-    leave some idle.  Over a 4-bit cache, rows whose positions (read on the device) lie beyond the page table are not computed, nor are
+    ``scratch`` (4-bit caches, from ``attn_prefill_scratch``, one to a stream): lets the keys be divided over all SMs where the rows, and
+    clusters of up to eight SMs to 256 (row, query head) pairs of a kv head, would leave some idle.  Over a 4-bit cache, rows whose positions (read on the device) lie beyond the page table are not computed, nor are
     those that share 256 (row, query head) pairs of a kv head with them, and the device status tells."""
     if k_cache.dtype is torch.uint8 and k_cache.shape[-1] == head_dim // 2 + 4:
         return _attn_prefill_q4(qkv, out, k_cache, v_cache, page_table, n_tokens, pos0, n_heads, n_kv_heads, head_dim, q_off, window or 0, pos0_dev, impl, scratch)
@@ -399,8 +399,7 @@ def attn_prefill_error(clear: bool = True) -> int:
 
 
 def attn_prefill_scratch(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
-    """Workspace with which ``attn_prefill`` divides chunks over a 4-bit cache along the keys when the rows alone leave SMs idle: the same
-    size for any number of rows.  One to a stream; it keeps nothing from one call for the next."""
+    """Workspace with which ``attn_prefill`` divides the keys of a 4-bit cache evenly over the SMs: the same size for any number of rows.  One to a stream; it keeps nothing from one call for the next."""
     return torch.zeros(int(lib().rlz_attn_prefill_q4_scratch_floats(int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim))), device=device, dtype=torch.float32)
 
 
