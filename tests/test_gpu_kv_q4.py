@@ -421,6 +421,16 @@ def test_prompt_attention_divided_evenly(cuda_device, h, kvh, d, rows, pos0, kw)
     _prompt(h, kvh, d, rows, pos0, **kw)
 
 
+@pytest.mark.parametrize("h, kvh, d, rows, pos0, kw", [
+    (64, 1, 128, 3, 700, {}), (300, 1, 64, 2, 100, {}), (160, 160, 64, 9, 40, {}), (160, 160, 80, 300, 5, dict(with_scratch=False)), (2, 1, 128, 129, 5000, {}),
+    (18, 18, 64, 100, 900, {}), (19, 19, 128, 200, 1500, dict(window=700)), (1, 1, 64, 1, 60000, {}), (1, 1, 64, 1, 60000, dict(with_scratch=False)),
+    (4, 4, 128, 129, 2047, {}), (74, 74, 64, 16, 5000, {}), (75, 75, 64, 16, 5000, {})])
+def test_prompt_attention_at_the_borders_of_the_split(cuda_device, h, kvh, d, rows, pos0, kw):
+    """More query heads than rows of a tile, more kv heads than SMs, one row over a long context, row tiles that just fill or just miss two
+    CTAs each, a second group of one row."""
+    _prompt(h, kvh, d, rows, pos0, **kw)
+
+
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 600])
 def test_prompt_attention_window_beyond_the_positions(cuda_device, window):
     _prompt(4, 2, 64, 90, 500, window=window)
