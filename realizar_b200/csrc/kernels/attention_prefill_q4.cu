@@ -3,9 +3,9 @@
 // A CTA has two groups of 128 rows of one kv head, row = (token, query head of the group): the group's heads share the keys and values
 // that the CTA turns into fp16, 128 keys at a time.  Per group and half a tile (64 keys):
 //   S = Q K^T      128 x 64 x D, accumulated in TMEM
-//   P = 2^(S - m)  one thread to a row; P goes back to TMEM as fp16, over the columns of S, and is the A operand of
-//   O += P V       128 x D x 64, accumulated in TMEM.  The running maximum moves only when a score passes it by 2^8, so that O is
-//                  rarely read, scaled and written back.
+//   P = 2^(S - m + 11)  one thread to a row; P goes back to TMEM as fp16, over the columns of S, and is the A operand of
+//   O += P V       128 x D x 64, accumulated in TMEM.  The running maximum m moves only when a score passes it by 4 (a factor of 2^4),
+//                  so that O is rarely read, scaled and written back.
 // Warps 0..7 do the softmax of the groups, 8..11 decode keys and 12..15 values (code x scale + minimum in fp16, rounded once) into two
 // buffers each of swizzled operand tiles, warps 16 and 17 issue the products of a group each.  The scores of one half are computed while
 // the softmax is at the other (whole tiles, whose scores have to wait for the product that reads P in their place: 280 instead of
@@ -16,7 +16,9 @@
 // cores work 2560 (products of 64 keys read the queries from shared memory twice as often: 384 instead of 256 clocks), the exponentials
 // take 2048 (16 a clock) and the decoding 9% of the issue slots' time.
 //
-// Range: K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
+// Range: fp16 holds P from 2^15 down to 2^-14 with all of its bits and to 2^-25 with fewer: weights count in full to 2^-25 of the row's
+// largest and at all to 2^-36, which matters where the largest belongs to a value near zero (32768 keys, one with 99.9% of the weight
+// and a zero value: the sum of the others is off by 6e-3, which is the rounding of the query to fp16; with P = 2^(S - m) by 0.28).  K and V tiles are scaled by powers of two so that fp16 holds them whatever the cache's scales are (K per tile, undone in the
 // softmax scale; V by one that changes only when a tile needs it, with O), q by one to a row.
 //
 // Split, in tiles of 128 keys.  Few row tiles (256 rows of a kv head): to each a cluster of nsplit CTAs, which take the keys in parts
@@ -40,6 +42,9 @@ constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS 
 constexpr int QP_MAX_SPLIT = 8;                // CTAs to a cluster
 constexpr int QP_MIN_TILES = 2, QP_SEG_COST = 5;      // least share of a CTA; what another row tile costs it, in key tiles
 constexpr int QP_REGS_SOFTMAX = 128, QP_REGS_DECODE = 96, QP_REGS_ISSUE = 32;      // 256, 256 and 128 threads: the launch's 640 x 96
+// Weights as fp16: 2^(S - m + QP_SHIFT), at most 2^15, where the maximum m of a row moves only when a score passes it by QP_LAG.  What it may
+// not lag is range for small weights; 2048 rows behind 6144 keys of 128 dims: 271 us with 8 and with 4, 278 with 2, 293 with 1
+constexpr int QP_LAG = 4, QP_SHIFT = 15 - QP_LAG;
 constexpr int QP_SLAB = 128 * 128;            // [128 rows x 64 fp16], 128-byte swizzle
 constexpr int QP_COUNTERS = 640;               // floats in front of the parts: arrival counters, one to each of a CTA's two slots and group
 
@@ -383,7 +388,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
               top1 = max3(top1, score(k + 2), score(k + 3));
             }
             top = fmaxf(top, top1) * sc;
-            if (__any_sync(0xFFFFFFFFu, top > m + 8.f || vn != vf)) {
+            if (__any_sync(0xFFFFFFFFu, top > m + (float)QP_LAG || vn != vf)) {
               const float mn = fmaxf(m, top), corr = m == -INFINITY ? 0.f : qp_ex2(m - mn), co = corr * (vn / vf);
               if (i > 0) {
                 ok = __all_sync(0xFFFFFFFFu, qp_wait(&sm.o_full[grp][half ^ 1], (uint32_t)((i - 1) >> 1) & 1u));      // the product before has ended
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) attn_prefill_q4_kernel(const __
               }
               l2.x *= corr; l2.y *= corr; m = mn; vf = vn;
             }
-            const float base = m == -INFINITY ? 0.f : -m;              // a row that has seen no key yet: all of its entries are masked
+            const float base = m == -INFINITY ? 0.f : (float)QP_SHIFT - m;              // a row that has seen no key yet: all of its entries are masked
             const float2 sc2 = make_float2(sc, sc), b2 = make_float2(base, base);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
