@@ -682,3 +682,46 @@ def test_engine_serves_from_the_4_bit_cache(cuda_device, name):
     assert res["q4"][1] * 2 * hd == res["bf16"][1] * (hd // 2 + 4)
     for a, b in zip(res["bf16"][0], res["q4"][0]):
         assert _cos(a, b) > 0.9, _cos(a, b)
+
+
+# ------------------------------------------------------------------------------------------------ a key that takes nearly all of the weight
+def _one_key_takes(share, kc, vc, pt, n, h, kvh, d, rows, seed=0):
+    """Query rows whose scores have a spread of about 1 over the first ``n`` rows of the table, but for the row at position 0: its key is
+    a constant that every query scores alike, so that it takes ``share`` of the weight, and its value row is zero.  What is left of
+    the result is the sum of the small weights.  Returns the queries and the constant."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    total = 0.4                                                   # sum(q) / sqrt(d)
+    q = 0.6 * torch.randn(rows, h, d, generator=g, device="cuda")
+    q += total / math.sqrt(d) - q.mean(-1, keepdim=True)
+    top = (math.log(share / (1 - share)) + math.log(n) + 0.5) / total
+    for c, low in ((kc, top), (vc, 0.0)):
+        flat = c.flatten(-2)
+        flat[int(pt[0]), :, 8 * d: 8 * d + 4] = torch.tensor([0.0, low], device="cuda").bfloat16().view(torch.uint8)
+    return q.reshape(rows, h * d), top
+
+
+@pytest.mark.parametrize("d, share, with_scratch", [(64, 0.97, False), (128, 0.97, True), (80, 0.999, False), (96, 0.999, True)])
+def test_prompt_with_one_key_that_takes_the_weight(cuda_device, d, share, with_scratch):
+    """The file's 4e-3 where the largest weight belongs to a value of zero, and what the rounding of the queries does to that weight.  The row
+    tiles leave no CTAs for a cluster (without a workspace a CTA takes all keys of a row), so that the small weights are held against the
+    large one.
+
+    The key of the large weight is ``top`` in all dims, and its score the sum of top q_i / sqrt(d), in which the q_i (rms 0.6) cancel but their
+    roundings do not: each q_i is off by at most half a step of fp16, 2^-11 |q_i|, in the mean square by at most 2^-11 |q_i| / sqrt(3).  The score is
+    off by top x 0.6 x 2^-11 / sqrt(3) in the root mean square over the heads, the weight and with it the sum of the weights by that fraction of
+    itself, and the result by the same."""
+    from realizar_b200 import ops
+    kvh, rows, n = 80, 8, 32768
+    per = n // 16
+    kc, vc = _cache(per + 2, kvh, d, seed=d)
+    pt = torch.randperm(per + 2, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d)).to(torch.int32)[:per].contiguous()
+    qkv = torch.zeros(rows, 3 * kvh * d, device="cuda")
+    qkv[:, : kvh * d], top = _one_key_takes(share, kc, vc, pt, n, kvh, kvh, d, rows)
+    out = torch.empty(rows, kvh * d, device="cuda")
+    scratch = ops.attn_prefill_scratch(rows, kvh, kvh, d, "cuda") if with_scratch else None
+    ops.attn_prefill(qkv, out, kc, vc, pt, rows, n - rows, kvh, kvh, d, scratch=scratch)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    ks, vs = _gather(kc, pt, d, False, n), _gather(vc, pt, d, True, n)
+    worst = max(_rel(out[r], _attend64(qkv[r, : kvh * d].double().view(kvh, d), ks[:, : n - rows + r + 1], vs[:, : n - rows + r + 1], 0)) for r in range(rows))
+    assert worst < 4e-3 + top * 0.6 * 2.0 ** -11 / math.sqrt(3), worst
