@@ -4,18 +4,21 @@
 //   s_t = q . k_t = scale_t (q . code_t) + min_t sum(q)        o = sum_t p_t v_t = sum_t (p_t scale'_t) code'_t + sum_t p_t min'_t
 //
 // Bound by the bytes of the cache as long as the arithmetic of the codes is cheap (96 sequences of 8192 tokens of 128 dims, 8 kv heads:
-// 130 us, 4.5 TB/s of the 6.6 that a copy reaches):
+// 129 us, 4.5 TB/s of the 6.6 that a copy reaches):
 //   * Keys: a masked word holds four codes as bytes, and the 8-bit integer product takes them as they are; q comes as three 8-bit
 //     digits of a 24-bit integer (its largest value in [2^22, 2^23) x 127 / 128), so the sums over the dims are exact; sum(q) is that of
 //     the integers.
 //   * Values: a nibble under the exponent of 1024 is the fp16 1024 + code (or 1024 + 16 code), which one subtraction (or
 //     multiply-add) turns into code - 8 exactly: 9 instructions to 8 codes.  The 8 goes into the minimum: without it, sum p scale code
 //     and sum p min cancel, over 131072 tokens to 1 / 900, and so do the digits of the result (2e-4 of it instead of 1e-6).
-//     p x scale' comes as its fp16 head and what that leaves, also fp16: 22 bits; its power of two follows the scales.
+//     p x scale' comes as its fp16 head and 2^11 times what that leaves, also fp16: 22 bits down to 2^-23 of the largest weight (and 1
+//     less to each factor of 2 below), because where the largest belongs to a value near zero the result is the sum of the small ones
+//     (32768 keys, one with 99.9% of the weight: 1.7e-3 off when the rest was not scaled).  Its power of two follows the scales.
 //   * Tokens (keys) and dims (values) are the 16 rows of the instruction and 4 heads its 8 columns, two digits or halves each, so
 //     the parts of a head's sum meet in one lane.  Up to 8 heads take two such tiles and share the other operand.
 //   * The pages lie in fragment order: a lane takes its operands with one wide shared-memory load and no shuffles.
-//   * The running maximum moves only when a score passes it by 2^8, so that the accumulators are rarely rescaled.
+//   * The running maximum moves only when a score passes it by 4, a factor of 2^4, so that the accumulators are rarely rescaled (2, 6 and 8
+//     take the same time).
 //
 // One CTA to an SM.  The main warps do nothing but pages: each has a ring of page pairs (K and V) that its lanes fill by 16-byte
 // asynchronous copies, and its pages follow one another across tiles.  (Bulk copies need a dozen instructions each, and a warp that
@@ -41,6 +44,10 @@ constexpr int QD_STAGES = 3, QD_MAX_SMS = 148, QD_HELPERS = 128;
 constexpr int QD_PAIR = 2 * Q4_PAGE;          // tokens of a pair of pages
 constexpr int QD_TILE_COST = 40;              // a second tile costs a CTA about as much time as this many pairs
 constexpr int QD_FLUSH = 8;                   // pairs whose values a warp adds up in the tensor core's accumulators, a power of two
+// p x scale' as fp16: p is at most 2^QD_LAG, by which a score may pass the running maximum before that moves, and scale' carries a power of
+// two that keeps it below QD_TOP, so that the product stays below 2^15 and what its fp16 head leaves, times QD_REST, below 2^14
+constexpr int QD_LAG = 4;
+constexpr float QD_TOP = 63.f / 64.f * (float)(1 << (15 - QD_LAG)), QD_REST = 2048.f;
 constexpr int QD_POSITIONS = 512;
 constexpr int QD_MAX_PARTS = 64;              // CTAs that share a tile: bounds the time of the last one, which joins their parts
 // query heads of a CTA (HN tiles of 4) and its main warps: with the four others 16 warps of 128 registers, or 12 of 168
@@ -96,11 +103,11 @@ __device__ __forceinline__ uint32_t digits(int q) {
   return (uint32_t)(d0 & 255) | (uint32_t)(d1 & 255) << 8 | (uint32_t)(d2 & 255) << 16;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// fp16 head of a value (low half) and of what the head leaves (high half)
-__device__ __forceinline__ uint32_t split_f16(float x) {
-  const __half h = __float2half_rn(x);
-  const __half2 r = __halves2half2(h, __float2half_rn(x - __half2float(h)));
-  return *(const uint32_t*)&r;
+// fp16 heads of two values (low halves) and QD_REST times what the heads leave (high halves)
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t (&w)[2]) {
+  const float2 h = __half22float2(__floats2half2_rn(x0, x1));
+  const __half2 a = __floats2half2_rn(x0, (x0 - h.x) * QD_REST), b = __floats2half2_rn(x1, (x1 - h.y) * QD_REST);
+  w[0] = *(const uint32_t*)&a; w[1] = *(const uint32_t*)&b;
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {       // of 16-bit values, row = lane / 4
   uint32_t y;
@@ -393,13 +400,13 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
                   }
                 }
             }
-            // ---- running maximum and scale: moved only where they fall behind by 2^8 and 2^2 ----
+            // ---- running maximum and scale: moved only where they fall behind (QD_LAG, QD_TOP) ----
             float mx[HN], top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-            bool behind = top * vf > 126.f;
+            bool behind = top * vf > QD_TOP;
 #pragma unroll
             for (int h = 0; h < HN; ++h) {
               mx[h] = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
-              behind |= mx[h] > m[h] + 8.f;
+              behind |= mx[h] > m[h] + (float)QD_LAG;
             }
             if (__any_sync(0xFFFFFFFFu, behind)) {
 #pragma unroll
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
 #pragma unroll
                 for (int h = 0; h < HN; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], k));
               }
-              const float vn = top * vf > 126.f ? pow2_for(top, 5) : vf, vr = vn / vf;
+              const float vn = top * vf > QD_TOP ? pow2_for(top, 13 - QD_LAG) : vf, vr = vn / vf;
               vf = vn;
 #pragma unroll
               for (int h = 0; h < HN; ++h) {
@@ -424,16 +431,14 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               uint32_t pb[HN][2];
+              const float f[2] = {sv[j][0] * vf, sv[j][1] * vf};
 #pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const float f = sv[j][n] * vf;
+              for (int h = 0; h < HN; ++h) {
+                const float e[2] = {ex2(sc[h][j][0] - m[h]), ex2(sc[h][j][1] - m[h])};
 #pragma unroll
-                for (int h = 0; h < HN; ++h) {
-                  const float e = ex2(sc[h][j][n] - m[h]);
-                  l[h] += e;
-                  om[h] = fmaf(e, mv[j][n], om[h]);
-                  pb[h][n] = transpose_8x8(split_f16(e * f));
-                }
+                for (int n = 0; n < 2; ++n) { l[h] += e[n]; om[h] = fmaf(e[n], mv[j][n], om[h]); }
+                split_f16(e[0] * f[0], e[1] * f[1], pb[h]);
+                pb[h][0] = transpose_8x8(pb[h][0]); pb[h][1] = transpose_8x8(pb[h][1]);
               }
               const uint8_t* vp = kp[j] + PB;
               uint32_t w0[NG], w1[NG];
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
           if (kb == k0 && it >= 2) ok = qd_wait(&sm.part_empty[buf], phase ^ 1u, ok) && ok;
           const float e0 = inverse_pow2(vf);
           for_part([&](int h, int n, int i, float v) {
-            const float add = (o[h][n][2 * i] + o[h][n][2 * i + 1]) * e0;
+            const float add = fmaf(o[h][n][2 * i + 1], 1.f / QD_REST, o[h][n][2 * i]) * e0;
             o[h][n][2 * i] = o[h][n][2 * i + 1] = 0.f;
             return kb == k0 ? add : v + add;
           });
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) { l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], k); om[h] += __shfl_xor_sync(0xFFFFFFFFu, om[h], k); }
         for_part([&](int h, int n, int i, float v) {
-          const float add = fmaf(o[h][n][2 * i] + o[h][n][2 * i + 1], e0, om[h]);
+          const float add = fmaf(fmaf(o[h][n][2 * i + 1], 1.f / QD_REST, o[h][n][2 * i]), e0, om[h]);
           return begun ? v + add : add;
         });
 #pragma unroll

@@ -700,6 +700,28 @@ def _one_key_takes(share, kc, vc, pt, n, h, kvh, d, rows, seed=0):
     return q.reshape(rows, h * d), top
 
 
+@pytest.mark.parametrize("h, kvh, d, share", [(8, 2, 64, 0.97), (14, 2, 128, 0.97), (8, 2, 80, 0.999), (6, 1, 96, 0.999)])
+def test_decode_with_one_key_that_takes_the_weight(cuda_device, h, kvh, d, share):
+    """The file's 1e-5 where the largest weight belongs to a value of zero, and what the rounding of the queries does to that weight.  A weight
+    times its value's scale is held to 22 bits of itself, so the small ones count as exactly as large ones.
+
+    The key of the large weight is ``top`` in all dims, and its score the sum of top q_i / sqrt(d), in which the q_i cancel but their roundings
+    to integers do not: half a step is at most 2^-23 x 128 / 127 of the row's largest |q|, in the root mean square 1 / sqrt(3) of that.  The
+    score is off by top x max|q| x 2^-23 x 1.008 / sqrt(3), and the result by that fraction of itself."""
+    from realizar_b200 import ops
+    B, n = 64 if kvh == 2 else 128, 32768
+    check = _decode(h, kvh, d, [n] * B, seed=d, no_append=True, shared_table=True, garbage=False)
+    qkv, out, kc, vc, pos, pt = check.keep[:6]
+    qkv[:, : h * d], top = _one_key_takes(share, kc, vc, pt, n, h, kvh, d, B)
+    ops.attn_decode_launch(check.params)
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    ks, vs = _gather(kc, pt, d, False, n), _gather(vc, pt, d, True, n)
+    room = top * float(qkv[:, : h * d].abs().max()) * 2.0 ** -23 * 1.008 / math.sqrt(3)
+    worst = max(_rel(out[b], _attend64(qkv[b, : h * d].double().view(h, d), ks, vs, 0)) for b in range(0, B, 5))
+    assert worst < 1e-5 + room, worst
+
+
 @pytest.mark.parametrize("d, share, with_scratch", [(64, 0.97, False), (128, 0.97, True), (80, 0.999, False), (96, 0.999, True)])
 def test_prompt_with_one_key_that_takes_the_weight(cuda_device, d, share, with_scratch):
     """The file's 4e-3 where the largest weight belongs to a value of zero, and what the rounding of the queries does to that weight.  The row
