@@ -31,11 +31,12 @@ struct AttnDecodeParams {
   float* partial;          // scratch [B, H, splits, head_dim + 2]
   int32_t* counters;       // scratch [B, n_kv_heads * head_groups], zero before first use
   int64_t ld_qkv, ld_out;
+  double eps;              // of the norms, as the caller has it: 4-bit caches normalise keys in 64 bits, as the append of a token batch does
   int32_t n_heads, n_kv_heads, head_dim, max_pages;
   int32_t rope_dim, rope_type, splits, batch;
   int32_t q_off, k_off, v_off;         // element offsets of the q / k / v sections in a qkv row
   int32_t pt_stride;                   // page_table elements between batch rows (0: every row shares one table)
-  float rope_theta, eps, scale;
+  float rope_theta, scale;
   int32_t no_append;                   // 1: the new rows are already in the cache (prefill), only attend
   int32_t window;                      // > 0: attend to positions (pos - window, pos] only
   int32_t rope_table_len;              // positions covered by rope_table
@@ -242,7 +243,7 @@ __device__ __forceinline__ void attn_decode_body(const AttnDecodeParams& p, cons
       float ss = 0.f;
       for (int j = lane; j < d; j += 32) ss += v[j] * v[j];
       ss = warp_sum(ss);
-      const float r = rsqrtf(ss / (float)d + p.eps);
+      const float r = rsqrtf(ss / (float)d + (float)p.eps);
       for (int j = lane; j < d; j += 32) v[j] = v[j] * r * w[j];
     }
     ATT_SYNC();

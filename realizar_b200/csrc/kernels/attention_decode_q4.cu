@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
       int isum = 0;
       if (g < gn) {
         load(row + p.q_off + (int64_t)(kvh * G + g0 + g) * D, half, p.rope_type, xa, xb);
-        norm_rope_f<D>(xa, xb, p.q_norm_w, p.eps, rope, cs, lane);
+        norm_rope_f<D>(xa, xb, p.q_norm_w, (float)p.eps, rope, cs, lane);
         float top = 0.f;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(32 * qd_warps(HN) + QD_HELPERS, 1) attn_decode
     // the new token's rows, behind the fragments: only the warp that has its pair waits for them
     if (own) {
       const bool v = own_v;
-      if (!v) norm_rope_d<D>(ra, rb, p.q_norm_w ? p.k_norm_w : nullptr, (double)p.eps, rope, cs, lane);
+      if (!v) norm_rope_d<D>(ra, rb, p.q_norm_w ? p.k_norm_w : nullptr, p.eps, rope, cs, lane);
       const uint32_t meta = q4_quantise<D>(ra, rb, v ? 0 : half, v ? 0 : p.rope_type, lane, sm.codes[buf][v]);
       __syncwarp();
       if (lane == 0) sm.meta[buf][v] = meta;

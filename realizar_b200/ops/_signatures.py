@@ -51,10 +51,10 @@ class CandExchange(Structure):
 class AttnDecodeParams(Structure):
     _fields_ = [("qkv", c_void_p), ("out", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("positions", c_void_p),
                 ("page_table", c_void_p), ("q_norm_w", c_void_p), ("k_norm_w", c_void_p), ("partial", c_void_p),
-                ("counters", c_void_p), ("ld_qkv", c_int64), ("ld_out", c_int64), ("n_heads", c_int32), ("n_kv_heads", c_int32),
+                ("counters", c_void_p), ("ld_qkv", c_int64), ("ld_out", c_int64), ("eps", c_double), ("n_heads", c_int32), ("n_kv_heads", c_int32),
                 ("head_dim", c_int32), ("max_pages", c_int32), ("rope_dim", c_int32), ("rope_type", c_int32), ("splits", c_int32),
                 ("batch", c_int32), ("q_off", c_int32), ("k_off", c_int32), ("v_off", c_int32), ("pt_stride", c_int32),
-                ("rope_theta", c_float), ("eps", c_float), ("scale", c_float), ("no_append", c_int32), ("window", c_int32),
+                ("rope_theta", c_float), ("scale", c_float), ("no_append", c_int32), ("window", c_int32),
                 ("rope_table_len", c_int32), ("rope_table", c_void_p), ("kv_q8", c_int32), ("num_pages", c_int32)]
 
 

@@ -747,3 +747,32 @@ def test_prompt_with_one_key_that_takes_the_weight(cuda_device, d, share, with_s
     ks, vs = _gather(kc, pt, d, False, n), _gather(vc, pt, d, True, n)
     worst = max(_rel(out[r], _attend64(qkv[r, : kvh * d].double().view(kvh, d), ks[:, : n - rows + r + 1], vs[:, : n - rows + r + 1], 0)) for r in range(rows))
     assert worst < 4e-3 + top * 0.6 * 2.0 ** -11 / math.sqrt(3), worst
+
+
+def test_append_and_decode_take_eps_alike(cuda_device):
+    """Keys so small that eps decides their norm, of them those that the definition caches differently with eps and with eps rounded to 32
+    bits (some in a million): both kernels write what the definition says."""
+    from realizar_b200 import ops
+    d, eps = 64, 1e-5
+    ones = torch.ones(d, device="cuda")
+    g, found = torch.Generator(device="cuda").manual_seed(1), []
+    for _ in range(8):
+        x = 1e-3 * torch.randn(1 << 20, 1, d, generator=g, device="cuda")
+        a, b = (_quant64(_head64(x, ones, None, None, 0, 0, eps=e)) for e in (eps, float(np.float32(eps))))
+        found.append(x[(a != b).any(-1)[:, 0], 0])
+    k = torch.cat(found)
+    n = k.shape[0]
+    assert n >= 8
+    want = _quant64(_head64(k[:, None], ones, None, None, 0, 0, eps=eps))
+    qkv = torch.cat([torch.randn(n, d, device="cuda"), k, k], -1).contiguous()
+    pos, pages = torch.zeros(n, device="cuda", dtype=torch.int32), torch.arange(n, device="cuda", dtype=torch.int32)
+    kv = [ops.kv_cache_alloc(1, n, 1, d, "cuda", "q4")[:, 0] for _ in range(2)]
+    ops.qk_norm_rope_append(qkv, pos, pages, kv[0][0], kv[0][1], 1, 1, d, q_out=torch.empty(n, d, device="cuda"), q_norm_w=ones, k_norm_w=ones, eps=eps)
+    partial, counters = ops.attn_decode_scratch(n, 1, 1, d, "cuda", kv_dtype="q4")
+    ops.attn_decode_launch(ops.build_attn_decode_params(qkv, torch.empty(n, d, device="cuda"), kv[1][0], kv[1][1], pos, pages[:, None], partial, counters, 1, 1, d, 1, n,
+                                                        0, 0, 1e4, 0, d, 2 * d, ones, ones, eps))
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+    for c in kv:
+        assert torch.equal(ops.kv_pages_to_float(c[0], d, False)[:, 0, 0], want[:, 0])
+    assert torch.equal(kv[0], kv[1])
