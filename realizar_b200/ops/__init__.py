@@ -271,20 +271,8 @@ def build_attn_decode_params(qkv, out, k_cache, v_cache, positions, page_table, 
                              eps=1e-6, ld_qkv=None, ld_out=None, shared_table=False, no_append=False, window=0, rope_table=None) -> S.AttnDecodeParams:
     fmt = kv_format(k_cache, head_dim)
     if fmt == KV_Q4:
-        _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, out, positions, page_table, partial, counters)
-        if batch < 1 or qkv.shape[0] < batch or out.shape[0] < batch or positions.numel() < batch or counters.numel() < batch * n_heads:
-            raise ValueError(f"batch {batch}: qkv, out, positions or counters hold fewer rows")
-        if not shared_table and page_table.dim() > 1 and page_table.shape[0] < batch:
-            raise ValueError(f"page_table has {page_table.shape[0]} rows for a batch of {batch}")
-        if qkv.dtype != torch.float32 or out.dtype != torch.float32 or qkv.stride(-1) != 1 or out.stride(-1) != 1 or page_table.stride(-1) != 1:
-            raise ValueError("qkv and out must be float32 with contiguous rows, page_table rows contiguous")
-        if positions.dtype != torch.int32 or page_table.dtype != torch.int32 or not positions.is_contiguous():
-            raise ValueError("positions and page_table must be contiguous int32")
-        if (q_norm_w is None) != (k_norm_w is None):
-            raise ValueError("q_norm_w and k_norm_w come together")
-        _check_current_device(k_cache)
-        if partial.numel() < int(lib().rlz_attn_q4_partial_floats(head_dim)):
-            raise ValueError("partial is too small for a 4-bit cache: take it from attn_decode_scratch(..., kv_dtype='q4')")
+        _check_decode_q4(qkv, out, k_cache, v_cache, positions, page_table, partial, counters, n_heads, n_kv_heads, head_dim, batch, rope_dim, q_off, k_off, v_off,
+                         q_norm_w, k_norm_w, ld_qkv, ld_out, shared_table, no_append, window or 0, rope_table)
     p = S.AttnDecodeParams()
     p.qkv, p.out, p.k_cache, p.v_cache = qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     p.positions, p.page_table = positions.data_ptr(), page_table.data_ptr()
@@ -306,6 +294,48 @@ def build_attn_decode_params(qkv, out, k_cache, v_cache, positions, page_table, 
             raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim / 2, 2] (cos, sin) tensor")
         p.rope_table, p.rope_table_len = rope_table.data_ptr(), rope_table.shape[0]
     return p
+
+
+def _check_decode_q4(qkv, out, k_cache, v_cache, positions, page_table, partial, counters, n_heads, n_kv_heads, head_dim, batch, rope_dim, q_off, k_off, v_off,
+                     q_norm_w, k_norm_w, ld_qkv, ld_out, shared_table, no_append, window, rope_table) -> None:
+    width = n_heads * head_dim
+    _check_q4_caches(k_cache, v_cache, n_kv_heads, head_dim, qkv, out, positions, page_table, partial, counters, q_norm_w, k_norm_w, rope_table)
+    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads:
+        raise ValueError(f"{n_heads} query heads do not divide over {n_kv_heads} kv heads")
+    if batch < 1 or qkv.shape[0] < batch or out.shape[0] < batch or positions.numel() < batch or counters.numel() < batch * n_heads:
+        raise ValueError(f"batch {batch}: qkv, out, positions or counters hold fewer rows")
+    if page_table.dim() not in (1, 2) or (not shared_table and page_table.dim() == 1 and batch > 1) or (not shared_table and page_table.dim() == 2 and page_table.shape[0] < batch):
+        raise ValueError(f"page_table is [{batch}, pages] for a batch of {batch}, or with shared_table one row, got {tuple(page_table.shape)}")
+    if qkv.dtype != torch.float32 or out.dtype != torch.float32 or qkv.stride(-1) != 1 or out.stride(-1) != 1 or page_table.stride(-1) != 1:
+        raise ValueError("qkv and out must be float32 with contiguous rows, page_table rows contiguous")
+    sections = [(q_off, width)] if no_append else [(q_off, width), (k_off, n_kv_heads * head_dim), (v_off, n_kv_heads * head_dim)]
+    if qkv.dim() != 2 or any(at < 0 or at + n > qkv.shape[1] for at, n in sections) or (batch > 1 and ld_qkv not in (None, qkv.stride(0))):
+        raise ValueError(f"qkv must be float32 [rows, columns] with the heads' sections inside a row and ld_qkv its row stride, got {tuple(qkv.shape)}")
+    if out.dim() != 2 or out.shape[1] < width or (batch > 1 and ld_out not in (None, out.stride(0))):
+        raise ValueError(f"out must be float32 [rows, >= {width}] with ld_out its row stride, got {tuple(out.shape)}")
+    if batch > 1 and out.stride(0) < width:
+        raise ValueError("rows of out overlap")
+    if positions.dtype != torch.int32 or page_table.dtype != torch.int32 or not positions.is_contiguous():
+        raise ValueError("positions and page_table must be contiguous int32")
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise ValueError("q_norm_w and k_norm_w come together")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != head_dim or not w.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous float32 of {head_dim} entries")
+    if rope_dim < 0 or rope_dim > head_dim or rope_dim % 2:
+        raise ValueError(f"rope_dim must be even and at most {head_dim}, got {rope_dim}")
+    if rope_table is not None and (rope_table.dtype != torch.float32 or rope_table.dim() != 3 or tuple(rope_table.shape[1:]) != (rope_dim // 2, 2)
+                                   or not rope_table.is_contiguous()):
+        raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim / 2, 2] (cos, sin) tensor")
+    if window < 0:
+        raise ValueError(f"window must be 0 (none) or more, got {window}")
+    if partial.dtype != torch.float32 or not partial.is_contiguous() or partial.data_ptr() % 16:
+        raise ValueError("partial must be a contiguous float32 tensor from attn_decode_scratch")
+    if counters.dtype != torch.int32 or not counters.is_contiguous():
+        raise ValueError("counters must be a contiguous int32 tensor from attn_decode_scratch")
+    _check_current_device(k_cache)
+    if partial.numel() < int(lib().rlz_attn_q4_partial_floats(head_dim)):
+        raise ValueError("partial is too small for a 4-bit cache: take it from attn_decode_scratch(..., kv_dtype='q4')")
 
 
 def make_rope_table(max_positions: int, rope_dim: int, theta: float, device) -> torch.Tensor:

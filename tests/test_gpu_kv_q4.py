@@ -776,3 +776,17 @@ def test_append_and_decode_take_eps_alike(cuda_device):
     for c in kv:
         assert torch.equal(ops.kv_pages_to_float(c[0], d, False)[:, 0, 0], want[:, 0])
     assert torch.equal(kv[0], kv[1])
+
+
+@pytest.mark.parametrize("name", ["q_norm_w", "k_norm_w", "rope_table", "partial", "counters"])
+def test_decode_refuses_tensors_of_another_device(cuda_device, name):
+    from realizar_b200 import ops
+    kv = ops.kv_cache_alloc(1, 3, 2, 64, "cuda", "q4")
+    z = lambda *s: torch.zeros(*s, device="cuda")                                                           # noqa: E731
+    partial, counters = ops.attn_decode_scratch(2, 4, 1, 64, "cuda", kv_dtype="q4")
+    a = dict(qkv=z(2, 512), out=z(2, 256), k_cache=kv[0, 0], v_cache=kv[1, 0], positions=z(2).int(), page_table=z(2, 2).int(), partial=partial, counters=counters, n_heads=4,
+             n_kv_heads=2, head_dim=64, splits=1, batch=2, rope_dim=64, rope_type=0, rope_theta=1e4, q_off=0, k_off=256, v_off=384, q_norm_w=z(64), k_norm_w=z(64),
+             rope_table=z(5, 32, 2))
+    ops.build_attn_decode_params(**a)
+    with pytest.raises(ValueError, match="one device"):
+        ops.build_attn_decode_params(**{**a, name: a[name].cpu()})

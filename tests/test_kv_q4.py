@@ -82,6 +82,31 @@ def test_decode_refuses(change, word):
 
 
 @pytest.mark.parametrize("change, word", [
+    (dict(qkv=torch.zeros(2, 511)), "qkv"), (dict(qkv=torch.zeros(2, 384)), "qkv"), (dict(q_off=-64), "qkv"), (dict(q_off=320), "qkv"), (dict(k_off=448), "qkv"),
+    (dict(v_off=448), "qkv"), (dict(v_off=-1), "qkv"), (dict(q_off=320, no_append=True), "qkv"), (dict(qkv=torch.zeros(1024)), "qkv"), (dict(ld_qkv=256), "qkv"),
+    (dict(out=torch.zeros(2, 255)), "out"), (dict(out=torch.zeros(512)), "out"), (dict(ld_out=512), "out"), (dict(out=torch.zeros(1, 256).expand(2, 256)), "overlap"),
+    (dict(out=torch.zeros(512).as_strided((2, 256), (192, 1))), "overlap"),
+    (dict(page_table=torch.zeros(4, dtype=torch.int32)), "page_table"), (dict(page_table=torch.zeros(2, 2, 2, dtype=torch.int32)), "page_table"),
+    (dict(q_norm_w=torch.ones(64), k_norm_w=torch.ones(32)), "norm weights"), (dict(q_norm_w=torch.ones(64).half(), k_norm_w=torch.ones(64)), "norm weights"),
+    (dict(q_norm_w=torch.ones(128)[::2], k_norm_w=torch.ones(64)), "norm weights"), (dict(rope_dim=64, rope_table=torch.zeros(5, 16, 2)), "rope_table"),
+    (dict(rope_dim=64, rope_table=torch.zeros(5, 32, 2).half()), "rope_table"), (dict(rope_dim=33), "rope_dim"), (dict(rope_dim=66), "rope_dim"), (dict(window=-1), "window"),
+    (dict(partial=torch.zeros(10).half()), "partial"), (dict(partial=torch.zeros(20)[::2]), "partial"), (dict(counters=torch.zeros(8)), "counters"),
+    (dict(counters=torch.zeros(16, dtype=torch.int32)[::2]), "counters"), (dict(n_heads=3), "divide"), (dict(n_heads=0), "divide")])
+def test_decode_refuses_what_append_and_prompt_refuse(change, word):
+    """What would be read or written out of range, or read as another type."""
+    with pytest.raises(ValueError, match=word):
+        ops.build_attn_decode_params(**{**_decode_args(), **change})
+
+
+@pytest.mark.parametrize("change", [dict(no_append=True, k_off=0, v_off=0, qkv=torch.zeros(2, 256)), dict(page_table=torch.zeros(4, dtype=torch.int32), shared_table=True),
+                                    dict(qkv=torch.zeros(2, 600)[:, 8:], out=torch.zeros(2, 300)[:, 4:]), dict(batch=1, ld_qkv=7, ld_out=7)])
+def test_decode_takes_calls_that_are_in_order(change):
+    """(up to the check of the device, which is the last but one)"""
+    with pytest.raises(ValueError, match="current CUDA device"):
+        ops.build_attn_decode_params(**{**_decode_args(), **change})
+
+
+@pytest.mark.parametrize("change, word", [
     (dict(n_tokens=0), "n_tokens"), (dict(n_tokens=5), "qkv"), (dict(pos0=29), "not covered"), (dict(pos0=-1), "not covered"), (dict(out=torch.zeros(4, 100)), "out"),
     (dict(out=torch.zeros(4, 256).half()), "out"), (dict(page_table=torch.zeros(2, 2, dtype=torch.int32)), "page_table"), (dict(window=-1), "covered"),
     (dict(scratch=torch.zeros(4, dtype=torch.int32)), "scratch"), (dict(pos0_dev=torch.zeros(1)), "pos0_dev"), ({}, "current CUDA device")])
