@@ -89,6 +89,12 @@ class BatchedForward:
         self._chunk_seen: dict = {}
         self.chunk_graphs = os.environ.get("RLZ_PREFILL_GRAPHS", "1") != "0"
 
+    def clear_workspace(self) -> None:
+        """Arrival counters of the prompt attention back to zero: a launch whose bounded wait ran out (a status word tells) leaves some of
+        them raised, and a later launch would join parts that are not written yet."""
+        if self.prefill_scratch is not None:
+            self.prefill_scratch.zero_()
+
     def forward_chunk(self, T: int, page_table_row: torch.Tensor, pos0: int) -> torch.Tensor:
         """Rows 0..T-1 are positions ``pos0 .. pos0+T-1`` of the sequence whose page-table row is given (``tokens`` /
         ``positions`` / ``page_rows`` must be set).  The first pass of a given T runs launch by launch; full-size chunks (and

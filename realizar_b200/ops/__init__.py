@@ -429,7 +429,9 @@ def attn_prefill_error(clear: bool = True) -> int:
 
 
 def attn_prefill_scratch(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
-    """Workspace with which ``attn_prefill`` divides the keys of a 4-bit cache evenly over the SMs: the same size for any number of rows.  One to a stream; it keeps nothing from one call for the next."""
+    """Workspace with which ``attn_prefill`` divides the keys of a 4-bit cache evenly over the SMs: the same size for any number of rows.  One to a stream.
+    Its first words are arrival counters, zero between launches; a launch whose bounded wait ran out (status 3115) may leave some raised:
+    ``zero_()`` it before the next one, as the engine does."""
     return torch.zeros(int(lib().rlz_attn_prefill_q4_scratch_floats(int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim))), device=device, dtype=torch.float32)
 
 

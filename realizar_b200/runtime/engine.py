@@ -332,12 +332,17 @@ class DecodeEngine:
         if not code and self.comm is not None and hasattr(self.comm, "check_status"):
             code = self.comm.check_status()
         if code:
+            self._clear_workspaces()
             raise ops.KernelError(f"a device-side check failed with status {code}: a bounded wait expired or an index left its range; "
                                   "results since the last check are not valid")
         if self.guards is not None:
             bad = self.guards.check()
             if bad:
                 raise ops.KernelError("guard bands overwritten next to: " + "; ".join(bad))
+
+    def _clear_workspaces(self) -> None:
+        if self._batched is not None:
+            self._batched.clear_workspace()
 
     def profile_step(self, batch: int = 1, steps: int = 4) -> dict:
         """Per-operation timing of the decode step at this batch: the plan is run launch by launch (no graph) with every launch
@@ -803,12 +808,13 @@ class DecodeEngine:
     def reset(self) -> None:
         """Back to the post-load state after a failed step: probe the device (a lost context makes the synchronise raise, and
         then nothing in this process can use the GPU again), close every open sequence, clear the device-side status words and
-        mark every row idle.  Weights, captured graphs and launch plans stay: they do not depend on sequence state."""
+        the workspaces' arrival counters, and mark every row idle.  Weights, captured graphs and launch plans stay: they do not depend on sequence state."""
         torch.cuda.synchronize(self.device)                  # raises when the context is poisoned
         for slot, s in enumerate(self.slots):
             if s.active:
                 self.close_slot(slot)
         ops.device_error(clear=True)
+        self._clear_workspaces()
         if self.comm is not None and hasattr(self.comm, "check_status"):
             self.comm.check_status()
         self._h_tok_pos[1].fill_(-1)

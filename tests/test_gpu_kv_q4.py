@@ -790,3 +790,33 @@ def test_decode_refuses_tensors_of_another_device(cuda_device, name):
     ops.build_attn_decode_params(**a)
     with pytest.raises(ValueError, match="one device"):
         ops.build_attn_decode_params(**{**a, name: a[name].cpu()})
+
+
+@pytest.mark.parametrize("how", ["reset", "status"])
+def test_engine_leaves_no_arrival_counter_raised(cuda_device, how, monkeypatch):
+    """After a failed launch (stood in for by a counter that is not zero, and by the status that is read) the engine's next prompt starts
+    from counters of zero."""
+    from test_gpu_engine import _kq_llama
+    from realizar_b200 import ops
+    from realizar_b200.models.weights import synthetic_weights
+    from realizar_b200.runtime.engine import DecodeEngine, EngineConfig
+    cfg = _kq_llama()
+    eng = DecodeEngine(synthetic_weights(cfg, seed=21, std=0.05), EngineConfig(max_batch=2, max_seq_len=160, greedy_only=True, kv_dtype="q4", prefill_chunk=64))
+    toks = [int(t) for t in np.random.default_rng(8).integers(0, cfg.vocab_size, 90)]
+    eng.open_slot(0, 128)
+    first = eng.prefill(0, toks)
+    counters = eng.batched().prefill_scratch.view(torch.int32)[:640]
+    assert not bool(counters.any())
+    counters[::3] = 1
+    if how == "reset":
+        eng.reset()
+    else:
+        with monkeypatch.context() as m:
+            m.setattr(ops, "device_error", lambda clear=True: 3115)
+            with pytest.raises(ops.KernelError, match="3115"):
+                eng.check_health()
+        eng.close_slot(0)
+    assert not bool(counters.any())
+    eng.open_slot(0, 128)
+    assert eng.prefill(0, toks) == first
+    eng.close()
