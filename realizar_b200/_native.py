@@ -79,9 +79,10 @@ def cuda_lib() -> ctypes.CDLL:
                 if built is None:
                     raise RuntimeError("librlz_cuda.so is missing and nvcc was not found to build it")
                 path = built
-            _cuda = ctypes.CDLL(str(path))
+            lib = ctypes.CDLL(str(path))
             from .ops import _signatures
-            _signatures.declare(_cuda)
+            _signatures.declare(lib)
+            _cuda = lib                                  # last: whoever sees it takes it without the lock
         return _cuda
 
 

@@ -145,3 +145,33 @@ def test_append_parameters_are_packed_as_the_structure_lies():
     values = [11 * (i + 1) for i in range(11)] + [1e-6] + list(range(1, 9)) + [5e5, 0]
     assert bytes(S.QkAppendParams(*values)) == S.pack_qk_append(*values)
     assert len(S.pack_qk_append(*values)) == ctypes.sizeof(S.QkAppendParams)
+
+
+def test_library_handle_is_published_with_its_signatures(monkeypatch):
+    """Another thread that asks for the kernel library while its signatures are being declared waits for them: calls through an undeclared
+    function would pass pointers as 32-bit integers."""
+    import threading
+    from realizar_b200 import _native
+    from realizar_b200.ops import _signatures
+    if not _native.cuda_lib_path().exists():
+        pytest.skip("kernel library not built")
+    declared, entered, seen = threading.Event(), threading.Event(), []
+    declare = _signatures.declare
+
+    def slow(lib):
+        entered.set()
+        second.join(0.3)                                             # time enough to take the handle, if it is there to be taken
+        declare(lib)
+        declared.set()
+
+    def other():
+        entered.wait(10)
+        _native.cuda_lib()
+        seen.append(declared.is_set())
+    monkeypatch.setattr(_native, "_cuda", None)
+    monkeypatch.setattr(_signatures, "declare", slow)
+    second = threading.Thread(target=other)
+    second.start()
+    _native.cuda_lib()
+    second.join(10)
+    assert seen == [True]
