@@ -820,3 +820,143 @@ def test_engine_leaves_no_arrival_counter_raised(cuda_device, how, monkeypatch):
     eng.open_slot(0, 128)
     assert eng.prefill(0, toks) == first
     eng.close()
+
+
+# ------------------------------------------------------------------------------------------------ prompt attention divided evenly over the SMs
+class _Divided:
+    """A prompt chunk for which the launcher divides the key tiles evenly (few row tiles over many keys: a cluster of eight CTAs to each would
+    leave most SMs idle), with a workspace of its own.  ``used`` tells whether parts went through it since the last ``fresh``."""
+
+    def __init__(self, h, kvh, d, rows, pos0, seed=0, window=0, dtype=torch.bfloat16, scales=None):
+        from realizar_b200 import ops
+        self.ops, self.shape, self.rows, self.pos0, self.window = ops, (h, kvh, d), rows, pos0, window
+        g, total = torch.Generator(device="cuda").manual_seed(seed + d), pos0 + rows
+        per = -(-total // 16)
+        self.kc, self.vc = _cache(per + 2, kvh, d, seed=seed)
+        self.pt = torch.randperm(per + 2, generator=g, device="cuda").to(torch.int32)[:per].contiguous()
+        if scales is not None:
+            sc = scales(torch.arange(16 * per, device="cuda").float())
+            for k in range(kvh):
+                self.vc.flatten(-2)[self.pt.long(), k, 8 * d:] = torch.stack([sc, -7.5 * sc], -1).bfloat16().view(torch.uint8).view(-1, 64)
+        self.qkv = torch.randn(rows, (h + 2 * kvh) * d, generator=g, device="cuda")
+        self.out = torch.full((rows, h * d), 9.0, device="cuda", dtype=dtype)
+        self.scratch = ops.attn_prefill_scratch(rows, h, kvh, d, "cuda")
+        self.fresh()
+
+    def fresh(self):
+        self.scratch[640:] = 7.0
+        self.out.fill_(9.0)
+
+    def used(self):
+        assert not bool(self.scratch[:640].any())                  # the arrival counters are zero again
+        return bool((self.scratch[640:] != 7.0).any())
+
+    def launch(self, **kw):
+        h, kvh, d = self.shape
+        a = dict(window=self.window, scratch=self.scratch, pos0=self.pos0)
+        a.update(kw)
+        self.ops.attn_prefill(self.qkv, a.pop("out", self.out), self.kc, self.vc, self.pt, self.rows, a.pop("pos0"), h, kvh, d, **a)
+
+    def check(self, out=None, pos0=None):
+        torch.cuda.synchronize()
+        assert self.ops.device_error() == 0
+        h, kvh, d = self.shape
+        pos0 = self.pos0 if pos0 is None else pos0
+        n, out = pos0 + self.rows, self.out if out is None else out
+        ks, vs = _gather(self.kc, self.pt, d, False, n), _gather(self.vc, self.pt, d, True, n)
+        worst = 0.0
+        for r in range(self.rows):
+            p1 = pos0 + r + 1
+            want = _attend64(self.qkv[r, : h * d].double().view(h, d), ks[:, :p1], vs[:, :p1], max(0, p1 - self.window) if self.window else 0)
+            worst = max(worst, _rel(out[r], want))
+        assert worst < 3 * 4e-3, worst                              # (of a single row, as in _prompt)
+
+
+@pytest.mark.parametrize("h, kvh, d, rows, pos0, kw", [
+    (4, 2, 128, 40, 9000, {}), (2, 2, 96, 40, 9000, {}), (14, 2, 64, 40, 9001, {}), (3, 3, 80, 70, 12345, {}), (6, 1, 96, 100, 20000, dict(window=9000)),
+    (8, 2, 128, 40, 9000, dict(dtype=torch.float32)), (2, 2, 96, 200, 7777, {})])
+@pytest.mark.parametrize("dev_pos", [False, True])
+def test_prompt_of_few_rows_divided_evenly(cuda_device, h, kvh, d, rows, pos0, kw, dev_pos):
+    c = _Divided(h, kvh, d, rows, pos0, **kw)
+    pd = torch.tensor([pos0], device="cuda", dtype=torch.int32) if dev_pos else None
+    for _ in range(2):
+        c.launch(**(dict(pos0=0, pos0_dev=pd) if dev_pos else {}))
+    c.check()
+    assert c.used()
+    first = c.out.clone()
+    c.fresh()
+    c.launch(**(dict(pos0=0, pos0_dev=pd) if dev_pos else {}))
+    assert torch.equal(c.out, first) and c.used()                  # the same bits from any workspace
+
+
+@pytest.mark.parametrize("kind", ["constant first", "growing", "shrinking"])
+def test_prompt_divided_evenly_with_wide_ranges_of_scales(cuda_device, kind):
+    """The parts of a row come with powers of two of their own."""
+    c = _Divided(4, 2, 64, 40, 9000, dtype=torch.float32, scales={"constant first": lambda i: torch.where(i < 4000, 0.0, 1e-6), "growing": lambda i: torch.exp2(i / 400 - 20),
+                                                                  "shrinking": lambda i: torch.exp2(5 - i / 400)}[kind])
+    c.launch()
+    c.check()
+    assert c.used()
+
+
+def test_prompt_divided_evenly_only_with_a_workspace_that_is_large_enough(cuda_device):
+    from realizar_b200 import ops
+    c = _Divided(4, 2, 128, 40, 9000)
+    c.launch()
+    c.check()
+    assert c.used()
+    small = torch.zeros(c.scratch.numel() - 4, device="cuda")
+    for scratch in (None, small, ops.attn_prefill_scratch(40, 4, 2, 64, "cuda")):
+        out = torch.full_like(c.out, 9.0)
+        c.launch(scratch=scratch, out=out)
+        c.check(out)
+        assert scratch is None or not bool(scratch.any())
+    larger = torch.zeros(c.scratch.numel() + 1000, device="cuda")
+    out = torch.full_like(c.out, 9.0)
+    c.launch(scratch=larger, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, c.out) and bool(larger[640:].any()) and not bool(larger[:640].any()) and not bool(larger[c.scratch.numel():].any())
+
+
+def test_prompts_divided_evenly_on_two_streams_with_their_own_workspaces(cuda_device):
+    jobs = [_Divided(4, 2, 128, 40, 9000, seed=1), _Divided(14, 2, 64, 70, 12000, seed=2)]
+    want = []
+    for c in jobs:
+        c.launch()
+        c.check()
+        assert c.used()
+        want.append(c.out.clone())
+        c.fresh()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(20):
+        for c, s in zip(jobs, streams):
+            with torch.cuda.stream(s):
+                c.launch()
+    torch.cuda.synchronize()
+    for c, w in zip(jobs, want):
+        assert torch.equal(c.out, w) and c.used()
+
+
+def test_captured_prompts_divided_evenly_share_a_workspace(cuda_device):
+    """Two graphs with one workspace, replayed in turn at several positions; one of the positions leaves hardly any keys to divide."""
+    a, b = _Divided(4, 2, 96, 40, 9000, seed=1), _Divided(8, 2, 96, 40, 11000, seed=2)
+    b.scratch = a.scratch
+    pos = [torch.tensor([c.pos0], device="cuda", dtype=torch.int32) for c in (a, b)]
+    graphs = []
+    for c, p in zip((a, b), pos):
+        c.launch(pos0=0, pos0_dev=p)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            c.launch(pos0=0, pos0_dev=p)
+    for back in (0, 1234, 8990):
+        for c, p in zip((a, b), pos):
+            p.fill_(c.pos0 - back)
+            c.fresh()
+        for _ in range(3):
+            for g in graphs:
+                g.replay()
+        for c in (a, b):
+            c.check(pos0=c.pos0 - back)
+        assert a.used()
