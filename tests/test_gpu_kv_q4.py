@@ -960,3 +960,43 @@ def test_captured_prompts_divided_evenly_share_a_workspace(cuda_device):
         for c in (a, b):
             c.check(pos0=c.pos0 - back)
         assert a.used()
+
+
+# ------------------------------------------------------------------------------------------------ engine, decode steps of a batch
+@pytest.mark.parametrize("name", ["llama", "phi2"])
+def test_engine_batch_step_over_the_4_bit_cache(cuda_device, name):
+    """Several sequences of unequal length with an idle slot between them, in one decode step: on the tensor-core path (append, then attention
+    without append over per-row page tables) and on the fused one, both against the same sequences fed one at a time.
+
+    The prompts' rows are the same bytes.  The tensor-core path takes bf16 activations and the other int8 ones, some 1% apart, which moves
+    one code in thirty of the few new rows by a step of 0.31 sigma: 0.31 x sqrt(0.03) = 5% of such a row, 1 - 0.05^2 / 2 = 0.999 of its cosine.
+    Two layers and the activations themselves stay above the 0.99 that the engine's other tests hold the two paths to."""
+    from test_gpu_engine import _cos, _kq_llama, small_phi2
+    from realizar_b200.models.weights import synthetic_weights
+    from realizar_b200.runtime.engine import DecodeEngine, EngineConfig
+    cfg = _kq_llama() if name == "llama" else small_phi2()
+    w = synthetic_weights(cfg, seed=21, std=0.05, **({} if name == "llama" else {"scheme": "Q4_K_M"}))
+    rng = np.random.default_rng(3)
+    lens = {0: 40, 1: 17, 3: 90, 4: 3, 5: 64}                     # slot 2 stays idle
+    prompts = {s: [int(t) for t in rng.integers(0, cfg.vocab_size, n)] for s, n in lens.items()}
+    steps = [{s: int(rng.integers(0, cfg.vocab_size)) for s in lens} for _ in range(3)]
+    res = {}
+    for how, min_batch in (("tensor core", 4), ("fused", 64), ("alone", 64)):
+        eng = DecodeEngine(w, EngineConfig(max_batch=6, max_seq_len=128, greedy_only=True, kv_dtype="q4", prefill_chunk=64, gemm_decode_min_batch=min_batch))
+        assert eng._use_batched_step(eng.bucket_for(6)) == (how == "tensor core")
+        for s, p in prompts.items():
+            eng.open_slot(s, 128)
+            eng.prefill(s, p)
+        res[how] = []
+        for feed in steps:
+            row = {}
+            for part in [{s: feed[s]} for s in lens] if how == "alone" else [feed]:
+                eng.feed(part)
+                row.update({s: eng.logits_of_last_step(s).float().cpu().numpy() for s in part})
+            res[how].append(row)
+        eng.check_health()
+        eng.close()
+    for how in ("tensor core", "fused"):
+        for a, b in zip(res[how], res["alone"]):
+            for s in lens:
+                assert _cos(a[s], b[s]) > 0.99, (how, s)
