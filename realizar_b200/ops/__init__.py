@@ -306,6 +306,8 @@ def _check_decode_q4(qkv, out, k_cache, v_cache, positions, page_table, partial,
         raise ValueError(f"batch {batch}: qkv, out, positions or counters hold fewer rows")
     if page_table.dim() not in (1, 2) or (not shared_table and page_table.dim() == 1 and batch > 1) or (not shared_table and page_table.dim() == 2 and page_table.shape[0] < batch):
         raise ValueError(f"page_table is [{batch}, pages] for a batch of {batch}, or with shared_table one row, got {tuple(page_table.shape)}")
+    if shared_table and batch > 1 and not no_append:
+        raise ValueError("rows of one sequence (shared_table) need no_append: they would read each other's new rows while those are written")
     if qkv.dtype != torch.float32 or out.dtype != torch.float32 or qkv.stride(-1) != 1 or out.stride(-1) != 1 or page_table.stride(-1) != 1:
         raise ValueError("qkv and out must be float32 with contiguous rows, page_table rows contiguous")
     sections = [(q_off, width)] if no_append else [(q_off, width), (k_off, n_kv_heads * head_dim), (v_off, n_kv_heads * head_dim)]

@@ -98,7 +98,14 @@ def test_decode_refuses_what_append_and_prompt_refuse(change, word):
         ops.build_attn_decode_params(**{**_decode_args(), **change})
 
 
-@pytest.mark.parametrize("change", [dict(no_append=True, k_off=0, v_off=0, qkv=torch.zeros(2, 256)), dict(page_table=torch.zeros(4, dtype=torch.int32), shared_table=True),
+def test_decode_refuses_rows_that_append_to_one_sequence():
+    """Rows of one sequence would read each other's new rows while they are written."""
+    with pytest.raises(ValueError, match="no_append"):
+        ops.build_attn_decode_params(**{**_decode_args(), "page_table": torch.zeros(4, dtype=torch.int32), "shared_table": True})
+
+
+@pytest.mark.parametrize("change", [dict(no_append=True, k_off=0, v_off=0, qkv=torch.zeros(2, 256)), dict(page_table=torch.zeros(4, dtype=torch.int32), shared_table=True, no_append=True),
+                                    dict(page_table=torch.zeros(4, dtype=torch.int32), shared_table=True, batch=1), dict(page_table=torch.zeros(4, dtype=torch.int32), batch=1),
                                     dict(qkv=torch.zeros(2, 600)[:, 8:], out=torch.zeros(2, 300)[:, 4:]), dict(batch=1, ld_qkv=7, ld_out=7)])
 def test_decode_takes_calls_that_are_in_order(change):
     """(up to the check of the device, which is the last but one)"""
