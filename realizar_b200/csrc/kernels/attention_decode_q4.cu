@@ -33,12 +33,14 @@
 #include "attention_q4.cuh"
 #include "kv_q4.cuh"
 #include <algorithm>
+#include <atomic>
 
 namespace rlz {
 
 // 3211: a tile's helpers or main warps never answered (bounded wait ran out); 3311: a position beyond the page-table row (the sequence is skipped);
 // 3312: a page id outside the cache (read as page 0, not written)
 __device__ int g_attn_q4_error = 0;
+static std::atomic<bool> attn_q4_ran{false};         // until a launch there is no status to fetch, which takes a synchronous copy
 
 constexpr int QD_STAGES = 3, QD_MAX_SMS = 148, QD_HELPERS = 128;
 constexpr int QD_PAIR = 2 * Q4_PAGE;          // tokens of a pair of pages
@@ -709,6 +711,7 @@ int attn_decode_q4_dispatch(const AttnDecodeParams& p, cudaStream_t st) {
   if (p.rope_dim < 0 || p.rope_dim > p.head_dim || (p.rope_dim & 1)) return -3;
   if (((uintptr_t)p.k_cache & 15) || ((uintptr_t)p.v_cache & 15) || ((uintptr_t)p.partial & 15)) return -4;
   if (p.window < 0) return -5;
+  attn_q4_ran.store(true, std::memory_order_relaxed);
   const bool narrow = p.n_heads / p.n_kv_heads <= qd_heads(1);
   switch (p.head_dim) {
     case 64: return narrow ? launch_decode_q4<64, 1>(p, st) : launch_decode_q4<64, 2>(p, st);
@@ -731,6 +734,7 @@ long long rlz_attn_q4_partial_floats(int head_dim) {
 // 0 / 3211 / 3311 / 3312
 int rlz_attn_q4_error(int clear) {
   int v = 0;
+  if (!rlz::attn_q4_ran.load(std::memory_order_relaxed)) return 0;
   if (cudaMemcpyFromSymbol(&v, rlz::g_attn_q4_error, sizeof(int)) != cudaSuccess) return -1;
   if (clear && v) { int z = 0; cudaMemcpyToSymbol(rlz::g_attn_q4_error, &z, sizeof(int)); }
   return v;

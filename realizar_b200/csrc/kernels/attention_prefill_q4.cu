@@ -31,12 +31,14 @@
 #include "kv_q4.cuh"
 #include "tcgen05_common.cuh"
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace rlz {
 
 // 3113: a page id outside the cache (read as page 0); 3114: rows beyond the page table (not computed); 3115: a bounded wait ran out
 __device__ int g_prefill_q4_error = 0;
+static std::atomic<bool> prefill_q4_ran{false};      // until a launch there is no status to fetch, which takes a synchronous copy
 
 constexpr int QP_THREADS = 640, QP_GROUP = 128, QP_ROWS = 2 * QP_GROUP, QP_KEYS = 128, QP_MAX_CTAS = 148;
 constexpr int QP_MAX_SPLIT = 8;                // CTAs to a cluster
@@ -786,6 +788,7 @@ int attn_prefill_q4_dispatch(const AttnPrefillParams& given, cudaStream_t st) {
   // row tiles x key tiles are counted in 32 bits
   const int64_t mtiles = ((int64_t)p.n_tokens * (p.n_heads / p.n_kv_heads) + QP_ROWS - 1) / QP_ROWS;
   if (mtiles * p.n_kv_heads * ((int64_t)p.pt_len * Q4_PAGE / QP_KEYS + 2) > INT32_MAX) return -6;
+  prefill_q4_ran.store(true, std::memory_order_relaxed);
   switch (p.head_dim) {
     case 64: return launch_prefill_q4<64>(p, st);
     case 80: return launch_prefill_q4<80>(p, st);
@@ -807,6 +810,7 @@ long long rlz_attn_prefill_q4_scratch_floats(int n_tokens, int n_heads, int n_kv
 // 0 / 3113 / 3114 / 3115
 int rlz_attn_prefill_q4_error(int clear) {
   int v = 0;
+  if (!rlz::prefill_q4_ran.load(std::memory_order_relaxed)) return 0;
   if (cudaMemcpyFromSymbol(&v, rlz::g_prefill_q4_error, sizeof(int)) != cudaSuccess) return -1;
   if (clear && v) { int z = 0; cudaMemcpyToSymbol(rlz::g_prefill_q4_error, &z, sizeof(int)); }
   return v;

@@ -1,5 +1,5 @@
-// Parameter block of the prompt attention, and the launchers of the kernels over 4-bit caches (attention_q4.cu) that the
-// general entry points hand over to.
+// Parameter block of the prompt attention, and the launchers of the kernels over 4-bit caches (attention_decode_q4.cu,
+// attention_prefill_q4.cu) that the general entry points hand over to.
 #pragma once
 #include "attention_decode_body.cuh"
 

@@ -10,11 +10,13 @@
 // registers that the compiler takes by itself (three blocks to an SM) it is 86 us, with 64 (four) 71, with 48 (five) 73; 4 query heads
 // to a warp and five blocks 71, one key head 83.
 #include "kv_q4.cuh"
+#include <atomic>
 
 namespace rlz {
 
 // 3405: a page id outside the cache (the row's K and V are not written)
 __device__ int g_q4_append_error = 0;
+static std::atomic<bool> q4_append_ran{false};       // until a launch there is no status to fetch, which takes a synchronous copy
 
 struct QkAppendParams {
   const float* qkv;            // [rows, ld]: q heads | k heads | v heads
@@ -198,6 +200,7 @@ int rlz_qk_norm_rope_append(const rlz::QkAppendParams* pp, void* stream) {
   if (!p.q_norm_w != !p.k_norm_w) return -5;
   if (((uintptr_t)p.qkv & 7) || ((uintptr_t)p.q_out & 7) || (p.ld & 1) || (p.ld_q & 1)) return -6;       // pairs are moved as 8 bytes
   cudaStream_t st = (cudaStream_t)stream;
+  q4_append_ran.store(true, std::memory_order_relaxed);
   switch (p.head_dim) {
     case 64: return launch_qk_append<64>(p, st);
     case 80: return launch_qk_append<80>(p, st);
@@ -209,6 +212,7 @@ int rlz_qk_norm_rope_append(const rlz::QkAppendParams* pp, void* stream) {
 // 0 / 3405
 int rlz_q4_append_error(int clear) {
   int v = 0;
+  if (!rlz::q4_append_ran.load(std::memory_order_relaxed)) return 0;
   if (cudaMemcpyFromSymbol(&v, rlz::g_q4_append_error, sizeof(int)) != cudaSuccess) return -1;
   if (clear && v) { int z = 0; cudaMemcpyToSymbol(rlz::g_q4_append_error, &z, sizeof(int)); }
   return v;

@@ -182,3 +182,14 @@ def test_library_handle_is_published_with_its_signatures(monkeypatch):
     _native.cuda_lib()
     second.join(10)
     assert seen == [True]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="other tests may have launched the kernels")
+def test_status_of_kernels_that_never_ran_is_not_fetched():
+    """Each status word is a synchronous copy from the device (12 us) after every prompt pass: programs without a 4-bit cache do not pay for
+    those of its kernels.  (Without a device a copy would answer -1.)"""
+    from realizar_b200 import _native
+    if not _native.cuda_lib_path().exists():
+        pytest.skip("kernel library not built")
+    lib = ops.lib()
+    assert [lib.rlz_q4_append_error(1), lib.rlz_attn_q4_error(1), lib.rlz_attn_prefill_q4_error(1)] == [0, 0, 0]
