@@ -1000,3 +1000,21 @@ def test_engine_batch_step_over_the_4_bit_cache(cuda_device, name):
         for a, b in zip(res[how], res["alone"]):
             for s in lens:
                 assert _cos(a[s], b[s]) > 0.99, (how, s)
+
+
+@pytest.mark.parametrize("size", [0.0, 1e-20, 1e-32, 1e-38])
+def test_prompt_with_tiny_queries_behind_zero_keys(cuda_device, size):
+    """Key tiles of zeros and queries near the smallest numbers: all scores are 0 or next to it, and no tile's keys drop out of the mean."""
+    from realizar_b200 import ops
+    h, kvh, d, n, rows = 4, 2, 64, 700, 90
+    kc, vc = _cache(46, kvh, d)
+    pt = torch.randperm(46, device="cuda").to(torch.int32)[:44].contiguous()
+    kc.flatten(-2)[pt[:20].long(), :, 8 * d:] = 0                    # the first 320 keys; the rows before the last begin in a tile that is masked in part
+    qkv = size * torch.randn(rows, (h + 2 * kvh) * d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    ks, vs = _gather(kc, pt, d, False, n), _gather(vc, pt, d, True, n)
+    for first in (n - rows, 100):
+        out = torch.empty(rows, h * d, device="cuda")
+        ops.attn_prefill(qkv, out, kc, vc, pt, rows, first, h, kvh, d)
+        for r in range(0, rows, 7):
+            p1 = first + r + 1
+            assert _rel(out[r], _attend64(qkv[r, : h * d].double().view(h, d), ks[:, :p1], vs[:, :p1], 0)) < 4e-3, (first, r)
