@@ -3,8 +3,9 @@
 //
 //   s_t = q . k_t = scale_t (q . code_t) + min_t sum(q)        o = sum_t p_t v_t = sum_t (p_t scale'_t) code'_t + sum_t p_t min'_t
 //
-// Bound by the bytes of the cache as long as the arithmetic of the codes is cheap (96 sequences of 8192 tokens of 128 dims, 8 kv heads:
-// 129 us, 4.5 TB/s of the 6.6 that a copy reaches):
+// Meant to be bound by the bytes of the cache, so the arithmetic of the codes has to be cheap (96 ragged sequences of up to 8192 tokens of
+// 128 dims, 8 kv heads: 129 us, 4.5 TB/s of the 6.6 that a copy reaches; what is missing is latency, a warp's steps from a pair's keys to
+// its values one after another, with 0.53 of the issue slots used):
 //   * Keys: a masked word holds four codes as bytes, and the 8-bit integer product takes them as they are; q comes as three 8-bit
 //     digits of a 24-bit integer (its largest value in [2^22, 2^23) x 127 / 128), so the sums over the dims are exact; sum(q) is that of
 //     the integers.
