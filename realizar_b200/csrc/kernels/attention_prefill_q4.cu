@@ -803,7 +803,7 @@ int attn_prefill_q4_dispatch(const AttnPrefillParams& given, cudaStream_t st) {
 extern "C" {
 
 // floats of scratch with which the keys can be split, whatever the number of rows is
-long long rlz_attn_prefill_q4_scratch_floats(int n_tokens, int n_heads, int n_kv_heads, int head_dim) {
+long long rlz_attn_prefill_q4_scratch_floats(int head_dim) {
   return 2LL * rlz::QP_MAX_CTAS * rlz::QP_ROWS * (head_dim + 4) + rlz::QP_COUNTERS;
 }
 

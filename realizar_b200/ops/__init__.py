@@ -269,6 +269,12 @@ def attn_decode_scratch(batch: int, n_heads: int, splits: int, head_dim: int, de
 def build_attn_decode_params(qkv, out, k_cache, v_cache, positions, page_table, partial, counters, n_heads, n_kv_heads, head_dim,
                              splits, batch, rope_dim, rope_type, rope_theta, q_off, k_off, v_off, q_norm_w=None, k_norm_w=None,
                              eps=1e-6, ld_qkv=None, ld_out=None, shared_table=False, no_append=False, window=0, rope_table=None) -> S.AttnDecodeParams:
+    """Description of a decode attention launch (``attn_decode_launch``), which holds no references: the tensors have to outlive it.  Rows
+    ``0 .. batch-1`` of ``qkv`` (q, k and v heads at the offsets) are the new tokens at ``positions`` (below 0: the row is idle) of the sequences
+    whose pages ``page_table [batch, pages]`` lists, or with ``shared_table`` of one sequence.  Their heads are normalised (when the weights are
+    given) and rotated, k and v written to the cache unless ``no_append``, and ``out`` is the attention over positions up to their own.  4-bit
+    caches: the arguments are checked here, and ``shared_table`` with several rows needs ``no_append``.  No two rows may append at the same
+    place, and ``out`` shares no memory with ``qkv`` or the caches."""
     fmt = kv_format(k_cache, head_dim)
     if fmt == KV_Q4:
         _check_decode_q4(qkv, out, k_cache, v_cache, positions, page_table, partial, counters, n_heads, n_kv_heads, head_dim, batch, rope_dim, q_off, k_off, v_off,
@@ -286,7 +292,7 @@ def build_attn_decode_params(qkv, out, k_cache, v_cache, positions, page_table, 
     p.rope_theta, p.eps, p.scale = rope_theta, eps, head_dim ** -0.5
     p.pt_stride = 0 if shared_table else (page_table.stride(0) if page_table.dim() > 1 else page_table.shape[-1])
     p.no_append = 1 if no_append else 0
-    p.window = int(window or 0)
+    p.window = min(int(window or 0), 2 ** 31 - 1)                         # (a field of 32 bits; positions have no more)
     p.kv_q8 = fmt
     p.num_pages = int(k_cache.shape[0]) if k_cache.dim() >= 4 else 0      # [pages, kv_heads, page, row]: page ids are checked on the device
     if rope_table is not None:
@@ -364,7 +370,7 @@ def attn_prefill(qkv: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     ``impl``: "tc" (128-query tiles on tcgen05) or "mma" (16-query tiles on mma.sync); None = the launcher's choice.
     ``scratch`` (4-bit caches, from ``attn_prefill_scratch``, one to a stream): lets the keys be divided over all SMs where the rows, and
     clusters of up to eight SMs to 256 (row, query head) pairs of a kv head, would leave some idle.  Over a 4-bit cache, rows whose positions (read on the device) lie beyond the page table are not computed, nor are
-    those that share 256 (row, query head) pairs of a kv head with them, and the device status tells."""
+    those that share 256 (row, query head) pairs of a kv head with them, and the device status tells.  ``out`` shares no memory with ``qkv``."""
     if k_cache.dtype is torch.uint8 and k_cache.shape[-1] == head_dim // 2 + 4:
         return _attn_prefill_q4(qkv, out, k_cache, v_cache, page_table, n_tokens, pos0, n_heads, n_kv_heads, head_dim, q_off, window or 0, pos0_dev, impl, scratch)
     p = S.AttnPrefillParams()
@@ -396,7 +402,7 @@ def _attn_prefill_q4(qkv, out, k_cache, v_cache, page_table, n_tokens, pos0, n_h
             and dev >= 0 and dev == torch._C._cuda_getDevice()):
         _refuse_prefill(qkv, out, k_cache, v_cache, page_table, n, pos0, n_heads, n_kv_heads, d, q_off, window, pos0_dev, impl, scratch)
     p = S.AttnPrefillParams(qkv.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), ld, ld_out, n_heads, n_kv_heads, d, q_off,
-                            n, int(pos0), int(window), KV_Q4, d ** -0.5, bf16, ptr(pos0_dev), shape[0], pages, ptr(scratch), 0 if scratch is None else scratch.numel())
+                            n, int(pos0), min(int(window), 2 ** 31 - 1), KV_Q4, d ** -0.5, bf16, ptr(pos0_dev), shape[0], pages, ptr(scratch), 0 if scratch is None else scratch.numel())
     check(lib().rlz_attn_prefill_impl(ctypes.byref(p), stream_ptr(), -1), "attn_prefill")
 
 
@@ -434,7 +440,7 @@ def attn_prefill_scratch(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim:
     """Workspace with which ``attn_prefill`` divides the keys of a 4-bit cache evenly over the SMs: the same size for any number of rows.  One to a stream.
     Its first words are arrival counters, zero between launches; a launch whose bounded wait ran out (status 3115) may leave some raised:
     ``zero_()`` it before the next one, as the engine does."""
-    return torch.zeros(int(lib().rlz_attn_prefill_q4_scratch_floats(int(n_tokens), int(n_heads), int(n_kv_heads), int(head_dim))), device=device, dtype=torch.float32)
+    return torch.zeros(int(lib().rlz_attn_prefill_q4_scratch_floats(int(head_dim))), device=device, dtype=torch.float32)
 
 
 KV_BF16, KV_Q8, KV_Q4 = 0, 1, 2

@@ -187,7 +187,7 @@ def declare(lib: ctypes.CDLL) -> None:
     lib.rlz_attn_prefill_q4_error.argtypes = [c_int]
     lib.rlz_attn_q4_partial_floats.argtypes = [c_int]
     lib.rlz_attn_q4_partial_floats.restype = c_longlong
-    lib.rlz_attn_prefill_q4_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
+    lib.rlz_attn_prefill_q4_scratch_floats.argtypes = [c_int]
     lib.rlz_attn_prefill_q4_scratch_floats.restype = c_longlong
     lib.rlz_ll_reduce.argtypes = [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p]
     lib.rlz_advance.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]

@@ -1018,3 +1018,9 @@ def test_prompt_with_tiny_queries_behind_zero_keys(cuda_device, size):
         for r in range(0, rows, 7):
             p1 = first + r + 1
             assert _rel(out[r], _attend64(qkv[r, : h * d].double().view(h, d), ks[:, :p1], vs[:, :p1], 0)) < 4e-3, (first, r)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5])
+def test_windows_beyond_32_bits_hide_nothing(cuda_device, window):
+    _prompt(4, 2, 64, 90, 500, window=window)
+    _decode(4, 2, 64, [40, 17], seed=1, window=window)()
