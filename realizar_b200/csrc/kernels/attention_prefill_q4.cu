@@ -8,8 +8,8 @@
 //                  so that O is rarely read, scaled and written back.
 // Warps 0..7 do the softmax of the groups, 8..11 decode keys and 12..15 values (code x scale + minimum in fp16, rounded once) into two
 // buffers each of swizzled operand tiles, warps 16 and 17 issue the products of a group each.  The scores of one half are computed while
-// the softmax is at the other (whole tiles, whose scores have to wait for the product that reads P in their place: 280 instead of
-// 268 us for 2048 rows behind 6144 keys, 32 query and 8 kv heads of 128).  Registers are moved from the decoding and issuing warps to
+// the softmax is at the other (whole tiles, whose scores have to wait for the product that reads P in their place: 4% more
+// than the 271 us of 2048 rows behind 6144 keys, 32 query and 8 kv heads of 128).  Registers are moved from the decoding and issuing warps to
 // the softmax.
 //
 // Bound, for 256 rows and 128 keys of 128 dims, by the chain of product, softmax and product, about 4000 clocks: of them the tensor
